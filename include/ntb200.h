@@ -343,6 +343,66 @@ int ntb200_varlen_attention_weights(const void* q, int64_t ldq, const void* k, i
 int ntb200_transpose_ragged(const void* in, void* out, const int64_t* offsets, int64_t batch, int64_t regular,
                             int regular_is_rows, int64_t max_ragged, int elem_size, void* stream);
 
+/* ------------------------------------------------------------------ training: forward passes that keep what their gradients need
+ * and the gradients themselves.  No counterparts in the reference (its autograd tests are skipped).  Sums, statistics and
+ * softmax denominators are fp32 whatever the dtype; every gradient is a sum in a fixed order (no floating-point atomics), so
+ * the same inputs give the same bits.  Workspaces are the caller's and hold nothing between calls; calls that may run at the
+ * same time need one each.
+ *
+ * LayerNorm: ntb200_layer_norm that also writes mean and rstd of every row ([rows] fp32 each); then, from the output's
+ * gradient `grad`, grad_x (any of the three gradients may be NULL: not wanted) and the column sums
+ *   grad_gamma[c] = sum_t grad[t,c] (x[t,c] - mean[t]) rstd[t],   grad_beta[c] = sum_t grad[t,c]
+ * gamma NULL: no affine, then grad_gamma and grad_beta must be NULL.  workspace (needed with gamma): 4-byte aligned.
+ */
+int ntb200_layer_norm_train(const void* x, const void* gamma, const void* beta, float eps, void* out, float* mean,
+                            float* rstd, int64_t rows, int64_t cols, int dtype, void* stream);
+size_t ntb200_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int ntb200_layer_norm_backward(const void* grad, const void* x, const float* mean, const float* rstd,
+                               const void* gamma, void* grad_x, void* grad_gamma, void* grad_beta, int64_t rows,
+                               int64_t cols, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Embedding: out[t, :] = scale * weight[index[t], :] (the product in fp32, rounded once; errors as ntb200_embedding), and
+ *   grad_weight[v, :] = scale * sum over { t : index[t] = v } of grad[t, :]
+ * for every v in [0, vocab): zeros where v does not occur and for v = padding_idx (-1: none); indices out of range
+ * contribute nothing.  The sums run over the tokens in ascending groups of 32, sorted by index.  workspace: 16-byte aligned;
+ * tokens, vocab < 2^31 - 1.
+ */
+int ntb200_embedding_scaled(const void* weight, const void* index, int index_bytes, void* out, int64_t tokens,
+                            int64_t vocab, int64_t embed_dim, float scale, int dtype, void* stream);
+size_t ntb200_embedding_backward_workspace_bytes(int64_t tokens, int64_t embed_dim);
+int ntb200_embedding_backward(const void* grad, const void* index, int index_bytes, void* grad_weight, int64_t tokens,
+                              int64_t vocab, int64_t embed_dim, int64_t padding_idx, float scale, int dtype,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention: as ntb200_varlen_cross_attention_ws (self-attention: the same offsets twice; where q, k and v are the three
+ * thirds of one [T, 3*H*d] matrix the kernels and results are those of ntb200_varlen_attention), and
+ *   lse[h*q_tokens + t] = log2( sum_j exp2(scaling * log2(e) * q_t,h . k_j,h) )      (left unwritten for rows without keys)
+ * offsets_q / offsets_k count elements of matrices with row_elems_q / row_elems_k elements per token (1: token offsets).
+ *   path  0 = best available;  1 = SIMT;  2 = mma.sync kernel;  3 = tcgen05 kernel (1-3: for cross-checks)
+ * workspace: ntb200_varlen_cross_attention_workspace_bytes(batch, q_tokens, ...), 16-byte aligned, or NULL.
+ */
+int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                  void* out, float* lse, const int64_t* offsets_q, int64_t row_elems_q,
+                                  const int64_t* offsets_k, int64_t row_elems_k, int64_t batch, int64_t q_tokens,
+                                  int64_t k_tokens, int num_heads, int head_dim, int64_t max_len_q, float scaling,
+                                  int dtype, int path, void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradients from grad_out [q_tokens, H*d] (contiguous, as out): grad_q / grad_k / grad_v, row strides ld_grad_* in elements
+ * (they may be the three thirds of one [T, 3*H*d] matrix), must not overlap the inputs.  Rows of every sequence are written
+ * (zeros where the other side is empty); rows outside the sequences are left as they were.  The probabilities are computed
+ * again from q, k and lse.
+ *   path  0 = best available;  1 = the 32-bit tile kernels (any dtype and head_dim <= 256)
+ * workspace: 16-byte aligned.
+ */
+size_t ntb200_varlen_attention_backward_workspace_bytes(int64_t batch, int64_t q_tokens, int64_t k_tokens, int num_heads,
+                                                        int head_dim, int dtype);
+int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                                     const void* v, int64_t ldv, const void* out, const float* lse, void* grad_q,
+                                     int64_t ld_grad_q, void* grad_k, int64_t ld_grad_k, void* grad_v, int64_t ld_grad_v,
+                                     const int64_t* offsets_q, int64_t row_elems_q, const int64_t* offsets_k,
+                                     int64_t row_elems_k, int64_t batch, int64_t q_tokens, int64_t k_tokens,
+                                     int num_heads, int head_dim, int64_t max_len_q, int64_t max_len_k, float scaling,
+                                     int dtype, int path, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ reference-shaped helpers
  * q/k/v_buf[b, h, l, :] = qkv[tok(b,l), {0,E,2E} + h*d + :] + bias  for valid tokens (padded
  * positions are left untouched): bias add fused with packed -> padded head-major scatter.

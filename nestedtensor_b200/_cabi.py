@@ -57,6 +57,23 @@ SIGNATURES = {
                                                  c_void_p, c_size_t, c_void_p]),
     "ntb200_varlen_attention_weights": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                                 c_int64, c_int, c_int, c_int64, c_float, c_int, c_int, c_void_p]),
+    "ntb200_layer_norm_train": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int,
+                                        c_void_p]),
+    "ntb200_layer_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "ntb200_layer_norm_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                           c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    "ntb200_embedding_scaled": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_float, c_int, c_void_p]),
+    "ntb200_embedding_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "ntb200_embedding_backward": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_float, c_int,
+                                          c_void_p, c_size_t, c_void_p]),
+    "ntb200_varlen_attention_train": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                              c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int64, c_float,
+                                              c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "ntb200_varlen_attention_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),
+    "ntb200_varlen_attention_backward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                                 c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                                 c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int64, c_int64, c_float, c_int,
+                                                 c_int, c_void_p, c_size_t, c_void_p]),
     "ntb200_add_qkv_bias_pad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                         c_int, c_int, c_int64, c_int, c_void_p]),
     "ntb200_transpose_rm_padding": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int64,

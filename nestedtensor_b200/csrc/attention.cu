@@ -59,11 +59,11 @@ constexpr int kMaxHeadDim = 256;
 template <typename T>
 __global__ void __launch_bounds__(kSimtWarps * 32)
 attn_simt_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, int64_t ldv,
-                 T* __restrict__ out, const int64_t* __restrict__ offsets_q, const int64_t* __restrict__ offsets_k,
-                 int64_t batch, int64_t total_tokens, int H, int d, float scale) {
+                 T* __restrict__ out, const int64_t* __restrict__ offsets_q, const int64_t* __restrict__ offsets_k, int64_t row_elems_q,
+                 int64_t row_elems_k, int64_t batch, int64_t total_tokens, int H, int d, float scale, LseOut lse) {
   // q / k / v: first element of head 0 of token 0, row strides ldq / ldk / ldv (self-attention on a packed
   // [T, 3E] buffer: the three thirds of one row, all strides 3E, offsets_k == offsets_q); offsets in elements
-  // of the [tokens, E] matrices of the query and of the key / value nested tensors
+  // of matrices with row_elems_q / row_elems_k elements per token (E for the nested tensors of the inputs)
   __shared__ float s_q[kSimtWarps][kMaxHeadDim];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t wg = (int64_t)blockIdx.x * kSimtWarps + warp;
@@ -71,9 +71,9 @@ attn_simt_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, 
   const int64_t t = wg / H;
   const int h = (int)(wg % H);
   const int64_t E = (int64_t)H * d;
-  const int64_t b = find_entry(offsets_q, batch, t * E);
-  const int64_t tok0 = offsets_k[b] / E;
-  const int L = (int)((offsets_k[b + 1] - offsets_k[b]) / E);
+  const int64_t b = find_entry(offsets_q, batch, t * row_elems_q);
+  const int64_t tok0 = offsets_k[b] / row_elems_k;
+  const int L = (int)((offsets_k[b + 1] - offsets_k[b]) / row_elems_k);
   const T* qrow = q + t * ldq + (int64_t)h * d;
   for (int i = lane; i < d; i += 32) s_q[warp][i] = Cvt<T>::to_f(qrow[i]) * scale;
   __syncwarp();
@@ -118,6 +118,7 @@ attn_simt_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, 
     m = m_new;
   }
   const float inv = L > 0 ? 1.0f / l : 0.0f;  // a query whose key sequence is empty gets zeros
+  if (lse.ptr != nullptr && lane == 0 && L > 0) lse.ptr[(int64_t)h * lse.ld + t] = (m + logf(l)) * 1.4426950408889634f;
   T* orow = out + t * E + (int64_t)h * d;
 #pragma unroll
   for (int i = 0; i < DPL; ++i) {
@@ -148,7 +149,7 @@ template <typename T, int kD>
 __global__ void __launch_bounds__(kFaThreads)
 attn_fa_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v,
                    int64_t ldv, T* __restrict__ out, const int64_t* __restrict__ offsets_q, const int64_t* __restrict__ offsets_k,
-                   int H, float scale_log2e) {  // arguments as in attn_simt_kernel
+                   int64_t row_elems_q, int64_t row_elems_k, int H, float scale_log2e, LseOut lse) {  // arguments as in attn_simt_kernel
   extern __shared__ __align__(128) uint8_t fa_smem[];  // Q tile, two K tiles, two V tiles of 64 x kD each
   constexpr uint32_t kTileBytes = kBKV * kD * 2;
   uint8_t* s_q = fa_smem;
@@ -158,12 +159,12 @@ attn_fa_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, in
   const int b = blockIdx.z, h = blockIdx.y;
   const int64_t E = (int64_t)H * kD;
   const int64_t off_b = offsets_q[b];
-  const int Lq = (int)((offsets_q[b + 1] - off_b) / E);
+  const int Lq = (int)((offsets_q[b + 1] - off_b) / row_elems_q);
   const int q0 = blockIdx.x * kBQ;
   if (q0 >= Lq) return;
-  const int64_t tok0 = off_b / E;  // first query token (also the first output row)
-  const int64_t tokk0 = offsets_k[b] / E;
-  const int L = (int)((offsets_k[b + 1] - offsets_k[b]) / E);  // keys
+  const int64_t tok0 = off_b / row_elems_q;  // first query token (also the first output row)
+  const int64_t tokk0 = offsets_k[b] / row_elems_k;
+  const int L = (int)((offsets_k[b + 1] - offsets_k[b]) / row_elems_k);  // keys
   const T* qbase = q + tok0 * ldq + (int64_t)h * kD;
   const T* kbase = k + tokk0 * ldk + (int64_t)h * kD;
   const T* vbase = v + tokk0 * ldv + (int64_t)h * kD;
@@ -295,6 +296,11 @@ attn_fa_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, in
   l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
   const float i0 = 1.0f / l0, i1 = 1.0f / l1;
   const int r0 = q0 + warp * 16 + (lane >> 2), r1 = r0 + 8;
+  if (lse.ptr != nullptr && (lane & 3) == 0) {
+    float* lrow = lse.ptr + (int64_t)h * lse.ld + tok0;
+    if (r0 < Lq) lrow[r0] = m0 + log2f(l0);
+    if (r1 < Lq) lrow[r1] = m1 + log2f(l1);
+  }
   uint32_t* obase = reinterpret_cast<uint32_t*>(out + (tok0 + r0) * E + (int64_t)h * kD);
   uint32_t* obase1 = reinterpret_cast<uint32_t*>(out + (tok0 + r1) * E + (int64_t)h * kD);
 #pragma unroll
@@ -475,6 +481,8 @@ struct QkvSrc {
   const void *q, *k, *v;
   int64_t ldq, ldk, ldv;
   const int64_t *offsets_q, *offsets_k;
+  int64_t row_elems_q, row_elems_k;  // elements per token in offsets_q / offsets_k
+  LseOut lse = {nullptr, 0};
 };
 
 template <typename T>
@@ -483,7 +491,8 @@ int launch_attn_simt(const QkvSrc& s, void* out, int64_t batch, int64_t q_tokens
   if (blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
   attn_simt_kernel<T><<<(unsigned)blocks, kSimtWarps * 32, 0, st>>>(static_cast<const T*>(s.q), s.ldq, static_cast<const T*>(s.k),
                                                                     s.ldk, static_cast<const T*>(s.v), s.ldv, static_cast<T*>(out),
-                                                                    s.offsets_q, s.offsets_k, batch, q_tokens, H, d, scale);
+                                                                    s.offsets_q, s.offsets_k, s.row_elems_q, s.row_elems_k, batch,
+                                                                    q_tokens, H, d, scale, s.lse);
   return status_from_cuda(cudaGetLastError());
 }
 
@@ -500,7 +509,7 @@ int launch_attn_fa(const QkvSrc& s, void* out, int64_t batch, int H, int64_t max
   dim3 grid((unsigned)ceil_div(max_len_q, kBQ), (unsigned)H, (unsigned)batch);
   attn_fa_kernel<T, D><<<grid, kFaThreads, kSmem, st>>>(static_cast<const T*>(s.q), s.ldq, static_cast<const T*>(s.k), s.ldk,
                                                         static_cast<const T*>(s.v), s.ldv, static_cast<T*>(out), s.offsets_q,
-                                                        s.offsets_k, H, scale * 1.4426950408889634f);
+                                                        s.offsets_k, s.row_elems_q, s.row_elems_k, H, scale * 1.4426950408889634f, s.lse);
   return status_from_cuda(cudaGetLastError());
 }
 
@@ -519,7 +528,7 @@ int launch_attn_tiny_dr(const QkvSrc& s, void* out, int64_t batch, int H, float 
   if (blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
   attn_tiny_kernel<T, D, R, kWarps><<<(unsigned)blocks, kWarps * 32, kWarps * kPerWarp, st>>>(
       static_cast<const T*>(s.q), s.ldq, static_cast<const T*>(s.k), s.ldk, static_cast<const T*>(s.v), s.ldv, static_cast<T*>(out),
-      s.offsets_q, s.offsets_k, batch, H, scale * 1.4426950408889634f);
+      s.offsets_q, s.offsets_k, s.row_elems_q, s.row_elems_k, batch, H, scale * 1.4426950408889634f, s.lse);
   return status_from_cuda(cudaGetLastError());
 }
 
@@ -585,7 +594,7 @@ int ntb200_varlen_attention(const void* qkv, void* out, const int64_t* offsets, 
     if (path == 4 || (path == 0 && tiny_ok)) {
       if (!tiny_ok) return NTB200_UNSUPPORTED_SHAPE;
       const char* base = static_cast<const char*>(qkv);
-      const QkvSrc src = {base, base + E * 2, base + 2 * E * 2, 3 * E, 3 * E, 3 * E, offsets, offsets};
+      const QkvSrc src = {base, base + E * 2, base + 2 * E * 2, 3 * E, 3 * E, 3 * E, offsets, offsets, E, E};
       if (dtype == NTB200_F16) return launch_attn_tiny<__half>(src, out, batch, num_heads, head_dim, max_len, scaling, st);
       return launch_attn_tiny<__nv_bfloat16>(src, out, batch, num_heads, head_dim, max_len, scaling, st);
     }
@@ -602,12 +611,13 @@ int ntb200_varlen_attention(const void* qkv, void* out, const int64_t* offsets, 
     // 128-row item.  Which kernel computes a sequence thus depends on the sequence alone, never on the batch around it,
     // so a batch cut into shards or ranges reproduces the one-call result bit for bit.
     const int skip_short = path == 0 ? (int)kTinyMaxLen : 0;
-    return attn_tcgen05_launch(qkv, out, offsets, batch, total_tokens, num_heads, scaling, dtype, workspace, st, skip_short);
+    return attn_tcgen05_launch(qkv, out, AttnRows{offsets, offsets, (int64_t)num_heads * head_dim, (int64_t)num_heads * head_dim, nullptr},
+                               batch, total_tokens, num_heads, scaling, dtype, workspace, st, skip_short);
   }
   const int64_t E = (int64_t)num_heads * head_dim;
   const size_t es = dtype == NTB200_F32 ? 4 : 2;
   const char* base = static_cast<const char*>(qkv);
-  const QkvSrc src = {base, base + E * es, base + 2 * E * es, 3 * E, 3 * E, 3 * E, offsets, offsets};
+  const QkvSrc src = {base, base + E * es, base + 2 * E * es, 3 * E, 3 * E, 3 * E, offsets, offsets, E, E};
   return launch_attn_generic(src, out, batch, total_tokens, num_heads, head_dim, max_len, scaling, dtype, force_simt ? 1 : path, st);
 }
 
@@ -623,7 +633,7 @@ int ntb200_varlen_cross_attention(const void* q, int64_t ldq, const void* k, int
   if (batch == 0 || q_tokens == 0) return NTB200_OK;
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || offsets_q == nullptr || offsets_k == nullptr)
     return NTB200_INVALID_ARG;
-  const QkvSrc src = {q, k, v, ldq, ldk, ldv, offsets_q, offsets_k};
+  const QkvSrc src = {q, k, v, ldq, ldk, ldv, offsets_q, offsets_k, E, E};
   return launch_attn_generic(src, out, batch, q_tokens, num_heads, head_dim, max_len_q, scaling, dtype, path,
                              static_cast<cudaStream_t>(stream));
 }
@@ -656,12 +666,54 @@ int ntb200_varlen_cross_attention_ws(const void* q, int64_t ldq, const void* k, 
     const size_t need = attn_tcgen05_workspace_bytes(batch, q_tokens);
     if (workspace == nullptr || workspace_bytes < need) return NTB200_WORKSPACE_TOO_SMALL;
     if (!aligned16(workspace)) return NTB200_MISALIGNED;
-    return attn_tcgen05_cross_launch(q, ldq, k, ldk, v, ldv, out, offsets_q, offsets_k, batch, q_tokens, k_tokens, num_heads, scaling,
-                                     dtype, workspace, static_cast<cudaStream_t>(stream));
+    return attn_tcgen05_cross_launch(q, ldq, k, ldk, v, ldv, out, AttnRows{offsets_q, offsets_k, E, E, nullptr}, batch, q_tokens, k_tokens,
+                                     num_heads, scaling, dtype, workspace, static_cast<cudaStream_t>(stream));
   }
-  const QkvSrc src = {q, k, v, ldq, ldk, ldv, offsets_q, offsets_k};
+  const QkvSrc src = {q, k, v, ldq, ldk, ldv, offsets_q, offsets_k, E, E};
   return launch_attn_generic(src, out, batch, q_tokens, num_heads, head_dim, max_len_q, scaling, dtype, path,
                              static_cast<cudaStream_t>(stream));
+}
+
+int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* out, float* lse,
+                                  const int64_t* offsets_q, int64_t row_elems_q, const int64_t* offsets_k, int64_t row_elems_k,
+                                  int64_t batch, int64_t q_tokens, int64_t k_tokens, int num_heads, int head_dim, int64_t max_len_q,
+                                  float scaling, int dtype, int path, void* workspace, size_t workspace_bytes, void* stream) {
+  if (batch < 0 || q_tokens < 0 || k_tokens < 0 || num_heads < 1 || head_dim < 1 || max_len_q < 0 || row_elems_q < 1 || row_elems_k < 1 ||
+      path < 0 || path > 3)
+    return NTB200_INVALID_ARG;
+  if (dtype != NTB200_F32 && dtype != NTB200_F16 && dtype != NTB200_BF16) return NTB200_UNSUPPORTED_DTYPE;
+  if (head_dim > kMaxHeadDim) return NTB200_UNSUPPORTED_SHAPE;
+  const int64_t E = (int64_t)num_heads * head_dim;
+  if (ldq < E || ldk < E || ldv < E) return NTB200_INVALID_ARG;
+  if (batch == 0 || q_tokens == 0) return NTB200_OK;
+  if (q == nullptr || out == nullptr || lse == nullptr || offsets_q == nullptr || offsets_k == nullptr) return NTB200_INVALID_ARG;
+  if (k_tokens > 0 && (k == nullptr || v == nullptr)) return NTB200_INVALID_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const QkvSrc src = {q, k, v, ldq, ldk, ldv, offsets_q, offsets_k, row_elems_q, row_elems_k, {lse, q_tokens}};
+  // one packed [T, 3E] matrix of a self-attention: q, k and v are its three column blocks over the same sequences
+  const size_t es = dtype == NTB200_F32 ? 4 : 2;
+  const bool packed = offsets_q == offsets_k && row_elems_q == row_elems_k && q_tokens == k_tokens && ldq == 3 * E && ldk == 3 * E &&
+                      ldv == 3 * E && static_cast<const char*>(k) == static_cast<const char*>(q) + E * es &&
+                      static_cast<const char*>(v) == static_cast<const char*>(q) + 2 * E * es;
+  // the same choices as the inference entry points
+  if (path == 0 && packed && dtype != NTB200_F32 && (head_dim == 32 || head_dim == 64 || head_dim == 128) && E % 8 == 0 && aligned16(q) &&
+      aligned16(out) && max_len_q >= 1 && max_len_q <= kTinyMaxLen) {
+    if (dtype == NTB200_F16) return launch_attn_tiny<__half>(src, out, batch, num_heads, head_dim, max_len_q, scaling, st);
+    return launch_attn_tiny<__nv_bfloat16>(src, out, batch, num_heads, head_dim, max_len_q, scaling, st);
+  }
+  const bool tc_ok = dtype != NTB200_F32 && attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype) && k_tokens > 0 &&
+                     k_tokens < (1ll << 31) - 128 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && ldq % 8 == 0 &&
+                     ldk % 8 == 0 && ldv % 8 == 0;
+  if (path == 3 || (path == 0 && tc_ok && workspace != nullptr)) {
+    if (!tc_ok) return NTB200_UNSUPPORTED_SHAPE;
+    if (workspace == nullptr || workspace_bytes < attn_tcgen05_workspace_bytes(batch, q_tokens)) return NTB200_WORKSPACE_TOO_SMALL;
+    if (!aligned16(workspace)) return NTB200_MISALIGNED;
+    const AttnRows rows = {offsets_q, offsets_k, row_elems_q, row_elems_k, lse};
+    if (packed)
+      return attn_tcgen05_launch(q, out, rows, batch, q_tokens, num_heads, scaling, dtype, workspace, st, path == 0 ? (int)kTinyMaxLen : 0);
+    return attn_tcgen05_cross_launch(q, ldq, k, ldk, v, ldv, out, rows, batch, q_tokens, k_tokens, num_heads, scaling, dtype, workspace, st);
+  }
+  return launch_attn_generic(src, out, batch, q_tokens, num_heads, head_dim, max_len_q, scaling, dtype, path, st);
 }
 
 int ntb200_varlen_attention_weights(const void* q, int64_t ldq, const void* k, int64_t ldk, void* weights,

@@ -8,18 +8,26 @@
 
 namespace ntb200 {
 
+// Where the sequences lie in the query and key / value matrices: B+1 offsets in elements, row_elems of them per token; lse:
+// NULL, or [H, q_tokens] fp32 for the base-2 logarithms of the softmax denominators.
+struct AttnRows {
+  const int64_t *offsets_q, *offsets_k;
+  int64_t row_elems_q, row_elems_k;
+  float* lse;
+};
+
 int64_t attn_tcgen05_item_capacity(int64_t batch, int64_t total_tokens);
 size_t attn_tcgen05_workspace_bytes(int64_t batch, int64_t total_tokens);
 bool attn_tcgen05_supported(int64_t batch, int64_t total_tokens, int num_heads, int head_dim, int dtype);
 // skip_short > 0 (then it must be 32): sequences of at most that many tokens get no work item; single warps of the
 // launch that builds the work list compute them
-int attn_tcgen05_launch(const void* qkv, void* out, const int64_t* offsets, int64_t batch, int64_t total_tokens, int H,
-                        float scaling, int dtype, void* workspace, cudaStream_t st, int skip_short);
+int attn_tcgen05_launch(const void* qkv, void* out, const AttnRows& rows, int64_t batch, int64_t total_tokens, int H, float scaling,
+                        int dtype, void* workspace, cudaStream_t st, int skip_short);
 // queries of sequence b over the keys / values of sequence b of other matrices (row strides in elements, multiples of 8;
 // k_tokens = rows of the key / value matrices); workspace as for the self-attention launch with (batch, q_tokens)
 int attn_tcgen05_cross_launch(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* out,
-                              const int64_t* offsets_q, const int64_t* offsets_k, int64_t batch, int64_t q_tokens, int64_t k_tokens,
-                              int H, float scaling, int dtype, void* workspace, cudaStream_t st);
+                              const AttnRows& rows, int64_t batch, int64_t q_tokens, int64_t k_tokens, int H, float scaling, int dtype,
+                              void* workspace, cudaStream_t st);
 int attn_tcgen05_error_flags_read_and_clear();
 int construct_error_flags_read_and_clear();  // construct.cu: bit 0 = embedding index out of range
 

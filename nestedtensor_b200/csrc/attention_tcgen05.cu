@@ -107,16 +107,16 @@ constexpr int kBuckets = 9;  // key blocks 1..8+, (0 unused)
 
 template <bool SELF>  // SELF: queries and keys are the same sequences, so none has queries without keys
 __device__ __forceinline__ void build_items_block(const int64_t* __restrict__ offsets_q, const int64_t* __restrict__ offsets_k,
-                                                  int64_t batch, int64_t row_elems, int4* __restrict__ items,
-                                                  int* __restrict__ count, int64_t capacity, uint16_t* __restrict__ out,
-                                                  int skip_short) {
+                                                  int64_t row_elems_q, int64_t row_elems_k, int64_t E, int64_t batch,
+                                                  int4* __restrict__ items, int* __restrict__ count, int64_t capacity,
+                                                  uint16_t* __restrict__ out, int skip_short) {
   const int nthreads = (int)blockDim.x;  // 1024 alone, 256 beside the short-sequence warps
   __shared__ int s_cnt[kBuckets];
   __shared__ int s_base[kBuckets];
   if (threadIdx.x < kBuckets) s_cnt[threadIdx.x] = 0;
   __syncthreads();
   for (int64_t b = threadIdx.x; b < batch; b += nthreads) {
-    const int64_t Lq = (offsets_q[b + 1] - offsets_q[b]) / row_elems, Lk = (offsets_k[b + 1] - offsets_k[b]) / row_elems;
+    const int64_t Lq = (offsets_q[b + 1] - offsets_q[b]) / row_elems_q, Lk = (offsets_k[b + 1] - offsets_k[b]) / row_elems_k;
     if (Lq <= 0 || Lk <= 0 || (Lq <= skip_short && Lk <= skip_short)) continue;
     const int nq = (int)((Lq + kQT - 1) / kQT);
     int nb = (int)((Lk + kKV - 1) / kKV);
@@ -134,13 +134,13 @@ __device__ __forceinline__ void build_items_block(const int64_t* __restrict__ of
   }
   __syncthreads();
   for (int64_t b = threadIdx.x; b < batch; b += nthreads) {
-    const int64_t Lq = (offsets_q[b + 1] - offsets_q[b]) / row_elems, Lk = (offsets_k[b + 1] - offsets_k[b]) / row_elems;
+    const int64_t Lq = (offsets_q[b + 1] - offsets_q[b]) / row_elems_q, Lk = (offsets_k[b + 1] - offsets_k[b]) / row_elems_k;
     if (Lq <= 0 || Lk <= 0 || (Lq <= skip_short && Lk <= skip_short)) continue;
     const int nq = (int)((Lq + kQT - 1) / kQT);
     int nb = (int)((Lk + kKV - 1) / kKV);
     nb = nb >= kBuckets ? kBuckets - 1 : nb;
     const int pos = atomicAdd(&s_base[nb], nq);
-    const int tq0 = (int)(offsets_q[b] / row_elems), tk0 = (int)(offsets_k[b] / row_elems);
+    const int tq0 = (int)(offsets_q[b] / row_elems_q), tk0 = (int)(offsets_k[b] / row_elems_k);
     for (int t = 0; t < nq; ++t) {
       const int64_t rows = Lq - (int64_t)t * kQT < kQT ? Lq - (int64_t)t * kQT : kQT;
       if (pos + t < capacity) items[pos + t] = make_int4(tq0 + t * kQT, (int)rows, tk0, (int)Lk);
@@ -159,23 +159,23 @@ __device__ __forceinline__ void build_items_block(const int64_t* __restrict__ of
     if (pos < kListThreads) {
       s_empty[pos] = (int)b;
     } else {  // more than the list holds: this thread clears the rows itself
-      for (int64_t e = offsets_q[b]; e < offsets_q[b + 1]; ++e) out[e] = 0;
+      for (int64_t e = offsets_q[b] / row_elems_q * E; e < offsets_q[b + 1] / row_elems_q * E; ++e) out[e] = 0;
     }
   }
   __syncthreads();
   const int n_listed = s_nempty < kListThreads ? s_nempty : kListThreads;
   for (int i = 0; i < n_listed; ++i) {
-    const int64_t e0 = offsets_q[s_empty[i]], e1 = offsets_q[s_empty[i] + 1];
+    const int64_t e0 = offsets_q[s_empty[i]] / row_elems_q * E, e1 = offsets_q[s_empty[i] + 1] / row_elems_q * E;
     for (int64_t e = e0 + threadIdx.x; e < e1; e += nthreads) out[e] = 0;
   }
 }
 
 __global__ void __launch_bounds__(kListThreads) build_items_kernel(const int64_t* __restrict__ offsets_q,
-                                                                   const int64_t* __restrict__ offsets_k, int64_t batch,
-                                                                   int64_t row_elems, int4* __restrict__ items,
-                                                                   int* __restrict__ count, int64_t capacity,
-                                                                   uint16_t* __restrict__ out) {
-  build_items_block<false>(offsets_q, offsets_k, batch, row_elems, items, count, capacity, out, 0);
+                                                                   const int64_t* __restrict__ offsets_k, int64_t row_elems_q,
+                                                                   int64_t row_elems_k, int64_t E, int64_t batch,
+                                                                   int4* __restrict__ items, int* __restrict__ count,
+                                                                   int64_t capacity, uint16_t* __restrict__ out) {
+  build_items_block<false>(offsets_q, offsets_k, row_elems_q, row_elems_k, E, batch, items, count, capacity, out, 0);
 }
 
 // The same list for self-attention on the default path, in one launch with the short sequences: block 0 builds the list
@@ -187,18 +187,20 @@ constexpr int kPrepSmem = kPrepWarps * 3 * (int)kTinyMaxLen * kHD * 2;  // 96 KB
 
 template <typename T>
 __global__ void __launch_bounds__(kPrepWarps * 32)
-prepare_self_attention_kernel(const int64_t* __restrict__ offsets, int64_t batch, int64_t row_elems, int4* __restrict__ items,
-                              int* __restrict__ count, int64_t capacity, const T* __restrict__ qkv, T* __restrict__ out, int H,
-                              float scale_log2e) {
+prepare_self_attention_kernel(const int64_t* __restrict__ offsets, int64_t row_elems, int64_t batch, int64_t E,
+                              int4* __restrict__ items, int* __restrict__ count, int64_t capacity, const T* __restrict__ qkv,
+                              T* __restrict__ out, int H, float scale_log2e, LseOut lse) {
   extern __shared__ __align__(128) uint8_t prep_smem[];
   if (blockIdx.x == 0) {
-    build_items_block<true>(offsets, offsets, batch, row_elems, items, count, capacity, reinterpret_cast<uint16_t*>(out), (int)kTinyMaxLen);
+    build_items_block<true>(offsets, offsets, row_elems, row_elems, E, batch, items, count, capacity, reinterpret_cast<uint16_t*>(out),
+                            (int)kTinyMaxLen);
     return;
   }
   const int warp = threadIdx.x >> 5;
-  attn_tiny_warp<T, kHD, (int)kTinyMaxLen>(qkv, 3 * row_elems, qkv + row_elems, 3 * row_elems, qkv + 2 * row_elems, 3 * row_elems, out,
-                                           offsets, offsets, batch, H, scale_log2e, ((int64_t)blockIdx.x - 1) * kPrepWarps + warp,
-                                           (uint32_t)__cvta_generic_to_shared(prep_smem) + (uint32_t)warp * (uint32_t)(kPrepSmem / kPrepWarps));
+  attn_tiny_warp<T, kHD, (int)kTinyMaxLen>(qkv, 3 * E, qkv + E, 3 * E, qkv + 2 * E, 3 * E, out, offsets, offsets, row_elems, row_elems,
+                                           batch, H, scale_log2e, ((int64_t)blockIdx.x - 1) * kPrepWarps + warp,
+                                           (uint32_t)__cvta_generic_to_shared(prep_smem) + (uint32_t)warp * (uint32_t)(kPrepSmem / kPrepWarps),
+                                           lse);
 }
 
 // ------------------------------------------------------------------ attention
@@ -217,11 +219,12 @@ prepare_self_attention_kernel(const int64_t* __restrict__ offsets, int64_t batch
 // and reduced, instead of being waited for.  The softmax warps sit at their register budget; this only pays
 // because the write needs about 30 registers (it spilled, and lost 20 %, before the row sums were cut to two
 // packed accumulators).
-template <int FMT>
+// STATS: the rows' softmax denominators are stored too (LseOut), for a backward pass.
+template <int FMT, bool STATS>
 __global__ void __launch_bounds__(kAttnThreads, 2)
 attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, int col_q, int col_k, int col_v, void* __restrict__ out,
-                    const int4* __restrict__ items, const int* __restrict__ count, int H, float scale_log2e) {
+                    const int4* __restrict__ items, const int* __restrict__ count, int H, float scale_log2e, LseOut lse) {
   const int n_items = *count;
   if ((int64_t)blockIdx.x >= (int64_t)n_items * H) return;
   extern __shared__ uint8_t smem_raw[];
@@ -619,6 +622,7 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       pend.inv = 1.0f / l;
       pend.rows = it.rows;
       pend.out_row0 = (int64_t)it.tq * E + (int64_t)it.h * kHD;
+      if (STATS && ok && row < it.rows) lse.ptr[(int64_t)it.h * lse.ld + it.tq + row] = m + log2f(l);
     }
     if (ok && pend.any) {  // the last item of this CTA
       if (!wait_or_abort(ptx::smem_u32(&ctrl->o_ready), (g - 1) & 1, &ctrl->abort)) ok = false;
@@ -675,17 +679,17 @@ bool make_tile_map(CUtensorMap* map, const TileSource& src, int dtype) {
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int FMT>
+template <int FMT, bool STATS>
 int launch(const TileSource& q, int col_q, const TileSource& k, int col_k, const TileSource& v, int col_v, void* out,
-           const int64_t* offsets_q, const int64_t* offsets_k, int64_t batch, int64_t q_tokens, int H, float scaling, int dtype,
-           void* workspace, cudaStream_t st, int skip_short) {  // skip_short > 0: self-attention only
+           const AttnRows& rows, int64_t batch, int64_t q_tokens, int H, float scaling, int dtype, void* workspace, cudaStream_t st,
+           int skip_short) {  // skip_short > 0: self-attention only
   const int64_t E = (int64_t)H * kHD;
   CUtensorMap map_q, map_k, map_v;
   if (!make_tile_map(&map_q, q, dtype) || !make_tile_map(&map_k, k, dtype) || !make_tile_map(&map_v, v, dtype))
     return NTB200_LAUNCH_FAILED;
   static std::atomic<int> attr_set[kMaxDevices];
   if (!once_per_device(attr_set, [] {
-        return cudaFuncSetAttribute(attn_tcgen05_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem) == cudaSuccess;
+        return cudaFuncSetAttribute(attn_tcgen05_kernel<FMT, STATS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem) == cudaSuccess;
       }))
     return NTB200_LAUNCH_FAILED;
   const int64_t capacity = attn_tcgen05_item_capacity(batch, q_tokens);
@@ -702,16 +706,18 @@ int launch(const TileSource& q, int col_q, const TileSource& k, int col_k, const
     const int64_t blocks = 1 + (batch * H + kPrepWarps - 1) / kPrepWarps;
     if (blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
     prepare_self_attention_kernel<T16><<<(unsigned)blocks, kPrepWarps * 32, kPrepSmem, st>>>(
-        offsets_q, batch, E, items, count, capacity, static_cast<const T16*>(q.base), static_cast<T16*>(out), H, scaling * 1.4426950408889634f);
+        rows.offsets_q, rows.row_elems_q, batch, E, items, count, capacity, static_cast<const T16*>(q.base), static_cast<T16*>(out), H,
+        scaling * 1.4426950408889634f, LseOut{rows.lse, q_tokens});
   } else {
-    build_items_kernel<<<1, kListThreads, 0, st>>>(offsets_q, offsets_k, batch, E, items, count, capacity, static_cast<uint16_t*>(out));
+    build_items_kernel<<<1, kListThreads, 0, st>>>(rows.offsets_q, rows.offsets_k, rows.row_elems_q, rows.row_elems_k, E, batch, items,
+                                                   count, capacity, static_cast<uint16_t*>(out));
   }
   int dev = 0, sms = kNumSMs;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   int64_t grid = 2ll * sms;  // two resident CTAs per SM, each loops over its share of the items
   if (grid > capacity * H) grid = capacity * H;
-  attn_tcgen05_kernel<FMT><<<(unsigned)grid, kAttnThreads, kAttnSmem, st>>>(map_q, map_k, map_v, col_q, col_k, col_v, out, items, count, H,
-                                                                            scaling * 1.4426950408889634f);
+  attn_tcgen05_kernel<FMT, STATS><<<(unsigned)grid, kAttnThreads, kAttnSmem, st>>>(map_q, map_k, map_v, col_q, col_k, col_v, out, items, count, H,
+                                                                            scaling * 1.4426950408889634f, LseOut{rows.lse, q_tokens});
   return status_from_cuda(cudaGetLastError());
 }
 
@@ -729,25 +735,23 @@ bool attn_tcgen05_supported(int64_t batch, int64_t total_tokens, int num_heads, 
          attn_tcgen05_item_capacity(batch, total_tokens) < (1ll << 31);
 }
 
-int attn_tcgen05_launch(const void* qkv, void* out, const int64_t* offsets, int64_t batch, int64_t total_tokens, int H,
-                        float scaling, int dtype, void* workspace, cudaStream_t st, int skip_short) {
+int attn_tcgen05_launch(const void* qkv, void* out, const AttnRows& rows, int64_t batch, int64_t total_tokens, int H, float scaling,
+                        int dtype, void* workspace, cudaStream_t st, int skip_short) {
   const int64_t E = (int64_t)H * kHD;
   const TileSource src = {qkv, total_tokens, 3 * E, 3 * E};  // one map, three column offsets
-  if (dtype == NTB200_F16)
-    return launch<0>(src, 0, src, (int)E, src, (int)(2 * E), out, offsets, offsets, batch, total_tokens, H, scaling, dtype, workspace, st,
-                     skip_short);
-  return launch<1>(src, 0, src, (int)E, src, (int)(2 * E), out, offsets, offsets, batch, total_tokens, H, scaling, dtype, workspace, st,
-                   skip_short);
+  const bool f16 = dtype == NTB200_F16, stats = rows.lse != nullptr;
+  auto fn = f16 ? (stats ? launch<0, true> : launch<0, false>) : (stats ? launch<1, true> : launch<1, false>);
+  return fn(src, 0, src, (int)E, src, (int)(2 * E), out, rows, batch, total_tokens, H, scaling, dtype, workspace, st, skip_short);
 }
 
 int attn_tcgen05_cross_launch(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* out,
-                              const int64_t* offsets_q, const int64_t* offsets_k, int64_t batch, int64_t q_tokens, int64_t k_tokens,
-                              int H, float scaling, int dtype, void* workspace, cudaStream_t st) {
+                              const AttnRows& rows, int64_t batch, int64_t q_tokens, int64_t k_tokens, int H, float scaling, int dtype,
+                              void* workspace, cudaStream_t st) {
   const int64_t E = (int64_t)H * kHD;
   const TileSource sq = {q, q_tokens, E, ldq}, sk = {k, k_tokens, E, ldk}, sv = {v, k_tokens, E, ldv};
-  if (dtype == NTB200_F16)
-    return launch<0>(sq, 0, sk, 0, sv, 0, out, offsets_q, offsets_k, batch, q_tokens, H, scaling, dtype, workspace, st, 0);
-  return launch<1>(sq, 0, sk, 0, sv, 0, out, offsets_q, offsets_k, batch, q_tokens, H, scaling, dtype, workspace, st, 0);
+  const bool f16 = dtype == NTB200_F16, stats = rows.lse != nullptr;
+  auto fn = f16 ? (stats ? launch<0, true> : launch<0, false>) : (stats ? launch<1, true> : launch<1, false>);
+  return fn(sq, 0, sk, 0, sv, 0, out, rows, batch, q_tokens, H, scaling, dtype, workspace, st, 0);
 }
 
 int attn_tcgen05_error_flags_read_and_clear() {

@@ -76,12 +76,22 @@ __device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src,
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
 }
 
+// Where a forward kernel leaves the statistics that a backward pass needs: the base-2 logarithm of every row's softmax
+// denominator, log2(sum_j exp2(scaling * log2(e) * q.k_j)), as [H, ld] fp32 with one row per query token.  ptr NULL: not
+// wanted (inference).  Rows of a sequence without keys are left unwritten.
+struct LseOut {
+  float* ptr;
+  int64_t ld;
+};
+
 // The work of one warp: (sequence, head) number w of the flattened list; warp_smem = this warp's 3 * kR * kD * 2 bytes.
+// row_elems_q / row_elems_k: elements per token in offsets_q / offsets_k (H * kD for offsets of [tokens, H * kD] inputs).
 template <typename T, int kD, int kR>
 __device__ __forceinline__ void attn_tiny_warp(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, int64_t ldk,
                                                const T* __restrict__ v, int64_t ldv, T* __restrict__ out,
                                                const int64_t* __restrict__ offsets_q, const int64_t* __restrict__ offsets_k,
-                                               int64_t batch, int H, float scale_log2e, int64_t w, uint32_t warp_smem) {
+                                               int64_t row_elems_q, int64_t row_elems_k, int64_t batch, int H, float scale_log2e,
+                                               int64_t w, uint32_t warp_smem, const LseOut& lse) {
   constexpr uint32_t kTileBytes = kR * kD * 2;
   constexpr int kChunks = kD / 8;   // 16-byte chunks per row
   constexpr int kGroups = kR / 16;  // 16-key groups (and 16-query tiles) at most
@@ -91,17 +101,18 @@ __device__ __forceinline__ void attn_tiny_warp(const T* __restrict__ q, int64_t 
   const int h = (int)(w - b * H);
   const int64_t E = (int64_t)H * kD;
   const int64_t oq = offsets_q[b], ok = offsets_k[b];
-  const int64_t Lq64 = (offsets_q[b + 1] - oq) / E, L64 = (offsets_k[b + 1] - ok) / E;
+  const int64_t Lq64 = (offsets_q[b + 1] - oq) / row_elems_q, L64 = (offsets_k[b + 1] - ok) / row_elems_k;
   if (Lq64 <= 0 || Lq64 > kR || L64 > kR) return;
   const int Lq = (int)Lq64, L = (int)L64;
-  T* obase = out + (oq / E) * E + (int64_t)h * kD;
+  const int64_t tq0 = oq / row_elems_q, tk0 = ok / row_elems_k;
+  T* obase = out + tq0 * E + (int64_t)h * kD;
   if (L <= 0) {  // no keys: an empty softmax, the rows are zeros
     for (int i = lane; i < Lq * (kD / 2); i += 32) reinterpret_cast<uint32_t*>(obase + (int64_t)(i / (kD / 2)) * E)[i % (kD / 2)] = 0u;
     return;
   }
-  const T* qbase = q + (oq / E) * ldq + (int64_t)h * kD;
-  const T* kbase = k + (ok / E) * ldk + (int64_t)h * kD;
-  const T* vbase = v + (ok / E) * ldv + (int64_t)h * kD;
+  const T* qbase = q + tq0 * ldq + (int64_t)h * kD;
+  const T* kbase = k + tk0 * ldk + (int64_t)h * kD;
+  const T* vbase = v + tk0 * ldv + (int64_t)h * kD;
   const uint32_t sq = warp_smem;
   const uint32_t sk = sq + kTileBytes, sv = sk + kTileBytes;
   const int rows_q = (Lq + 15) & ~15, rows_k = (L + 15) & ~15;
@@ -193,6 +204,11 @@ __device__ __forceinline__ void attn_tiny_warp(const T* __restrict__ q, int64_t 
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     const float i0 = 1.0f / l0, i1 = 1.0f / l1;
     const int r0 = qt * 16 + (lane >> 2), r1 = r0 + 8;
+    if (lse.ptr != nullptr && (lane & 3) == 0) {
+      float* lrow = lse.ptr + (int64_t)h * lse.ld + tq0;
+      if (r0 < Lq) lrow[r0] = mn0 + log2f(l0);
+      if (r1 < Lq) lrow[r1] = mn1 + log2f(l1);
+    }
     uint32_t* orow0 = reinterpret_cast<uint32_t*>(obase + (int64_t)r0 * E);
     uint32_t* orow1 = reinterpret_cast<uint32_t*>(obase + (int64_t)r1 * E);
 #pragma unroll
@@ -207,13 +223,13 @@ __device__ __forceinline__ void attn_tiny_warp(const T* __restrict__ q, int64_t 
 template <typename T, int kD, int kR, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32)
 attn_tiny_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, int64_t ldv,
-                 T* __restrict__ out, const int64_t* __restrict__ offsets_q, const int64_t* __restrict__ offsets_k, int64_t batch,
-                 int H, float scale_log2e) {
+                 T* __restrict__ out, const int64_t* __restrict__ offsets_q, const int64_t* __restrict__ offsets_k, int64_t row_elems_q,
+                 int64_t row_elems_k, int64_t batch, int H, float scale_log2e, LseOut lse) {
   extern __shared__ __align__(128) uint8_t tiny_smem[];  // per warp: Q, K and V tiles of kR x kD each
   const int warp = threadIdx.x >> 5;
-  attn_tiny_warp<T, kD, kR>(q, ldq, k, ldk, v, ldv, out, offsets_q, offsets_k, batch, H, scale_log2e,
+  attn_tiny_warp<T, kD, kR>(q, ldq, k, ldk, v, ldv, out, offsets_q, offsets_k, row_elems_q, row_elems_k, batch, H, scale_log2e,
                             (int64_t)blockIdx.x * kWarps + warp,
-                            (uint32_t)__cvta_generic_to_shared(tiny_smem) + (uint32_t)warp * (3u * kR * kD * 2u));
+                            (uint32_t)__cvta_generic_to_shared(tiny_smem) + (uint32_t)warp * (3u * kR * kD * 2u), lse);
 }
 
 }  // namespace

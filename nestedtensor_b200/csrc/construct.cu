@@ -8,7 +8,7 @@
 // embedding replaces the packed fast path of NestedTensor_embedding (nestedtensor/csrc/functions.cpp:29-56,
 // at::embedding on the index buffer).
 
-#include "common.cuh"
+#include "row_vec.cuh"
 
 namespace ntb200 {
 namespace {
@@ -116,6 +116,59 @@ embedding_kernel(const void* __restrict__ weight, const IDX* __restrict__ index,
   }
 }
 
+// out[t] = scale * weight[index[t]]: the product in fp32, rounded once to the table's type.  One warp per token.
+template <typename IDX, int DT, bool VEC>
+__global__ void __launch_bounds__(kEmbThreads)
+embedding_scaled_kernel(const void* __restrict__ weight, const IDX* __restrict__ index, void* __restrict__ out, int64_t tokens,
+                        int64_t vocab, int64_t cols, float scale) {
+  constexpr int EPV = Vec16<DT>::kElems;
+  const int64_t t = (int64_t)blockIdx.x * (kEmbThreads / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (t >= tokens) return;
+  const int64_t i = (int64_t)index[t];
+  const bool ok = i >= 0 && i < vocab;
+  if (!ok && lane == 0) atomicOr(&g_construct_error, 1);
+  if (VEC) {
+    const int64_t nv = cols / EPV;
+    const uint4* src = static_cast<const uint4*>(weight) + (ok ? i : 0) * nv;
+    uint4* dst = static_cast<uint4*>(out) + t * nv;
+    for (int64_t v = lane; v < nv; v += 32) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (ok) {
+        float f[EPV];
+        Vec16<DT>::unpack(src[v], f);
+#pragma unroll
+        for (int k = 0; k < EPV; ++k) f[k] *= scale;
+        x = Vec16<DT>::pack(f);
+      }
+      dst[v] = x;
+    }
+  } else {
+    for (int64_t c = lane; c < cols; c += 32)
+      Vec16<DT>::store1(out, t * cols + c, ok ? Vec16<DT>::load1(weight, i * cols + c) * scale : 0.0f);
+  }
+}
+
+template <int DT>
+int launch_embedding_scaled(const void* weight, const void* index, int index_bytes, void* out, int64_t tokens, int64_t vocab, int64_t cols,
+                            float scale, cudaStream_t st) {
+  const bool vec = cols % Vec16<DT>::kElems == 0 && aligned16(weight) && aligned16(out);
+  const int64_t grid = (tokens + kEmbThreads / 32 - 1) / (kEmbThreads / 32);
+  if (grid > 0x7fffffff) return NTB200_INVALID_ARG;
+#define NTB200_EMB(IDX, VEC)                                                                                                     \
+  embedding_scaled_kernel<IDX, DT, VEC><<<(unsigned)grid, kEmbThreads, 0, st>>>(weight, static_cast<const IDX*>(index), out, tokens, \
+                                                                               vocab, cols, scale)
+  if (index_bytes == 8) {
+    if (vec) NTB200_EMB(int64_t, true);
+    else NTB200_EMB(int64_t, false);
+  } else {
+    if (vec) NTB200_EMB(int32_t, true);
+    else NTB200_EMB(int32_t, false);
+  }
+#undef NTB200_EMB
+  return status_from_cuda(cudaGetLastError());
+}
+
 }  // namespace
 
 int construct_error_flags_read_and_clear() {
@@ -177,6 +230,20 @@ int ntb200_embedding(const void* weight, const void* index, int index_bytes, voi
   }
 #undef NTB200_EMB
   return status_from_cuda(cudaGetLastError());
+}
+
+int ntb200_embedding_scaled(const void* weight, const void* index, int index_bytes, void* out, int64_t tokens, int64_t vocab,
+                            int64_t embed_dim, float scale, int dtype, void* stream) {
+  if (tokens < 0 || vocab < 0 || embed_dim < 0 || (index_bytes != 4 && index_bytes != 8)) return NTB200_INVALID_ARG;
+  if (dtype != NTB200_F32 && dtype != NTB200_F16 && dtype != NTB200_BF16) return NTB200_UNSUPPORTED_DTYPE;
+  if (tokens == 0 || embed_dim == 0) return NTB200_OK;
+  if (weight == nullptr || index == nullptr || out == nullptr || vocab == 0) return NTB200_INVALID_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case NTB200_F32: return launch_embedding_scaled<NTB200_F32>(weight, index, index_bytes, out, tokens, vocab, embed_dim, scale, st);
+    case NTB200_F16: return launch_embedding_scaled<NTB200_F16>(weight, index, index_bytes, out, tokens, vocab, embed_dim, scale, st);
+    default: return launch_embedding_scaled<NTB200_BF16>(weight, index, index_bytes, out, tokens, vocab, embed_dim, scale, st);
+  }
 }
 
 }  // extern "C"

@@ -11,137 +11,29 @@
 // (transformer_kernels.cu:64-156, cuda_kernels.cu:114-159) and add_bias_act / add_bias_gelu
 // (cuda_kernels.cu:73-104, transformer_kernels.cu:52-62).
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include "common.cuh"
-#include "sm100_ptx.cuh"
+#include "row_vec.cuh"
 
 namespace ntb200 {
 namespace {
 
-// 16 bytes of storage <-> fp32 lanes
-template <int DT>
-struct Vec16;
-template <>
-struct Vec16<NTB200_F32> {
-  static constexpr int kElems = 4;
-  static __device__ __forceinline__ void unpack(const uint4& r, float* f) {
-    f[0] = __uint_as_float(r.x), f[1] = __uint_as_float(r.y), f[2] = __uint_as_float(r.z), f[3] = __uint_as_float(r.w);
-  }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-  }
-  static __device__ __forceinline__ float load1(const void* p, int64_t i) { return reinterpret_cast<const float*>(p)[i]; }
-  static __device__ __forceinline__ void store1(void* p, int64_t i, float v) { reinterpret_cast<float*>(p)[i] = v; }
-};
-template <>
-struct Vec16<NTB200_F16> {
-  static constexpr int kElems = 8;
-  static __device__ __forceinline__ void unpack(const uint4& r, float* f) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-      f[2 * k] = t.x, f[2 * k + 1] = t.y;
-    }
-  }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const __half2 h = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
-      w[k] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  static __device__ __forceinline__ float load1(const void* p, int64_t i) { return __half2float(reinterpret_cast<const __half*>(p)[i]); }
-  static __device__ __forceinline__ void store1(void* p, int64_t i, float v) { reinterpret_cast<__half*>(p)[i] = __float2half_rn(v); }
-};
-template <>
-struct Vec16<NTB200_BF16> {
-  static constexpr int kElems = 8;
-  static __device__ __forceinline__ void unpack(const uint4& r, float* f) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {  // a bf16 is the upper half of an fp32
-      f[2 * k] = __uint_as_float(w[k] << 16);
-      f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-    }
-  }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
-      w[k] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  static __device__ __forceinline__ float load1(const void* p, int64_t i) {
-    return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  }
-  static __device__ __forceinline__ void store1(void* p, int64_t i, float v) {
-    reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-  }
-};
-
-// The same 16 bytes as kElems / 2 packed fp32 pairs (sm_100 adds, subtracts and multiplies two fp32 values
-// held in a 64-bit register pair with one instruction: the LayerNorm kernel is otherwise bound by its issue
-// slots, not by memory).
-template <int DT>
-__device__ __forceinline__ void unpack_pairs(const uint4& r, uint64_t* p) {
-  float f[Vec16<DT>::kElems];
-  Vec16<DT>::unpack(r, f);
-#pragma unroll
-  for (int k = 0; k < Vec16<DT>::kElems / 2; ++k) p[k] = ptx::f32x2_pack(f[2 * k], f[2 * k + 1]);
-}
-template <int DT>
-__device__ __forceinline__ uint4 pack_pairs(const uint64_t* p) {
-  float f[Vec16<DT>::kElems];
-#pragma unroll
-  for (int k = 0; k < Vec16<DT>::kElems / 2; ++k) ptx::f32x2_unpack(p[k], f[2 * k], f[2 * k + 1]);
-  return Vec16<DT>::pack(f);
-}
-
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// Sum over the GROUP threads that share a row: part of a warp (GROUP == 8, 16: neighbouring lanes), a warp
-// (GROUP == 32) or the whole block.
-template <int GROUP>
-__device__ __forceinline__ float group_sum(float v, float* scratch) {
-  if (GROUP < 32) {
-#pragma unroll
-    for (int o = GROUP / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  }
-  v = warp_sum(v);
-  if (GROUP == 32) return v;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __syncthreads();  // scratch may still be read from the previous reduction
-  if (lane == 0) scratch[warp] = v;
-  __syncthreads();
-  float t = lane < GROUP / 32 ? scratch[lane] : 0.0f;
-  return warp_sum(t);
-}
-
 constexpr int kLnThreads = 256;
+
+struct RowStats {  // [rows] fp32 each, or NULL
+  float *mean, *rstd;
+};
 
 // One row per GROUP threads, the row held in registers between the passes (one global read, one global
 // write per element).  VPL = 16-byte vectors per thread; vector v of the row belongs to thread v % GROUP.
 // Mean and variance are the two-pass forms of the reference kernel (sum, then sum of squared deviations).
 // A 16-bit row without the fused additions stays in its packed form (4 registers per vector instead of 8) and is
 // widened again in each pass, which is exact: half the registers, twice the rows in flight per SM.
-// FULL: the row is exactly VPL * GROUP vectors (no per-vector bound test).
-template <int DT, int VPL, int GROUP, bool FUSED, bool FULL>
+// FULL: the row is exactly VPL * GROUP vectors (no per-vector bound test).  STATS: mean and rstd of every row are stored too,
+// for a backward pass.
+template <int DT, int VPL, int GROUP, bool FUSED, bool FULL, bool STATS>
 __global__ void __launch_bounds__(kLnThreads, (!FUSED && FULL && DT != NTB200_F32 && VPL <= 4) ? 6 : 1)
 layer_norm_kernel(const void* x, const void* __restrict__ residual, const void* __restrict__ bias,
                   const void* __restrict__ gamma, const void* __restrict__ beta, float eps, void* out, int64_t rows,
-                  int cols) {  // out may alias x: a thread has read all it needs of the row before it writes
+                  int cols, RowStats stats) {  // out may alias x: a thread has read all it needs of the row before it writes
   constexpr int EPV = Vec16<DT>::kElems;
   constexpr int kRowsPerBlock = kLnThreads / GROUP;
   constexpr bool RAW = !FUSED && DT != NTB200_F32;
@@ -232,6 +124,10 @@ layer_norm_kernel(const void* x, const void* __restrict__ residual, const void* 
   ptx::f32x2_unpack(sq2, s_lo, s_hi);
   const float rstd = rsqrtf(group_sum<GROUP>(s_lo + s_hi, scratch) / (float)cols + eps);
   if (!live) return;
+  if (STATS && t == 0) {
+    stats.mean[row] = mean;
+    stats.rstd[row] = rstd;
+  }
   const uint64_t rstd2 = ptx::f32x2_pack(rstd, rstd);
   uint4* orow = reinterpret_cast<uint4*>(out) + row * nv;
 #pragma unroll
@@ -267,7 +163,7 @@ template <int DT>
 __global__ void __launch_bounds__(kLnThreads)
 layer_norm_generic_kernel(const void* x, const void* __restrict__ residual, const void* __restrict__ bias,
                           const void* __restrict__ gamma, const void* __restrict__ beta, float eps, void* out, int64_t rows,
-                          int cols) {
+                          int cols, RowStats stats) {
   __shared__ float scratch[kLnThreads / 32];
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const int64_t base = row * cols;
@@ -286,6 +182,10 @@ layer_norm_generic_kernel(const void* x, const void* __restrict__ residual, cons
       sq += d * d;
     }
     const float rstd = rsqrtf(group_sum<kLnThreads>(sq, scratch) / (float)cols + eps);
+    if (stats.mean != nullptr && threadIdx.x == 0) {
+      stats.mean[row] = mean;
+      stats.rstd[row] = rstd;
+    }
     for (int i = threadIdx.x; i < cols; i += kLnThreads) {
       float o = (value(i) - mean) * rstd;
       if (gamma != nullptr) o = o * Vec16<DT>::load1(gamma, i) + Vec16<DT>::load1(beta, i);
@@ -329,11 +229,9 @@ add_bias_gelu_scalar_kernel(const void* x, const void* __restrict__ bias, void* 
   }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-template <int DT, bool FUSED>
+template <int DT, bool FUSED, bool STATS = false>
 int launch_layer_norm(const void* x, const void* residual, const void* bias, const void* gamma, const void* beta, float eps,
-                      void* out, int64_t rows, int64_t cols, cudaStream_t st) {
+                      void* out, int64_t rows, int64_t cols, cudaStream_t st, RowStats stats = {nullptr, nullptr}) {
   constexpr int EPV = Vec16<DT>::kElems;
   const bool vec_ok = cols % EPV == 0 && aligned16(x) && aligned16(out) && (residual == nullptr || aligned16(residual)) &&
                       (bias == nullptr || aligned16(bias)) && (gamma == nullptr || (aligned16(gamma) && aligned16(beta)));
@@ -344,11 +242,11 @@ int launch_layer_norm(const void* x, const void* residual, const void* bias, con
     const int64_t grid = (rows + rpb - 1) / rpb;                                                                  \
     if (grid > 0x7fffffff) return NTB200_INVALID_ARG;                                                             \
     if (nv == (int64_t)(VPL) * (GROUP))                                                                           \
-      layer_norm_kernel<DT, VPL, GROUP, FUSED, true><<<(unsigned)grid, kLnThreads, 0, st>>>(x, residual, bias, gamma, beta, \
-                                                                                           eps, out, rows, (int)cols); \
+      layer_norm_kernel<DT, VPL, GROUP, FUSED, true, STATS><<<(unsigned)grid, kLnThreads, 0, st>>>(x, residual, bias, gamma, beta, \
+                                                                                           eps, out, rows, (int)cols, stats); \
     else                                                                                                          \
-      layer_norm_kernel<DT, VPL, GROUP, FUSED, false><<<(unsigned)grid, kLnThreads, 0, st>>>(x, residual, bias, gamma, beta, \
-                                                                                            eps, out, rows, (int)cols); \
+      layer_norm_kernel<DT, VPL, GROUP, FUSED, false, STATS><<<(unsigned)grid, kLnThreads, 0, st>>>(x, residual, bias, gamma, beta, \
+                                                                                            eps, out, rows, (int)cols, stats); \
   } while (0)
   // Vectors per thread = ceil(nv / GROUP): widths such as 768, 1280 or 1536 get an exact fit (3, 5 or 6 vectors per
   // lane, no idle slots, the variant without bound tests) instead of the next power of two.  A packed 16-bit row
@@ -378,7 +276,7 @@ int launch_layer_norm(const void* x, const void* residual, const void* bias, con
     const int64_t grid = rows < 148 * 32 ? rows : 148 * 32;
     layer_norm_generic_kernel<DT><<<(unsigned)grid, kLnThreads, 0, st>>>(x, FUSED ? residual : nullptr,
                                                                         FUSED ? bias : nullptr, gamma, beta, eps, out, rows,
-                                                                        (int)cols);
+                                                                        (int)cols, stats);
   }
 #undef NTB200_LN_LAUNCH
   return status_from_cuda(cudaGetLastError());
@@ -432,6 +330,23 @@ extern "C" {
 int ntb200_layer_norm(const void* x, const void* gamma, const void* beta, float eps, void* out, int64_t rows, int64_t cols,
                       int dtype, void* stream) {
   return ntb200::layer_norm_entry(x, nullptr, nullptr, gamma, beta, eps, out, rows, cols, dtype, stream);
+}
+
+int ntb200_layer_norm_train(const void* x, const void* gamma, const void* beta, float eps, void* out, float* mean, float* rstd,
+                            int64_t rows, int64_t cols, int dtype, void* stream) {
+  if (rows < 0 || cols < 0 || cols > 0x7fffffff || !(eps >= 0.0f)) return NTB200_INVALID_ARG;
+  if ((gamma == nullptr) != (beta == nullptr)) return NTB200_INVALID_ARG;
+  if (dtype != NTB200_F32 && dtype != NTB200_F16 && dtype != NTB200_BF16) return NTB200_UNSUPPORTED_DTYPE;
+  if (rows == 0 || cols == 0) return NTB200_OK;
+  if (x == nullptr || out == nullptr || mean == nullptr || rstd == nullptr) return NTB200_INVALID_ARG;
+  using namespace ntb200;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const RowStats stats = {mean, rstd};
+  switch (dtype) {
+    case NTB200_F32: return launch_layer_norm<NTB200_F32, false, true>(x, nullptr, nullptr, gamma, beta, eps, out, rows, cols, st, stats);
+    case NTB200_F16: return launch_layer_norm<NTB200_F16, false, true>(x, nullptr, nullptr, gamma, beta, eps, out, rows, cols, st, stats);
+    default: return launch_layer_norm<NTB200_BF16, false, true>(x, nullptr, nullptr, gamma, beta, eps, out, rows, cols, st, stats);
+  }
 }
 
 int ntb200_add_bias_residual_layer_norm(const void* x, const void* residual, const void* bias, const void* gamma,

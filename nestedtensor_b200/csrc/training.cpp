@@ -1,0 +1,376 @@
+// Differentiable operators of the torch layer: LayerNorm, embedding and varlen attention on packed ragged batches, each a
+// C++ autograd function over the C ABI's forward pass (which keeps what the gradients need) and backward pass.  First
+// derivatives only: differentiating a gradient raises.  Host validation, allocation through torch's caching allocator and
+// launches on the current stream as in dispatch.cpp; nothing is kept between calls, so captured CUDA graphs share nothing.
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <algorithm>
+
+#include "dispatch_common.h"
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Passes a gradient computed with create_graph=True on to the graph, with an error in the place of its own derivative.
+struct FirstOrderOnly : public torch::autograd::Function<FirstOrderOnly> {
+  static Tensor forward(AutogradContext*, const Tensor& grad, const Tensor&, const Tensor&, const Tensor&, const Tensor&) { return grad.detach(); }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "nestedtensor_b200: the training operators have first derivatives only");
+  }
+};
+
+// Runs `compute` (the gradients) without recording it; with create_graph=True every result keeps its dependence on `deps`.
+template <typename F>
+variable_list first_order(const std::array<Tensor, 4>& deps, F&& compute) {
+  const bool create_graph = at::GradMode::is_enabled();
+  variable_list grads;
+  {
+    at::AutoGradMode no_grad(false);
+    grads = compute();
+  }
+  if (create_graph)
+    for (auto& g : grads)
+      if (g.defined()) g = FirstOrderOnly::apply(g, deps[0], deps[1], deps[2], deps[3]);
+  return grads;
+}
+
+Tensor byte_workspace(size_t bytes, const Tensor& like) {
+  return at::empty({(int64_t)std::max<size_t>(bytes, 16)}, like.options().dtype(at::kByte));
+}
+
+bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+void same_kind(const Tensor& t, const Tensor& like, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == like.scalar_type(), "nestedtensor_b200: ", name,
+              " must be on the input's device and of its dtype");
+}
+
+// The rows of a ragged batch: host lengths (first column of `sizes`) and device offsets with `row_elems` elements per token.
+struct Rows {
+  int64_t B, tokens, longest;
+};
+
+Rows make_rows(const Tensor& sizes, const Tensor& meta, int64_t row_elems, const Tensor& like, const char* name) {
+  TORCH_CHECK(sizes.device().is_cpu() && sizes.scalar_type() == at::kLong && sizes.dim() == 2 && sizes.is_contiguous() &&
+                  (sizes.size(1) >= 1 || sizes.size(0) == 0),
+              "nestedtensor_b200: sizes must be a contiguous CPU int64 [B, tensor_dim] tensor");
+  Rows r = {sizes.size(0), 0, 0};
+  TORCH_CHECK(meta.is_cuda() && meta.device() == like.device(), "nestedtensor_b200: this operator needs a CUDA ", name,
+              " (this build has no CPU implementation)");
+  TORCH_CHECK(meta.scalar_type() == at::kLong && meta.is_contiguous() && meta.numel() >= r.B + 1,
+              "nestedtensor_b200: meta must be a CUDA int64 tensor that begins with B+1 offsets");
+  TORCH_CHECK(row_elems >= 1, "nestedtensor_b200: row_elems must be at least 1");
+  const int64_t* p = sizes.data_ptr<int64_t>();
+  const int64_t td = sizes.size(1);
+  for (int64_t b = 0; b < r.B; ++b) {
+    TORCH_CHECK(p[b * td] >= 0, "nestedtensor_b200: negative size");
+    r.tokens += p[b * td];
+    r.longest = std::max(r.longest, p[b * td]);
+  }
+  return r;
+}
+
+// ------------------------------------------------------------------ LayerNorm
+struct LayerNormTrain : public torch::autograd::Function<LayerNormTrain> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t cols, double eps) {
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t rows = x.numel() / cols;
+    Tensor out = at::empty({rows, cols}, x.options());
+    Tensor stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
+    Tensor w, b;
+    if (weight.defined()) w = weight.contiguous(), b = bias.contiguous();
+    float* st = stats.data_ptr<float>();
+    check_rc(ntb200_layer_norm_train(x.data_ptr(), w.defined() ? w.data_ptr() : nullptr, b.defined() ? b.data_ptr() : nullptr, (float)eps,
+                                     out.data_ptr(), st, st + rows, rows, cols, dtype_code(x.scalar_type()), cur_stream()),
+             "ntb200_layer_norm_train");
+    ctx->save_for_backward({x, w, stats});
+    ctx->saved_data["wants_x"] = wants(x);
+    ctx->saved_data["wants_w"] = wants(weight);
+    ctx->saved_data["wants_b"] = wants(bias);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
+    return first_order({grads[0], x, w, Tensor()}, [&]() -> variable_list {
+      c10::cuda::CUDAGuard guard(x.device());
+      const Tensor g = grads[0].contiguous();
+      const int64_t rows = g.size(0), cols = g.size(1);
+      const bool wx = ctx->saved_data["wants_x"].toBool(), ww = ctx->saved_data["wants_w"].toBool(), wb = ctx->saved_data["wants_b"].toBool();
+      Tensor gx, gw, gb;
+      if (wx) gx = at::empty(x.sizes(), x.options());
+      if (ww) gw = at::empty({cols}, x.options());
+      if (wb) gb = at::empty({cols}, x.options());
+      const size_t bytes = w.defined() ? ntb200_layer_norm_backward_workspace_bytes(rows, cols) : 0;
+      Tensor ws = byte_workspace(bytes, x);
+      const float* st = stats.data_ptr<float>();
+      check_rc(ntb200_layer_norm_backward(g.data_ptr(), x.data_ptr(), st, st + rows, w.defined() ? w.data_ptr() : nullptr,
+                                          wx ? gx.data_ptr() : nullptr, ww ? gw.data_ptr() : nullptr, wb ? gb.data_ptr() : nullptr, rows, cols,
+                                          dtype_code(x.scalar_type()), ws.data_ptr(), bytes, cur_stream()),
+               "ntb200_layer_norm_backward");
+      return {gx, gw, gb, Tensor(), Tensor()};
+    });
+  }
+};
+
+// LayerNorm over the last dimension of the packed rows; x is the buffer of the record, in any contiguous shape.  [T, E].
+Tensor layer_norm_train(const Tensor& x_, const Tensor& sizes, at::IntArrayRef normalized_shape, const c10::optional<Tensor>& weight,
+                        const c10::optional<Tensor>& bias, double eps) {
+  TORCH_CHECK(normalized_shape.size() == 1, "Currently only singleton tuples of integers supported for layer_norm.");
+  const int64_t E = normalized_shape[0];
+  TORCH_CHECK(E > 0, "nestedtensor_b200: layer_norm over an empty dimension");
+  TORCH_CHECK(x_.is_cuda(), "nestedtensor_b200: layer_norm needs a CUDA nested tensor (this build has no CPU implementation)");
+  TORCH_CHECK(sizes.device().is_cpu() && sizes.scalar_type() == at::kLong && sizes.dim() == 2 && sizes.is_contiguous(),
+              "nestedtensor_b200: sizes must be a contiguous CPU int64 [B, tensor_dim] tensor");
+  const int64_t B = sizes.size(0), td = sizes.size(1);
+  TORCH_CHECK(B == 0 || td >= 1, "Cannot normalize across irregular dimension ", td);
+  const int64_t* p = sizes.data_ptr<int64_t>();
+  int64_t numel = 0;
+  for (int64_t b = 0; b < B; ++b) {
+    TORCH_CHECK(p[b * td + td - 1] == p[td - 1], "Cannot normalize across irregular dimension ", td);
+    int64_t n = 1;
+    for (int64_t j = 0; j < td; ++j) n *= p[b * td + j];
+    numel += n;
+  }
+  TORCH_CHECK(B == 0 || p[td - 1] == E, "Normalized shape [", E, "] does not match the size of the last dimension (", p[td - 1], ") of input.");
+  TORCH_CHECK(x_.numel() == numel, "nestedtensor_b200: buffer must have sum(numel) elements");
+  dtype_code(x_.scalar_type());
+  const bool has_w = weight && weight->defined(), has_b = bias && bias->defined();
+  TORCH_CHECK(has_w == has_b, "Either both weight and bias are used or not.");
+  if (has_w) {
+    same_kind(*weight, x_, "weight");
+    same_kind(*bias, x_, "bias");
+    TORCH_CHECK(weight->dim() == 1 && weight->size(0) == E, "nestedtensor_b200: weight must have ", E, " entries");
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == E, "nestedtensor_b200: bias must have ", E, " entries");
+  }
+  TORCH_CHECK(eps >= 0, "nestedtensor_b200: eps must not be negative");
+  return LayerNormTrain::apply(x_.contiguous(), has_w ? *weight : Tensor(), has_b ? *bias : Tensor(), E, eps);
+}
+
+// ------------------------------------------------------------------ embedding
+struct EmbeddingTrain : public torch::autograd::Function<EmbeddingTrain> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& index, int64_t padding_idx, double scale) {
+    c10::cuda::CUDAGuard guard(weight.device());
+    Tensor w = weight.contiguous();
+    const int64_t T = index.numel(), V = w.size(0), E = w.size(1);
+    Tensor out = at::empty({T, E}, w.options());
+    if (scale == 1.0)  // rows copied bit for bit
+      check_rc(ntb200_embedding(w.data_ptr(), index.data_ptr(), (int)index.element_size(), out.data_ptr(), T, V, E, (int)w.element_size(),
+                                cur_stream()),
+               "ntb200_embedding");
+    else
+      check_rc(ntb200_embedding_scaled(w.data_ptr(), index.data_ptr(), (int)index.element_size(), out.data_ptr(), T, V, E, (float)scale,
+                                       dtype_code(w.scalar_type()), cur_stream()),
+               "ntb200_embedding_scaled");
+    ctx->save_for_backward({index});
+    ctx->saved_data["padding_idx"] = padding_idx;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["vocab"] = V;
+    maybe_check_device_errors("embedding");
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor index = ctx->get_saved_variables()[0];
+    return first_order({grads[0], Tensor(), Tensor(), Tensor()}, [&]() -> variable_list {
+      c10::cuda::CUDAGuard guard(index.device());
+      const Tensor g = grads[0].contiguous();
+      const int64_t T = g.size(0), E = g.size(1), V = ctx->saved_data["vocab"].toInt();
+      Tensor gw = at::empty({V, E}, g.options());
+      const size_t bytes = ntb200_embedding_backward_workspace_bytes(T, E);
+      Tensor ws = byte_workspace(bytes, g);
+      check_rc(ntb200_embedding_backward(g.data_ptr(), index.data_ptr(), (int)index.element_size(), gw.data_ptr(), T, V, E,
+                                         ctx->saved_data["padding_idx"].toInt(), (float)ctx->saved_data["scale"].toDouble(),
+                                         dtype_code(g.scalar_type()), ws.data_ptr(), bytes, cur_stream()),
+               "ntb200_embedding_backward");
+      return {gw, Tensor(), Tensor(), Tensor()};
+    });
+  }
+};
+
+// scale * weight[index] for the packed index buffer of 1-D sequences: [T, E]
+Tensor embedding_train(const Tensor& weight, const Tensor& index, const Tensor& sizes, c10::optional<int64_t> padding_idx, double scale) {
+  TORCH_CHECK(weight.is_cuda() && weight.dim() == 2, "nestedtensor_b200: embedding needs a 2-D CUDA weight");
+  dtype_code(weight.scalar_type());
+  TORCH_CHECK(index.is_cuda() && index.device() == weight.device() && index.dim() == 1 && index.is_contiguous(),
+              "nestedtensor_b200: the index buffer must be 1-D contiguous on the weight's device");
+  TORCH_CHECK(index.scalar_type() == at::kLong || index.scalar_type() == at::kInt,
+              "Expected tensor for argument #1 'indices' to have one of the following scalar types: Long, Int");
+  TORCH_CHECK(sizes.device().is_cpu() && sizes.scalar_type() == at::kLong && sizes.dim() == 2 && (sizes.size(1) == 1 || sizes.size(0) == 0),
+              "nestedtensor_b200: embedding expects a nested tensor of 1-D index sequences");
+  TORCH_CHECK(index.numel() == (sizes.size(0) > 0 ? sizes.sum().item<int64_t>() : 0),
+              "nestedtensor_b200: the index buffer must hold sum(L_i) entries");
+  const int64_t V = weight.size(0);
+  TORCH_CHECK(V > 0 || index.numel() == 0, "nestedtensor_b200: embedding needs a weight with at least one row");
+  TORCH_CHECK(V < (1ll << 31) - 1 && index.numel() < (1ll << 31) - 1, "nestedtensor_b200: embedding supports fewer than 2^31 - 1 rows and tokens");
+  int64_t pad = -1;
+  if (padding_idx) {
+    TORCH_CHECK(*padding_idx >= -V && *padding_idx < V, "padding_idx must be within num_embeddings");
+    pad = *padding_idx < 0 ? *padding_idx + V : *padding_idx;
+  }
+  return EmbeddingTrain::apply(weight, index, pad, scale);
+}
+
+// ------------------------------------------------------------------ attention
+struct AttentionShape {
+  int64_t B, Tq, Tk, longest_q, longest_k, row_q, row_k, H, d;
+  double scaling;
+};
+
+void attention_forward(const AttentionShape& s, const void* q, const void* k, const void* v, int64_t ldq, int64_t ldkv, const Tensor& meta_q,
+                       const Tensor& meta_k, Tensor& out, Tensor& lse) {
+  const int dt = dtype_code(out.scalar_type());
+  const size_t bytes = ntb200_varlen_cross_attention_workspace_bytes(s.B, s.Tq, (int)s.H, (int)s.d, dt);
+  Tensor ws;
+  if (bytes > 0) ws = byte_workspace(bytes, out);
+  check_rc(ntb200_varlen_attention_train(q, ldq, k, ldkv, v, ldkv, out.data_ptr(), lse.data_ptr<float>(), meta_q.data_ptr<int64_t>(), s.row_q,
+                                         meta_k.data_ptr<int64_t>(), s.row_k, s.B, s.Tq, s.Tk, (int)s.H, (int)s.d, s.longest_q,
+                                         (float)s.scaling, dt, 0, bytes > 0 ? ws.data_ptr() : nullptr, bytes, cur_stream()),
+           "ntb200_varlen_attention_train");
+  maybe_check_device_errors("attention");
+}
+
+void attention_backward(const AttentionShape& s, const Tensor& grad, const void* q, const void* k, const void* v, int64_t ldq, int64_t ldkv,
+                        const Tensor& out, const Tensor& lse, void* dq, void* dk, void* dv, const Tensor& meta_q, const Tensor& meta_k) {
+  const int dt = dtype_code(out.scalar_type());
+  const size_t bytes = ntb200_varlen_attention_backward_workspace_bytes(s.B, s.Tq, s.Tk, (int)s.H, (int)s.d, dt);
+  Tensor ws = byte_workspace(bytes, out);
+  check_rc(ntb200_varlen_attention_backward(grad.data_ptr(), q, ldq, k, ldkv, v, ldkv, out.data_ptr(), lse.data_ptr<float>(), dq, ldq, dk, ldkv,
+                                            dv, ldkv, meta_q.data_ptr<int64_t>(), s.row_q, meta_k.data_ptr<int64_t>(), s.row_k, s.B, s.Tq, s.Tk,
+                                            (int)s.H, (int)s.d, s.longest_q, s.longest_k, (float)s.scaling, dt, 0, ws.data_ptr(), bytes,
+                                            cur_stream()),
+           "ntb200_varlen_attention_backward");
+  maybe_check_device_errors("attention backward");
+}
+
+void save_shape(AutogradContext* ctx, const AttentionShape& s) {
+  ctx->saved_data["shape"] = std::vector<int64_t>{s.B, s.Tq, s.Tk, s.longest_q, s.longest_k, s.row_q, s.row_k, s.H, s.d};
+  ctx->saved_data["scaling"] = s.scaling;
+}
+
+AttentionShape load_shape(AutogradContext* ctx) {
+  const auto v = ctx->saved_data["shape"].toIntVector();
+  return {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], ctx->saved_data["scaling"].toDouble()};
+}
+
+// q | k | v of every token in one [T, 3E] matrix; the gradient has the same form
+struct SelfAttentionTrain : public torch::autograd::Function<SelfAttentionTrain> {
+  static const void* part(const Tensor& t, int64_t elems) { return static_cast<const char*>(t.data_ptr()) + elems * t.element_size(); }
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& meta, const AttentionShape& s) {
+    c10::cuda::CUDAGuard guard(qkv.device());
+    const int64_t E = s.H * s.d;
+    Tensor out = at::empty({s.Tq, E}, qkv.options()), lse = at::empty({s.H, s.Tq}, qkv.options().dtype(at::kFloat));
+    if (s.Tq > 0) attention_forward(s, qkv.data_ptr(), part(qkv, E), part(qkv, 2 * E), 3 * E, 3 * E, meta, meta, out, lse);
+    ctx->save_for_backward({qkv, meta, out, lse});
+    save_shape(ctx, s);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &qkv = saved[0], &meta = saved[1], &out = saved[2], &lse = saved[3];
+    return first_order({grads[0], qkv, Tensor(), Tensor()}, [&]() -> variable_list {
+      c10::cuda::CUDAGuard guard(qkv.device());
+      const AttentionShape s = load_shape(ctx);
+      const int64_t E = s.H * s.d;
+      const Tensor g = grads[0].contiguous();
+      Tensor dqkv = at::empty(qkv.sizes(), qkv.options());
+      if (s.Tq > 0)
+        attention_backward(s, g, qkv.data_ptr(), part(qkv, E), part(qkv, 2 * E), 3 * E, 3 * E, out, lse, dqkv.data_ptr(),
+                           const_cast<void*>(part(dqkv, E)), const_cast<void*>(part(dqkv, 2 * E)), meta, meta);
+      return {dqkv, Tensor(), Tensor()};
+    });
+  }
+};
+
+struct AttentionTrain : public torch::autograd::Function<AttentionTrain> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& meta_q, const Tensor& meta_k,
+                        const AttentionShape& s) {
+    c10::cuda::CUDAGuard guard(q.device());
+    const int64_t E = s.H * s.d;
+    Tensor out = at::empty({s.Tq, E}, q.options()), lse = at::empty({s.H, s.Tq}, q.options().dtype(at::kFloat));
+    if (s.Tq > 0) attention_forward(s, q.data_ptr(), k.data_ptr(), v.data_ptr(), E, E, meta_q, meta_k, out, lse);
+    ctx->save_for_backward({q, k, v, meta_q, meta_k, out, lse});
+    save_shape(ctx, s);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &meta_q = saved[3], &meta_k = saved[4], &out = saved[5], &lse = saved[6];
+    return first_order({grads[0], q, k, v}, [&]() -> variable_list {
+      c10::cuda::CUDAGuard guard(q.device());
+      const AttentionShape s = load_shape(ctx);
+      const int64_t E = s.H * s.d;
+      const Tensor g = grads[0].contiguous();
+      Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
+      if (s.Tq > 0 || s.Tk > 0)
+        attention_backward(s, g, q.data_ptr(), k.data_ptr(), v.data_ptr(), E, E, out, lse, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), meta_q,
+                           meta_k);
+      return {dq, dk, dv, Tensor(), Tensor(), Tensor()};
+    });
+  }
+};
+
+int64_t check_heads(int64_t num_heads, int64_t E) {
+  TORCH_CHECK(num_heads >= 1 && E >= num_heads && E % num_heads == 0, "embed_dim must be divisible by num_heads");
+  TORCH_CHECK(E / num_heads <= 256, "nestedtensor_b200: head_dim must be in [1, 256]");
+  return E / num_heads;
+}
+
+// Self-attention of packed q|k|v rows: qkv is the buffer of (L_i, 3E) constituents in any contiguous shape; [T, E].
+Tensor self_attention_train(const Tensor& qkv, const Tensor& sizes, const Tensor& meta, int64_t row_elems, int64_t num_heads, double scaling) {
+  TORCH_CHECK(qkv.is_cuda(), "nestedtensor_b200: self_attention needs a CUDA nested tensor (this build has no CPU implementation)");
+  dtype_code(qkv.scalar_type());
+  const Rows r = make_rows(sizes, meta, row_elems, qkv, "nested tensor");
+  TORCH_CHECK(sizes.size(0) == 0 || sizes.size(1) == 2, "nestedtensor_b200: self_attention expects (L_i, 3 * embed_dim) constituents");
+  int64_t F = 3 * num_heads;
+  const int64_t* p = sizes.data_ptr<int64_t>();
+  for (int64_t b = 0; b < r.B; ++b) {
+    TORCH_CHECK(p[2 * b + 1] == p[1], "query's third dimension must be regular.");
+    F = p[1];
+  }
+  TORCH_CHECK(F % 3 == 0, "nestedtensor_b200: self_attention expects (L_i, 3 * embed_dim) constituents");
+  TORCH_CHECK(qkv.numel() == r.tokens * F, "nestedtensor_b200: buffer must have sum(numel) elements");
+  const int64_t d = check_heads(num_heads, F / 3);
+  const AttentionShape s = {r.B, r.tokens, r.tokens, r.longest, r.longest, row_elems, row_elems, num_heads, d, scaling};
+  return SelfAttentionTrain::apply(qkv.contiguous(), meta, s);
+}
+
+// Attention of the queries of sequence b over the keys and values of sequence b: buffers of (L_i, E) constituents; [Tq, E].
+Tensor attention_train(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_sizes, const Tensor& q_meta, int64_t q_row_elems,
+                       const Tensor& k_sizes, const Tensor& k_meta, int64_t k_row_elems, int64_t embed_dim, int64_t num_heads, double scaling) {
+  TORCH_CHECK(q.is_cuda(), "nestedtensor_b200: attention needs a CUDA nested tensor (this build has no CPU implementation)");
+  dtype_code(q.scalar_type());
+  same_kind(k, q, "key");
+  same_kind(v, q, "value");
+  const Rows rq = make_rows(q_sizes, q_meta, q_row_elems, q, "query"), rk = make_rows(k_sizes, k_meta, k_row_elems, q, "key");
+  TORCH_CHECK(rq.B == rk.B, "nestedtensor_b200: query and key must hold the same number of sequences");
+  const int64_t d = check_heads(num_heads, embed_dim);
+  auto regular = [&](const Tensor& sizes, const char* name) {
+    const int64_t* p = sizes.data_ptr<int64_t>();
+    TORCH_CHECK(sizes.size(0) == 0 || sizes.size(1) == 2, name, " needs to be 3 dim.");
+    for (int64_t b = 0; b < sizes.size(0); ++b) TORCH_CHECK(p[2 * b + 1] == embed_dim, name, "'s third dimension must be regular.");
+  };
+  regular(q_sizes, "query");
+  regular(k_sizes, "key");
+  TORCH_CHECK(q.numel() == rq.tokens * embed_dim && k.numel() == rk.tokens * embed_dim && v.numel() == k.numel(),
+              "nestedtensor_b200: buffer must have sum(numel) elements");
+  const AttentionShape s = {rq.B, rq.tokens, rk.tokens, rq.longest, rk.longest, q_row_elems, k_row_elems, num_heads, d, scaling};
+  return AttentionTrain::apply(q.contiguous(), k.contiguous(), v.contiguous(), q_meta, k_meta, s);
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(nestedtensor, m) {
+  m.def("layer_norm_train(Tensor x, Tensor sizes, int[] normalized_shape, Tensor? weight, Tensor? bias, float eps) -> Tensor", &layer_norm_train);
+  m.def("embedding_train(Tensor weight, Tensor index, Tensor sizes, int? padding_idx, float scale) -> Tensor", &embedding_train);
+  m.def("self_attention_train(Tensor qkv, Tensor sizes, Tensor meta, int row_elems, int num_heads, float scaling) -> Tensor",
+        &self_attention_train);
+  m.def(
+      "attention_train(Tensor q, Tensor k, Tensor v, Tensor q_sizes, Tensor q_meta, int q_row_elems, Tensor k_sizes, Tensor k_meta, "
+      "int k_row_elems, int embed_dim, int num_heads, float scaling) -> Tensor",
+      &attention_train);
+}

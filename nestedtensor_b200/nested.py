@@ -58,6 +58,10 @@ class NestedTensor(object):
         # the logical (C, H_i, W_i), every constituent is STORED as (H_i, W_i, C), i.e. with strides (1, W_i*C, C).
         self._channels_last = bool(channels_last)
         self._nchw = None  # cached contiguous copy of a channels_last tensor, made on first use by an operator
+        # set by with_values(): the [rows, ...] matrix behind _buffer (it carries the autograd graph), and (offsets, elements
+        # per row in them) of the nested tensor whose ragged structure this one shares
+        self._packed = None
+        self._rows = None
 
     # ---- record access -------------------------------------------------------------------
     def _record(self):
@@ -67,6 +71,9 @@ class NestedTensor(object):
             if self._nchw is None:
                 self._nchw = self.contiguous()
             return self._nchw._record()
+        if self._packed is not None and self._packed.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("nestedtensor_b200: this operator does not track gradients and would drop them; use "
+                               "nestedtensor_b200.nn.training, torch.no_grad() or detach the values")
         if self._meta is None or self._meta.device != self._buffer.device:
             self._meta = build_meta(self._sizes, self._buffer.device)
         return self._buffer, self._sizes, self._meta
@@ -74,6 +81,61 @@ class NestedTensor(object):
     def _stored_sizes(self):
         """Constituent shapes as they lie in the buffer."""
         return self._sizes[:, [1, 2, 0]].contiguous() if self._channels_last else self._sizes
+
+    # ---- packed rows, for torch operators and training -------------------------------------
+    def values(self):
+        """The rows of all constituents as one ``[sum(L_i), ...]`` tensor: the buffer in the shape of ``(L_i, ...)`` constituents
+        whose dimensions after the first are regular.  Shares the buffer's memory and its autograd graph."""
+        if self._packed is not None:
+            return self._packed
+        if len(self) == 0:
+            return self._buffer
+        if self._channels_last or self.tensor_dim() < 1:
+            raise RuntimeError("values() needs constituents of shape (L_i, ...)")
+        trailing = self._sizes[:, 1:]
+        if bool((trailing != trailing[0]).any()):
+            raise RuntimeError("values() needs regular dimensions after the first.")
+        return self._buffer.view([int(self._sizes[:, 0].sum())] + trailing[0].tolist())
+
+    def with_values(self, values):
+        """A NestedTensor of the same lengths ``L_i`` over another tensor of ``sum(L_i)`` rows: constituents
+        ``(L_i, *values.shape[1:])``.  Made contiguous if it is not; otherwise shares the memory and the autograd graph."""
+        if not torch.is_tensor(values) or values.dim() < 1:
+            raise TypeError("values must be a tensor of at least one dimension")
+        if self._channels_last or (self.tensor_dim() < 1 and len(self) > 0):
+            raise RuntimeError("with_values() needs constituents of shape (L_i, ...)")
+        B = len(self)
+        rows = int(self._sizes[:, 0].sum()) if B > 0 else 0
+        if values.size(0) != rows:
+            raise RuntimeError("with_values(): got %d rows for %d" % (values.size(0), rows))
+        if values.device != self._buffer.device:
+            raise RuntimeError("with_values(): values must be on the nested tensor's device")
+        sizes = torch.empty((B, values.dim()), dtype=torch.int64)
+        if B > 0:
+            sizes[:, 0] = self._sizes[:, 0]
+            for j in range(1, values.dim()):
+                sizes[:, j] = values.size(j)
+        return self._of_rows(values.contiguous(), sizes)
+
+    def _of_rows(self, packed, sizes):
+        out = NestedTensor(packed.view(-1), sizes)
+        out._packed = packed
+        out._rows = self._row_offsets() if self._buffer.is_cuda and len(self) > 0 else None
+        return out
+
+    def _row_offsets(self):
+        """(device offsets of the constituents, elements per row in them)."""
+        if self._rows is not None:
+            return self._rows
+        if self._meta is None or self._meta.device != self._buffer.device:
+            self._meta = build_meta(self._sizes, self._buffer.device)
+        return self._meta, int(self._sizes[0, 1:].prod()) if len(self) > 0 else 1
+
+    def _tracked(self):
+        """The packed rows as an operator that tracks gradients takes them."""
+        if self._channels_last:
+            raise RuntimeError("nestedtensor_b200: the training operators need contiguous constituents")
+        return self._packed if self._packed is not None else self._buffer
 
     # ---- attributes ----------------------------------------------------------------------
     @property
@@ -90,7 +152,7 @@ class NestedTensor(object):
 
     @property
     def requires_grad(self):
-        return False
+        return self._packed is not None and self._packed.requires_grad
 
     @property
     def is_cuda(self):
@@ -213,6 +275,12 @@ class NestedTensor(object):
         raise NotImplementedError("nestedtensor_b200: only integer indexing of constituents is implemented")
 
     def to(self, *args, **kwargs):
+        if self._packed is not None:
+            packed = self._packed.to(*args, **kwargs)
+            out = NestedTensor(packed.view(-1), self._sizes)
+            out._packed = packed
+            out._rows = self._rows if packed.device == self._buffer.device else None
+            return out
         buf = self._buffer.to(*args, **kwargs)
         meta = self._meta if (self._meta is not None and self._meta.device == buf.device) else None
         return NestedTensor(buf, self._sizes, meta, channels_last=self._channels_last)
