@@ -16,11 +16,14 @@ using torch::autograd::variable_list;
 
 // Passes a gradient computed with create_graph=True on to the graph, with an error in the place of its own derivative.
 struct FirstOrderOnly : public torch::autograd::Function<FirstOrderOnly> {
-  static Tensor forward(AutogradContext*, const Tensor& grad, const Tensor&, const Tensor&, const Tensor&, const Tensor&) { return grad.detach(); }
+  using Maybe = c10::optional<Tensor>;
+  static Tensor forward(AutogradContext*, const Tensor& grad, const Maybe&, const Maybe&, const Maybe&, const Maybe&) { return grad.detach(); }
   static variable_list backward(AutogradContext*, variable_list) {
     TORCH_CHECK_NOT_IMPLEMENTED(false, "nestedtensor_b200: the training operators have first derivatives only");
   }
 };
+
+c10::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
 
 // Runs `compute` (the gradients) without recording it; with create_graph=True every result keeps its dependence on `deps`.
 template <typename F>
@@ -33,7 +36,7 @@ variable_list first_order(const std::array<Tensor, 4>& deps, F&& compute) {
   }
   if (create_graph)
     for (auto& g : grads)
-      if (g.defined()) g = FirstOrderOnly::apply(g, deps[0], deps[1], deps[2], deps[3]);
+      if (g.defined()) g = FirstOrderOnly::apply(g, maybe(deps[0]), maybe(deps[1]), maybe(deps[2]), maybe(deps[3]));
   return grads;
 }
 
@@ -75,21 +78,22 @@ Rows make_rows(const Tensor& sizes, const Tensor& meta, int64_t row_elems, const
 
 // ------------------------------------------------------------------ LayerNorm
 struct LayerNormTrain : public torch::autograd::Function<LayerNormTrain> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t cols, double eps) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& bias,
+                        int64_t cols, double eps) {
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t rows = x.numel() / cols;
     Tensor out = at::empty({rows, cols}, x.options());
     Tensor stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
     Tensor w, b;
-    if (weight.defined()) w = weight.contiguous(), b = bias.contiguous();
+    if (weight) w = weight->contiguous(), b = bias->contiguous();
     float* st = stats.data_ptr<float>();
     check_rc(ntb200_layer_norm_train(x.data_ptr(), w.defined() ? w.data_ptr() : nullptr, b.defined() ? b.data_ptr() : nullptr, (float)eps,
                                      out.data_ptr(), st, st + rows, rows, cols, dtype_code(x.scalar_type()), cur_stream()),
              "ntb200_layer_norm_train");
     ctx->save_for_backward({x, w, stats});
     ctx->saved_data["wants_x"] = wants(x);
-    ctx->saved_data["wants_w"] = wants(weight);
-    ctx->saved_data["wants_b"] = wants(bias);
+    ctx->saved_data["wants_w"] = weight && wants(*weight);
+    ctx->saved_data["wants_b"] = bias && wants(*bias);
     return out;
   }
 
@@ -148,7 +152,7 @@ Tensor layer_norm_train(const Tensor& x_, const Tensor& sizes, at::IntArrayRef n
     TORCH_CHECK(bias->dim() == 1 && bias->size(0) == E, "nestedtensor_b200: bias must have ", E, " entries");
   }
   TORCH_CHECK(eps >= 0, "nestedtensor_b200: eps must not be negative");
-  return LayerNormTrain::apply(x_.contiguous(), has_w ? *weight : Tensor(), has_b ? *bias : Tensor(), E, eps);
+  return LayerNormTrain::apply(x_.contiguous(), has_w ? weight : c10::nullopt, has_b ? bias : c10::nullopt, E, eps);
 }
 
 // ------------------------------------------------------------------ embedding
