@@ -6,6 +6,8 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <array>
+#include <cmath>
 
 #include "dispatch_common.h"
 
@@ -51,29 +53,48 @@ void same_kind(const Tensor& t, const Tensor& like, const char* name) {
               " must be on the input's device and of its dtype");
 }
 
-// The rows of a ragged batch: host lengths (first column of `sizes`) and device offsets with `row_elems` elements per token.
+// The rows of a ragged batch.  `sizes` holds the lengths in its first column; features >= 0: the rows are a packed matrix of that
+// width, which the sizes of another nested tensor with the same lengths describe; -1: `sizes` are the tensor's own, and its
+// trailing dimensions must be regular.
 struct Rows {
-  int64_t B, tokens, longest;
+  int64_t B, tokens, longest, features;  // features: elements of the last dimension (-1: no sequences to tell)
 };
 
-Rows make_rows(const Tensor& sizes, const Tensor& meta, int64_t row_elems, const Tensor& like, const char* name) {
+Rows make_rows(const Tensor& t, const Tensor& sizes, int64_t features, const char* name) {
   TORCH_CHECK(sizes.device().is_cpu() && sizes.scalar_type() == at::kLong && sizes.dim() == 2 && sizes.is_contiguous() &&
                   (sizes.size(1) >= 1 || sizes.size(0) == 0),
               "nestedtensor_b200: sizes must be a contiguous CPU int64 [B, tensor_dim] tensor");
-  Rows r = {sizes.size(0), 0, 0};
-  TORCH_CHECK(meta.is_cuda() && meta.device() == like.device(), "nestedtensor_b200: this operator needs a CUDA ", name,
-              " (this build has no CPU implementation)");
-  TORCH_CHECK(meta.scalar_type() == at::kLong && meta.is_contiguous() && meta.numel() >= r.B + 1,
-              "nestedtensor_b200: meta must be a CUDA int64 tensor that begins with B+1 offsets");
-  TORCH_CHECK(row_elems >= 1, "nestedtensor_b200: row_elems must be at least 1");
+  TORCH_CHECK(t.is_cuda(), "nestedtensor_b200: this operator needs a CUDA ", name, " (this build has no CPU implementation)");
+  Rows r = {sizes.size(0), 0, 0, features};
   const int64_t* p = sizes.data_ptr<int64_t>();
   const int64_t td = sizes.size(1);
+  int64_t numel = 0;
   for (int64_t b = 0; b < r.B; ++b) {
-    TORCH_CHECK(p[b * td] >= 0, "nestedtensor_b200: negative size");
-    r.tokens += p[b * td];
-    r.longest = std::max(r.longest, p[b * td]);
+    const int64_t* s = p + b * td;
+    TORCH_CHECK(s[0] >= 0, "nestedtensor_b200: negative size");
+    r.tokens += s[0];
+    r.longest = std::max(r.longest, s[0]);
+    if (features < 0) {
+      TORCH_CHECK(s[td - 1] == p[td - 1] || td == 1, name, "'s last dimension must be regular.");
+      int64_t n = 1;
+      for (int64_t j = 0; j < td; ++j) n *= s[j];
+      numel += n;
+    }
   }
+  if (features < 0) {
+    if (r.B > 0) r.features = td > 1 ? p[td - 1] : 1;
+  } else {
+    TORCH_CHECK(t.dim() >= 1 && t.size(0) == r.tokens, "nestedtensor_b200: ", name, " must have sum(L_i) rows");
+    numel = t.numel();
+  }
+  TORCH_CHECK(t.numel() == numel, "nestedtensor_b200: buffer must have sum(numel) elements");
   return r;
+}
+
+void check_meta(const Tensor& meta, int64_t row_elems, int64_t B, const Tensor& like) {
+  TORCH_CHECK(meta.is_cuda() && meta.device() == like.device() && meta.scalar_type() == at::kLong && meta.is_contiguous() && meta.numel() >= B + 1,
+              "nestedtensor_b200: meta must be a CUDA int64 tensor that begins with B+1 offsets, on the input's device");
+  TORCH_CHECK(row_elems >= 1 || B == 0, "nestedtensor_b200: row_elems must be at least 1");
 }
 
 // ------------------------------------------------------------------ LayerNorm
@@ -122,26 +143,17 @@ struct LayerNormTrain : public torch::autograd::Function<LayerNormTrain> {
 };
 
 // LayerNorm over the last dimension of the packed rows; x is the buffer of the record, in any contiguous shape.  [T, E].
-Tensor layer_norm_train(const Tensor& x_, const Tensor& sizes, at::IntArrayRef normalized_shape, const c10::optional<Tensor>& weight,
-                        const c10::optional<Tensor>& bias, double eps) {
+Tensor layer_norm_train(const Tensor& x_, const Tensor& sizes, int64_t features, at::IntArrayRef normalized_shape,
+                        const c10::optional<Tensor>& weight, const c10::optional<Tensor>& bias, double eps) {
   TORCH_CHECK(normalized_shape.size() == 1, "Currently only singleton tuples of integers supported for layer_norm.");
   const int64_t E = normalized_shape[0];
   TORCH_CHECK(E > 0, "nestedtensor_b200: layer_norm over an empty dimension");
-  TORCH_CHECK(x_.is_cuda(), "nestedtensor_b200: layer_norm needs a CUDA nested tensor (this build has no CPU implementation)");
-  TORCH_CHECK(sizes.device().is_cpu() && sizes.scalar_type() == at::kLong && sizes.dim() == 2 && sizes.is_contiguous(),
-              "nestedtensor_b200: sizes must be a contiguous CPU int64 [B, tensor_dim] tensor");
-  const int64_t B = sizes.size(0), td = sizes.size(1);
-  TORCH_CHECK(B == 0 || td >= 1, "Cannot normalize across irregular dimension ", td);
-  const int64_t* p = sizes.data_ptr<int64_t>();
-  int64_t numel = 0;
-  for (int64_t b = 0; b < B; ++b) {
-    TORCH_CHECK(p[b * td + td - 1] == p[td - 1], "Cannot normalize across irregular dimension ", td);
-    int64_t n = 1;
-    for (int64_t j = 0; j < td; ++j) n *= p[b * td + j];
-    numel += n;
-  }
-  TORCH_CHECK(B == 0 || p[td - 1] == E, "Normalized shape [", E, "] does not match the size of the last dimension (", p[td - 1], ") of input.");
-  TORCH_CHECK(x_.numel() == numel, "nestedtensor_b200: buffer must have sum(numel) elements");
+  TORCH_CHECK(features >= 0 || sizes.size(0) == 0 || sizes.size(1) > 1 ||
+                  (sizes.numel() > 0 && (sizes == sizes[0][0]).all().item<bool>()),
+              "Cannot normalize across irregular dimension 1");
+  const Rows r = make_rows(x_, sizes, features, "input");
+  const int64_t last = features < 0 && r.B > 0 && sizes.size(1) == 1 ? r.longest : r.features;
+  TORCH_CHECK(last < 0 || last == E, "Normalized shape [", E, "] does not match the size of the last dimension (", last, ") of input.");
   dtype_code(x_.scalar_type());
   const bool has_w = weight && weight->defined(), has_b = bias && bias->defined();
   TORCH_CHECK(has_w == has_b, "Either both weight and bias are used or not.");
@@ -206,8 +218,7 @@ Tensor embedding_train(const Tensor& weight, const Tensor& index, const Tensor& 
               "Expected tensor for argument #1 'indices' to have one of the following scalar types: Long, Int");
   TORCH_CHECK(sizes.device().is_cpu() && sizes.scalar_type() == at::kLong && sizes.dim() == 2 && (sizes.size(1) == 1 || sizes.size(0) == 0),
               "nestedtensor_b200: embedding expects a nested tensor of 1-D index sequences");
-  TORCH_CHECK(index.numel() == (sizes.size(0) > 0 ? sizes.sum().item<int64_t>() : 0),
-              "nestedtensor_b200: the index buffer must hold sum(L_i) entries");
+  make_rows(index, sizes, -1, "index tensor");
   const int64_t V = weight.size(0);
   TORCH_CHECK(V > 0 || index.numel() == 0, "nestedtensor_b200: embedding needs a weight with at least one row");
   TORCH_CHECK(V < (1ll << 31) - 1 && index.numel() < (1ll << 31) - 1, "nestedtensor_b200: embedding supports fewer than 2^31 - 1 rows and tokens");
@@ -324,57 +335,54 @@ int64_t check_heads(int64_t num_heads, int64_t E) {
   return E / num_heads;
 }
 
+double scaling_or_default(c10::optional<double> scaling, int64_t d) { return scaling ? *scaling : 1.0 / std::sqrt((double)d); }
+
 // Self-attention of packed q|k|v rows: qkv is the buffer of (L_i, 3E) constituents in any contiguous shape; [T, E].
-Tensor self_attention_train(const Tensor& qkv, const Tensor& sizes, const Tensor& meta, int64_t row_elems, int64_t num_heads, double scaling) {
-  TORCH_CHECK(qkv.is_cuda(), "nestedtensor_b200: self_attention needs a CUDA nested tensor (this build has no CPU implementation)");
+Tensor self_attention_train(const Tensor& qkv, const Tensor& sizes, int64_t features, const Tensor& meta, int64_t row_elems, int64_t num_heads,
+                            c10::optional<double> scaling) {
   dtype_code(qkv.scalar_type());
-  const Rows r = make_rows(sizes, meta, row_elems, qkv, "nested tensor");
-  TORCH_CHECK(sizes.size(0) == 0 || sizes.size(1) == 2, "nestedtensor_b200: self_attention expects (L_i, 3 * embed_dim) constituents");
-  int64_t F = 3 * num_heads;
-  const int64_t* p = sizes.data_ptr<int64_t>();
-  for (int64_t b = 0; b < r.B; ++b) {
-    TORCH_CHECK(p[2 * b + 1] == p[1], "query's third dimension must be regular.");
-    F = p[1];
-  }
-  TORCH_CHECK(F % 3 == 0, "nestedtensor_b200: self_attention expects (L_i, 3 * embed_dim) constituents");
-  TORCH_CHECK(qkv.numel() == r.tokens * F, "nestedtensor_b200: buffer must have sum(numel) elements");
+  const Rows r = make_rows(qkv, sizes, features, "nested tensor");
+  check_meta(meta, row_elems, r.B, qkv);
+  const int64_t F = r.features < 0 ? 3 * num_heads : r.features;
+  TORCH_CHECK(F % 3 == 0 && qkv.numel() == r.tokens * F, "nestedtensor_b200: self_attention expects (L_i, 3 * embed_dim) constituents");
   const int64_t d = check_heads(num_heads, F / 3);
-  const AttentionShape s = {r.B, r.tokens, r.tokens, r.longest, r.longest, row_elems, row_elems, num_heads, d, scaling};
+  const AttentionShape s = {r.B, r.tokens, r.tokens, r.longest, r.longest, row_elems, row_elems, num_heads, d, scaling_or_default(scaling, d)};
   return SelfAttentionTrain::apply(qkv.contiguous(), meta, s);
 }
 
 // Attention of the queries of sequence b over the keys and values of sequence b: buffers of (L_i, E) constituents; [Tq, E].
-Tensor attention_train(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_sizes, const Tensor& q_meta, int64_t q_row_elems,
-                       const Tensor& k_sizes, const Tensor& k_meta, int64_t k_row_elems, int64_t embed_dim, int64_t num_heads, double scaling) {
-  TORCH_CHECK(q.is_cuda(), "nestedtensor_b200: attention needs a CUDA nested tensor (this build has no CPU implementation)");
+Tensor attention_train(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_sizes, int64_t q_features, const Tensor& q_meta,
+                       int64_t q_row_elems, const Tensor& k_sizes, int64_t k_features, const Tensor& k_meta, int64_t k_row_elems,
+                       int64_t num_heads, c10::optional<double> scaling) {
   dtype_code(q.scalar_type());
+  const Rows rq = make_rows(q, q_sizes, q_features, "query");
   same_kind(k, q, "key");
   same_kind(v, q, "value");
-  const Rows rq = make_rows(q_sizes, q_meta, q_row_elems, q, "query"), rk = make_rows(k_sizes, k_meta, k_row_elems, q, "key");
+  const Rows rk = make_rows(k, k_sizes, k_features, "key");
+  check_meta(q_meta, q_row_elems, rq.B, q);
+  check_meta(k_meta, k_row_elems, rk.B, q);
   TORCH_CHECK(rq.B == rk.B, "nestedtensor_b200: query and key must hold the same number of sequences");
-  const int64_t d = check_heads(num_heads, embed_dim);
-  auto regular = [&](const Tensor& sizes, const char* name) {
-    const int64_t* p = sizes.data_ptr<int64_t>();
-    TORCH_CHECK(sizes.size(0) == 0 || sizes.size(1) == 2, name, " needs to be 3 dim.");
-    for (int64_t b = 0; b < sizes.size(0); ++b) TORCH_CHECK(p[2 * b + 1] == embed_dim, name, "'s third dimension must be regular.");
-  };
-  regular(q_sizes, "query");
-  regular(k_sizes, "key");
-  TORCH_CHECK(q.numel() == rq.tokens * embed_dim && k.numel() == rk.tokens * embed_dim && v.numel() == k.numel(),
-              "nestedtensor_b200: buffer must have sum(numel) elements");
-  const AttentionShape s = {rq.B, rq.tokens, rk.tokens, rq.longest, rk.longest, q_row_elems, k_row_elems, num_heads, d, scaling};
+  const int64_t E = rq.features < 0 ? num_heads : rq.features;
+  TORCH_CHECK((rk.features < 0 || rk.features == E) && q.numel() == rq.tokens * E && k.numel() == rk.tokens * E && v.numel() == k.numel(),
+              "nestedtensor_b200: query, key and value need the same last dimension and constituents of (L_i, embed_dim)");
+  const int64_t d = check_heads(num_heads, E);
+  const AttentionShape s = {rq.B, rq.tokens, rk.tokens, rq.longest, rk.longest, q_row_elems, k_row_elems, num_heads, d,
+                            scaling_or_default(scaling, d)};
   return AttentionTrain::apply(q.contiguous(), k.contiguous(), v.contiguous(), q_meta, k_meta, s);
 }
 
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(nestedtensor, m) {
-  m.def("layer_norm_train(Tensor x, Tensor sizes, int[] normalized_shape, Tensor? weight, Tensor? bias, float eps) -> Tensor", &layer_norm_train);
-  m.def("embedding_train(Tensor weight, Tensor index, Tensor sizes, int? padding_idx, float scale) -> Tensor", &embedding_train);
-  m.def("self_attention_train(Tensor qkv, Tensor sizes, Tensor meta, int row_elems, int num_heads, float scaling) -> Tensor",
-        &self_attention_train);
   m.def(
-      "attention_train(Tensor q, Tensor k, Tensor v, Tensor q_sizes, Tensor q_meta, int q_row_elems, Tensor k_sizes, Tensor k_meta, "
-      "int k_row_elems, int embed_dim, int num_heads, float scaling) -> Tensor",
+      "layer_norm_train(Tensor x, Tensor sizes, int features, int[] normalized_shape, Tensor? weight, Tensor? bias, float eps) -> Tensor",
+      &layer_norm_train);
+  m.def("embedding_train(Tensor weight, Tensor index, Tensor sizes, int? padding_idx, float scale) -> Tensor", &embedding_train);
+  m.def(
+      "self_attention_train(Tensor qkv, Tensor sizes, int features, Tensor meta, int row_elems, int num_heads, float? scaling) -> Tensor",
+      &self_attention_train);
+  m.def(
+      "attention_train(Tensor q, Tensor k, Tensor v, Tensor q_sizes, int q_features, Tensor q_meta, int q_row_elems, Tensor k_sizes, "
+      "int k_features, Tensor k_meta, int k_row_elems, int num_heads, float? scaling) -> Tensor",
       &attention_train);
 }

@@ -51,17 +51,44 @@ class NestedTensor(object):
             raise TypeError("sizes must be a CPU int64 [B, tensor_dim] tensor")
         if channels_last and sizes.size(1) != 3:
             raise RuntimeError("channels_last needs constituents of shape (C, H_i, W_i)")
-        self._buffer = buffer
-        self._sizes = sizes.contiguous()
+        self._flat = buffer
+        self._extents = sizes.contiguous()
         self._meta = meta
         # channels_last (nestedtensor/csrc/nested_tensor_impl.cpp:46, storage_is_contiguous_channels_last): the sizes are
         # the logical (C, H_i, W_i), every constituent is STORED as (H_i, W_i, C), i.e. with strides (1, W_i*C, C).
         self._channels_last = bool(channels_last)
         self._nchw = None  # cached contiguous copy of a channels_last tensor, made on first use by an operator
-        # set by with_values(): the [rows, ...] matrix behind _buffer (it carries the autograd graph), and (offsets, elements
-        # per row in them) of the nested tensor whose ragged structure this one shares
         self._packed = None
-        self._rows = None
+        self._root = None
+
+    @classmethod
+    def _over(cls, packed, root):
+        """A nested tensor over the [rows, ...] matrix `packed` (contiguous; it carries the autograd graph) with the lengths of
+        `root`, whose offsets it shares; the flat buffer and the sizes are made when something asks for them."""
+        out = cls.__new__(cls)
+        out._flat = out._extents = out._meta = out._nchw = None
+        out._channels_last = False
+        out._packed = packed
+        out._root = root
+        return out
+
+    @property
+    def _buffer(self):
+        if self._flat is None:
+            self._flat = self._packed.view(-1)
+        return self._flat
+
+    @property
+    def _sizes(self):
+        if self._extents is None:
+            lengths, p = self._root._sizes, self._packed
+            sizes = torch.empty((lengths.size(0), p.dim()), dtype=torch.int64)
+            if lengths.size(0) > 0:
+                sizes[:, 0] = lengths[:, 0]
+                for j in range(1, p.dim()):
+                    sizes[:, j] = p.size(j)
+            self._extents = sizes
+        return self._extents
 
     # ---- record access -------------------------------------------------------------------
     def _record(self):
@@ -104,47 +131,53 @@ class NestedTensor(object):
             raise TypeError("values must be a tensor of at least one dimension")
         if self._channels_last or (self.tensor_dim() < 1 and len(self) > 0):
             raise RuntimeError("with_values() needs constituents of shape (L_i, ...)")
-        B = len(self)
-        rows = int(self._sizes[:, 0].sum()) if B > 0 else 0
+        rows = self._packed.size(0) if self._packed is not None else int(self._sizes[:, 0].sum()) if len(self) > 0 else 0
         if values.size(0) != rows:
             raise RuntimeError("with_values(): got %d rows for %d" % (values.size(0), rows))
-        if values.device != self._buffer.device:
+        if values.device != self.device:
             raise RuntimeError("with_values(): values must be on the nested tensor's device")
-        sizes = torch.empty((B, values.dim()), dtype=torch.int64)
-        if B > 0:
-            sizes[:, 0] = self._sizes[:, 0]
-            for j in range(1, values.dim()):
-                sizes[:, j] = values.size(j)
-        return self._of_rows(values.contiguous(), sizes)
+        return self._with_rows(values.contiguous())
 
-    def _of_rows(self, packed, sizes):
-        out = NestedTensor(packed.view(-1), sizes)
-        out._packed = packed
-        out._rows = self._row_offsets() if self._buffer.is_cuda and len(self) > 0 else None
-        return out
+    def _with_rows(self, packed):
+        return NestedTensor._over(packed, self if self._root is None else self._root)
 
     def _row_offsets(self):
         """(device offsets of the constituents, elements per row in them)."""
-        if self._rows is not None:
-            return self._rows
-        if self._meta is None or self._meta.device != self._buffer.device:
-            self._meta = build_meta(self._sizes, self._buffer.device)
-        return self._meta, int(self._sizes[0, 1:].prod()) if len(self) > 0 else 1
+        root = self if self._root is None else self._root
+        if root._meta is None or root._meta.device != self.device:
+            if root._buffer.device != self.device:  # moved away from the structure it was made from
+                self._meta = build_meta(self._sizes, self.device) if self._meta is None else self._meta
+                return self._meta, self._row_elems()
+            root._meta = build_meta(root._sizes, root._buffer.device)
+        return root._meta, root._row_elems()
+
+    def _row_elems(self):
+        sizes = self._sizes
+        if sizes.size(0) == 0 or sizes.size(1) == 1:
+            return 1
+        return int(sizes[0, 1]) if sizes.size(1) == 2 else int(sizes[0, 1:].prod())
 
     def _tracked(self):
-        """The packed rows as an operator that tracks gradients takes them."""
+        """(rows, sizes, features) as an operator that tracks gradients takes them: the packed rows with their last extent and
+        sizes whose first column holds the lengths, or the buffer with its own sizes and -1."""
         if self._channels_last:
             raise RuntimeError("nestedtensor_b200: the training operators need contiguous constituents")
-        return self._packed if self._packed is not None else self._buffer
+        if self._packed is not None:
+            return self._packed, self._root._sizes, self._packed.size(-1) if self._packed.dim() > 1 else 1
+        buf = self._flat
+        base = buf._base
+        if base is not None and base.requires_grad and base.numel() == buf.numel() and base.is_contiguous():
+            buf = base  # a flat view of a whole tensor: the gradient goes to the tensor itself, without the view's own step
+        return buf, self._extents, -1
 
     # ---- attributes ----------------------------------------------------------------------
     @property
     def dtype(self):
-        return self._buffer.dtype
+        return (self._flat if self._packed is None else self._packed).dtype
 
     @property
     def device(self):
-        return self._buffer.device
+        return (self._flat if self._packed is None else self._packed).device
 
     @property
     def layout(self):
@@ -177,13 +210,13 @@ class NestedTensor(object):
         return 1
 
     def tensor_dim(self):
-        return int(self._sizes.size(1))
+        return int(self._sizes.size(1)) if self._packed is None else self._packed.dim()
 
     def dim(self):
         return 1 + self.tensor_dim()
 
     def __len__(self):
-        return int(self._sizes.size(0))
+        return int((self if self._root is None else self._root)._sizes.size(0))
 
     def size(self, dim=None):
         """``None`` for ragged dimensions (nestedtensor/csrc/py_init.cpp:169-172)."""
@@ -276,11 +309,7 @@ class NestedTensor(object):
 
     def to(self, *args, **kwargs):
         if self._packed is not None:
-            packed = self._packed.to(*args, **kwargs)
-            out = NestedTensor(packed.view(-1), self._sizes)
-            out._packed = packed
-            out._rows = self._rows if packed.device == self._buffer.device else None
-            return out
+            return NestedTensor._over(self._packed.to(*args, **kwargs), self._root)
         buf = self._buffer.to(*args, **kwargs)
         meta = self._meta if (self._meta is not None and self._meta.device == buf.device) else None
         return NestedTensor(buf, self._sizes, meta, channels_last=self._channels_last)

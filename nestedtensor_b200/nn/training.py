@@ -37,9 +37,11 @@ def layer_norm(input: NestedTensor, normalized_shape, weight=None, bias=None, ep
     _check(input, "input")
     if isinstance(normalized_shape, int):
         normalized_shape = (normalized_shape,)
-    x = input._tracked()
-    out = _ops.ops().layer_norm_train(x, input._sizes, list(normalized_shape), weight, bias, float(eps))
-    return input._of_rows(out, input._sizes)
+    x, sizes, features = input._tracked()
+    out = _ops.ops().layer_norm_train(x, sizes, features, normalized_shape, weight, bias, eps)
+    if input.tensor_dim() != 2:  # (L_i, ..., E): the rows of the operator are finer than the constituents'
+        out = out.view(input.values().shape)
+    return input._with_rows(out)
 
 
 def embedding(input: NestedTensor, weight: torch.Tensor, padding_idx: Optional[int] = None, max_norm=None, norm_type=2.0,
@@ -53,8 +55,8 @@ def embedding(input: NestedTensor, weight: torch.Tensor, padding_idx: Optional[i
     _check(input, "input")
     if input.dim() != 2 and len(input) > 0:
         raise NotImplementedError("nestedtensor_b200: embedding expects a nested tensor of 1-D index sequences")
-    out = _ops.ops().embedding_train(weight, input._buffer, input._sizes, padding_idx, float(scale))
-    return input.with_values(out)
+    out = _ops.ops().embedding_train(weight, input._buffer, input._sizes, padding_idx, scale)
+    return input._with_rows(out)
 
 
 def self_attention(qkv: NestedTensor, num_heads: int, scaling: Optional[float] = None) -> NestedTensor:
@@ -64,13 +66,10 @@ def self_attention(qkv: NestedTensor, num_heads: int, scaling: Optional[float] =
     _check(qkv, "qkv")
     if qkv.dim() != 3 and len(qkv) > 0:
         raise RuntimeError("query needs to be 3 dim.")
-    x = qkv._tracked()
-    if scaling is None:
-        features = int(qkv._sizes[0, 1]) if len(qkv) > 0 else 3 * num_heads
-        scaling = float(max(features // (3 * num_heads), 1)) ** -0.5
+    x, sizes, features = qkv._tracked()
     meta, row_elems = qkv._row_offsets()
-    out = _ops.ops().self_attention_train(x, qkv._sizes, meta, row_elems, num_heads, float(scaling))
-    return qkv.with_values(out)
+    out = _ops.ops().self_attention_train(x, sizes, features, meta, row_elems, num_heads, scaling)
+    return qkv._with_rows(out)
 
 
 def attention(query: NestedTensor, key: NestedTensor, value: NestedTensor, num_heads: int,
@@ -84,12 +83,10 @@ def attention(query: NestedTensor, key: NestedTensor, value: NestedTensor, num_h
             raise RuntimeError(name + " needs to be 3 dim.")
     if value is not key and not torch.equal(key._sizes, value._sizes):
         raise RuntimeError("nestedtensor_b200: key and value must have the same nested size")
-    embed_dim = int(query._sizes[0, 1]) if len(query) > 0 else num_heads
-    if scaling is None:
-        scaling = float(max(embed_dim // num_heads, 1)) ** -0.5
-    q, k, v = query._tracked(), key._tracked(), value._tracked()
+    q, q_sizes, features = query._tracked()
+    k, k_sizes, k_features = key._tracked()
+    v = value._tracked()[0]
     q_meta, q_row = query._row_offsets()
     k_meta, k_row = key._row_offsets()
-    out = _ops.ops().attention_train(q, k, v, query._sizes, q_meta, q_row, key._sizes, k_meta, k_row, embed_dim, num_heads,
-                                     float(scaling))
-    return query.with_values(out)
+    out = _ops.ops().attention_train(q, k, v, q_sizes, features, q_meta, q_row, k_sizes, k_features, k_meta, k_row, num_heads, scaling)
+    return query._with_rows(out)
