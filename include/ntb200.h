@@ -390,7 +390,8 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
  * (they may be the three thirds of one [T, 3*H*d] matrix), must not overlap the inputs.  Rows of every sequence are written
  * (zeros where the other side is empty); rows outside the sequences are left as they were.  The probabilities are computed
  * again from q, k and lse.
- *   path  0 = best available;  1 = the 32-bit tile kernels (any dtype and head_dim <= 256)
+ *   path  0 = best available;  1 = the 32-bit tile kernels (any dtype and head_dim <= 256);  2 = mma.sync kernels (fp16 /
+ *         bf16, head_dim 32 / 64 / 128, 16-byte aligned rows)                                (1, 2: for cross-checks)
  * workspace: 16-byte aligned.
  */
 size_t ntb200_varlen_attention_backward_workspace_bytes(int64_t batch, int64_t q_tokens, int64_t k_tokens, int num_heads,

@@ -14,6 +14,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "attention_internal.cuh"
 #include "attention_tiny.cuh"
 #include "common.cuh"
@@ -46,6 +48,7 @@ struct BwdArgs {
   const void *grad, *q, *k, *v, *out;
   const float* lse;  // [H, q_tokens]
   float* delta;      // [H, q_tokens]: D
+  const unsigned* top;  // [batch, H]: bits of the largest |dO| of the sequence and head (fp16 kernels only, else NULL)
   void *dq, *dk, *dv;
   int64_t ldq, ldk, ldv, lddq, lddk, lddv;  // grad and out are contiguous: their stride is H * d
   const int64_t *offsets_q, *offsets_k;
@@ -55,16 +58,21 @@ struct BwdArgs {
   float scaling;
 };
 
-// ------------------------------------------------------------------ work list
-// items[i] = (first row of the tile, valid rows in it, first row of the sequence's other side, its length) for every `tile`
-// rows of the own side (keys for dK / dV, queries for dQ), longest other side first.  A sequence whose other side is empty
-// keeps its items: their gradients are zeros, written by the kernel that walks no tile at all.  One block.
-constexpr int kListThreads = 1024;
+// ------------------------------------------------------------------ work lists and D = rowsum(dO * O), one launch
+// items[i] = (first row of the tile, valid rows in it, sequence, tile number) for every `tile` rows of the own side (keys for
+// dK / dV, queries for dQ), longest other side first.  A sequence whose other side is empty keeps its items: their gradients
+// are zeros, written by a block that walks no tile at all.  One block.
 constexpr int kListBuckets = 32;
+constexpr int kPrepThreads = 256;
 
-__global__ void __launch_bounds__(kListThreads)
-backward_items_kernel(const int64_t* __restrict__ offsets_own, int64_t row_elems_own, const int64_t* __restrict__ offsets_other,
-                      int64_t row_elems_other, int64_t batch, int tile, int4* __restrict__ items, int* __restrict__ count) {
+struct ListOut {
+  int4* items;
+  int* count;
+};
+
+__device__ __forceinline__ void build_backward_items(const int64_t* __restrict__ offsets_own, int64_t row_elems_own,
+                                                     const int64_t* __restrict__ offsets_other, int64_t row_elems_other, int64_t batch,
+                                                     int tile, const ListOut& out) {
   __shared__ int s_cnt[kListBuckets], s_base[kListBuckets];
   if (threadIdx.x < kListBuckets) s_cnt[threadIdx.x] = 0;
   __syncthreads();
@@ -72,7 +80,7 @@ backward_items_kernel(const int64_t* __restrict__ offsets_own, int64_t row_elems
     const int t = (int)((n + tile - 1) / tile);
     return t < 16 ? t : 16 + (27 - __clz(t) < kListBuckets - 17 ? 27 - __clz(t) : kListBuckets - 17);
   };
-  for (int64_t b = threadIdx.x; b < batch; b += kListThreads) {
+  for (int64_t b = threadIdx.x; b < batch; b += kPrepThreads) {
     const int64_t n = (offsets_own[b + 1] - offsets_own[b]) / row_elems_own, m = (offsets_other[b + 1] - offsets_other[b]) / row_elems_other;
     if (n > 0) atomicAdd(&s_cnt[bucket(m)], (int)((n + tile - 1) / tile));
   }
@@ -83,37 +91,109 @@ backward_items_kernel(const int64_t* __restrict__ offsets_own, int64_t row_elems
       s_base[k] = acc;
       acc += s_cnt[k];
     }
-    *count = acc;
+    *out.count = acc;
   }
   __syncthreads();
-  for (int64_t b = threadIdx.x; b < batch; b += kListThreads) {
+  for (int64_t b = threadIdx.x; b < batch; b += kPrepThreads) {
     const int64_t n = (offsets_own[b + 1] - offsets_own[b]) / row_elems_own, m = (offsets_other[b + 1] - offsets_other[b]) / row_elems_other;
     if (n <= 0) continue;
     const int tiles = (int)((n + tile - 1) / tile);
     const int pos = atomicAdd(&s_base[bucket(m)], tiles);  // (the order inside a bucket decides nothing but the schedule)
-    const int t0 = (int)(offsets_own[b] / row_elems_own), o0 = (int)(offsets_other[b] / row_elems_other);
+    const int t0 = (int)(offsets_own[b] / row_elems_own);
     for (int t = 0; t < tiles; ++t) {
       const int64_t rows = n - (int64_t)t * tile;
-      items[pos + t] = make_int4(t0 + t * tile, (int)(rows < tile ? rows : tile), o0, (int)m);
+      out.items[pos + t] = make_int4(t0 + t * tile, (int)(rows < tile ? rows : tile), (int)b, t);
     }
   }
 }
 
-// ------------------------------------------------------------------ D = rowsum(dO * O)
-template <typename T>
-__global__ void __launch_bounds__(256) attn_delta_kernel(BwdArgs a) {
-  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+// Blocks 0 and 1 build the lists; every warp of the others takes one query token: D of all its heads, and (fp16) the largest
+// |dO| of its sequence and head.  VEC: heads of 32, 64 or 128 elements on 16-byte boundaries: a head on d / 8 lanes.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kPrepThreads)
+backward_prepare_kernel(BwdArgs a, int tile, ListOut kv, ListOut qi, unsigned* __restrict__ top) {
+  if (blockIdx.x == 0) {
+    build_backward_items(a.offsets_k, a.row_elems_k, a.offsets_q, a.row_elems_q, a.batch, tile, kv);
+    return;
+  }
+  if (blockIdx.x == 1) {
+    build_backward_items(a.offsets_q, a.row_elems_q, a.offsets_k, a.row_elems_k, a.batch, tile, qi);
+    return;
+  }
+  const int64_t t = ((int64_t)blockIdx.x - 2) * (kPrepThreads / 32) + (threadIdx.x >> 5);
+  if (t >= a.q_tokens) return;
   const int lane = threadIdx.x & 31;
-  if (w >= a.q_tokens * a.H) return;
-  const int64_t t = w / a.H;
-  const int h = (int)(w - t * a.H);
-  const int64_t base = t * ((int64_t)a.H * a.d) + (int64_t)h * a.d;
-  float s = 0.0f;
-  for (int i = lane; i < a.d; i += 32)
-    s = fmaf(to_f32(static_cast<const T*>(a.grad)[base + i]), to_f32(static_cast<const T*>(a.out)[base + i]), s);
+  const int64_t E = (int64_t)a.H * a.d;
+  const T* g = static_cast<const T*>(a.grad) + t * E;
+  const T* o = static_cast<const T*>(a.out) + t * E;
+  int64_t b = 0;
+  if (top != nullptr) b = find_entry_warp(a.offsets_q, 0, a.batch - 1, t * a.row_elems_q);
+  if (VEC) {
+    const int per = a.d / 8;  // lanes per head
+    for (int v0 = 0; v0 < E / 8; v0 += 32) {
+      const int v = v0 + lane;
+      float s = 0.0f, m = 0.0f;
+      if (v < E / 8) {
+        T x[8], y[8];
+        *reinterpret_cast<uint4*>(x) = reinterpret_cast<const uint4*>(g)[v];
+        *reinterpret_cast<uint4*>(y) = reinterpret_cast<const uint4*>(o)[v];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) a.delta[(int64_t)h * a.q_tokens + t] = s;
+        for (int k = 0; k < 8; ++k) {
+          s = fmaf(to_f32(x[k]), to_f32(y[k]), s);
+          m = fmaxf(m, fabsf(to_f32(x[k])));
+        }
+      }
+      for (int w = per / 2; w > 0; w >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, w);
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+      }
+      if (v < E / 8 && lane % per == 0) {
+        const int h = v / per;
+        a.delta[(int64_t)h * a.q_tokens + t] = s;
+        if (top != nullptr) atomicMax(top + b * a.H + h, __float_as_uint(m));
+      }
+    }
+  } else {
+    for (int h = 0; h < a.H; ++h) {
+      float s = 0.0f;
+      for (int i = lane; i < a.d; i += 32) s = fmaf(to_f32(g[(int64_t)h * a.d + i]), to_f32(o[(int64_t)h * a.d + i]), s);
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+      if (lane == 0) a.delta[(int64_t)h * a.q_tokens + t] = s;
+    }
+  }
+}
+
+// One work item: a tile of the own side, and the other side of its sequence
+struct Item {
+  int64_t row0;   // first row of the tile
+  int rows;       // valid rows in it
+  int64_t other;  // first row of the other side
+  int n_other;    // and its length
+  int seq;
+};
+
+template <bool KV>
+__device__ __forceinline__ Item decode(const BwdArgs& a, const int4& w) {
+  Item it;
+  it.row0 = w.x;
+  it.rows = w.y;
+  it.seq = w.z;
+  const int64_t* off = KV ? a.offsets_q : a.offsets_k;
+  const int64_t re = KV ? a.row_elems_q : a.row_elems_k;
+  it.other = off[w.z] / re;
+  it.n_other = (int)(off[w.z + 1] / re - it.other);
+  return it;
+}
+
+// fp16 holds dS only between 2^-24 and 65504, while gradients come at any scale: dS is computed from dO times a power of two
+// that brings the largest |dO| of the sequence and head to [1, 2), and the product's sum is divided by it again (both exact).
+__device__ __forceinline__ float grad_scale(const BwdArgs& a, int seq, int h) {
+  if (a.top == nullptr) return 1.0f;
+  const int e = (int)(a.top[(int64_t)seq * a.H + h] >> 23);  // biased exponent of a non-negative number
+  if (e == 0 || e == 255) return 1.0f;                       // zeros; Inf or NaN, which no factor mends
+  const int f = 254 - e;                                     // 2^(127 - e)
+  return __uint_as_float((unsigned)(f < 27 ? 27 : (f > 227 ? 227 : f)) << 23);
 }
 
 // ------------------------------------------------------------------ tiles in 32 bits, any type and head size
@@ -152,22 +232,22 @@ attn_bwd_simt_kernel(BwdArgs a, const int4* __restrict__ items, const int* __res
   const float scale = a.scaling * kLog2e;
   const int d4 = (a.d + 3) & ~3;
   for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
-    const int4 it = items[w / a.H];
+    const Item it = decode<KV>(a, items[w / a.H]);
     const int h = (int)(w % a.H);
     const int64_t col = (int64_t)h * a.d;
-    const T* ga_own = (KV ? static_cast<const T*>(a.k) + it.x * a.ldk : static_cast<const T*>(a.q) + it.x * a.ldq) + col;
-    const T* gb_own = (KV ? static_cast<const T*>(a.v) + it.x * a.ldv : static_cast<const T*>(a.grad) + it.x * E) + col;
+    const T* ga_own = (KV ? static_cast<const T*>(a.k) + it.row0 * a.ldk : static_cast<const T*>(a.q) + it.row0 * a.ldq) + col;
+    const T* gb_own = (KV ? static_cast<const T*>(a.v) + it.row0 * a.ldv : static_cast<const T*>(a.grad) + it.row0 * E) + col;
     const int64_t ld_a_own = KV ? a.ldk : a.ldq, ld_b_own = KV ? a.ldv : E;
     const int64_t ld_a = KV ? a.ldq : a.ldk, ld_b = KV ? E : a.ldv;
     const float* g_lse = a.lse + (int64_t)h * a.q_tokens;
     const float* g_delta = a.delta + (int64_t)h * a.q_tokens;
     __syncthreads();  // the previous item's tiles have been read
-    load_rows<T, BT, DP>(own_a, ga_own, ld_a_own, it.y, a.d);
-    load_rows<T, BT, DP>(own_b, gb_own, ld_b_own, it.y, a.d);
+    load_rows<T, BT, DP>(own_a, ga_own, ld_a_own, it.rows, a.d);
+    load_rows<T, BT, DP>(own_b, gb_own, ld_b_own, it.rows, a.d);
     if (!KV && threadIdx.x < BT) {
-      const bool ok = (int)threadIdx.x < it.y && it.w > 0;  // (rows without keys have no statistics)
-      s_lse[threadIdx.x] = ok ? g_lse[it.x + threadIdx.x] : INFINITY;
-      s_delta[threadIdx.x] = ok ? g_delta[it.x + threadIdx.x] : 0.0f;
+      const bool ok = (int)threadIdx.x < it.rows && it.n_other > 0;  // (rows without keys have no statistics)
+      s_lse[threadIdx.x] = ok ? g_lse[it.row0 + threadIdx.x] : INFINITY;
+      s_delta[threadIdx.x] = ok ? g_delta[it.row0 + threadIdx.x] : 0.0f;
     }
     float acc1[KV ? MI : 1][KV ? NC : 1], acc2[MI][NC];
 #pragma unroll
@@ -177,9 +257,9 @@ attn_bwd_simt_kernel(BwdArgs a, const int4* __restrict__ items, const int* __res
         acc2[i][j] = 0.0f;
         if (KV) acc1[i][j] = 0.0f;
       }
-    for (int c0 = 0; c0 < it.w; c0 += BT) {
-      const int nc = it.w - c0 < BT ? it.w - c0 : BT;
-      const int64_t o0 = (int64_t)it.z + c0;
+    for (int c0 = 0; c0 < it.n_other; c0 += BT) {
+      const int nc = it.n_other - c0 < BT ? it.n_other - c0 : BT;
+      const int64_t o0 = it.other + c0;
       __syncthreads();
       load_rows<T, BT, DP>(oth_a, (KV ? static_cast<const T*>(a.q) + o0 * a.ldq : static_cast<const T*>(a.k) + o0 * a.ldk) + col, ld_a, nc, a.d);
       load_rows<T, BT, DP>(oth_b, (KV ? static_cast<const T*>(a.grad) + o0 * E : static_cast<const T*>(a.v) + o0 * a.ldv) + col, ld_b, nc, a.d);
@@ -260,9 +340,9 @@ attn_bwd_simt_kernel(BwdArgs a, const int4* __restrict__ items, const int* __res
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int r = ty * MI + i;
-      if (r >= it.y) continue;
-      T* o2 = (KV ? static_cast<T*>(a.dk) + (it.x + r) * a.lddk : static_cast<T*>(a.dq) + (it.x + r) * a.lddq) + col;
-      T* o1 = KV ? static_cast<T*>(a.dv) + (it.x + r) * a.lddv + col : nullptr;
+      if (r >= it.rows) continue;
+      T* o2 = (KV ? static_cast<T*>(a.dk) + (it.row0 + r) * a.lddk : static_cast<T*>(a.dq) + (it.row0 + r) * a.lddq) + col;
+      T* o1 = KV ? static_cast<T*>(a.dv) + (it.row0 + r) * a.lddv + col : nullptr;
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
         const int c = tx * 4 + 64 * (j / 4) + j % 4;
@@ -275,23 +355,244 @@ attn_bwd_simt_kernel(BwdArgs a, const int4* __restrict__ items, const int* __res
   }
 }
 
+// ------------------------------------------------------------------ tensor cores (mma.sync), heads of 32, 64, 128 in 16 bits
+// The same walk as the 32-bit tile kernels, a block of four warps per 64 own rows: a warp's 16 rows r are the M rows of every
+// product, so S and dP come out as accumulators, become P and dS in registers and are at once the A operands of the products
+// with the other side's rows (no shared-memory round trip):
+//     S = A_own A_c^T,  dP = B_own B_c^T        (B operands: rows of the other side's tiles)
+//     acc1 += P B_c,    acc2 += dS A_c          (B operands: the same tiles, transposed by ldmatrix)
+// Other side's tiles of 64 rows come double-buffered through cp.async.  P and dS are rounded to the 16-bit type for the products
+// (as the forward pass rounds P); all sums are fp32.
+constexpr int kMmaThreads = 128, kMmaTile = 64;
+
+template <typename T, int D>
+__device__ __forceinline__ void load_tile_zfill(uint32_t dst, const T* __restrict__ g, int64_t ld, int rows) {
+  constexpr int kChunks = D / 8;
+#pragma unroll
+  for (int i = 0; i < kMmaTile * kChunks / kMmaThreads; ++i) {
+    const int idx = threadIdx.x + i * kMmaThreads;
+    const int r = idx / kChunks, c = idx % kChunks;
+    const bool ok = r < rows;
+    cp_async_16_zfill(dst + tile_off<D>(r, c), g + (int64_t)(ok ? r : 0) * ld + c * 8, ok ? 16u : 0u);
+  }
+}
+
+template <int D>
+constexpr int bwd_mma_smem() { return 6 * kMmaTile * D * 2 + 4 * kMmaTile * 4; }
+
+template <typename T, int D, bool KV>
+__device__ __forceinline__ void bwd_mma_tile(const BwdArgs& a, const Item& it, int h, uint8_t* smem) {
+  constexpr int KS = D / 16, NO = D / 8;
+  constexpr int CW = D <= 64 ? 64 : 32;  // other rows whose S and dP are in registers at a time
+  constexpr bool kKeep = D <= 64;        // own fragments in registers, or read again from shared memory
+  constexpr uint32_t kBytes = kMmaTile * D * 2;
+  const uint32_t s_own_a = (uint32_t)__cvta_generic_to_shared(smem), s_own_b = s_own_a + kBytes, s_oth = s_own_b + kBytes;
+  float* s_lse = reinterpret_cast<float*>(smem + 6 * kBytes);  // [2][64]
+  float* s_delta = s_lse + 2 * kMmaTile;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t E = (int64_t)a.H * D, col = (int64_t)h * D;
+  const T* ga = (KV ? static_cast<const T*>(a.k) + it.row0 * a.ldk : static_cast<const T*>(a.q) + it.row0 * a.ldq) + col;
+  const T* gb = (KV ? static_cast<const T*>(a.v) + it.row0 * a.ldv : static_cast<const T*>(a.grad) + it.row0 * E) + col;
+  const T* oa = (KV ? static_cast<const T*>(a.q) + it.other * a.ldq : static_cast<const T*>(a.k) + it.other * a.ldk) + col;
+  const T* ob = (KV ? static_cast<const T*>(a.grad) + it.other * E : static_cast<const T*>(a.v) + it.other * a.ldv) + col;
+  const int64_t ld_oa = KV ? a.ldq : a.ldk, ld_ob = KV ? E : a.ldv;
+  const float* g_lse = a.lse + (int64_t)h * a.q_tokens;
+  const float* g_delta = a.delta + (int64_t)h * a.q_tokens;
+  const float gs = grad_scale(a, it.seq, h);
+  const float scale = a.scaling * kLog2e;
+  const int n_tiles = (it.n_other + kMmaTile - 1) / kMmaTile;
+  auto load_other = [&](int j) {
+    const int st = j & 1, n = it.n_other - j * kMmaTile;
+    load_tile_zfill<T, D>(s_oth + st * 2 * kBytes, oa + (int64_t)j * kMmaTile * ld_oa, ld_oa, n);
+    load_tile_zfill<T, D>(s_oth + st * 2 * kBytes + kBytes, ob + (int64_t)j * kMmaTile * ld_ob, ld_ob, n);
+    if (KV && threadIdx.x < kMmaTile) {
+      const bool ok = (int)threadIdx.x < n;
+      s_lse[st * kMmaTile + threadIdx.x] = ok ? g_lse[it.other + j * kMmaTile + threadIdx.x] : INFINITY;  // 2^(x - inf) = 0
+      s_delta[st * kMmaTile + threadIdx.x] = ok ? g_delta[it.other + j * kMmaTile + threadIdx.x] * gs : 0.0f;
+    }
+  };
+  if (n_tiles > 0) {
+    load_tile_zfill<T, D>(s_own_a, ga, KV ? a.ldk : a.ldq, it.rows);
+    load_tile_zfill<T, D>(s_own_b, gb, KV ? a.ldv : E, it.rows);
+    load_other(0);
+    cp_async_commit();
+  }
+  const int r0 = warp * 16 + (lane >> 2), r1 = r0 + 8;
+  float lse0 = INFINITY, lse1 = INFINITY, dl0 = 0.0f, dl1 = 0.0f;
+  if (!KV && n_tiles > 0) {
+    if (r0 < it.rows) lse0 = g_lse[it.row0 + r0], dl0 = g_delta[it.row0 + r0] * gs;
+    if (r1 < it.rows) lse1 = g_lse[it.row0 + r1], dl1 = g_delta[it.row0 + r1] * gs;
+  }
+  const bool active = warp * 16 < it.rows;
+  float acc1[KV ? NO : 1][4], acc2[NO][4];
+#pragma unroll
+  for (int i = 0; i < NO; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      acc2[i][j] = 0.0f;
+      if (KV) acc1[KV ? i : 0][j] = 0.0f;
+    }
+  uint32_t fa[kKeep ? KS : 1][4], fb[kKeep ? KS : 1][4];
+  for (int j = 0; j < n_tiles; ++j) {
+    if (j + 1 < n_tiles) {
+      load_other(j + 1);
+      cp_async_commit();
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncthreads();
+    if (active) {
+      const uint32_t ta = s_oth + (j & 1) * 2 * kBytes, tb = ta + kBytes;
+      const float* lse_c = s_lse + (j & 1) * kMmaTile;
+      const float* delta_c = s_delta + (j & 1) * kMmaTile;
+      const int nc = it.n_other - j * kMmaTile < kMmaTile ? it.n_other - j * kMmaTile : kMmaTile;
+      if (kKeep && j == 0) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          ldmatrix_x4(fa[kKeep ? ks : 0], s_own_a + tile_off<D>(warp * 16 + (lane & 15), ks * 2 + (lane >> 4)));
+          ldmatrix_x4(fb[kKeep ? ks : 0], s_own_b + tile_off<D>(warp * 16 + (lane & 15), ks * 2 + (lane >> 4)));
+        }
+      }
+#pragma unroll 1
+      for (int c0 = 0; c0 < nc; c0 += CW) {
+        const int groups = (nc - c0 + 15) / 16;  // of 16 other rows, CW / 16 at most
+        float s[CW / 8][4], dp[CW / 8][4];
+#pragma unroll
+        for (int i = 0; i < CW / 8; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[i][k] = dp[i][k] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t xa[4], xb[4];
+          if (!kKeep) {
+            ldmatrix_x4(xa, s_own_a + tile_off<D>(warp * 16 + (lane & 15), ks * 2 + (lane >> 4)));
+            ldmatrix_x4(xb, s_own_b + tile_off<D>(warp * 16 + (lane & 15), ks * 2 + (lane >> 4)));
+          }
+          const uint32_t(&ua)[4] = kKeep ? fa[kKeep ? ks : 0] : xa;
+          const uint32_t(&ub)[4] = kKeep ? fb[kKeep ? ks : 0] : xb;
+#pragma unroll
+          for (int np = 0; np < CW / 16; ++np) {
+            if (np < groups) {
+              uint32_t f[4];
+              const uint32_t off = tile_off<D>(c0 + np * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1));
+              ldmatrix_x4(f, ta + off);
+              MmaOp<T>::mma(s[np * 2], ua, f[0], f[1]);
+              MmaOp<T>::mma(s[np * 2 + 1], ua, f[2], f[3]);
+              ldmatrix_x4(f, tb + off);
+              MmaOp<T>::mma(dp[np * 2], ub, f[0], f[1]);
+              MmaOp<T>::mma(dp[np * 2 + 1], ub, f[2], f[3]);
+            }
+          }
+        }
+        uint32_t pf[CW / 16][4], df[CW / 16][4];  // P and dS as A fragments
+#pragma unroll
+        for (int nt = 0; nt < CW / 8; ++nt) {
+          const int c = c0 + nt * 8 + 2 * (lane & 3);
+          float p[4], ds[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float l = KV ? lse_c[c + (k & 1)] : (k < 2 ? lse0 : lse1);
+            const float dl = KV ? delta_c[c + (k & 1)] : (k < 2 ? dl0 : dl1);
+            p[k] = exp2f(fmaf(s[nt][k], scale, -l));
+            // a key past the end has no probability (its zeroed row scores 0); a query past the end has lse = inf
+            if (!KV && c + (k & 1) >= nc) p[k] = 0.0f;
+            ds[k] = p[k] * fmaf(dp[nt][k], gs, -dl);
+          }
+          pf[nt >> 1][(nt & 1) * 2] = MmaOp<T>::pack(p[0], p[1]);
+          pf[nt >> 1][(nt & 1) * 2 + 1] = MmaOp<T>::pack(p[2], p[3]);
+          df[nt >> 1][(nt & 1) * 2] = MmaOp<T>::pack(ds[0], ds[1]);
+          df[nt >> 1][(nt & 1) * 2 + 1] = MmaOp<T>::pack(ds[2], ds[3]);
+        }
+#pragma unroll
+        for (int ks = 0; ks < CW / 16; ++ks) {
+          if (ks < groups) {
+#pragma unroll
+            for (int np = 0; np < NO / 2; ++np) {
+              uint32_t f[4];
+              const uint32_t off = tile_off<D>(c0 + ks * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), np * 2 + (lane >> 4));
+              ldmatrix_x4_trans(f, ta + off);
+              MmaOp<T>::mma(acc2[np * 2], df[ks], f[0], f[1]);
+              MmaOp<T>::mma(acc2[np * 2 + 1], df[ks], f[2], f[3]);
+              if (KV) {
+                ldmatrix_x4_trans(f, tb + off);
+                MmaOp<T>::mma(acc1[KV ? np * 2 : 0], pf[ks], f[0], f[1]);
+                MmaOp<T>::mma(acc1[KV ? np * 2 + 1 : 0], pf[ks], f[2], f[3]);
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();  // this stage is refilled next
+  }
+  const float f2 = a.scaling / gs;
+  T* out2 = (KV ? static_cast<T*>(a.dk) + it.row0 * a.lddk : static_cast<T*>(a.dq) + it.row0 * a.lddq) + col;
+  T* out1 = KV ? static_cast<T*>(a.dv) + it.row0 * a.lddv + col : nullptr;
+  const int64_t ld2 = KV ? a.lddk : a.lddq;
+#pragma unroll
+  for (int nt = 0; nt < NO; ++nt) {
+    const int c = nt * 8 + 2 * (lane & 3);
+    if (r0 < it.rows) {
+      *reinterpret_cast<uint32_t*>(out2 + r0 * ld2 + c) = MmaOp<T>::pack(acc2[nt][0] * f2, acc2[nt][1] * f2);
+      if (KV) *reinterpret_cast<uint32_t*>(out1 + r0 * a.lddv + c) = MmaOp<T>::pack(acc1[KV ? nt : 0][0], acc1[KV ? nt : 0][1]);
+    }
+    if (r1 < it.rows) {
+      *reinterpret_cast<uint32_t*>(out2 + r1 * ld2 + c) = MmaOp<T>::pack(acc2[nt][2] * f2, acc2[nt][3] * f2);
+      if (KV) *reinterpret_cast<uint32_t*>(out1 + r1 * a.lddv + c) = MmaOp<T>::pack(acc1[KV ? nt : 0][2], acc1[KV ? nt : 0][3]);
+    }
+  }
+}
+
+// blocks [0, kv_blocks): dK and dV of a (key tile, head); the others dQ of a (query tile, head)
+template <typename T, int D>
+__global__ void __launch_bounds__(kMmaThreads) attn_bwd_mma_kernel(BwdArgs a, ListOut kv, ListOut qi, int64_t kv_blocks) {
+  extern __shared__ __align__(128) uint8_t mma_smem[];
+  const bool is_kv = (int64_t)blockIdx.x < kv_blocks;
+  const int64_t w = is_kv ? (int64_t)blockIdx.x : (int64_t)blockIdx.x - kv_blocks;
+  const int64_t i = w / a.H;
+  const int h = (int)(w - i * a.H);
+  if (i >= *(is_kv ? kv : qi).count) return;
+  if (is_kv) bwd_mma_tile<T, D, true>(a, decode<true>(a, kv.items[i]), h, mma_smem);
+  else bwd_mma_tile<T, D, false>(a, decode<false>(a, qi.items[i]), h, mma_smem);
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-int64_t item_capacity(int64_t batch, int64_t tokens) { return batch + tokens / 32 + 1; }  // tiles of 32 rows or more
+int64_t item_capacity(int64_t batch, int64_t tokens, int tile) { return batch + tokens / tile + 1; }
 
-// delta | count, KV items | count, Q items; every part on a 16-byte boundary
+// delta | largest |dO| | count, KV items | count, Q items; every part on a 16-byte boundary
 struct BwdWorkspace {
-  size_t delta, kv, q, bytes;
+  size_t delta, top, kv, q, bytes;
   BwdWorkspace(int64_t batch, int64_t q_tokens, int64_t k_tokens, int H) {
+    auto up = [](size_t v) { return (v + 15) / 16 * 16; };
     delta = 0;
-    kv = ((size_t)q_tokens * H * 4 + 15) / 16 * 16;
-    q = kv + 16 + sizeof(int4) * (size_t)item_capacity(batch, k_tokens);
-    bytes = q + 16 + sizeof(int4) * (size_t)item_capacity(batch, q_tokens);
+    top = up((size_t)q_tokens * H * 4);
+    kv = top + up((size_t)batch * H * 4);
+    q = kv + 16 + sizeof(int4) * (size_t)item_capacity(batch, k_tokens, 32);  // (tiles of 32 rows or more)
+    bytes = q + 16 + sizeof(int4) * (size_t)item_capacity(batch, q_tokens, 32);
   }
 };
 
+struct Lists {
+  ListOut kv, qi;
+  Lists(uint8_t* ws, const BwdWorkspace& at)
+      : kv{reinterpret_cast<int4*>(ws + at.kv + 16), reinterpret_cast<int*>(ws + at.kv)},
+        qi{reinterpret_cast<int4*>(ws + at.q + 16), reinterpret_cast<int*>(ws + at.q)} {}
+};
+
+template <typename T, bool VEC>
+int launch_prepare(const BwdArgs& a, int tile, const Lists& l, unsigned* top, cudaStream_t st) {
+  const int64_t blocks = 2 + ceil_div(a.q_tokens, kPrepThreads / 32);
+  if (blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
+  if (top != nullptr && cudaMemsetAsync(top, 0, (size_t)a.batch * a.H * 4, st) != cudaSuccess) return NTB200_LAUNCH_FAILED;
+  backward_prepare_kernel<T, VEC><<<(unsigned)blocks, kPrepThreads, 0, st>>>(a, tile, l.kv, l.qi, top);
+  return status_from_cuda(cudaGetLastError());
+}
+
 template <typename T, int BT, int DP>
-int launch_bwd_simt(const BwdArgs& a, int64_t k_tokens, uint8_t* ws, const BwdWorkspace& at, cudaStream_t st) {
+int launch_bwd_simt(const BwdArgs& a, int64_t k_tokens, const Lists& l, cudaStream_t st) {
   constexpr int kSmem = bwd_simt_smem<BT, DP>();
   static std::atomic<int> configured[kMaxDevices];
   if (!once_per_device(configured, [] {
@@ -299,34 +600,56 @@ int launch_bwd_simt(const BwdArgs& a, int64_t k_tokens, uint8_t* ws, const BwdWo
                cudaFuncSetAttribute(attn_bwd_simt_kernel<T, BT, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess;
       }))
     return NTB200_LAUNCH_FAILED;
-  int *n_kv = reinterpret_cast<int*>(ws + at.kv), *n_q = reinterpret_cast<int*>(ws + at.q);
-  int4 *kv = reinterpret_cast<int4*>(ws + at.kv + 16), *qi = reinterpret_cast<int4*>(ws + at.q + 16);
+  const int rc = launch_prepare<T, false>(a, BT, l, nullptr, st);
+  if (rc != NTB200_OK) return rc;
   const int per_sm = 227 * 1024 / (kSmem + 1024);
   auto grid = [&](int64_t tokens) {
-    const int64_t most = (a.batch + tokens / BT + 1) * a.H;
+    const int64_t most = item_capacity(a.batch, tokens, BT) * a.H;
     return (unsigned)(most < (int64_t)kNumSMs * per_sm ? most : (int64_t)kNumSMs * per_sm);
   };
-  if (k_tokens > 0) {
-    backward_items_kernel<<<1, kListThreads, 0, st>>>(a.offsets_k, a.row_elems_k, a.offsets_q, a.row_elems_q, a.batch, BT, kv, n_kv);
-    attn_bwd_simt_kernel<T, BT, DP, true><<<grid(k_tokens), 256, kSmem, st>>>(a, kv, n_kv);
-  }
-  if (a.q_tokens > 0) {
-    backward_items_kernel<<<1, kListThreads, 0, st>>>(a.offsets_q, a.row_elems_q, a.offsets_k, a.row_elems_k, a.batch, BT, qi, n_q);
-    attn_bwd_simt_kernel<T, BT, DP, false><<<grid(a.q_tokens), 256, kSmem, st>>>(a, qi, n_q);
-  }
+  if (k_tokens > 0) attn_bwd_simt_kernel<T, BT, DP, true><<<grid(k_tokens), 256, kSmem, st>>>(a, l.kv.items, l.kv.count);
+  if (a.q_tokens > 0) attn_bwd_simt_kernel<T, BT, DP, false><<<grid(a.q_tokens), 256, kSmem, st>>>(a, l.qi.items, l.qi.count);
+  return status_from_cuda(cudaGetLastError());
+}
+
+template <typename T, int D>
+int launch_bwd_mma(BwdArgs a, int64_t k_tokens, unsigned* top, const Lists& l, cudaStream_t st) {
+  constexpr int kSmem = bwd_mma_smem<D>();
+  static std::atomic<int> configured[kMaxDevices];
+  if (!once_per_device(configured, [] {
+        return cudaFuncSetAttribute(attn_bwd_mma_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess;
+      }))
+    return NTB200_LAUNCH_FAILED;
+  a.top = std::is_same<T, __half>::value ? top : nullptr;
+  const int rc = launch_prepare<T, true>(a, kMmaTile, l, const_cast<unsigned*>(a.top), st);
+  if (rc != NTB200_OK) return rc;
+  const int64_t kv_blocks = k_tokens > 0 ? item_capacity(a.batch, k_tokens, kMmaTile) * a.H : 0;
+  const int64_t q_blocks = a.q_tokens > 0 ? item_capacity(a.batch, a.q_tokens, kMmaTile) * a.H : 0;
+  if (kv_blocks + q_blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
+  attn_bwd_mma_kernel<T, D><<<(unsigned)(kv_blocks + q_blocks), kMmaThreads, kSmem, st>>>(a, l.kv, l.qi, kv_blocks);
   return status_from_cuda(cudaGetLastError());
 }
 
 template <typename T>
-int launch_bwd(const BwdArgs& a, int64_t k_tokens, uint8_t* ws, const BwdWorkspace& at, cudaStream_t st) {
-  if (a.q_tokens > 0 && k_tokens > 0) {
-    const int64_t blocks = ceil_div(a.q_tokens * a.H, 8);
-    if (blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
-    attn_delta_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(a);
+int launch_bwd(const BwdArgs& a, int64_t k_tokens, uint8_t* ws, const BwdWorkspace& at, int path, cudaStream_t st) {
+  const Lists l(ws, at);
+  if constexpr (!std::is_same<T, float>::value) {
+    const bool mma = (a.d == 32 || a.d == 64 || a.d == 128) && aligned16(a.grad) && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) &&
+                     aligned16(a.out) && aligned16(a.dq) && aligned16(a.dk) && aligned16(a.dv) && a.ldq % 8 == 0 && a.ldk % 8 == 0 &&
+                     a.ldv % 8 == 0 && a.lddq % 8 == 0 && a.lddk % 8 == 0 && a.lddv % 8 == 0;
+    if (path == 2 && !mma) return NTB200_UNSUPPORTED_SHAPE;
+    if (mma && path != 1) {
+      unsigned* top = reinterpret_cast<unsigned*>(ws + at.top);
+      if (a.d == 32) return launch_bwd_mma<T, 32>(a, k_tokens, top, l, st);
+      if (a.d == 64) return launch_bwd_mma<T, 64>(a, k_tokens, top, l, st);
+      return launch_bwd_mma<T, 128>(a, k_tokens, top, l, st);
+    }
+  } else if (path > 1) {
+    return NTB200_UNSUPPORTED_SHAPE;
   }
-  if (a.d <= 64) return launch_bwd_simt<T, 64, 64>(a, k_tokens, ws, at, st);
-  if (a.d <= 128) return launch_bwd_simt<T, 64, 128>(a, k_tokens, ws, at, st);
-  return launch_bwd_simt<T, 32, 256>(a, k_tokens, ws, at, st);
+  if (a.d <= 64) return launch_bwd_simt<T, 64, 64>(a, k_tokens, l, st);
+  if (a.d <= 128) return launch_bwd_simt<T, 64, 128>(a, k_tokens, l, st);
+  return launch_bwd_simt<T, 32, 256>(a, k_tokens, l, st);
 }
 
 }  // namespace
@@ -350,7 +673,7 @@ int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_
                                      int num_heads, int head_dim, int64_t max_len_q, int64_t max_len_k, float scaling, int dtype, int path,
                                      void* workspace, size_t workspace_bytes, void* stream) {
   if (batch < 0 || q_tokens < 0 || k_tokens < 0 || num_heads < 1 || head_dim < 1 || row_elems_q < 1 || row_elems_k < 1 || max_len_q < 0 ||
-      max_len_k < 0 || path < 0 || path > 1)
+      max_len_k < 0 || path < 0 || path > 2)
     return NTB200_INVALID_ARG;
   if (dtype != NTB200_F32 && dtype != NTB200_F16 && dtype != NTB200_BF16) return NTB200_UNSUPPORTED_DTYPE;
   if (head_dim > kMaxHeadDim) return NTB200_UNSUPPORTED_SHAPE;
@@ -365,14 +688,14 @@ int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_
   if (workspace_bytes < at.bytes) return NTB200_WORKSPACE_TOO_SMALL;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return NTB200_MISALIGNED;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const BwdArgs a = {grad_out, q, k, v, out, lse, reinterpret_cast<float*>(ws + at.delta), grad_q, grad_k, grad_v,
+  const BwdArgs a = {grad_out, q, k, v, out, lse, reinterpret_cast<float*>(ws + at.delta), nullptr, grad_q, grad_k, grad_v,
                      ldq, ldk, ldv, ld_grad_q, ld_grad_k, ld_grad_v, offsets_q, offsets_k, row_elems_q, row_elems_k,
                      batch, q_tokens, num_heads, head_dim, scaling};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case NTB200_F32: return launch_bwd<float>(a, k_tokens, ws, at, st);
-    case NTB200_F16: return launch_bwd<__half>(a, k_tokens, ws, at, st);
-    default: return launch_bwd<__nv_bfloat16>(a, k_tokens, ws, at, st);
+    case NTB200_F32: return launch_bwd<float>(a, k_tokens, ws, at, path, st);
+    case NTB200_F16: return launch_bwd<__half>(a, k_tokens, ws, at, path, st);
+    default: return launch_bwd<__nv_bfloat16>(a, k_tokens, ws, at, path, st);
   }
 }
 

@@ -111,8 +111,10 @@ def attention(q, k, v, g, lq, lk, heads, scaling):
         e_d = (G.abs() * (e_o + (u if half else W) * (O.abs() + e_o))).sum(2, keepdim=True) + (d + 2) * W * (G * O).abs().sum(2, keepdim=True)
         e_dp = (d + 2) * W * (G.abs() @ V.abs().transpose(1, 2))
         e_ds = e_p * (dP - D).abs() + P * (e_dp + e_d + 2 * W * (dP.abs() + D.abs()))
-        e_ds = e_ds + up * (dS.abs() + e_ds)
-        e_pr = e_p + up * (P + e_p)
+        # rounded for the products; below the type's normal range by half its smallest step, where dS is held relative to the
+        # power of two at or below the head's largest |dO| (at most that number times 2)
+        e_ds = e_ds + up * (dS.abs() + e_ds) + half * tiny(dt) * G.abs().amax((1, 2), keepdim=True) * 2
+        e_pr = e_p + up * (P + e_p) + half * tiny(dt)
         sc = abs(scaling)
         out = {"out": (O, e_o, rows), "dq": (scaling * (dS @ K), sc * (e_ds @ K.abs() + (m + 4) * W * (dS.abs() @ K.abs())), rows),
                "dk": (scaling * (dS.transpose(1, 2) @ Q), sc * (e_ds.transpose(1, 2) @ Q.abs() + (n + 4) * W * (dS.abs().transpose(1, 2) @ Q.abs())), cols),
