@@ -212,7 +212,7 @@ int ntb200_gemm_bias_act(const void* A, const void* W, const void* bias, const v
 
 /* Bit mask of device-side conditions recorded since the last call (0 = none): bounded waits of the tcgen05
  * kernels that ran out (projection GEMM: bit 0 TMA producer, bit 1 MMA issuer, bit 2 epilogue; attention:
- * the same roles in bits 8-10) and bit 16 = ntb200_embedding met an index outside [0, vocab) (that row
+ * the same roles in bits 8-10, its backward pass in bits 12-14) and bit 16 = ntb200_embedding met an index outside [0, vocab) (that row
  * was zero-filled); synchronises the device; negative on a CUDA error.  No counterpart in the reference. */
 int ntb200_device_error_flags(void);
 
@@ -391,7 +391,8 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
  * (zeros where the other side is empty); rows outside the sequences are left as they were.  The probabilities are computed
  * again from q, k and lse.
  *   path  0 = best available;  1 = the 32-bit tile kernels (any dtype and head_dim <= 256);  2 = mma.sync kernels (fp16 /
- *         bf16, head_dim 32 / 64 / 128, 16-byte aligned rows)                                (1, 2: for cross-checks)
+ *         bf16, head_dim 32 / 64 / 128, 16-byte aligned rows);  3 = tcgen05 kernel (the same with head_dim 64 / 128 and rows
+ *         on both sides)                                                                     (1-3: for cross-checks)
  * workspace: 16-byte aligned.
  */
 size_t ntb200_varlen_attention_backward_workspace_bytes(int64_t batch, int64_t q_tokens, int64_t k_tokens, int num_heads,

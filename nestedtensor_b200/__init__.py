@@ -33,7 +33,7 @@ del _os, _b, _o
 
 def device_error_flags():
     """Bit mask of device-side conditions recorded since the last call (0 = none): a bounded wait of a tcgen05
-    kernel that ran out (projection: bits 0-2, attention: bits 8-10; the affected output tiles were left unwritten)
+    kernel that ran out (projection: bits 0-2, attention: bits 8-10, its backward pass: bits 12-14; the affected output tiles were left unwritten)
     or an embedding index out of range (bit 16).  Synchronises the device.  The torch operators do not read it on
     every call; a caller that wants the check after each of them sets ``NTB200_CHECK_DEVICE_ERRORS=1``."""
     from . import _cabi

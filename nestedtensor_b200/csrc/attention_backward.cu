@@ -16,6 +16,7 @@
 
 #include <type_traits>
 
+#include "attention_backward.cuh"
 #include "attention_internal.cuh"
 #include "attention_tiny.cuh"
 #include "common.cuh"
@@ -23,52 +24,11 @@
 namespace ntb200 {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxHeadDim = 256;
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
-
-// What every kernel of the backward pass reads and writes; strides in elements, all matrices [tokens, H * d] at head 0.
-struct BwdArgs {
-  const void *grad, *q, *k, *v, *out;
-  const float* lse;  // [H, q_tokens]
-  float* delta;      // [H, q_tokens]: D
-  const unsigned* top;  // [batch, H]: bits of the largest |dO| of the sequence and head (fp16 kernels only, else NULL)
-  void *dq, *dk, *dv;
-  int64_t ldq, ldk, ldv, lddq, lddk, lddv;  // grad and out are contiguous: their stride is H * d
-  const int64_t *offsets_q, *offsets_k;
-  int64_t row_elems_q, row_elems_k;
-  int64_t batch, q_tokens;
-  int H, d;
-  float scaling;
-};
-
 // ------------------------------------------------------------------ work lists and D = rowsum(dO * O), one launch
-// items[i] = (first row of the tile, valid rows in it, sequence, tile number) for every `tile` rows of the own side (keys for
-// dK / dV, queries for dQ), longest other side first.  A sequence whose other side is empty keeps its items: their gradients
+// An item for every `tile` rows of the own side (keys for dK / dV, queries for dQ), longest other side first.  A sequence whose other side is empty keeps its items: their gradients
 // are zeros, written by a block that walks no tile at all.  One block.
 constexpr int kListBuckets = 32;
 constexpr int kPrepThreads = 256;
-
-struct ListOut {
-  int4* items;
-  int* count;
-};
 
 __device__ __forceinline__ void build_backward_items(const int64_t* __restrict__ offsets_own, int64_t row_elems_own,
                                                      const int64_t* __restrict__ offsets_other, int64_t row_elems_other, int64_t batch,
@@ -99,10 +59,11 @@ __device__ __forceinline__ void build_backward_items(const int64_t* __restrict__
     if (n <= 0) continue;
     const int tiles = (int)((n + tile - 1) / tile);
     const int pos = atomicAdd(&s_base[bucket(m)], tiles);  // (the order inside a bucket decides nothing but the schedule)
-    const int t0 = (int)(offsets_own[b] / row_elems_own);
+    const int t0 = (int)(offsets_own[b] / row_elems_own), o0 = (int)(offsets_other[b] / row_elems_other);
     for (int t = 0; t < tiles; ++t) {
       const int64_t rows = n - (int64_t)t * tile;
-      out.items[pos + t] = make_int4(t0 + t * tile, (int)(rows < tile ? rows : tile), (int)b, t);
+      out.items[pos + t] = make_int4(t0 + t * tile, (int)(rows < tile ? rows : tile), o0, (int)m);
+      out.seq[pos + t] = (int)b;
     }
   }
 }
@@ -164,38 +125,6 @@ backward_prepare_kernel(BwdArgs a, int tile, ListOut kv, ListOut qi, unsigned* _
   }
 }
 
-// One work item: a tile of the own side, and the other side of its sequence
-struct Item {
-  int64_t row0;   // first row of the tile
-  int rows;       // valid rows in it
-  int64_t other;  // first row of the other side
-  int n_other;    // and its length
-  int seq;
-};
-
-template <bool KV>
-__device__ __forceinline__ Item decode(const BwdArgs& a, const int4& w) {
-  Item it;
-  it.row0 = w.x;
-  it.rows = w.y;
-  it.seq = w.z;
-  const int64_t* off = KV ? a.offsets_q : a.offsets_k;
-  const int64_t re = KV ? a.row_elems_q : a.row_elems_k;
-  it.other = off[w.z] / re;
-  it.n_other = (int)(off[w.z + 1] / re - it.other);
-  return it;
-}
-
-// fp16 holds dS only between 2^-24 and 65504, while gradients come at any scale: dS is computed from dO times a power of two
-// that brings the largest |dO| of the sequence and head to [1, 2), and the product's sum is divided by it again (both exact).
-__device__ __forceinline__ float grad_scale(const BwdArgs& a, int seq, int h) {
-  if (a.top == nullptr) return 1.0f;
-  const int e = (int)(a.top[(int64_t)seq * a.H + h] >> 23);  // biased exponent of a non-negative number
-  if (e == 0 || e == 255) return 1.0f;                       // zeros; Inf or NaN, which no factor mends
-  const int f = 254 - e;                                     // 2^(127 - e)
-  return __uint_as_float((unsigned)(f < 27 ? 27 : (f > 227 ? 227 : f)) << 23);
-}
-
 // ------------------------------------------------------------------ tiles in 32 bits, any type and head size
 // One block owns BT rows r of one side and walks the other side's rows c in tiles of BT:
 //     KV:  r = keys,    A_own = K, B_own = V;   c = queries, A = Q, B = dO:   dV_r += P_cr dO_c,  dK_r += dS_cr Q_c
@@ -232,7 +161,7 @@ attn_bwd_simt_kernel(BwdArgs a, const int4* __restrict__ items, const int* __res
   const float scale = a.scaling * kLog2e;
   const int d4 = (a.d + 3) & ~3;
   for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
-    const Item it = decode<KV>(a, items[w / a.H]);
+    const Item it = decode(items[w / a.H]);
     const int h = (int)(w % a.H);
     const int64_t col = (int64_t)h * a.d;
     const T* ga_own = (KV ? static_cast<const T*>(a.k) + it.row0 * a.ldk : static_cast<const T*>(a.q) + it.row0 * a.ldq) + col;
@@ -381,7 +310,7 @@ template <int D>
 constexpr int bwd_mma_smem() { return 6 * kMmaTile * D * 2 + 4 * kMmaTile * 4; }
 
 template <typename T, int D, bool KV>
-__device__ __forceinline__ void bwd_mma_tile(const BwdArgs& a, const Item& it, int h, uint8_t* smem) {
+__device__ __forceinline__ void bwd_mma_tile(const BwdArgs& a, const Item& it, float gs, int h, uint8_t* smem) {
   constexpr int KS = D / 16, NO = D / 8;
   constexpr int CW = D <= 64 ? 64 : 32;  // other rows whose S and dP are in registers at a time
   constexpr bool kKeep = D <= 64;        // own fragments in registers, or read again from shared memory
@@ -398,7 +327,6 @@ __device__ __forceinline__ void bwd_mma_tile(const BwdArgs& a, const Item& it, i
   const int64_t ld_oa = KV ? a.ldq : a.ldk, ld_ob = KV ? E : a.ldv;
   const float* g_lse = a.lse + (int64_t)h * a.q_tokens;
   const float* g_delta = a.delta + (int64_t)h * a.q_tokens;
-  const float gs = grad_scale(a, it.seq, h);
   const float scale = a.scaling * kLog2e;
   const int n_tiles = (it.n_other + kMmaTile - 1) / kMmaTile;
   auto load_other = [&](int j) {
@@ -553,8 +481,8 @@ __global__ void __launch_bounds__(kMmaThreads) attn_bwd_mma_kernel(BwdArgs a, Li
   const int64_t i = w / a.H;
   const int h = (int)(w - i * a.H);
   if (i >= *(is_kv ? kv : qi).count) return;
-  if (is_kv) bwd_mma_tile<T, D, true>(a, decode<true>(a, kv.items[i]), h, mma_smem);
-  else bwd_mma_tile<T, D, false>(a, decode<false>(a, qi.items[i]), h, mma_smem);
+  if (is_kv) bwd_mma_tile<T, D, true>(a, decode(kv.items[i]), grad_scale(a, kv.seq, i, h), h, mma_smem);
+  else bwd_mma_tile<T, D, false>(a, decode(qi.items[i]), grad_scale(a, qi.seq, i, h), h, mma_smem);
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -562,24 +490,27 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 int64_t item_capacity(int64_t batch, int64_t tokens, int tile) { return batch + tokens / tile + 1; }
 
-// delta | largest |dO| | count, KV items | count, Q items; every part on a 16-byte boundary
+// delta | largest |dO| | count, KV items, their sequences | count, Q items, their sequences; every part on a 16-byte boundary
 struct BwdWorkspace {
-  size_t delta, top, kv, q, bytes;
+  size_t delta, top, kv, kv_seq, q, q_seq, bytes;
   BwdWorkspace(int64_t batch, int64_t q_tokens, int64_t k_tokens, int H) {
     auto up = [](size_t v) { return (v + 15) / 16 * 16; };
+    const size_t nk = (size_t)item_capacity(batch, k_tokens, 32), nq = (size_t)item_capacity(batch, q_tokens, 32);  // (tiles of 32 rows or more)
     delta = 0;
     top = up((size_t)q_tokens * H * 4);
     kv = top + up((size_t)batch * H * 4);
-    q = kv + 16 + sizeof(int4) * (size_t)item_capacity(batch, k_tokens, 32);  // (tiles of 32 rows or more)
-    bytes = q + 16 + sizeof(int4) * (size_t)item_capacity(batch, q_tokens, 32);
+    kv_seq = kv + 16 + sizeof(int4) * nk;
+    q = kv_seq + up(4 * nk);
+    q_seq = q + 16 + sizeof(int4) * nq;
+    bytes = q_seq + up(4 * nq);
   }
 };
 
 struct Lists {
   ListOut kv, qi;
   Lists(uint8_t* ws, const BwdWorkspace& at)
-      : kv{reinterpret_cast<int4*>(ws + at.kv + 16), reinterpret_cast<int*>(ws + at.kv)},
-        qi{reinterpret_cast<int4*>(ws + at.q + 16), reinterpret_cast<int*>(ws + at.q)} {}
+      : kv{reinterpret_cast<int4*>(ws + at.kv + 16), reinterpret_cast<int*>(ws + at.kv_seq), reinterpret_cast<int*>(ws + at.kv)},
+        qi{reinterpret_cast<int4*>(ws + at.q + 16), reinterpret_cast<int*>(ws + at.q_seq), reinterpret_cast<int*>(ws + at.q)} {}
 };
 
 template <typename T, bool VEC>
@@ -631,13 +562,25 @@ int launch_bwd_mma(BwdArgs a, int64_t k_tokens, unsigned* top, const Lists& l, c
 }
 
 template <typename T>
+int launch_bwd_tcgen05(BwdArgs a, int64_t k_tokens, unsigned* top, int dtype, const Lists& l, cudaStream_t st) {
+  a.top = std::is_same<T, __half>::value ? top : nullptr;
+  const int rc = launch_prepare<T, true>(a, 128, l, const_cast<unsigned*>(a.top), st);
+  if (rc != NTB200_OK) return rc;
+  return attn_bwd_tcgen05_launch(a, k_tokens, dtype, l.kv, l.qi, item_capacity(a.batch, k_tokens, 128), item_capacity(a.batch, a.q_tokens, 128), st);
+}
+
+template <typename T>
 int launch_bwd(const BwdArgs& a, int64_t k_tokens, uint8_t* ws, const BwdWorkspace& at, int path, cudaStream_t st) {
   const Lists l(ws, at);
   if constexpr (!std::is_same<T, float>::value) {
     const bool mma = (a.d == 32 || a.d == 64 || a.d == 128) && aligned16(a.grad) && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) &&
                      aligned16(a.out) && aligned16(a.dq) && aligned16(a.dk) && aligned16(a.dv) && a.ldq % 8 == 0 && a.ldk % 8 == 0 &&
                      a.ldv % 8 == 0 && a.lddq % 8 == 0 && a.lddk % 8 == 0 && a.lddv % 8 == 0;
-    if (path == 2 && !mma) return NTB200_UNSUPPORTED_SHAPE;
+    if (path >= 2 && !mma) return NTB200_UNSUPPORTED_SHAPE;
+    constexpr int dtype = std::is_same<T, __half>::value ? NTB200_F16 : NTB200_BF16;
+    const bool tc = mma && a.d >= 64 && attn_bwd_tcgen05_supported(a, k_tokens, dtype);
+    if (path == 3 && !tc) return NTB200_UNSUPPORTED_SHAPE;
+    if (tc && (path == 3 || path == 0)) return launch_bwd_tcgen05<T>(a, k_tokens, reinterpret_cast<unsigned*>(ws + at.top), dtype, l, st);
     if (mma && path != 1) {
       unsigned* top = reinterpret_cast<unsigned*>(ws + at.top);
       if (a.d == 32) return launch_bwd_mma<T, 32>(a, k_tokens, top, l, st);
@@ -673,7 +616,7 @@ int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_
                                      int num_heads, int head_dim, int64_t max_len_q, int64_t max_len_k, float scaling, int dtype, int path,
                                      void* workspace, size_t workspace_bytes, void* stream) {
   if (batch < 0 || q_tokens < 0 || k_tokens < 0 || num_heads < 1 || head_dim < 1 || row_elems_q < 1 || row_elems_k < 1 || max_len_q < 0 ||
-      max_len_k < 0 || path < 0 || path > 2)
+      max_len_k < 0 || path < 0 || path > 3)
     return NTB200_INVALID_ARG;
   if (dtype != NTB200_F32 && dtype != NTB200_F16 && dtype != NTB200_BF16) return NTB200_UNSUPPORTED_DTYPE;
   if (head_dim > kMaxHeadDim) return NTB200_UNSUPPORTED_SHAPE;

@@ -29,6 +29,7 @@ int attn_tcgen05_cross_launch(const void* q, int64_t ldq, const void* k, int64_t
                               const AttnRows& rows, int64_t batch, int64_t q_tokens, int64_t k_tokens, int H, float scaling, int dtype,
                               void* workspace, cudaStream_t st);
 int attn_tcgen05_error_flags_read_and_clear();
+int attn_bwd_tcgen05_error_flags_read_and_clear();  // attention_backward_tcgen05.cu
 int construct_error_flags_read_and_clear();  // construct.cu: bit 0 = embedding index out of range
 
 }  // namespace ntb200

@@ -22,6 +22,7 @@
 #include <type_traits>
 
 #include "attention_internal.cuh"
+#include "attention_tc.cuh"
 #include "attention_tiny.cuh"
 #include "common.cuh"
 #include "sm100_ptx.cuh"
@@ -72,29 +73,6 @@ struct Ctrl {
 };
 
 static_assert(sizeof(Ctrl) <= 256, "control block exceeds its shared-memory slot");
-
-__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  if (ptx::mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = ptx::globaltimer_ns();
-  while (true) {
-#pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-      if (ptx::mbar_try_wait_suspend(bar, parity, 20000u)) return true;
-    if (*abort_flag) return false;
-    if (ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) return false;
-  }
-}
-
-template <int FMT>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if (FMT == 0) {
-    __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  } else {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
-}
 
 // ------------------------------------------------------------------ work list
 // items[i] = (first query token of the tile, valid query rows in the tile, first key token of the sequence, number
@@ -643,40 +621,6 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     ptx::tc_fence_after_sync();
     ptx::tmem_dealloc(tmem_base, kTmemCols);
   }
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
-  return fn;
-}
-
-// One source of 128-row x 64-column tiles: a row-major [rows, cols] two-byte matrix with row stride `ld` elements.
-struct TileSource {
-  const void* base;
-  int64_t rows, cols, ld;
-};
-
-bool make_tile_map(CUtensorMap* map, const TileSource& src, int dtype) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (fn == nullptr) return false;
-  const cuuint64_t gdim[2] = {(cuuint64_t)src.cols, (cuuint64_t)src.rows};
-  const cuuint64_t gstride[1] = {(cuuint64_t)(src.ld * 2)};
-  const cuuint32_t box[2] = {(cuuint32_t)kHD, (cuuint32_t)kQT};
-  const cuuint32_t estr[2] = {1, 1};
-  const CUtensorMapDataType dt = dtype == NTB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return fn(map, dt, 2, const_cast<void*>(src.base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int FMT, bool STATS>

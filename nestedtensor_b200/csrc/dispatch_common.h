@@ -29,7 +29,7 @@ using at::Tensor;
   if (!enabled) return;
   const int flags = ntb200_device_error_flags();
   TORCH_CHECK(flags == 0, "nestedtensor_b200: ", op, ": device error flags 0x", std::hex, flags,
-              " (bits 0-2 projection, 8-10 attention: a bounded device-side wait ran out; bit 16: embedding index out of range)");
+              " (bits 0-2 projection, 8-10 attention, 12-14 attention backward: a bounded device-side wait ran out; bit 16: embedding index out of range)");
 }
 
 [[maybe_unused]] void* cur_stream() { return static_cast<void*>(at::cuda::getCurrentCUDAStream().stream()); }

@@ -920,8 +920,9 @@ int ntb200_device_error_flags(void) {
   const int g = gemm_error_flags_read_and_clear();
   const int a = attn_tcgen05_error_flags_read_and_clear();
   const int c = construct_error_flags_read_and_clear();
-  if (g < 0 || a < 0 || c < 0) return -1;
-  return g | (a << 8) | (c << 16);
+  const int b = attn_bwd_tcgen05_error_flags_read_and_clear();
+  if (g < 0 || a < 0 || c < 0 || b < 0) return -1;
+  return g | (a << 8) | (b << 12) | (c << 16);
 }
 
 }  // extern "C"

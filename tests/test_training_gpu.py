@@ -7,6 +7,8 @@ import torch
 
 import nestedtensor_b200 as nt
 import _training_reference as ref
+from _helpers import stream_ptr
+from nestedtensor_b200 import _cabi
 from nestedtensor_b200.nn import training
 
 pytestmark = pytest.mark.gpu
@@ -254,6 +256,46 @@ def test_attention_large_logits_and_gradients(cuda_device, dtype):
         gs = (g.float() * factor).to(dtype)
         want, bound = ref.attention(q, k, v, gs, lengths, lengths, 2, scaling)
         _check(_run_self(q, k, v, gs, qs, 2, scaling), want, bound, "scaling %g, gradients times %g" % (scaling, factor))
+
+
+def _cabi_backward(q, k, v, g, lq, lk, heads, path, ld_extra=0):
+    """Forward with row statistics and backward through the C ABI on one path, token offsets, gradients in wider rows."""
+    lib, E, d = _cabi.load(), q.size(1), q.size(1) // heads
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[q.dtype]
+    off = [torch.tensor([0] + list(torch.tensor(n).cumsum(0))).cuda() for n in (lq, lk)]
+    out, lse = torch.empty_like(q), torch.empty(heads, q.size(0), device="cuda")
+    B, Tq, Tk, scaling = len(lq), q.size(0), k.size(0), d ** -0.5
+    n = lib.ntb200_varlen_cross_attention_workspace_bytes(B, Tq, heads, d, code)
+    ws = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
+    _cabi.check("train", lib.ntb200_varlen_attention_train(
+        q.data_ptr(), E, k.data_ptr(), E, v.data_ptr(), E, out.data_ptr(), lse.data_ptr(), off[0].data_ptr(), 1, off[1].data_ptr(), 1, B, Tq, Tk,
+        heads, d, max(lq), scaling, code, path if path < 3 or d == 64 else 2, ws.data_ptr(), n, stream_ptr()))
+    n = lib.ntb200_varlen_attention_backward_workspace_bytes(B, Tq, Tk, heads, d, code)
+    ws = torch.full((n + 64,), 0xAB, dtype=torch.uint8, device="cuda")
+    wide = E + ld_extra
+    grads = [torch.full((t.size(0) + 3, wide), 7.0, dtype=q.dtype, device="cuda") for t in (q, k, v)]
+    _cabi.check("backward", lib.ntb200_varlen_attention_backward(
+        g.data_ptr(), q.data_ptr(), E, k.data_ptr(), E, v.data_ptr(), E, out.data_ptr(), lse.data_ptr(), grads[0].data_ptr(), wide,
+        grads[1].data_ptr(), wide, grads[2].data_ptr(), wide, off[0].data_ptr(), 1, off[1].data_ptr(), 1, B, Tq, Tk, heads, d, max(lq), max(lk),
+        scaling, code, path, ws.data_ptr(), n, stream_ptr()))
+    torch.cuda.synchronize()
+    assert bool((ws[n:] == 0xAB).all()), "workspace overrun"
+    for t in grads:  # rows behind the last sequence and columns beside the heads are left as they were
+        assert bool((t[-3:] == 7.0).all()) and bool((t[:, E:] == 7.0).all())
+    assert lib.ntb200_device_error_flags() == 0
+    return dict(zip(("out", "dq", "dk", "dv"), (out, *(t[:-3, :E] for t in grads))))
+
+
+@pytest.mark.parametrize("path,dtype,d", [(1, torch.float32, 64), (1, torch.bfloat16, 64), (1, torch.float16, 72), (2, torch.float16, 32),
+                                          (2, torch.bfloat16, 64), (2, torch.float16, 64), (2, torch.bfloat16, 128), (2, torch.float16, 128),
+                                          (3, torch.bfloat16, 64), (3, torch.float16, 64), (3, torch.bfloat16, 128), (3, torch.float16, 128)],
+                         ids=str)
+def test_attention_backward_paths(cuda_device, path, dtype, d):
+    nt.device_error_flags()
+    lq, lk = [1, 0, 64, 130, 300, 17], [5, 3, 0, 257, 129, 16]
+    q, k, v, g, _, _ = _attend_inputs(lq, lk, 2, d, dtype, path + d)
+    want, bound = ref.attention(q, k, v, g, lq, lk, 2, d ** -0.5)
+    _check(_cabi_backward(q, k, v, g, lq, lk, 2, path, 24), want, bound, "path %d" % path)
 
 
 @pytest.mark.parametrize("op", ["norm", "attend"])
