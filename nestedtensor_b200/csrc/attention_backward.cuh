@@ -69,12 +69,14 @@ __device__ __forceinline__ Item decode(const int4& w) { return {w.x, w.y, w.z, w
 
 // fp16 holds dS only between 2^-24 and 65504, while gradients come at any scale: dS is computed from dO times a power of two
 // that brings the largest |dO| of the sequence and head to [1, 2), and the product's sum is divided by it again (both exact).
-__device__ __forceinline__ float grad_scale(const BwdArgs& a, const int* __restrict__ seq, int64_t i, int h) {
-  if (a.top == nullptr) return 1.0f;
-  const int e = (int)(a.top[(int64_t)seq[i] * a.H + h] >> 23);  // biased exponent of a non-negative number
-  if (e == 0 || e == 255) return 1.0f;                       // zeros; Inf or NaN, which no factor mends
-  const int f = 254 - e;                                     // 2^(127 - e)
+__device__ __forceinline__ float scale_of(unsigned top) {
+  const int e = (int)(top >> 23);       // biased exponent of a non-negative number
+  if (e == 0 || e == 255) return 1.0f;  // zeros; Inf or NaN, which no factor mends
+  const int f = 254 - e;                // 2^(127 - e)
   return __uint_as_float((unsigned)(f < 27 ? 27 : (f > 227 ? 227 : f)) << 23);
+}
+__device__ __forceinline__ float grad_scale(const BwdArgs& a, const int* __restrict__ seq, int64_t i, int h) {
+  return a.top == nullptr ? 1.0f : scale_of(a.top[(int64_t)seq[i] * a.H + h]);
 }
 
 }  // namespace

@@ -16,6 +16,8 @@
 // Tensor memory: S [0,128), dP [128,256), acc1 and acc2 from 256.  Heads of 64 leave room for P and dS of their own, so the next
 // tile's S and dP are computed while this tile's are still operands; at 128 P and dS take the columns of the S and dP chunks
 // they come from (a thread overwrites only what it has read itself), and the next S waits for this P's product.
+// Every step between the roles costs a warp some 150-200 cycles whether it waits or not, and eight warps hide little of that, so
+// a tile takes a softmax warp only two waits (S, dP) and two arrivals (P, dS): each commit also covers the product before it.
 // All barriers count tiles g of the CTA over its items.  Every wait is bounded: a wait that runs out sets an error flag, the
 // roles fall through and the CTA frees its tensor memory.
 
@@ -58,7 +60,7 @@ template <int D>
 struct Ctrl {
   uint64_t own_full[Cfg<D>::kOwn], own_empty[Cfg<D>::kOwn];
   uint64_t full[Cfg<D>::kStages], empty[Cfg<D>::kStages], aux[Cfg<D>::kStages];
-  uint64_t s_ready, s_free, p_ready, p_done, dp_ready, dp_free, ds_ready, ds_done, acc_free, done;
+  uint64_t s_ready, p_ready, p_done, dp_ready, ds_ready, ds_done, item_done, acc_free, done;
   uint32_t tmem_base;
   volatile int abort;
 };
@@ -96,13 +98,12 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       ptx::mbar_init(ptx::smem_u32(&ctrl->aux[s]), 2);  // both helper warps
     }
     ptx::mbar_init(ptx::smem_u32(&ctrl->s_ready), 1);
-    ptx::mbar_init(ptx::smem_u32(&ctrl->s_free), 8);
     ptx::mbar_init(ptx::smem_u32(&ctrl->p_ready), 8);
     ptx::mbar_init(ptx::smem_u32(&ctrl->p_done), 1);
     ptx::mbar_init(ptx::smem_u32(&ctrl->dp_ready), 1);
-    ptx::mbar_init(ptx::smem_u32(&ctrl->dp_free), 8);
     ptx::mbar_init(ptx::smem_u32(&ctrl->ds_ready), 8);
     ptx::mbar_init(ptx::smem_u32(&ctrl->ds_done), 1);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->item_done), 1);
     ptx::mbar_init(ptx::smem_u32(&ctrl->acc_free), 8);
     ptx::mbar_init(ptx::smem_u32(&ctrl->done), 1);
     ctrl->abort = 0;
@@ -272,31 +273,28 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
               }
             }
           };
-          if (C::kSep && more) {  // S of this tile is in registers: the next may overwrite it
-            if (!wait(&ctrl->s_free, g & 1) || !issue_s()) { ok = false; break; }
-          }
+          // p_ready: P is in place, and S has been read.  The commit behind the next S covers this product too, so that a warp that
+          // finds the next S ready may overwrite P; the same holds for dP and dS.
           if (!wait(&ctrl->aux[s], (g / C::kStages) & 1)) { ok = false; break; }
           if (j == 0 && n > 0 && !wait(&ctrl->acc_free, (n - 1) & 1)) { ok = false; break; }
           if (!wait(&ctrl->p_ready, g & 1)) { ok = false; break; }
           ptx::tc_fence_after_sync();
           if (kv) product(C::kAcc1, 1, true);
-          ptx::umma_commit(ptx::smem_u32(&ctrl->p_done));
-          if (!C::kSep && more) {  // the next S takes the columns of this P
-            if (!wait(&ctrl->p_done, g & 1) || !issue_s()) { ok = false; break; }
+          if (!C::kSep) {  // the next S takes the columns of this P
+            ptx::umma_commit(ptx::smem_u32(&ctrl->p_done));
+            if (more && !wait(&ctrl->p_done, g & 1)) { ok = false; break; }
           }
-          if (C::kSep && more) {
-            if (!wait(&ctrl->dp_free, g & 1)) { ok = false; break; }
-            issue_dp();
-          }
+          if (more && !issue_s()) { ok = false; break; }
           if (!wait(&ctrl->ds_ready, g & 1)) { ok = false; break; }
           ptx::tc_fence_after_sync();
           product(C::kAcc2, 0, false);
-          ptx::umma_commit(ptx::smem_u32(&ctrl->ds_done));
           ptx::umma_commit(ptx::smem_u32(&ctrl->empty[s]));
-          if (!C::kSep && more) {
-            if (!wait(&ctrl->ds_done, g & 1)) { ok = false; break; }
-            issue_dp();
+          if (j == nt - 1) ptx::umma_commit(ptx::smem_u32(&ctrl->item_done));
+          if (!C::kSep) {
+            ptx::umma_commit(ptx::smem_u32(&ctrl->ds_done));
+            if (more && !wait(&ctrl->ds_done, g & 1)) { ok = false; break; }
           }
+          if (more) issue_dp();
         }
         ++n;
       }
@@ -311,46 +309,70 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       const int me = warp - 10;
       bool ok = true;
       uint32_t g = 0;
-      int4 rec = fetch(blockIdx.x);
-      for (unsigned w = blockIdx.x; w < n_all && ok; w += gridDim.x) {
-        const Item it = decode(rec);
-        rec = fetch(w + gridDim.x);
-        const int nt = tiles_of(it);
-        const bool kv = w < n_kv;
-        const int h = head(w);
-        const float* src = (me == 0 ? a.lse : a.delta) + (int64_t)h * a.q_tokens + it.other;
-        const float f = me == 0 ? -1.0f : (kv && nt > 0 ? -grad_scale(a, t.kv.seq, w / H, h) : 0.0f);
-        for (int j = 0; j < nt; ++j, ++g) {
-          const uint32_t s = g % C::kStages;
-          int nc = it.n_other - j * kTR;
-          nc = nc > kTR ? kTR : nc;
-          float v[4];
-          if (kv) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int c = lane + 32 * k;
-              v[k] = c < nc ? src[j * kTR + c] * f : 0.0f;
-            }
-          }
-          if (!wait(&ctrl->full[s], (g / C::kStages) & 1)) {
-            ok = false;
-            break;
-          }
-          if (kv) {
-            float* dst = s_stats + s * (C::kStats / 4) + me * kTR;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) dst[lane + 32 * k] = v[k];
-          }
-          const int r_end = (nc + 15) & ~15;
-          for (int i = lane; i < (r_end - nc) * 8 * C::kHalves; i += 32) {
-            const int r = nc + i / (8 * C::kHalves), x = i % (8 * C::kHalves);
-            const uint32_t addr = s_oth + (s * 2 + me) * C::kTile + (x / 8) * kHalf + (r >> 3) * 1024 + (r & 7) * 128 + (x % 8) * 16;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0u) : "memory");
-          }
-          ptx::fence_proxy_async();  // the tensor core reads the cleared rows
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->aux[s]));
+      // cursor over the tiles, one ahead: its statistics are on the way while the current tile is waited for
+      unsigned w = blockIdx.x;
+      auto fetch_seq = [&](unsigned w) { return me == 1 && a.top != nullptr && w < n_kv ? __ldg(t.kv.seq + w / H) : 0; };
+      int4 rec = fetch(w), rec_next = fetch(w + gridDim.x);
+      int seq = fetch_seq(w), seq_next = fetch_seq(w + gridDim.x);
+      int j = 0, nt = 0;
+      unsigned top = 0;
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      Item it = decode(rec);
+      auto step = [&]() {
+        w += gridDim.x;
+        rec = rec_next, seq = seq_next;
+        rec_next = fetch(w + gridDim.x), seq_next = fetch_seq(w + gridDim.x);
+      };
+      auto open = [&]() {  // the next item that has tiles
+        for (; w < n_all; step()) {
+          it = decode(rec);
+          nt = tiles_of(it);
+          if (nt > 0) break;
         }
+        j = 0;
+        if (me == 1 && a.top != nullptr && w < n_kv) top = a.top[(int64_t)seq * H + head(w)];
+      };
+      auto load = [&]() {
+        if (w >= n_kv) return;
+        const float* src = (me == 0 ? a.lse : a.delta) + (int64_t)head(w) * a.q_tokens + it.other + j * kTR;
+        const int nc = it.n_other - j * kTR;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = lane + 32 * k < nc ? src[lane + 32 * k] : 0.0f;
+      };
+      open();
+      if (w < n_all) load();
+      while (w < n_all) {
+        const uint32_t s = g % C::kStages;
+        const bool kv = w < n_kv;
+        const unsigned top_c = top;
+        const float vc[4] = {v[0], v[1], v[2], v[3]};
+        int nc = it.n_other - j * kTR;
+        nc = nc > kTR ? kTR : nc;
+        if (++j == nt) {
+          step();
+          open();
+        }
+        if (w < n_all) load();
+        if (!wait(&ctrl->full[s], (g / C::kStages) & 1)) {
+          ok = false;
+          break;
+        }
+        if (kv) {
+          float* dst = s_stats + s * (C::kStats / 4) + me * kTR;
+          const float fc = me == 1 && a.top != nullptr ? -scale_of(top_c) : -1.0f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) dst[lane + 32 * k] = vc[k] * fc;
+        }
+        const int r_end = (nc + 15) & ~15;
+        for (int i = lane; i < (r_end - nc) * 8 * C::kHalves; i += 32) {
+          const int r = nc + i / (8 * C::kHalves), x = i % (8 * C::kHalves);
+          const uint32_t addr = s_oth + (s * 2 + me) * C::kTile + (x / 8) * kHalf + (r >> 3) * 1024 + (r & 7) * 128 + (x % 8) * 16;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0u) : "memory");
+        }
+        ptx::fence_proxy_async();  // the tensor core reads the cleared rows
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->aux[s]));
+        ++g;
       }
       if (!ok && lane == 0) {
         ctrl->abort = 1;
@@ -372,23 +394,142 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(bar));
     };
-    int4 rec = fetch(blockIdx.x);
+    // The gradients of an item are written during the first tile of the next one (its last product retires meanwhile).
+    struct Pending {
+      bool any, live;
+      T* out;
+      int rows, cols, acc;
+      float f;
+    } pend = {false, false, nullptr, 0, 0, 0, 0.0f};
+    auto write_out = [&](const Pending& o, bool zeros) {
+      for (int c = 0; c < o.cols; c += 32) {
+        uint32_t r[32];
+        if (!zeros) {
+          ptx::tmem_ld_32x32b_x32(tl + o.acc + c, r);
+          ptx::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0u;
+        }
+        if (row < o.rows) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 v;
+            v.x = pack2<FMT>(__uint_as_float(r[i]) * o.f, __uint_as_float(r[i + 1]) * o.f);
+            v.y = pack2<FMT>(__uint_as_float(r[i + 2]) * o.f, __uint_as_float(r[i + 3]) * o.f);
+            v.z = pack2<FMT>(__uint_as_float(r[i + 4]) * o.f, __uint_as_float(r[i + 5]) * o.f);
+            v.w = pack2<FMT>(__uint_as_float(r[i + 6]) * o.f, __uint_as_float(r[i + 7]) * o.f);
+            *reinterpret_cast<uint4*>(o.out + c + i) = v;
+          }
+        }
+      }
+    };
+    uint32_t n = 0;  // items with tiles whose gradients have been written
+    auto flush = [&]() {
+      if (!pend.any) return;
+      if (ok && !wait(&ctrl->item_done, n & 1)) ok = false;
+      ++n;
+      if (ok && pend.live) {
+        ptx::tc_fence_after_sync();
+        write_out(pend, false);
+      }
+      arrive(&ctrl->acc_free);
+      pend.any = false;
+    };
+    // P of this thread's (up to) 64 columns, 2^(scale S - lse); lse per column (KV items, from shared memory) or per row.  Columns
+    // past the end of the sequence have no probability, whatever was in their columns (cut in a loop of zero or one trips, so
+    // that whole chunks do not pay for the selects).
+    auto cut = [&](float (&x)[32], int c0, int nc) {
+#pragma unroll 1
+      for (int ragged = nc - c0 < 32 ? 1 : 0; ragged > 0; --ragged) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = c0 + i >= nc ? 0.0f : x[i];
+      }
+    };
+    auto exponentials = [&](auto is_kv, const uint32_t (&sv)[2][32], float (&p)[2][32], const float* stats, uint64_t nl, int nc) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int c0 = (wg + 2 * k) * 32;
+        if (c0 < nc) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            ulonglong2 n = make_ulonglong2(nl, nl);
+            if constexpr (decltype(is_kv)::value) n = *reinterpret_cast<const ulonglong2*>(stats + c0 + i);
+            const uint64_t x0 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[k][i]), __uint_as_float(sv[k][i + 1])), sc2, n.x);
+            const uint64_t x1 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[k][i + 2]), __uint_as_float(sv[k][i + 3])), sc2, n.y);
+            float e0, e1, e2, e3;
+            ptx::f32x2_unpack(x0, e0, e1);
+            ptx::f32x2_unpack(x1, e2, e3);
+            p[k][i] = ptx::ex2_approx(e0);
+            p[k][i + 1] = ptx::ex2_approx(e1);
+            p[k][i + 2] = ptx::ex2_approx(e2);
+            p[k][i + 3] = ptx::ex2_approx(e3);
+          }
+          cut(p[k], c0, nc);
+        }
+      }
+    };
+    // dS = P (gs dP - gs D), over P, and to tensor memory
+    auto products = [&](auto is_kv, const uint32_t (&sv)[2][32], float (&p)[2][32], const float* stats, uint64_t nd, uint64_t gs2, int nc) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int c0 = (wg + 2 * k) * 32;
+        if (c0 < nc) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            ulonglong2 n = make_ulonglong2(nd, nd);
+            if constexpr (decltype(is_kv)::value) n = *reinterpret_cast<const ulonglong2*>(stats + c0 + i);
+            const uint64_t x0 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[k][i]), __uint_as_float(sv[k][i + 1])), gs2, n.x);
+            const uint64_t x1 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[k][i + 2]), __uint_as_float(sv[k][i + 3])), gs2, n.y);
+            ptx::f32x2_unpack(ptx::f32x2_mul(ptx::f32x2_pack(p[k][i], p[k][i + 1]), x0), p[k][i], p[k][i + 1]);
+            ptx::f32x2_unpack(ptx::f32x2_mul(ptx::f32x2_pack(p[k][i + 2], p[k][i + 3]), x1), p[k][i + 2], p[k][i + 3]);
+          }
+          cut(p[k], c0, nc);
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pk[i] = pack2<FMT>(p[k][2 * i], p[k][2 * i + 1]);
+          ptx::tmem_st_32x32b_x16(tl + C::ds_col(wg + 2 * k), pk);
+        }
+      }
+    };
+    // what an item needs from memory is fetched one item ahead (its record two)
+    struct Ahead {
+      int4 rec;
+      unsigned top;    // bits of the largest |dO| (fp16)
+      float lse, delta;  // of this row (Q items)
+    };
+    auto fetch_seq = [&](unsigned w) {
+      if (a.top == nullptr || w >= n_all) return 0;
+      return __ldg(w < n_kv ? t.kv.seq + w / H : t.qi.seq + (w - n_kv) / H);
+    };
+    auto look = [&](unsigned w, const int4& r, int seq) {
+      Ahead x = {r, 0u, 0.0f, 0.0f};
+      if (w >= n_all) return x;
+      if (a.top != nullptr) x.top = a.top[(int64_t)seq * H + head(w)];
+      if (w >= n_kv && row < r.y && r.w > 0) {
+        const int64_t i = (int64_t)head(w) * a.q_tokens + r.x + row;
+        x.lse = a.lse[i];
+        x.delta = a.delta[i];
+      }
+      return x;
+    };
+    int4 rec = fetch(blockIdx.x), rec2 = fetch(blockIdx.x + gridDim.x);
+    int seq2 = fetch_seq(blockIdx.x + gridDim.x);
+    Ahead next = look(blockIdx.x, rec, fetch_seq(blockIdx.x));
     for (unsigned w = blockIdx.x; w < n_all; w += gridDim.x) {
-      const Item it = decode(rec);
-      rec = fetch(w + gridDim.x);
+      const Ahead cur = next;
+      next = look(w + gridDim.x, rec2, seq2);
+      rec2 = fetch(w + 2 * gridDim.x);
+      seq2 = fetch_seq(w + 2 * gridDim.x);
+      const Item it = decode(cur.rec);
       const bool kv = w < n_kv;
       const int h = head(w);
       const int nt = tiles_of(it);
       const bool live = q * 32 < it.rows;  // warp-uniform: this warp owns valid rows
-      const float gs = grad_scale(a, kv ? t.kv.seq : t.qi.seq, (kv ? w : w - n_kv) / H, h);
+      const float gs = a.top != nullptr ? scale_of(cur.top) : 1.0f;
       const uint64_t gs2 = ptx::f32x2_pack(gs, gs);
-      uint64_t nl2 = 0, nd2 = 0;  // -lse and -D of this row (Q items)
-      if (!kv && nt > 0 && row < it.rows) {
-        const int64_t i = (int64_t)h * a.q_tokens + it.row0 + row;
-        const float nl = -a.lse[i], nd = -a.delta[i] * gs;
-        nl2 = ptx::f32x2_pack(nl, nl);
-        nd2 = ptx::f32x2_pack(nd, nd);
-      }
+      const uint64_t nl2 = ptx::f32x2_pack(-cur.lse, -cur.lse);  // (Q items)
+      const uint64_t nd2 = ptx::f32x2_pack(-cur.delta * gs, -cur.delta * gs);
       for (int j = 0; j < nt; ++j, ++g) {
         const uint32_t s = g % C::kStages;
         int nc = it.n_other - j * kTR;
@@ -406,57 +547,24 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             if ((wg + 2 * k) * 32 < nc) ptx::tmem_ld_32x32b_x32(tl + (wg + 2 * k) * 32, sv[k]);
           ptx::tmem_ld_wait();
         }
-        arrive(&ctrl->s_free);
         if (ok && live) {
+          if (kv) exponentials(std::true_type{}, sv, p, stats, 0, nc);
+          else exponentials(std::false_type{}, sv, p, nullptr, nl2, nc);
+        }
+        if (ok && live && kv) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const int c0 = (wg + 2 * k) * 32;
-            if (c0 < nc) {
+            if ((wg + 2 * k) * 32 < nc) {
+              uint32_t pk[16];
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                uint64_t n0 = nl2, n1 = nl2;
-                if (kv) {
-                  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(stats + c0 + i);
-                  n0 = v.x, n1 = v.y;
-                }
-                const uint64_t x0 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[k][i]), __uint_as_float(sv[k][i + 1])), sc2, n0);
-                const uint64_t x1 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[k][i + 2]), __uint_as_float(sv[k][i + 3])), sc2, n1);
-                float e0, e1, e2, e3;
-                ptx::f32x2_unpack(x0, e0, e1);
-                ptx::f32x2_unpack(x1, e2, e3);
-                p[k][i] = ptx::ex2_approx(e0);
-                p[k][i + 1] = ptx::ex2_approx(e1);
-                p[k][i + 2] = ptx::ex2_approx(e2);
-                p[k][i + 3] = ptx::ex2_approx(e3);
-              }
-              // columns past the end of the sequence: no probability, whatever was there (a loop of zero or one trips, so that
-              // whole chunks do not pay for the selects)
-#pragma unroll 1
-              for (int ragged = nc - c0 < 32 ? 1 : 0; ragged > 0; --ragged) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) p[k][i] = c0 + i >= nc ? 0.0f : p[k][i];
-              }
+              for (int i = 0; i < 16; ++i) pk[i] = pack2<FMT>(p[k][2 * i], p[k][2 * i + 1]);
+              ptx::tmem_st_32x32b_x16(tl + C::p_col(wg + 2 * k), pk);
             }
           }
-        }
-        if (kv) {
-          // the product with the previous P must have read these columns
-          if (C::kSep && ok && g > 0 && !wait(&ctrl->p_done, (g - 1) & 1)) ok = false;
-          if (ok && live) {
-            ptx::tc_fence_after_sync();
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              if ((wg + 2 * k) * 32 < nc) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) pk[i] = pack2<FMT>(p[k][2 * i], p[k][2 * i + 1]);
-                ptx::tmem_st_32x32b_x16(tl + C::p_col(wg + 2 * k), pk);
-              }
-            }
-            ptx::tmem_st_wait();
-          }
+          ptx::tmem_st_wait();
         }
         arrive(&ctrl->p_ready);
+        if (j == 0) flush();
         // ---- dS
         if (ok && !wait(&ctrl->dp_ready, g & 1)) ok = false;
         if (ok && live) {
@@ -465,79 +573,27 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           for (int k = 0; k < 2; ++k)
             if ((wg + 2 * k) * 32 < nc) ptx::tmem_ld_32x32b_x32(tl + 128 + (wg + 2 * k) * 32, sv[k]);
           ptx::tmem_ld_wait();
-        }
-        arrive(&ctrl->dp_free);
-        if (C::kSep && ok && g > 0 && !wait(&ctrl->ds_done, (g - 1) & 1)) ok = false;
-        if (ok && live) {
-          ptx::tc_fence_after_sync();
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int c0 = (wg + 2 * k) * 32;
-            if (c0 < nc) {
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                uint64_t n0 = nd2, n1 = nd2;
-                if (kv) {
-                  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(stats + kTR + c0 + i);
-                  n0 = v.x, n1 = v.y;
-                }
-                const uint64_t x0 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[k][i]), __uint_as_float(sv[k][i + 1])), gs2, n0);
-                const uint64_t x1 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[k][i + 2]), __uint_as_float(sv[k][i + 3])), gs2, n1);
-                const uint64_t y0 = ptx::f32x2_mul(ptx::f32x2_pack(p[k][i], p[k][i + 1]), x0);
-                const uint64_t y1 = ptx::f32x2_mul(ptx::f32x2_pack(p[k][i + 2], p[k][i + 3]), x1);
-                ptx::f32x2_unpack(y0, p[k][i], p[k][i + 1]);
-                ptx::f32x2_unpack(y1, p[k][i + 2], p[k][i + 3]);
-              }
-#pragma unroll 1
-              for (int ragged = nc - c0 < 32 ? 1 : 0; ragged > 0; --ragged) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) p[k][i] = c0 + i >= nc ? 0.0f : p[k][i];
-              }
-              uint32_t pk[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) pk[i] = pack2<FMT>(p[k][2 * i], p[k][2 * i + 1]);
-              ptx::tmem_st_32x32b_x16(tl + C::ds_col(wg + 2 * k), pk);
-            }
-          }
+          if (kv) products(std::true_type{}, sv, p, stats + kTR, 0, gs2, nc);
+          else products(std::false_type{}, sv, p, nullptr, nd2, gs2, nc);
           ptx::tmem_st_wait();
         }
         arrive(&ctrl->ds_ready);
       }
       // ---- the item's gradients: KV: warps 0-3 dV, warps 4-7 dK; Q: half of dQ's columns each
-      if (nt > 0 && ok && !wait(&ctrl->ds_done, (g - 1) & 1)) ok = false;
-      if (ok && live) {
-        ptx::tc_fence_after_sync();
-        constexpr int kCols = D;
-        const int cols = kv ? kCols : kCols / 2;
-        const int col0 = kv ? 0 : wg * (kCols / 2);
-        const int acc = kv && wg == 0 ? C::kAcc1 : C::kAcc2;
-        const float f = kv && wg == 0 ? 1.0f : a.scaling / gs;
-        T* out = static_cast<T*>(kv ? (wg == 0 ? a.dv : a.dk) : a.dq) + (it.row0 + row) * (kv ? (wg == 0 ? a.lddv : a.lddk) : a.lddq) +
-                 (int64_t)h * D + col0;
-        for (int c = 0; c < cols; c += 32) {
-          uint32_t r[32];
-          if (nt > 0) {
-            ptx::tmem_ld_32x32b_x32(tl + acc + col0 + c, r);
-            ptx::tmem_ld_wait();
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = 0u;  // nothing on the other side: zeros
-          }
-          if (row < it.rows) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 v;
-              v.x = pack2<FMT>(__uint_as_float(r[i]) * f, __uint_as_float(r[i + 1]) * f);
-              v.y = pack2<FMT>(__uint_as_float(r[i + 2]) * f, __uint_as_float(r[i + 3]) * f);
-              v.z = pack2<FMT>(__uint_as_float(r[i + 4]) * f, __uint_as_float(r[i + 5]) * f);
-              v.w = pack2<FMT>(__uint_as_float(r[i + 6]) * f, __uint_as_float(r[i + 7]) * f);
-              *reinterpret_cast<uint4*>(out + c + i) = v;
-            }
-          }
-        }
-      }
-      if (nt > 0) arrive(&ctrl->acc_free);
+      const int col0 = kv ? 0 : wg * (D / 2);
+      Pending o;
+      o.any = true;
+      o.live = live;
+      o.rows = it.rows;
+      o.cols = kv ? D : D / 2;
+      o.acc = (kv && wg == 0 ? C::kAcc1 : C::kAcc2) + col0;
+      o.f = kv && wg == 0 ? 1.0f : a.scaling / gs;
+      o.out = static_cast<T*>(kv ? (wg == 0 ? a.dv : a.dk) : a.dq) + (it.row0 + row) * (kv ? (wg == 0 ? a.lddv : a.lddk) : a.lddq) +
+              (int64_t)h * D + col0;
+      if (nt > 0) pend = o;
+      else if (ok && live) write_out(o, true);  // nothing on the other side: zeros
     }
+    flush();
     if (!ok && lane == 0) {
       ctrl->abort = 1;
       atomicOr(&g_attn_bwd_error, 4);
