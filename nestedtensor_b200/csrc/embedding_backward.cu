@@ -40,25 +40,39 @@ struct PassIn {
 
 __device__ __forceinline__ uint32_t digit_of(uint32_t key, int shift, int bits) { return (key >> shift) & ((1u << bits) - 1u); }
 
-// counts of every digit in the block's tile: hist[block][digit]
+constexpr int kGroupTiles = 8;  // tiles whose counts one block makes, and their sum
+
+// counts of every digit: hist[tile][digit], and group[block][digit] over the block's kGroupTiles tiles
 template <typename IDX>
 __global__ void __launch_bounds__(kSortThreads)
-radix_count_kernel(PassIn<IDX> in, int64_t tokens, int tile, int shift, int bits, uint32_t* __restrict__ hist) {
-  __shared__ uint32_t cnt[1 << kMaxDigit];
+radix_count_kernel(PassIn<IDX> in, int64_t tokens, int tile, int tiles, int shift, int bits, uint32_t* __restrict__ hist,
+                   uint32_t* __restrict__ group) {
+  __shared__ uint32_t cnt[kGroupTiles << kMaxDigit];
   const int bins = 1 << bits;
-  for (int i = threadIdx.x; i < bins; i += kSortThreads) cnt[i] = 0;
+  for (int i = threadIdx.x; i < kGroupTiles * bins; i += kSortThreads) cnt[i] = 0;
   __syncthreads();
-  const int64_t t0 = (int64_t)blockIdx.x * tile, t1 = t0 + tile < tokens ? t0 + tile : tokens;
-  for (int64_t t = t0 + threadIdx.x; t < t1; t += kSortThreads) atomicAdd(&cnt[digit_of(in.key(t), shift, bits)], 1u);
+  const int64_t t0 = (int64_t)blockIdx.x * kGroupTiles * tile;
+  const int64_t t1 = t0 + (int64_t)kGroupTiles * tile < tokens ? t0 + (int64_t)kGroupTiles * tile : tokens;
+  for (int64_t t = t0 + threadIdx.x; t < t1; t += kSortThreads)
+    atomicAdd(&cnt[(int)(t - t0) / tile * bins + digit_of(in.key(t), shift, bits)], 1u);
   __syncthreads();
-  for (int i = threadIdx.x; i < bins; i += kSortThreads) hist[(int64_t)blockIdx.x * bins + i] = cnt[i];
+  for (int i = threadIdx.x; i < kGroupTiles * bins; i += kSortThreads) {
+    const int64_t tl = (int64_t)blockIdx.x * kGroupTiles + i / bins;
+    if (tl < tiles) hist[tl * bins + i % bins] = cnt[i];
+  }
+  if ((int)threadIdx.x < bins) {
+    uint32_t sum = 0;
+    for (int k = 0; k < kGroupTiles; ++k) sum += cnt[k * bins + threadIdx.x];
+    group[(int64_t)blockIdx.x * bins + threadIdx.x] = sum;
+  }
 }
 
-// One stable pass over the tile [t0, t1) of block `blk`: every warp owns a contiguous part of it.  hist == NULL: the tile is the
+// One stable pass over the tile [t0, t1), number `blk`: every warp owns a contiguous part of it.  hist == NULL: the tile is the
 // whole input.  smem: [kSortWarps][bins] counters.
 template <typename IDX>
 __device__ __forceinline__ void radix_scatter_tile(const PassIn<IDX>& in, int64_t t0, int64_t t1, int shift, int bits,
-                                                   const uint32_t* __restrict__ hist, int blk, int blocks, uint32_t* wcnt,
+                                                   const uint32_t* __restrict__ hist, const uint32_t* __restrict__ group, int blk,
+                                                   int groups, uint32_t* wcnt,
                                                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
   __shared__ uint32_t s_below[1 << kMaxDigit], s_total[1 << kMaxDigit], s_warp[kSortWarps];
   const int bins = 1 << bits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -70,15 +84,17 @@ __device__ __forceinline__ void radix_scatter_tile(const PassIn<IDX>& in, int64_
   for (int64_t t = w0 + lane; t < w1; t += 32) atomicAdd(&wcnt[warp * bins + digit_of(in.key(t), shift, bits)], 1u);
   __syncthreads();
   if (hist != nullptr) {
-    // every digit's count over the blocks before this one, and over all
+    // every digit's count over the tiles before this one (whole groups, then this group's), and over all
     const int bin = threadIdx.x % bins, part = threadIdx.x / bins, parts = kSortThreads / bins;
+    const int mine = blk / kGroupTiles;
     uint32_t below = 0, total = 0;
 #pragma unroll 8
-    for (int k = part; k < blocks; k += parts) {
-      const uint32_t c = hist[(int64_t)k * bins + bin];
+    for (int k = part; k < groups; k += parts) {
+      const uint32_t c = group[(int64_t)k * bins + bin];
       total += c;
-      below += k < blk ? c : 0u;
+      below += k < mine ? c : 0u;
     }
+    for (int k = mine * kGroupTiles + part; k < blk; k += parts) below += hist[(int64_t)k * bins + bin];
     atomicAdd(&s_below[bin], below);
     atomicAdd(&s_total[bin], total);
   } else if ((int)threadIdx.x < bins) {
@@ -128,11 +144,12 @@ __device__ __forceinline__ void radix_scatter_tile(const PassIn<IDX>& in, int64_
 template <typename IDX>
 __global__ void __launch_bounds__(kSortThreads)
 radix_scatter_kernel(PassIn<IDX> in, int64_t tokens, int tile, int shift, int bits, const uint32_t* __restrict__ hist,
-                     uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, int* __restrict__ n_long) {
+                     const uint32_t* __restrict__ group, int groups, uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out,
+                     int* __restrict__ n_long) {
   extern __shared__ uint32_t sort_smem[];
-  if (blockIdx.x == 0 && threadIdx.x == 0) *n_long = 0;
+  if (blockIdx.x == 0 && threadIdx.x < 2) n_long[threadIdx.x] = 0;
   const int64_t t0 = (int64_t)blockIdx.x * tile, t1 = t0 + tile < tokens ? t0 + tile : tokens;
-  radix_scatter_tile(in, t0, t1, shift, bits, hist, (int)blockIdx.x, (int)gridDim.x, sort_smem, keys_out, pos_out);
+  radix_scatter_tile(in, t0, t1, shift, bits, hist, group, (int)blockIdx.x, groups, sort_smem, keys_out, pos_out);
 }
 
 // All passes in one block; the result is in keys[passes & 1 ? 0 : 1] ... (see launch).
@@ -141,9 +158,9 @@ __global__ void __launch_bounds__(kSortThreads)
 radix_single_kernel(PassIn<IDX> in, int64_t tokens, int passes, int bits, uint32_t* __restrict__ ka, uint32_t* __restrict__ pa,
                     uint32_t* __restrict__ kb, uint32_t* __restrict__ pb, int* __restrict__ n_long) {
   extern __shared__ uint32_t sort_smem[];
-  if (threadIdx.x == 0) *n_long = 0;
+  if (threadIdx.x < 2) n_long[threadIdx.x] = 0;
   for (int p = 0; p < passes; ++p) {
-    radix_scatter_tile<IDX>(in, 0, tokens, p * bits, bits, nullptr, 0, 1, sort_smem, ka, pa);
+    radix_scatter_tile<IDX>(in, 0, tokens, p * bits, bits, nullptr, nullptr, 0, 0, sort_smem, ka, pa);
     __syncthreads();  // the pass's output is read by the whole block, its counters cleared
     in.first = false;
     in.keys = ka, in.pos = pa;
@@ -179,17 +196,20 @@ struct SumArgs {
   const uint32_t *keys, *pos;  // sorted
   void* dw;
   float* partial;  // [chunks][2][cols]: sums of the chunk's first run (begun before it) and of its last run (not ended in it)
-  int* n_long;     // chunks whose last run begins there and goes on
-  int* long_list;
+  // chunks whose last run begins there and goes on: n_long[0] of them at the front of long_list; those whose run covers the next
+  // kFar chunks, n_long[1] of them, at its back
+  int *n_long, *long_list;
+  int64_t chunks;
   int64_t tokens, vocab, cols;
   float scale;
 };
 
 constexpr int kSumWarps = 8;
 constexpr int kAhead = 4;  // rows loaded before they are added
+constexpr int kFar = 31;   // chunks after the first that one warp of embedding_long_runs_kernel adds up
 
 template <int DT, int EPV, int VPL>
-__global__ void __launch_bounds__(kSumWarps * 32)
+__global__ void __launch_bounds__(kSumWarps * 32, 2)
 embedding_sum_kernel(SumArgs a, int slabs, int64_t sum_warps) {
   using U = RowUnit<DT, EPV>;
   const int lane = threadIdx.x & 31;
@@ -257,17 +277,25 @@ embedding_sum_kernel(SumArgs a, int slabs, int64_t sum_warps) {
           for (int k = 0; k < EPV; ++k) p[(int64_t)(u0 + 32 * j) * EPV + k] = acc[j * EPV + k];
         }
       }
-      if (begun_here && w % slabs == 0 && lane == 0) a.long_list[atomicAdd(a.n_long, 1)] = (int)chunk;
+      if (begun_here && w % slabs == 0 && lane == 0) {
+        const int64_t far = t0 + (int64_t)(kFar + 1) * kChunk;
+        if (far < a.tokens && a.keys[far] == run) a.long_list[a.chunks - 1 - atomicAdd(a.n_long + 1, 1)] = (int)chunk;
+        else a.long_list[atomicAdd(a.n_long, 1)] = (int)chunk;
+      }
     }
   };
+  // (loads are clamped to the last row and unit instead of predicated: all of a step's are in flight together; what a lane past
+  // the row's end adds up is never stored)
+  int unit[VPL];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) unit[j] = u0 + 32 * j < nv ? u0 + 32 * j : nv - 1;
   for (int e0 = 0; e0 < n; e0 += kAhead) {
     typename U::Raw rows[kAhead][VPL];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int64_t base = (int64_t)__shfl_sync(0xffffffffu, pos, e0 + i < n ? e0 + i : n - 1) * nv;
 #pragma unroll
-      for (int j = 0; j < VPL; ++j)
-        if (e0 + i < n && u0 + 32 * j < nv) rows[i][j] = U::load(a.grad, base + u0 + 32 * j);
+      for (int j = 0; j < VPL; ++j) rows[i][j] = U::load(a.grad, base + unit[j]);
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -281,8 +309,7 @@ embedding_sum_kernel(SumArgs a, int slabs, int64_t sum_warps) {
           for (int c = 0; c < VPL * EPV; ++c) acc[c] = 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < VPL; ++j)
-          if (u0 + 32 * j < nv) U::add(acc + j * EPV, rows[i][j]);
+        for (int j = 0; j < VPL; ++j) U::add(acc + j * EPV, rows[i][j]);
       }
     }
   }
@@ -290,19 +317,19 @@ embedding_sum_kernel(SumArgs a, int slabs, int64_t sum_warps) {
 }
 
 // The runs over several chunks: the partial of the chunk where the run begins, then those of the chunks whose first key is the
-// run's, by the block's warps in turn and the warps' sums in order.
+// run's, in order.  Columns in blocks of 128.  Runs of at most kFar + 1 chunks: one warp each; longer ones first, a block each: its
+// warps in turn, and their sums in order.
 template <int DT>
 __global__ void __launch_bounds__(256) embedding_long_runs_kernel(SumArgs a, int col_blocks) {
   __shared__ float s[8][128];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t chunks = (a.tokens + kChunk - 1) / kChunk;
-  const int64_t n = (int64_t)*a.n_long * col_blocks;
-  for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
-    const int64_t c = a.long_list[i / col_blocks];
+  const int64_t n_far = (int64_t)a.n_long[1] * col_blocks, n_near = (int64_t)a.n_long[0] * col_blocks;
+  for (int64_t i = blockIdx.x; i < n_far; i += gridDim.x) {
+    const int64_t c = a.long_list[a.chunks - 1 - i / col_blocks];
     const int64_t col0 = (i % col_blocks) * 128;
     const uint32_t run = a.keys[c * kChunk + kChunk - 1];
     // last chunk whose first key is the run's (first keys are sorted; chunk c + 1's is): 32 probes per step
-    int64_t lo = c + 1, hi = chunks - 1;
+    int64_t lo = c + 1, hi = a.chunks - 1;
     while (hi > lo) {
       const int64_t step = (hi - lo + 31) / 32;
       int64_t probe = lo + step * (lane + 1);
@@ -338,11 +365,30 @@ __global__ void __launch_bounds__(256) embedding_long_runs_kernel(SumArgs a, int
       Vec16<DT>::store1(a.dw, (int64_t)run * a.cols + col0 + threadIdx.x, t * a.scale);
     }
   }
+  for (int64_t i = (int64_t)blockIdx.x * 8 + warp; i < n_near; i += (int64_t)gridDim.x * 8) {
+    const int64_t c = a.long_list[i / col_blocks];
+    const int64_t col0 = (i % col_blocks) * 128;
+    const uint32_t run = a.keys[c * kChunk + kChunk - 1];
+    // lane k: does chunk c + 1 + k begin with the run?  (sorted: the ones that do come first; at most kFar)
+    const unsigned on = __ballot_sync(0xffffffffu, c + 1 + lane < a.chunks && a.keys[(c + 1 + lane) * kChunk] == run);
+    const int m = __popc(on);
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int k = 0; k <= m; ++k) {
+      const float* p = a.partial + ((c + k) * 2 + (k == 0 ? 1 : 0)) * a.cols + col0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col0 + lane + 32 * j < a.cols) acc[j] += p[lane + 32 * j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col0 + lane + 32 * j < a.cols) Vec16<DT>::store1(a.dw, (int64_t)run * a.cols + col0 + lane + 32 * j, acc[j] * a.scale);
+  }
 }
 
 struct EmbWorkspace {
-  size_t k0, p0, k1, p1, hist, n_long, list, partial, bytes;
-  int64_t chunks, blocks;
+  size_t k0, p0, k1, p1, hist, group, n_long, list, partial, bytes;
+  int64_t chunks, blocks, groups;
   int tile;
   EmbWorkspace(int64_t tokens, int64_t cols) {
     auto up = [](size_t v) { return (v + 15) / 16 * 16; };
@@ -355,7 +401,9 @@ struct EmbWorkspace {
     const size_t arr = up((size_t)tokens * 4);
     k0 = 0, p0 = k0 + arr, k1 = p0 + arr, p1 = k1 + arr;
     hist = p1 + arr;
-    n_long = hist + (tokens > kSingleBlock ? up((size_t)blocks * (1 << kMaxDigit) * 4) : 0);
+    groups = (blocks + kGroupTiles - 1) / kGroupTiles;
+    group = hist + (tokens > kSingleBlock ? up((size_t)blocks * (1 << kMaxDigit) * 4) : 0);
+    n_long = group + (tokens > kSingleBlock ? up((size_t)groups * (1 << kMaxDigit) * 4) : 0);
     list = n_long + 16;
     partial = list + up((size_t)chunks * 4);
     bytes = partial + (size_t)chunks * 2 * (size_t)cols * 4;
@@ -372,6 +420,7 @@ int sort_tokens(const IDX* index, int64_t tokens, int64_t vocab, int64_t padding
   uint32_t* k[2] = {reinterpret_cast<uint32_t*>(ws + at.k0), reinterpret_cast<uint32_t*>(ws + at.k1)};
   uint32_t* p[2] = {reinterpret_cast<uint32_t*>(ws + at.p0), reinterpret_cast<uint32_t*>(ws + at.p1)};
   uint32_t* hist = reinterpret_cast<uint32_t*>(ws + at.hist);
+  uint32_t* group = reinterpret_cast<uint32_t*>(ws + at.group);
   int* n_long = reinterpret_cast<int*>(ws + at.n_long);
   const size_t smem = (size_t)kSortWarps * (1u << digit) * 4;
   static std::atomic<int> configured[kMaxDevices];
@@ -386,9 +435,9 @@ int sort_tokens(const IDX* index, int64_t tokens, int64_t vocab, int64_t padding
     radix_single_kernel<IDX><<<1, kSortThreads, smem, st>>>(in, tokens, passes, digit, k[0], p[0], k[1], p[1], n_long);
   } else {
     for (int i = 0; i < passes; ++i) {
-      radix_count_kernel<IDX><<<(unsigned)at.blocks, kSortThreads, 0, st>>>(in, tokens, at.tile, i * digit, digit, hist);
-      radix_scatter_kernel<IDX><<<(unsigned)at.blocks, kSortThreads, smem, st>>>(in, tokens, at.tile, i * digit, digit, hist, k[i & 1],
-                                                                                 p[i & 1], n_long);
+      radix_count_kernel<IDX><<<(unsigned)at.groups, kSortThreads, 0, st>>>(in, tokens, at.tile, (int)at.blocks, i * digit, digit, hist, group);
+      radix_scatter_kernel<IDX><<<(unsigned)at.blocks, kSortThreads, smem, st>>>(in, tokens, at.tile, i * digit, digit, hist, group,
+                                                                                 (int)at.groups, k[i & 1], p[i & 1], n_long);
       in.first = false;
       in.keys = k[i & 1], in.pos = p[i & 1];
     }
@@ -450,7 +499,7 @@ int ntb200_embedding_backward(const void* grad, const void* index, int index_byt
   if (tokens >= (1ll << 31) - 1 || vocab >= (1ll << 31) - 1 || embed_dim >= (1ll << 31) - 1) return NTB200_UNSUPPORTED_SHAPE;
   if (grad_weight == nullptr) return NTB200_INVALID_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  SumArgs a = {grad, nullptr, nullptr, grad_weight, nullptr, nullptr, nullptr, tokens, vocab, embed_dim, scale};
+  SumArgs a = {grad, nullptr, nullptr, grad_weight, nullptr, nullptr, nullptr, (tokens + kChunk - 1) / kChunk, tokens, vocab, embed_dim, scale};
   if (tokens > 0) {
     if (grad == nullptr || index == nullptr) return NTB200_INVALID_ARG;
     const EmbWorkspace at(tokens, embed_dim);

@@ -34,7 +34,8 @@ struct Unit<DT, 1> {
   static __device__ __forceinline__ Raw zero() { return 0.0f; }
 };
 
-// Sums of a and b over the GROUP threads that share a row (GROUP >= 32: whole warps of a block of GROUP or, at 32, kBlock threads).
+// Sums of a and b over the GROUP neighbouring threads that share a row.  GROUP > 32: whole warps, through `scratch` and (GROUP <
+// the block) a named barrier of their own.
 template <int GROUP>
 __device__ __forceinline__ void group_sum2(float& a, float& b, float2* scratch) {
 #pragma unroll
@@ -45,13 +46,18 @@ __device__ __forceinline__ void group_sum2(float& a, float& b, float2* scratch) 
   if (GROUP <= 32) return;
   constexpr int kWarps = GROUP / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __syncthreads();  // scratch of the previous row has been read
+  const int group = threadIdx.x / GROUP;
+  auto sync = [&]() {
+    if (GROUP == kBlock) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(GROUP) : "memory");
+  };
+  sync();  // scratch of the previous row has been read
   if (lane == 0) scratch[warp] = make_float2(a, b);
-  __syncthreads();
+  sync();
   a = b = 0.0f;
 #pragma unroll
   for (int k = 0; k < kWarps; ++k) {
-    const float2 v = scratch[k];
+    const float2 v = scratch[group * kWarps + k];
     a += v.x;
     b += v.y;
   }
@@ -59,23 +65,30 @@ __device__ __forceinline__ void group_sum2(float& a, float& b, float2* scratch) 
 
 // AFFINE: gamma given and column sums wanted.  nv = units per row (cols / EPV).
 template <int DT, int EPV, int VPL, int GROUP, bool AFFINE>
-__global__ void __launch_bounds__(GROUP > 32 ? GROUP : kBlock)
+__global__ void __launch_bounds__(kBlock, 2)
 layer_norm_backward_kernel(const void* __restrict__ grad, const void* __restrict__ x, const float* __restrict__ mean,
                            const float* __restrict__ rstd, const void* __restrict__ gamma, void* __restrict__ dx,
                            float* __restrict__ partial, int64_t rows, int nv) {
   using U = Unit<DT, EPV>;
-  constexpr int kThreads = GROUP > 32 ? GROUP : kBlock;
-  constexpr int kRows = kThreads / GROUP;  // rows a block works on at a time
-  extern __shared__ float ln_smem[];       // [2, cols] column sums of the block's warps
+  constexpr int kRows = kBlock / GROUP;  // rows a block works on at a time
+  // whole vectors keep gamma in shared memory (in registers it spilled at 32 columns a thread), single elements in registers
+  constexpr bool kGammaSmem = AFFINE && EPV > 1;
+  extern __shared__ __align__(16) float ln_smem[];  // kGammaSmem: gamma; then [2, cols] column sums of the block's warps
   __shared__ float2 scratch[8];
   const int t = threadIdx.x % GROUP;
   const float inv_cols = 1.0f / (float)(nv * EPV);
-  typename U::Raw gam[VPL];
+  typename U::Raw gam[kGammaSmem ? 1 : VPL];
+  typename U::Raw* s_gam = reinterpret_cast<typename U::Raw*>(ln_smem);
+  float* s_cols = ln_smem + (kGammaSmem ? nv * (int)(sizeof(typename U::Raw) / sizeof(float)) : 0);
+  if (kGammaSmem) {
+    for (int v = threadIdx.x; v < nv; v += kBlock) s_gam[v] = U::load(gamma, v);
+    __syncthreads();
+  }
   float acc_g[AFFINE ? VPL * EPV : 1], acc_b[AFFINE ? VPL * EPV : 1];
 #pragma unroll
-  for (int j = 0; j < VPL; ++j) {
+  for (int j = 0; j < (kGammaSmem ? 1 : VPL); ++j) {
     gam[j] = U::zero();
-    if (AFFINE && t + j * GROUP < nv) gam[j] = U::load(gamma, t + j * GROUP);
+    if (AFFINE && !kGammaSmem && t + j * GROUP < nv) gam[j] = U::load(gamma, t + j * GROUP);
   }
 #pragma unroll
   for (int k = 0; k < (AFFINE ? VPL * EPV : 1); ++k) acc_g[k] = acc_b[k] = 0.0f;
@@ -104,7 +117,7 @@ layer_norm_backward_kernel(const void* __restrict__ grad, const void* __restrict
         float xf[EPV], gf[EPV], wf[EPV];
         U::unpack(xr[j], xf);
         U::unpack(gr[j], gf);
-        U::unpack(gam[j], wf);
+        U::unpack(kGammaSmem ? s_gam[t + j * GROUP] : gam[kGammaSmem ? 0 : j], wf);
 #pragma unroll
         for (int k = 0; k < EPV; ++k) {
           const float n = (xf[k] - mu) * rs;
@@ -128,7 +141,7 @@ layer_norm_backward_kernel(const void* __restrict__ grad, const void* __restrict
         float xf[EPV], gf[EPV], wf[EPV];
         U::unpack(xr[j], xf);
         U::unpack(gr[j], gf);
-        U::unpack(gam[j], wf);
+        U::unpack(kGammaSmem ? s_gam[t + j * GROUP] : gam[kGammaSmem ? 0 : j], wf);
 #pragma unroll
         for (int k = 0; k < EPV; ++k) {
           const float n = (xf[k] - mu) * rs;
@@ -165,16 +178,17 @@ layer_norm_backward_kernel(const void* __restrict__ grad, const void* __restrict
           acc_b[k] += __shfl_xor_sync(0xffffffffu, acc_b[k], o);
         }
       }
-      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-      for (int w = 0; w < kThreads / 32; ++w) {
-        if (warp == w && lane < GROUP) {
+      const int lane = threadIdx.x & 31;
+      constexpr int kTurn = GROUP < 32 ? 32 : GROUP;  // threads that add their columns at a time
+      for (int w = 0; w < kBlock / kTurn; ++w) {
+        if ((int)threadIdx.x / kTurn == w && (GROUP >= 32 || lane < GROUP)) {
 #pragma unroll
           for (int j = 0; j < VPL; ++j) {
             const int v = t + j * GROUP;
             if (v < nv) {
 #pragma unroll
               for (int k = 0; k < EPV; ++k) {
-                float* g = ln_smem + v * EPV + k;
+                float* g = s_cols + v * EPV + k;
                 *g = (w == 0 ? 0.0f : *g) + acc_g[j * EPV + k];
                 g[cols] = (w == 0 ? 0.0f : g[cols]) + acc_b[j * EPV + k];
               }
@@ -183,7 +197,7 @@ layer_norm_backward_kernel(const void* __restrict__ grad, const void* __restrict
         }
         __syncthreads();
       }
-      for (int i = threadIdx.x; i < 2 * cols; i += kThreads) out[i] = ln_smem[i];
+      for (int i = threadIdx.x; i < 2 * cols; i += kBlock) out[i] = s_cols[i];
     }
   }
 }
@@ -235,24 +249,25 @@ layer_norm_backward_columns_kernel(const void* __restrict__ grad, const void* __
   out[cols + c] = b;
 }
 
-// out[c] = sum over the blocks' partials, in a fixed order: 8 running sums a column (one per warp), then those in turn.
+// out[c] = sum over the blocks' partials, in a fixed order: 32 running sums a column (one per warp), then those in turn.
+constexpr int kReduceWarps = 32;
 template <int DT>
-__global__ void __launch_bounds__(kBlock)
+__global__ void __launch_bounds__(kReduceWarps * 32)
 layer_norm_backward_reduce_kernel(const float* __restrict__ partial, int blocks, void* __restrict__ dgamma, void* __restrict__ dbeta,
                                   int64_t cols) {
-  __shared__ float s[8][33];
+  __shared__ float s[kReduceWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float a = 0.0f;
   if (c < 2 * cols) {
 #pragma unroll 8
-    for (int k = warp; k < blocks; k += 8) a += partial[(int64_t)k * 2 * cols + c];
+    for (int k = warp; k < blocks; k += kReduceWarps) a += partial[(int64_t)k * 2 * cols + c];
   }
   s[warp][lane] = a;
   __syncthreads();
   if (warp != 0 || c >= 2 * cols) return;
 #pragma unroll
-  for (int w = 1; w < 8; ++w) a += s[w][lane];
+  for (int w = 1; w < kReduceWarps; ++w) a += s[w][lane];
   if (c < cols) {
     if (dgamma != nullptr) Vec16<DT>::store1(dgamma, c, a);
   } else if (dbeta != nullptr) {
@@ -260,7 +275,7 @@ layer_norm_backward_reduce_kernel(const float* __restrict__ partial, int blocks,
   }
 }
 
-constexpr int kMaxPartials = 8 * kNumSMs;  // most blocks that leave a partial
+constexpr int kMaxPartials = 4 * kNumSMs;  // most blocks that leave a partial
 
 struct BwdCall {
   const void *grad, *x;
@@ -288,17 +303,20 @@ int resident_blocks(F kernel, int threads, size_t smem, std::atomic<int>* cache)
 
 template <int DT, int EPV, int VPL, int GROUP, bool AFFINE>
 int launch_rows(const BwdCall& c, int* blocks, cudaStream_t st) {
-  constexpr int kThreads = GROUP > 32 ? GROUP : kBlock;
-  constexpr int kRows = kThreads / GROUP;
-  const size_t smem = AFFINE && kRows > 1 ? 2 * (size_t)c.cols * sizeof(float) : 0;  // at most 2 * 32 * VPL * EPV floats: 16 KB
+  constexpr int kRows = kBlock / GROUP;
+  // gamma (whole vectors) and the column sums of several rows' threads: 48 KB at most
+  constexpr int kPerUnit = (AFFINE && EPV > 1 ? 16 : 0) + (AFFINE && kRows > 1 ? 2 * EPV * (int)sizeof(float) : 0);
+  constexpr int kMostSmem = GROUP * VPL * kPerUnit;
+  static_assert(kMostSmem <= 48 * 1024, "more shared memory than a launch may ask for without an opt-in");
+  const size_t smem = (size_t)(c.cols / EPV) * kPerUnit;
   auto kernel = layer_norm_backward_kernel<DT, EPV, VPL, GROUP, AFFINE>;
   static std::atomic<int> cache[kMaxDevices];
-  int64_t grid = resident_blocks(kernel, kThreads, 2 * 32 * VPL * EPV * sizeof(float) * (kRows > 1), cache);
+  int64_t grid = resident_blocks(kernel, kBlock, kMostSmem, cache);
   if (grid > kMaxPartials) grid = kMaxPartials;
   const int64_t need = (c.rows + kRows - 1) / kRows;
   if (grid > need) grid = need;
   *blocks = (int)grid;
-  kernel<<<(unsigned)grid, kThreads, smem, st>>>(c.grad, c.x, c.mean, c.rstd, c.gamma, c.dx, c.partial, c.rows, (int)(c.cols / EPV));
+  kernel<<<(unsigned)grid, kBlock, smem, st>>>(c.grad, c.x, c.mean, c.rstd, c.gamma, c.dx, c.partial, c.rows, (int)(c.cols / EPV));
   return status_from_cuda(cudaGetLastError());
 }
 
@@ -356,7 +374,7 @@ int backward(const BwdCall& c, cudaStream_t st) {
   }
   if (affine && (c.dgamma != nullptr || c.dbeta != nullptr)) {
     const int64_t grid = (2 * c.cols + 31) / 32;
-    layer_norm_backward_reduce_kernel<DT><<<(unsigned)grid, kBlock, 0, st>>>(c.partial, blocks, c.dgamma, c.dbeta, c.cols);
+    layer_norm_backward_reduce_kernel<DT><<<(unsigned)grid, kReduceWarps * 32, 0, st>>>(c.partial, blocks, c.dgamma, c.dbeta, c.cols);
   }
   return status_from_cuda(cudaGetLastError());
 }

@@ -194,6 +194,64 @@ layer_norm_generic_kernel(const void* x, const void* __restrict__ residual, cons
   }
 }
 
+// Rows that are not made of whole 16-byte vectors, with statistics for a backward pass: one row per GROUP threads, element by
+// element, held in registers between the passes (the generic kernel reads the row three times: 94 us against 2 x 12 us for
+// reading and writing 24 000 rows of 771 bf16 at the copy rate).
+template <int DT, int VPL, int GROUP>
+__global__ void __launch_bounds__(kLnThreads)
+layer_norm_elements_kernel(const void* __restrict__ x, const void* __restrict__ gamma, const void* __restrict__ beta, float eps,
+                           void* __restrict__ out, int64_t rows, int cols, RowStats stats) {
+  constexpr int kRows = kLnThreads / GROUP, kWarps = GROUP / 32;
+  __shared__ float scratch[kLnThreads / 32];
+  const int t = threadIdx.x % GROUP, group = threadIdx.x / GROUP, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto sum = [&](float v) {
+    v = warp_sum(v);
+    if (kWarps == 1) return v;
+    auto sync = [&]() {
+      if (GROUP == kLnThreads) __syncthreads();
+      else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(GROUP) : "memory");
+    };
+    sync();  // scratch of the previous sum has been read
+    if (lane == 0) scratch[warp] = v;
+    sync();
+    v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) v += scratch[group * kWarps + k];
+    return v;
+  };
+  for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < rows; row0 += (int64_t)gridDim.x * kRows) {
+    const int64_t row = row0 + group, base = row * cols;
+    const bool live = row < rows;
+    float v[VPL], s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) v[j] = live && t + j * GROUP < cols ? Vec16<DT>::load1(x, base + t + j * GROUP) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) s += v[j];
+    const float mean = sum(s) / (float)cols;
+    s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      v[j] -= mean;
+      if (t + j * GROUP < cols) s = fmaf(v[j], v[j], s);
+    }
+    const float rstd = rsqrtf(sum(s) / (float)cols + eps);
+    if (!live) continue;
+    if (t == 0) {
+      stats.mean[row] = mean;
+      stats.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      const int c = t + j * GROUP;
+      if (c < cols) {
+        float o = v[j] * rstd;
+        if (gamma != nullptr) o = fmaf(o, Vec16<DT>::load1(gamma, c), Vec16<DT>::load1(beta, c));
+        Vec16<DT>::store1(out, base + c, o);
+      }
+    }
+  }
+}
+
 // tanh form of GELU, the one the reference's fused kernels use (cuda_kernels.cu:29-36)
 __device__ __forceinline__ float gelu_tanh(float x) {
   return 0.5f * x * (1.0f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
@@ -272,7 +330,21 @@ int launch_layer_norm(const void* x, const void* residual, const void* bias, con
   else if (vec_ok && nv <= 1280) NTB200_LN_LAUNCH(5, kLnThreads);
   else if (vec_ok && nv <= 1536) NTB200_LN_LAUNCH(6, kLnThreads);
   else if (vec_ok && nv <= 2048) NTB200_LN_LAUNCH(8, kLnThreads);
-  else {
+  else if (STATS && !vec_ok && cols <= 4096) {
+#define NTB200_LN_ELEMENTS(VPL, GROUP)                                                                                     \
+  do {                                                                                                                     \
+    const int64_t need = (rows + kLnThreads / (GROUP) - 1) / (kLnThreads / (GROUP));                                       \
+    layer_norm_elements_kernel<DT, VPL, GROUP><<<(unsigned)(need < 148 * 32 ? need : 148 * 32), kLnThreads, 0, st>>>(      \
+        x, gamma, beta, eps, out, rows, (int)cols, stats);                                                                 \
+  } while (0)
+    if (cols <= 128) NTB200_LN_ELEMENTS(4, 32);
+    else if (cols <= 512) NTB200_LN_ELEMENTS(16, 32);
+    else if (cols <= 832) NTB200_LN_ELEMENTS(13, 64);
+    else if (cols <= 1024) NTB200_LN_ELEMENTS(16, 64);
+    else if (cols <= 2048) NTB200_LN_ELEMENTS(16, 128);
+    else NTB200_LN_ELEMENTS(16, 256);
+#undef NTB200_LN_ELEMENTS
+  } else {
     const int64_t grid = rows < 148 * 32 ? rows : 148 * 32;
     layer_norm_generic_kernel<DT><<<(unsigned)grid, kLnThreads, 0, st>>>(x, FUSED ? residual : nullptr,
                                                                         FUSED ? bias : nullptr, gamma, beta, eps, out, rows,
