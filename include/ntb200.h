@@ -378,9 +378,11 @@ int ntb200_embedding_backward(const void* grad, const void* index, int index_byt
  * thirds of one [T, 3*H*d] matrix the kernels and results are those of ntb200_varlen_attention), and
  *   lse[h*q_tokens + t] = log2( sum_j exp2(scaling * log2(e) * q_t,h . k_j,h) )      (left unwritten for rows without keys)
  * offsets_q / offsets_k count elements of matrices with row_elems_q / row_elems_k elements per token (1: token offsets).
- *   path  0 = best available;  1 = SIMT;  2 = mma.sync kernel;  3 = tcgen05 kernel (1-3: for cross-checks)
- * workspace: ntb200_varlen_cross_attention_workspace_bytes(batch, q_tokens, ...), 16-byte aligned, or NULL.
+ *   path  0 = best available;  1 = 32-bit tiles;  2 = mma.sync kernel;  3 = tcgen05 kernel (1-3: for cross-checks)
+ * workspace: 16-byte aligned.
  */
+size_t ntb200_varlen_attention_train_workspace_bytes(int64_t batch, int64_t q_tokens, int num_heads, int head_dim,
+                                                     int dtype);
 int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
                                   void* out, float* lse, const int64_t* offsets_q, int64_t row_elems_q,
                                   const int64_t* offsets_k, int64_t row_elems_k, int64_t batch, int64_t q_tokens,

@@ -59,11 +59,11 @@ constexpr int kMaxHeadDim = 256;
 template <typename T>
 __global__ void __launch_bounds__(kSimtWarps * 32)
 attn_simt_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v, int64_t ldv,
-                 T* __restrict__ out, const int64_t* __restrict__ offsets_q, const int64_t* __restrict__ offsets_k, int64_t row_elems_q,
-                 int64_t row_elems_k, int64_t batch, int64_t total_tokens, int H, int d, float scale, LseOut lse) {
+                 T* __restrict__ out, const int64_t* __restrict__ offsets_q, const int64_t* __restrict__ offsets_k,
+                 int64_t batch, int64_t total_tokens, int H, int d, float scale) {
   // q / k / v: first element of head 0 of token 0, row strides ldq / ldk / ldv (self-attention on a packed
   // [T, 3E] buffer: the three thirds of one row, all strides 3E, offsets_k == offsets_q); offsets in elements
-  // of matrices with row_elems_q / row_elems_k elements per token (E for the nested tensors of the inputs)
+  // of the [tokens, E] matrices of the query and of the key / value nested tensors
   __shared__ float s_q[kSimtWarps][kMaxHeadDim];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t wg = (int64_t)blockIdx.x * kSimtWarps + warp;
@@ -71,9 +71,9 @@ attn_simt_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, 
   const int64_t t = wg / H;
   const int h = (int)(wg % H);
   const int64_t E = (int64_t)H * d;
-  const int64_t b = find_entry(offsets_q, batch, t * row_elems_q);
-  const int64_t tok0 = offsets_k[b] / row_elems_k;
-  const int L = (int)((offsets_k[b + 1] - offsets_k[b]) / row_elems_k);
+  const int64_t b = find_entry(offsets_q, batch, t * E);
+  const int64_t tok0 = offsets_k[b] / E;
+  const int L = (int)((offsets_k[b + 1] - offsets_k[b]) / E);
   const T* qrow = q + t * ldq + (int64_t)h * d;
   for (int i = lane; i < d; i += 32) s_q[warp][i] = Cvt<T>::to_f(qrow[i]) * scale;
   __syncwarp();
@@ -118,7 +118,6 @@ attn_simt_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ k, 
     m = m_new;
   }
   const float inv = L > 0 ? 1.0f / l : 0.0f;  // a query whose key sequence is empty gets zeros
-  if (lse.ptr != nullptr && lane == 0 && L > 0) lse.ptr[(int64_t)h * lse.ld + t] = (m + logf(l)) * 1.4426950408889634f;
   T* orow = out + t * E + (int64_t)h * d;
 #pragma unroll
   for (int i = 0; i < DPL; ++i) {
@@ -491,8 +490,7 @@ int launch_attn_simt(const QkvSrc& s, void* out, int64_t batch, int64_t q_tokens
   if (blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
   attn_simt_kernel<T><<<(unsigned)blocks, kSimtWarps * 32, 0, st>>>(static_cast<const T*>(s.q), s.ldq, static_cast<const T*>(s.k),
                                                                     s.ldk, static_cast<const T*>(s.v), s.ldv, static_cast<T*>(out),
-                                                                    s.offsets_q, s.offsets_k, s.row_elems_q, s.row_elems_k, batch,
-                                                                    q_tokens, H, d, scale, s.lse);
+                                                                    s.offsets_q, s.offsets_k, batch, q_tokens, H, d, scale);
   return status_from_cuda(cudaGetLastError());
 }
 
@@ -713,7 +711,25 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
       return attn_tcgen05_launch(q, out, rows, batch, q_tokens, num_heads, scaling, dtype, workspace, st, path == 0 ? (int)kTinyMaxLen : 0);
     return attn_tcgen05_cross_launch(q, ldq, k, ldk, v, ldv, out, rows, batch, q_tokens, k_tokens, num_heads, scaling, dtype, workspace, st);
   }
-  return launch_attn_generic(src, out, batch, q_tokens, num_heads, head_dim, max_len_q, scaling, dtype, path, st);
+  if (path != 1 && dtype != NTB200_F32 && (head_dim == 32 || head_dim == 64 || head_dim == 128)) {
+    const int rc = launch_attn_generic(src, out, batch, q_tokens, num_heads, head_dim, max_len_q, scaling, dtype, 2, st);
+    if (rc != NTB200_UNSUPPORTED_SHAPE || path == 2) return rc;
+  }
+  if (path == 2) return NTB200_UNSUPPORTED_SHAPE;
+  // what no tensor-core kernel takes: 32-bit tiles (the inference entry points' kernel, one warp per query and head, rereads its
+  // keys for every query: 242 us against 45 us for 16 sequences of up to 200 tokens, 4 heads of 64 in fp32)
+  if (q_tokens >= (1ll << 31) - 256 || k_tokens >= (1ll << 31) - 256 || batch >= (1ll << 31) - 256) return NTB200_UNSUPPORTED_SHAPE;
+  if (workspace == nullptr || workspace_bytes < attn_fwd_tiles_workspace_bytes(batch, q_tokens)) return NTB200_WORKSPACE_TOO_SMALL;
+  if (!aligned16(workspace)) return NTB200_MISALIGNED;
+  return attn_fwd_tiles_launch(q, ldq, k, ldk, v, ldv, out, {offsets_q, offsets_k, row_elems_q, row_elems_k, lse}, batch, q_tokens, num_heads,
+                               head_dim, scaling, dtype, workspace, st);
+}
+
+size_t ntb200_varlen_attention_train_workspace_bytes(int64_t batch, int64_t q_tokens, int num_heads, int head_dim, int dtype) {
+  if (batch <= 0 || q_tokens <= 0) return 0;
+  const size_t tiles = attn_fwd_tiles_workspace_bytes(batch, q_tokens);
+  const size_t tc = attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype) ? attn_tcgen05_workspace_bytes(batch, q_tokens) : 0;
+  return tiles > tc ? tiles : tc;
 }
 
 int ntb200_varlen_attention_weights(const void* q, int64_t ldq, const void* k, int64_t ldk, void* weights,

@@ -68,6 +68,10 @@ __device__ __forceinline__ void build_backward_items(const int64_t* __restrict__
   }
 }
 
+__global__ void __launch_bounds__(kPrepThreads) query_items_kernel(BwdArgs a, int tile, ListOut l) {
+  build_backward_items(a.offsets_q, a.row_elems_q, a.offsets_k, a.row_elems_k, a.batch, tile, l);
+}
+
 // Blocks 0 and 1 build the lists; every warp of the others takes one query token: D of all its heads, and (fp16) the largest
 // |dO| of its sequence and head.  VEC: heads of 32, 64 or 128 elements on 16-byte boundaries: a head on d / 8 lanes.
 template <typename T, bool VEC>
@@ -279,6 +283,146 @@ attn_bwd_simt_kernel(BwdArgs a, const int4* __restrict__ items, const int* __res
           o2[c] = from_f32<T>(acc2[i][j] * a.scaling);
           if (KV) o1[c] = from_f32<T>(acc1[i][j]);
         }
+      }
+    }
+  }
+}
+
+// The forward pass in the same tiles, for training calls that no tensor-core kernel takes: r = queries, and the online softmax over
+// tiles of keys; a row's maximum and sum are kept in shared memory between tiles.
+template <int BT, int DP>
+constexpr int fwd_simt_smem() { return (3 * BT * (DP + 4) + BT * (BT + 4) + 3 * BT) * 4; }
+
+template <typename T, int BT, int DP>
+__global__ void __launch_bounds__(256)
+attn_fwd_simt_kernel(BwdArgs a, T* __restrict__ out, float* __restrict__ lse, const int4* __restrict__ items, const int* __restrict__ count) {
+  constexpr int MI = BT / 16, LD = DP + 4, LS = BT + 4, NC = DP / 16;
+  extern __shared__ __align__(16) float bwd_smem[];
+  float* s_q = bwd_smem;
+  float* s_k = s_q + BT * LD;
+  float* s_v = s_k + BT * LD;
+  float* s_p = s_v + BT * LD;  // [key][query]
+  float* s_top = s_p + BT * LS;
+  float* s_sum = s_top + BT;
+  float* s_corr = s_sum + BT;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int64_t n = (int64_t)*count * a.H;
+  const int64_t E = (int64_t)a.H * a.d;
+  const float scale = a.scaling * kLog2e;
+  const int d4 = (a.d + 3) & ~3;
+  for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
+    const Item it = decode(items[w / a.H]);
+    const int h = (int)(w % a.H);
+    const int64_t col = (int64_t)h * a.d;
+    __syncthreads();  // the previous item's tiles have been read
+    load_rows<T, BT, DP>(s_q, static_cast<const T*>(a.q) + it.row0 * a.ldq + col, a.ldq, it.rows, a.d);
+    if (threadIdx.x < BT) {
+      s_top[threadIdx.x] = -INFINITY;
+      s_sum[threadIdx.x] = 0.0f;
+    }
+    float acc[MI][NC];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) acc[i][j] = 0.0f;
+    for (int c0 = 0; c0 < it.n_other; c0 += BT) {
+      const int nc = it.n_other - c0 < BT ? it.n_other - c0 : BT;
+      __syncthreads();
+      load_rows<T, BT, DP>(s_k, static_cast<const T*>(a.k) + (it.other + c0) * a.ldk + col, a.ldk, nc, a.d);
+      load_rows<T, BT, DP>(s_v, static_cast<const T*>(a.v) + (it.other + c0) * a.ldv + col, a.ldv, nc, a.d);
+      __syncthreads();
+      float s[MI][MI];  // key ty + 16 i, query tx + 16 j
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j) s[i][j] = 0.0f;
+#pragma unroll 2
+      for (int c = 0; c < d4; c += 4) {
+        float4 x[MI], y[MI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) x[i] = *reinterpret_cast<const float4*>(s_k + (ty + 16 * i) * LD + c);
+#pragma unroll
+        for (int j = 0; j < MI; ++j) y[j] = *reinterpret_cast<const float4*>(s_q + (tx + 16 * j) * LD + c);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < MI; ++j) {
+            s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
+            s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
+            s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
+            s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < MI; ++j) s_p[(ty + 16 * i) * LS + tx + 16 * j] = s[i][j] * scale;
+      __syncthreads();
+      // one warp takes BT / 8 queries: 32 lanes over the tile's keys
+      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+      for (int r = 0; r < BT / 8; ++r) {
+        const int q = warp * (BT / 8) + r;
+        float v[BT / 32], top = s_top[q];
+#pragma unroll
+        for (int k = 0; k < BT / 32; ++k) {
+          v[k] = lane + 32 * k < nc ? s_p[(lane + 32 * k) * LS + q] : -INFINITY;
+          top = fmaxf(top, v[k]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < BT / 32; ++k) {
+          v[k] = lane + 32 * k < nc ? exp2f(v[k] - top) : 0.0f;
+          sum += v[k];
+          s_p[(lane + 32 * k) * LS + q] = v[k];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+          const float corr = exp2f(s_top[q] - top);  // 0 on the first tile
+          s_corr[q] = corr;
+          s_sum[q] = s_sum[q] * corr + sum;
+          s_top[q] = top;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const float corr = s_corr[ty * MI + i];
+#pragma unroll
+        for (int j = 0; j < NC; ++j) acc[i][j] *= corr;
+      }
+      for (int c = 0; c < nc; ++c) {
+        float p[MI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) p[i] = s_p[c * LS + ty * MI + i];
+#pragma unroll
+        for (int m = 0; m < NC / 4; ++m) {
+          const float4 x = *reinterpret_cast<const float4*>(s_v + c * LD + tx * 4 + 64 * m);
+#pragma unroll
+          for (int i = 0; i < MI; ++i) {
+            acc[i][4 * m] = fmaf(p[i], x.x, acc[i][4 * m]);
+            acc[i][4 * m + 1] = fmaf(p[i], x.y, acc[i][4 * m + 1]);
+            acc[i][4 * m + 2] = fmaf(p[i], x.z, acc[i][4 * m + 2]);
+            acc[i][4 * m + 3] = fmaf(p[i], x.w, acc[i][4 * m + 3]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (lse != nullptr && threadIdx.x < BT && (int)threadIdx.x < it.rows && it.n_other > 0)
+      lse[(int64_t)h * a.q_tokens + it.row0 + threadIdx.x] = s_top[threadIdx.x] + log2f(s_sum[threadIdx.x]);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int r = ty * MI + i;
+      if (r >= it.rows) continue;
+      const float inv = it.n_other > 0 ? 1.0f / s_sum[r] : 0.0f;  // no keys: zeros
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int c = tx * 4 + 64 * (j / 4) + j % 4;
+        if (c < a.d) out[(it.row0 + r) * E + col + c] = from_f32<T>(acc[i][j] * inv);
       }
     }
   }
@@ -543,6 +687,29 @@ int launch_bwd_simt(const BwdArgs& a, int64_t k_tokens, const Lists& l, cudaStre
   return status_from_cuda(cudaGetLastError());
 }
 
+template <typename T, int BT, int DP>
+int launch_fwd_simt(const BwdArgs& a, void* out, float* lse, const ListOut& l, cudaStream_t st) {
+  constexpr int kSmem = fwd_simt_smem<BT, DP>();
+  static std::atomic<int> configured[kMaxDevices];
+  if (!once_per_device(configured, [] {
+        return cudaFuncSetAttribute(attn_fwd_simt_kernel<T, BT, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess;
+      }))
+    return NTB200_LAUNCH_FAILED;
+  query_items_kernel<<<1, kPrepThreads, 0, st>>>(a, BT, l);
+  const int per_sm = 227 * 1024 / (kSmem + 1024);
+  const int64_t most = item_capacity(a.batch, a.q_tokens, BT) * a.H;
+  const unsigned grid = (unsigned)(most < (int64_t)kNumSMs * per_sm ? most : (int64_t)kNumSMs * per_sm);
+  attn_fwd_simt_kernel<T, BT, DP><<<grid, 256, kSmem, st>>>(a, static_cast<T*>(out), lse, l.items, l.count);
+  return status_from_cuda(cudaGetLastError());
+}
+
+template <typename T>
+int launch_fwd(const BwdArgs& a, void* out, float* lse, const ListOut& l, cudaStream_t st) {
+  if (a.d <= 64) return launch_fwd_simt<T, 64, 64>(a, out, lse, l, st);
+  if (a.d <= 128) return launch_fwd_simt<T, 64, 128>(a, out, lse, l, st);
+  return launch_fwd_simt<T, 32, 256>(a, out, lse, l, st);
+}
+
 template <typename T, int D>
 int launch_bwd_mma(BwdArgs a, int64_t k_tokens, unsigned* top, const Lists& l, cudaStream_t st) {
   constexpr int kSmem = bwd_mma_smem<D>();
@@ -596,6 +763,30 @@ int launch_bwd(const BwdArgs& a, int64_t k_tokens, uint8_t* ws, const BwdWorkspa
 }
 
 }  // namespace
+
+size_t attn_fwd_tiles_workspace_bytes(int64_t batch, int64_t q_tokens) {
+  return 16 + (sizeof(int4) + sizeof(int)) * (size_t)item_capacity(batch, q_tokens, 32);
+}
+
+int attn_fwd_tiles_launch(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* out, const AttnRows& rows,
+                          int64_t batch, int64_t q_tokens, int H, int d, float scaling, int dtype, void* workspace, cudaStream_t st) {
+  BwdArgs a = {};
+  a.q = q, a.k = k, a.v = v;
+  a.ldq = ldq, a.ldk = ldk, a.ldv = ldv;
+  a.offsets_q = rows.offsets_q, a.offsets_k = rows.offsets_k;
+  a.row_elems_q = rows.row_elems_q, a.row_elems_k = rows.row_elems_k;
+  a.batch = batch, a.q_tokens = q_tokens;
+  a.H = H, a.d = d, a.scaling = scaling;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int64_t cap = item_capacity(batch, q_tokens, 32);
+  const ListOut l = {reinterpret_cast<int4*>(ws + 16), reinterpret_cast<int*>(ws + 16 + sizeof(int4) * cap), reinterpret_cast<int*>(ws)};
+  switch (dtype) {
+    case NTB200_F32: return launch_fwd<float>(a, out, rows.lse, l, st);
+    case NTB200_F16: return launch_fwd<__half>(a, out, rows.lse, l, st);
+    default: return launch_fwd<__nv_bfloat16>(a, out, rows.lse, l, st);
+  }
+}
+
 }  // namespace ntb200
 
 using namespace ntb200;

@@ -28,6 +28,10 @@ int attn_tcgen05_launch(const void* qkv, void* out, const AttnRows& rows, int64_
 int attn_tcgen05_cross_launch(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* out,
                               const AttnRows& rows, int64_t batch, int64_t q_tokens, int64_t k_tokens, int H, float scaling, int dtype,
                               void* workspace, cudaStream_t st);
+// attention_backward.cu: forward pass of training calls in 32-bit tiles (any dtype, head_dim <= 256; tokens and batch < 2^31 - 256)
+size_t attn_fwd_tiles_workspace_bytes(int64_t batch, int64_t q_tokens);
+int attn_fwd_tiles_launch(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* out, const AttnRows& rows,
+                          int64_t batch, int64_t q_tokens, int H, int d, float scaling, int dtype, void* workspace, cudaStream_t st);
 int attn_tcgen05_error_flags_read_and_clear();
 int attn_bwd_tcgen05_error_flags_read_and_clear();  // attention_backward_tcgen05.cu
 int construct_error_flags_read_and_clear();  // construct.cu: bit 0 = embedding index out of range

@@ -239,12 +239,11 @@ struct AttentionShape {
 void attention_forward(const AttentionShape& s, const void* q, const void* k, const void* v, int64_t ldq, int64_t ldkv, const Tensor& meta_q,
                        const Tensor& meta_k, Tensor& out, Tensor& lse) {
   const int dt = dtype_code(out.scalar_type());
-  const size_t bytes = ntb200_varlen_cross_attention_workspace_bytes(s.B, s.Tq, (int)s.H, (int)s.d, dt);
-  Tensor ws;
-  if (bytes > 0) ws = byte_workspace(bytes, out);
+  const size_t bytes = ntb200_varlen_attention_train_workspace_bytes(s.B, s.Tq, (int)s.H, (int)s.d, dt);
+  Tensor ws = byte_workspace(bytes, out);
   check_rc(ntb200_varlen_attention_train(q, ldq, k, ldkv, v, ldkv, out.data_ptr(), lse.data_ptr<float>(), meta_q.data_ptr<int64_t>(), s.row_q,
                                          meta_k.data_ptr<int64_t>(), s.row_k, s.B, s.Tq, s.Tk, (int)s.H, (int)s.d, s.longest_q,
-                                         (float)s.scaling, dt, 0, bytes > 0 ? ws.data_ptr() : nullptr, bytes, cur_stream()),
+                                         (float)s.scaling, dt, 0, ws.data_ptr(), bytes, cur_stream()),
            "ntb200_varlen_attention_train");
   maybe_check_device_errors("attention");
 }

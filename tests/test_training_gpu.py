@@ -265,7 +265,7 @@ def _cabi_backward(q, k, v, g, lq, lk, heads, path, ld_extra=0):
     off = [torch.tensor([0] + list(torch.tensor(n).cumsum(0))).cuda() for n in (lq, lk)]
     out, lse = torch.empty_like(q), torch.empty(heads, q.size(0), device="cuda")
     B, Tq, Tk, scaling = len(lq), q.size(0), k.size(0), d ** -0.5
-    n = lib.ntb200_varlen_cross_attention_workspace_bytes(B, Tq, heads, d, code)
+    n = lib.ntb200_varlen_attention_train_workspace_bytes(B, Tq, heads, d, code)
     ws = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
     _cabi.check("train", lib.ntb200_varlen_attention_train(
         q.data_ptr(), E, k.data_ptr(), E, v.data_ptr(), E, out.data_ptr(), lse.data_ptr(), off[0].data_ptr(), 1, off[1].data_ptr(), 1, B, Tq, Tk,
