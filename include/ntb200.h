@@ -394,11 +394,12 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
  * again from q, k and lse.
  *   path  0 = best available;  1 = the 32-bit tile kernels (any dtype and head_dim <= 256);  2 = mma.sync kernels (fp16 /
  *         bf16, head_dim 32 / 64 / 128, 16-byte aligned rows);  3 = tcgen05 kernel (the same with head_dim 64 / 128 and rows
- *         on both sides)                                                                     (1-3: for cross-checks)
- * workspace: 16-byte aligned.
+ *         on both sides);  4 = tcgen05 kernel with whole sequences as items (head_dim 64)    (1-4: for cross-checks)
+ * max_len_q / max_len_k: the longest sequences, or more.  workspace: 16-byte aligned, sized for the same lengths and path.
  */
 size_t ntb200_varlen_attention_backward_workspace_bytes(int64_t batch, int64_t q_tokens, int64_t k_tokens, int num_heads,
-                                                        int head_dim, int dtype);
+                                                        int head_dim, int64_t max_len_q, int64_t max_len_k, int dtype,
+                                                        int path);
 int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_t ldq, const void* k, int64_t ldk,
                                      const void* v, int64_t ldv, const void* out, const float* lse, void* grad_q,
                                      int64_t ld_grad_q, void* grad_k, int64_t ld_grad_k, void* grad_v, int64_t ld_grad_v,

@@ -70,7 +70,7 @@ SIGNATURES = {
     "ntb200_varlen_attention_train": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
                                               c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int64, c_float,
                                               c_int, c_int, c_void_p, c_size_t, c_void_p]),
-    "ntb200_varlen_attention_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),
+    "ntb200_varlen_attention_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int, c_int64, c_int64, c_int, c_int]),
     "ntb200_varlen_attention_backward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                                  c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                                                  c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int64, c_int64, c_float, c_int,

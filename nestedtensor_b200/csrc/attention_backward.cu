@@ -72,11 +72,52 @@ __global__ void __launch_bounds__(kPrepThreads) query_items_kernel(BwdArgs a, in
   build_backward_items(a.offsets_q, a.row_elems_q, a.offsets_k, a.row_elems_k, a.batch, tile, l);
 }
 
-// Blocks 0 and 1 build the lists; every warp of the others takes one query token: D of all its heads, and (fp16) the largest
+// An item for every sequence with rows on either side: (first key, keys, first query, queries), most tile pairs first.  One block.
+__device__ __forceinline__ void build_sequence_items(const BwdArgs& a, const ListOut& out) {
+  __shared__ int s_cnt[kListBuckets], s_base[kListBuckets];
+  if (threadIdx.x < kListBuckets) s_cnt[threadIdx.x] = 0;
+  __syncthreads();
+  auto lengths = [&](int64_t b) {
+    const int q0 = (int)(a.offsets_q[b] / a.row_elems_q), k0 = (int)(a.offsets_k[b] / a.row_elems_k);
+    return make_int4(k0, (int)(a.offsets_k[b + 1] / a.row_elems_k) - k0, q0, (int)(a.offsets_q[b + 1] / a.row_elems_q) - q0);
+  };
+  auto bucket = [&](const int4& l) {
+    const long long t = (long long)((l.y + 127) / 128) * ((l.w + 127) / 128);
+    const int n = t > 1 << 20 ? 1 << 20 : (int)t;
+    return n < 16 ? n : (28 - __clz(n) + 15 < kListBuckets - 1 ? 28 - __clz(n) + 15 : kListBuckets - 1);
+  };
+  for (int64_t b = threadIdx.x; b < a.batch; b += kPrepThreads) {
+    const int4 l = lengths(b);
+    if (l.y > 0 || l.w > 0) atomicAdd(&s_cnt[bucket(l)], 1);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int acc = 0;
+    for (int k = kListBuckets - 1; k >= 0; --k) {
+      s_base[k] = acc;
+      acc += s_cnt[k];
+    }
+    *out.count = acc;
+  }
+  __syncthreads();
+  for (int64_t b = threadIdx.x; b < a.batch; b += kPrepThreads) {
+    const int4 l = lengths(b);
+    if (l.y <= 0 && l.w <= 0) continue;
+    const int pos = atomicAdd(&s_base[bucket(l)], 1);
+    out.items[pos] = l;
+    out.seq[pos] = (int)b;
+  }
+}
+
+// Blocks 0 and 1 build the lists (tile 0: block 0 the list of sequences); every warp of the others takes one query token: D of all its heads, and (fp16) the largest
 // |dO| of its sequence and head.  VEC: heads of 32, 64 or 128 elements on 16-byte boundaries: a head on d / 8 lanes.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kPrepThreads)
 backward_prepare_kernel(BwdArgs a, int tile, ListOut kv, ListOut qi, unsigned* __restrict__ top) {
+  if (tile == 0) {
+    if (blockIdx.x == 0) build_sequence_items(a, kv);
+    if (blockIdx.x <= 1) return;
+  }
   if (blockIdx.x == 0) {
     build_backward_items(a.offsets_k, a.row_elems_k, a.offsets_q, a.row_elems_q, a.batch, tile, kv);
     return;
@@ -147,8 +188,7 @@ template <int BT, int DP>
 constexpr int bwd_simt_smem() { return (4 * BT * (DP + 4) + 2 * BT * (BT + 4) + 2 * BT) * 4; }
 
 template <typename T, int BT, int DP, bool KV>
-__global__ void __launch_bounds__(256)
-attn_bwd_simt_kernel(BwdArgs a, const int4* __restrict__ items, const int* __restrict__ count) {
+__device__ __forceinline__ void bwd_simt_item(const BwdArgs& a, const Item& it, int h) {
   constexpr int MI = BT / 16, LD = DP + 4, LS = BT + 4, NC = DP / 16;
   extern __shared__ __align__(16) float bwd_smem[];
   float* own_a = bwd_smem;
@@ -160,131 +200,136 @@ attn_bwd_simt_kernel(BwdArgs a, const int4* __restrict__ items, const int* __res
   float* s_lse = s_ds + BT * LS;
   float* s_delta = s_lse + BT;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t n = (int64_t)*count * a.H;
   const int64_t E = (int64_t)a.H * a.d;
   const float scale = a.scaling * kLog2e;
   const int d4 = (a.d + 3) & ~3;
-  for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
-    const Item it = decode(items[w / a.H]);
-    const int h = (int)(w % a.H);
-    const int64_t col = (int64_t)h * a.d;
-    const T* ga_own = (KV ? static_cast<const T*>(a.k) + it.row0 * a.ldk : static_cast<const T*>(a.q) + it.row0 * a.ldq) + col;
-    const T* gb_own = (KV ? static_cast<const T*>(a.v) + it.row0 * a.ldv : static_cast<const T*>(a.grad) + it.row0 * E) + col;
-    const int64_t ld_a_own = KV ? a.ldk : a.ldq, ld_b_own = KV ? a.ldv : E;
-    const int64_t ld_a = KV ? a.ldq : a.ldk, ld_b = KV ? E : a.ldv;
-    const float* g_lse = a.lse + (int64_t)h * a.q_tokens;
-    const float* g_delta = a.delta + (int64_t)h * a.q_tokens;
-    __syncthreads();  // the previous item's tiles have been read
-    load_rows<T, BT, DP>(own_a, ga_own, ld_a_own, it.rows, a.d);
-    load_rows<T, BT, DP>(own_b, gb_own, ld_b_own, it.rows, a.d);
-    if (!KV && threadIdx.x < BT) {
-      const bool ok = (int)threadIdx.x < it.rows && it.n_other > 0;  // (rows without keys have no statistics)
-      s_lse[threadIdx.x] = ok ? g_lse[it.row0 + threadIdx.x] : INFINITY;
-      s_delta[threadIdx.x] = ok ? g_delta[it.row0 + threadIdx.x] : 0.0f;
+  const int64_t col = (int64_t)h * a.d;
+  const T* ga_own = (KV ? static_cast<const T*>(a.k) + it.row0 * a.ldk : static_cast<const T*>(a.q) + it.row0 * a.ldq) + col;
+  const T* gb_own = (KV ? static_cast<const T*>(a.v) + it.row0 * a.ldv : static_cast<const T*>(a.grad) + it.row0 * E) + col;
+  const int64_t ld_a_own = KV ? a.ldk : a.ldq, ld_b_own = KV ? a.ldv : E;
+  const int64_t ld_a = KV ? a.ldq : a.ldk, ld_b = KV ? E : a.ldv;
+  const float* g_lse = a.lse + (int64_t)h * a.q_tokens;
+  const float* g_delta = a.delta + (int64_t)h * a.q_tokens;
+  __syncthreads();  // the previous item's tiles have been read
+  load_rows<T, BT, DP>(own_a, ga_own, ld_a_own, it.rows, a.d);
+  load_rows<T, BT, DP>(own_b, gb_own, ld_b_own, it.rows, a.d);
+  if (!KV && threadIdx.x < BT) {
+    const bool ok = (int)threadIdx.x < it.rows && it.n_other > 0;  // (rows without keys have no statistics)
+    s_lse[threadIdx.x] = ok ? g_lse[it.row0 + threadIdx.x] : INFINITY;
+    s_delta[threadIdx.x] = ok ? g_delta[it.row0 + threadIdx.x] : 0.0f;
+  }
+  float acc1[KV ? MI : 1][KV ? NC : 1], acc2[MI][NC];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      acc2[i][j] = 0.0f;
+      if (KV) acc1[i][j] = 0.0f;
     }
-    float acc1[KV ? MI : 1][KV ? NC : 1], acc2[MI][NC];
+  for (int c0 = 0; c0 < it.n_other; c0 += BT) {
+    const int nc = it.n_other - c0 < BT ? it.n_other - c0 : BT;
+    const int64_t o0 = it.other + c0;
+    __syncthreads();
+    load_rows<T, BT, DP>(oth_a, (KV ? static_cast<const T*>(a.q) + o0 * a.ldq : static_cast<const T*>(a.k) + o0 * a.ldk) + col, ld_a, nc, a.d);
+    load_rows<T, BT, DP>(oth_b, (KV ? static_cast<const T*>(a.grad) + o0 * E : static_cast<const T*>(a.v) + o0 * a.ldv) + col, ld_b, nc, a.d);
+    if (KV && threadIdx.x < BT) {
+      const bool ok = (int)threadIdx.x < nc;
+      s_lse[threadIdx.x] = ok ? g_lse[o0 + threadIdx.x] : INFINITY;  // 2^(x - inf) = 0: a row past the end counts nothing
+      s_delta[threadIdx.x] = ok ? g_delta[o0 + threadIdx.x] : 0.0f;
+    }
+    __syncthreads();
+    float s[MI][MI], dp[MI][MI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        acc2[i][j] = 0.0f;
-        if (KV) acc1[i][j] = 0.0f;
-      }
-    for (int c0 = 0; c0 < it.n_other; c0 += BT) {
-      const int nc = it.n_other - c0 < BT ? it.n_other - c0 : BT;
-      const int64_t o0 = it.other + c0;
-      __syncthreads();
-      load_rows<T, BT, DP>(oth_a, (KV ? static_cast<const T*>(a.q) + o0 * a.ldq : static_cast<const T*>(a.k) + o0 * a.ldk) + col, ld_a, nc, a.d);
-      load_rows<T, BT, DP>(oth_b, (KV ? static_cast<const T*>(a.grad) + o0 * E : static_cast<const T*>(a.v) + o0 * a.ldv) + col, ld_b, nc, a.d);
-      if (KV && threadIdx.x < BT) {
-        const bool ok = (int)threadIdx.x < nc;
-        s_lse[threadIdx.x] = ok ? g_lse[o0 + threadIdx.x] : INFINITY;  // 2^(x - inf) = 0: a row past the end counts nothing
-        s_delta[threadIdx.x] = ok ? g_delta[o0 + threadIdx.x] : 0.0f;
-      }
-      __syncthreads();
-      float s[MI][MI], dp[MI][MI];
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < MI; ++j) s[i][j] = dp[i][j] = 0.0f;
-      auto products = [&](const float* oth, const float* own, float (&acc)[MI][MI]) {
+      for (int j = 0; j < MI; ++j) s[i][j] = dp[i][j] = 0.0f;
+    auto products = [&](const float* oth, const float* own, float (&acc)[MI][MI]) {
 #pragma unroll 2
-        for (int c = 0; c < d4; c += 4) {
-          float4 x[MI], y[MI];
+      for (int c = 0; c < d4; c += 4) {
+        float4 x[MI], y[MI];
 #pragma unroll
-          for (int i = 0; i < MI; ++i) x[i] = *reinterpret_cast<const float4*>(oth + (ty + 16 * i) * LD + c);
+        for (int i = 0; i < MI; ++i) x[i] = *reinterpret_cast<const float4*>(oth + (ty + 16 * i) * LD + c);
 #pragma unroll
-          for (int j = 0; j < MI; ++j) y[j] = *reinterpret_cast<const float4*>(own + (tx + 16 * j) * LD + c);
+        for (int j = 0; j < MI; ++j) y[j] = *reinterpret_cast<const float4*>(own + (tx + 16 * j) * LD + c);
 #pragma unroll
-          for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int j = 0; j < MI; ++j) {
-              acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
-              acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
-              acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
-              acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
-            }
-        }
-      };
-      products(oth_a, own_a, s);
-      products(oth_b, own_b, dp);
+          for (int j = 0; j < MI; ++j) {
+            acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
+            acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
+            acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
+            acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+          }
+      }
+    };
+    products(oth_a, own_a, s);
+    products(oth_b, own_b, dp);
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < MI; ++j) {
-          const int c = ty + 16 * i, r = tx + 16 * j;
-          const int qi = KV ? c : r;
-          // a key past the end of the sequence has no probability (its zeroed row would score 0)
-          const float p = (!KV && c >= nc) ? 0.0f : exp2f(fmaf(s[i][j], scale, -s_lse[qi]));
-          if (KV) s_p[c * LS + r] = p;
-          s_ds[c * LS + r] = p * (dp[i][j] - s_delta[qi]);
-        }
-      __syncthreads();
-      for (int c = 0; c < nc; ++c) {
-        float ds[MI], pv[MI];
+      for (int j = 0; j < MI; ++j) {
+        const int c = ty + 16 * i, r = tx + 16 * j;
+        const int qi = KV ? c : r;
+        // a key past the end of the sequence has no probability (its zeroed row would score 0)
+        const float p = (!KV && c >= nc) ? 0.0f : exp2f(fmaf(s[i][j], scale, -s_lse[qi]));
+        if (KV) s_p[c * LS + r] = p;
+        s_ds[c * LS + r] = p * (dp[i][j] - s_delta[qi]);
+      }
+    __syncthreads();
+    for (int c = 0; c < nc; ++c) {
+      float ds[MI], pv[MI];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        ds[i] = s_ds[c * LS + ty * MI + i];
+        if (KV) pv[i] = s_p[c * LS + ty * MI + i];
+      }
+#pragma unroll
+      for (int m = 0; m < NC / 4; ++m) {
+        const float4 x = *reinterpret_cast<const float4*>(oth_a + c * LD + tx * 4 + 64 * m);
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-          ds[i] = s_ds[c * LS + ty * MI + i];
-          if (KV) pv[i] = s_p[c * LS + ty * MI + i];
+          acc2[i][4 * m] = fmaf(ds[i], x.x, acc2[i][4 * m]);
+          acc2[i][4 * m + 1] = fmaf(ds[i], x.y, acc2[i][4 * m + 1]);
+          acc2[i][4 * m + 2] = fmaf(ds[i], x.z, acc2[i][4 * m + 2]);
+          acc2[i][4 * m + 3] = fmaf(ds[i], x.w, acc2[i][4 * m + 3]);
         }
-#pragma unroll
-        for (int m = 0; m < NC / 4; ++m) {
-          const float4 x = *reinterpret_cast<const float4*>(oth_a + c * LD + tx * 4 + 64 * m);
+        if (KV) {
+          const float4 y = *reinterpret_cast<const float4*>(oth_b + c * LD + tx * 4 + 64 * m);
 #pragma unroll
           for (int i = 0; i < MI; ++i) {
-            acc2[i][4 * m] = fmaf(ds[i], x.x, acc2[i][4 * m]);
-            acc2[i][4 * m + 1] = fmaf(ds[i], x.y, acc2[i][4 * m + 1]);
-            acc2[i][4 * m + 2] = fmaf(ds[i], x.z, acc2[i][4 * m + 2]);
-            acc2[i][4 * m + 3] = fmaf(ds[i], x.w, acc2[i][4 * m + 3]);
-          }
-          if (KV) {
-            const float4 y = *reinterpret_cast<const float4*>(oth_b + c * LD + tx * 4 + 64 * m);
-#pragma unroll
-            for (int i = 0; i < MI; ++i) {
-              acc1[i][4 * m] = fmaf(pv[i], y.x, acc1[i][4 * m]);
-              acc1[i][4 * m + 1] = fmaf(pv[i], y.y, acc1[i][4 * m + 1]);
-              acc1[i][4 * m + 2] = fmaf(pv[i], y.z, acc1[i][4 * m + 2]);
-              acc1[i][4 * m + 3] = fmaf(pv[i], y.w, acc1[i][4 * m + 3]);
-            }
+            acc1[i][4 * m] = fmaf(pv[i], y.x, acc1[i][4 * m]);
+            acc1[i][4 * m + 1] = fmaf(pv[i], y.y, acc1[i][4 * m + 1]);
+            acc1[i][4 * m + 2] = fmaf(pv[i], y.z, acc1[i][4 * m + 2]);
+            acc1[i][4 * m + 3] = fmaf(pv[i], y.w, acc1[i][4 * m + 3]);
           }
         }
       }
     }
+  }
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int r = ty * MI + i;
-      if (r >= it.rows) continue;
-      T* o2 = (KV ? static_cast<T*>(a.dk) + (it.row0 + r) * a.lddk : static_cast<T*>(a.dq) + (it.row0 + r) * a.lddq) + col;
-      T* o1 = KV ? static_cast<T*>(a.dv) + (it.row0 + r) * a.lddv + col : nullptr;
+  for (int i = 0; i < MI; ++i) {
+    const int r = ty * MI + i;
+    if (r >= it.rows) continue;
+    T* o2 = (KV ? static_cast<T*>(a.dk) + (it.row0 + r) * a.lddk : static_cast<T*>(a.dq) + (it.row0 + r) * a.lddq) + col;
+    T* o1 = KV ? static_cast<T*>(a.dv) + (it.row0 + r) * a.lddv + col : nullptr;
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        const int c = tx * 4 + 64 * (j / 4) + j % 4;
-        if (c < a.d) {
-          o2[c] = from_f32<T>(acc2[i][j] * a.scaling);
-          if (KV) o1[c] = from_f32<T>(acc1[i][j]);
-        }
+    for (int j = 0; j < NC; ++j) {
+      const int c = tx * 4 + 64 * (j / 4) + j % 4;
+      if (c < a.d) {
+        o2[c] = from_f32<T>(acc2[i][j] * a.scaling);
+        if (KV) o1[c] = from_f32<T>(acc1[i][j]);
       }
     }
+  }
+}
+
+// KV items, then Q items, in one launch: neither alone fills the GPU when the batch is small
+template <typename T, int BT, int DP>
+__global__ void __launch_bounds__(256) attn_bwd_simt_kernel(BwdArgs a, ListOut kv, ListOut qi) {
+  const int64_t n_kv = (int64_t)*kv.count * a.H, n = n_kv + (int64_t)*qi.count * a.H;
+  for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
+    if (w < n_kv) bwd_simt_item<T, BT, DP, true>(a, decode(kv.items[w / a.H]), (int)(w % a.H));
+    else bwd_simt_item<T, BT, DP, false>(a, decode(qi.items[(w - n_kv) / a.H]), (int)((w - n_kv) % a.H));
   }
 }
 
@@ -634,10 +679,11 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 int64_t item_capacity(int64_t batch, int64_t tokens, int tile) { return batch + tokens / tile + 1; }
 
-// delta | largest |dO| | count, KV items, their sequences | count, Q items, their sequences; every part on a 16-byte boundary
+// delta | largest |dO| | count, KV items, their sequences | count, Q items, their sequences | dQ in fp32 (the tcgen05 kernel with
+// whole sequences as items); every part on a 16-byte boundary
 struct BwdWorkspace {
-  size_t delta, top, kv, kv_seq, q, q_seq, bytes;
-  BwdWorkspace(int64_t batch, int64_t q_tokens, int64_t k_tokens, int H) {
+  size_t delta, top, kv, kv_seq, q, q_seq, scratch, bytes;
+  BwdWorkspace(int64_t batch, int64_t q_tokens, int64_t k_tokens, int H, size_t scratch_bytes) {
     auto up = [](size_t v) { return (v + 15) / 16 * 16; };
     const size_t nk = (size_t)item_capacity(batch, k_tokens, 32), nq = (size_t)item_capacity(batch, q_tokens, 32);  // (tiles of 32 rows or more)
     delta = 0;
@@ -646,7 +692,8 @@ struct BwdWorkspace {
     kv_seq = kv + 16 + sizeof(int4) * nk;
     q = kv_seq + up(4 * nk);
     q_seq = q + 16 + sizeof(int4) * nq;
-    bytes = q_seq + up(4 * nq);
+    scratch = q_seq + up(4 * nq);
+    bytes = scratch + up(scratch_bytes);
   }
 };
 
@@ -671,19 +718,15 @@ int launch_bwd_simt(const BwdArgs& a, int64_t k_tokens, const Lists& l, cudaStre
   constexpr int kSmem = bwd_simt_smem<BT, DP>();
   static std::atomic<int> configured[kMaxDevices];
   if (!once_per_device(configured, [] {
-        return cudaFuncSetAttribute(attn_bwd_simt_kernel<T, BT, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess &&
-               cudaFuncSetAttribute(attn_bwd_simt_kernel<T, BT, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess;
+        return cudaFuncSetAttribute(attn_bwd_simt_kernel<T, BT, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess;
       }))
     return NTB200_LAUNCH_FAILED;
   const int rc = launch_prepare<T, false>(a, BT, l, nullptr, st);
   if (rc != NTB200_OK) return rc;
   const int per_sm = 227 * 1024 / (kSmem + 1024);
-  auto grid = [&](int64_t tokens) {
-    const int64_t most = item_capacity(a.batch, tokens, BT) * a.H;
-    return (unsigned)(most < (int64_t)kNumSMs * per_sm ? most : (int64_t)kNumSMs * per_sm);
-  };
-  if (k_tokens > 0) attn_bwd_simt_kernel<T, BT, DP, true><<<grid(k_tokens), 256, kSmem, st>>>(a, l.kv.items, l.kv.count);
-  if (a.q_tokens > 0) attn_bwd_simt_kernel<T, BT, DP, false><<<grid(a.q_tokens), 256, kSmem, st>>>(a, l.qi.items, l.qi.count);
+  const int64_t most = (item_capacity(a.batch, k_tokens, BT) + item_capacity(a.batch, a.q_tokens, BT)) * a.H;
+  const unsigned grid = (unsigned)(most < (int64_t)kNumSMs * per_sm ? most : (int64_t)kNumSMs * per_sm);
+  attn_bwd_simt_kernel<T, BT, DP><<<grid, 256, kSmem, st>>>(a, l.kv, l.qi);
   return status_from_cuda(cudaGetLastError());
 }
 
@@ -736,8 +779,20 @@ int launch_bwd_tcgen05(BwdArgs a, int64_t k_tokens, unsigned* top, int dtype, co
   return attn_bwd_tcgen05_launch(a, k_tokens, dtype, l.kv, l.qi, item_capacity(a.batch, k_tokens, 128), item_capacity(a.batch, a.q_tokens, 128), st);
 }
 
+// Whether the tcgen05 kernel takes whole sequences as items (heads of 64).  It needs enough of them to fill the GPU, and none so
+// long that its CTA is still busy when the others are done.
+bool by_sequence(int64_t batch, int64_t max_len_q, int64_t max_len_k, int H, int d, int dtype, int path) {
+  if (d != 64 || dtype == NTB200_F32 || (path != 0 && path != 4)) return false;
+  return path == 4 || (batch * H >= 2 * kNumSMs && max_len_q <= 1024 && max_len_k <= 1024);
+}
+
+size_t scratch_bytes(int64_t batch, int64_t q_tokens, int64_t max_len_q, int64_t max_len_k, int H, int d, int dtype, int path) {
+  return by_sequence(batch, max_len_q, max_len_k, H, d, dtype, path) && max_len_k > 128 ? (size_t)q_tokens * H * d * 4 : 0;
+}
+
 template <typename T>
-int launch_bwd(const BwdArgs& a, int64_t k_tokens, uint8_t* ws, const BwdWorkspace& at, int path, cudaStream_t st) {
+int launch_bwd(const BwdArgs& a, int64_t k_tokens, int64_t max_len_q, int64_t max_len_k, uint8_t* ws, const BwdWorkspace& at, int path,
+               cudaStream_t st) {
   const Lists l(ws, at);
   if constexpr (!std::is_same<T, float>::value) {
     const bool mma = (a.d == 32 || a.d == 64 || a.d == 128) && aligned16(a.grad) && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) &&
@@ -746,7 +801,14 @@ int launch_bwd(const BwdArgs& a, int64_t k_tokens, uint8_t* ws, const BwdWorkspa
     if (path >= 2 && !mma) return NTB200_UNSUPPORTED_SHAPE;
     constexpr int dtype = std::is_same<T, __half>::value ? NTB200_F16 : NTB200_BF16;
     const bool tc = mma && a.d >= 64 && attn_bwd_tcgen05_supported(a, k_tokens, dtype);
-    if (path == 3 && !tc) return NTB200_UNSUPPORTED_SHAPE;
+    if ((path == 3 && !tc) || (path == 4 && (!tc || a.d != 64))) return NTB200_UNSUPPORTED_SHAPE;
+    if (tc && by_sequence(a.batch, max_len_q, max_len_k, a.H, a.d, dtype, path)) {
+      BwdArgs b = a;
+      b.top = std::is_same<T, __half>::value ? reinterpret_cast<unsigned*>(ws + at.top) : nullptr;
+      const int rc = launch_prepare<T, true>(b, 0, l, const_cast<unsigned*>(b.top), st);
+      if (rc != NTB200_OK) return rc;
+      return attn_bwd_fused_launch(b, k_tokens, dtype, l.kv, reinterpret_cast<float*>(ws + at.scratch), st);
+    }
     if (tc && (path == 3 || path == 0)) return launch_bwd_tcgen05<T>(a, k_tokens, reinterpret_cast<unsigned*>(ws + at.top), dtype, l, st);
     if (mma && path != 1) {
       unsigned* top = reinterpret_cast<unsigned*>(ws + at.top);
@@ -794,10 +856,9 @@ using namespace ntb200;
 extern "C" {
 
 size_t ntb200_varlen_attention_backward_workspace_bytes(int64_t batch, int64_t q_tokens, int64_t k_tokens, int num_heads, int head_dim,
-                                                        int dtype) {
-  (void)head_dim, (void)dtype;
-  if (batch <= 0 || q_tokens < 0 || k_tokens < 0 || num_heads < 1) return 0;
-  return BwdWorkspace(batch, q_tokens, k_tokens, num_heads).bytes;
+                                                        int64_t max_len_q, int64_t max_len_k, int dtype, int path) {
+  if (batch <= 0 || q_tokens < 0 || k_tokens < 0 || num_heads < 1 || head_dim < 1) return 0;
+  return BwdWorkspace(batch, q_tokens, k_tokens, num_heads, scratch_bytes(batch, q_tokens, max_len_q, max_len_k, num_heads, head_dim, dtype, path)).bytes;
 }
 
 int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
@@ -807,7 +868,7 @@ int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_
                                      int num_heads, int head_dim, int64_t max_len_q, int64_t max_len_k, float scaling, int dtype, int path,
                                      void* workspace, size_t workspace_bytes, void* stream) {
   if (batch < 0 || q_tokens < 0 || k_tokens < 0 || num_heads < 1 || head_dim < 1 || row_elems_q < 1 || row_elems_k < 1 || max_len_q < 0 ||
-      max_len_k < 0 || path < 0 || path > 3)
+      max_len_k < 0 || path < 0 || path > 4)
     return NTB200_INVALID_ARG;
   if (dtype != NTB200_F32 && dtype != NTB200_F16 && dtype != NTB200_BF16) return NTB200_UNSUPPORTED_DTYPE;
   if (head_dim > kMaxHeadDim) return NTB200_UNSUPPORTED_SHAPE;
@@ -818,7 +879,8 @@ int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_
   if (offsets_q == nullptr || offsets_k == nullptr || workspace == nullptr) return NTB200_INVALID_ARG;
   if (q_tokens > 0 && (grad_out == nullptr || q == nullptr || out == nullptr || lse == nullptr || grad_q == nullptr)) return NTB200_INVALID_ARG;
   if (k_tokens > 0 && (k == nullptr || v == nullptr || grad_k == nullptr || grad_v == nullptr)) return NTB200_INVALID_ARG;
-  const BwdWorkspace at(batch, q_tokens, k_tokens, num_heads);
+  const BwdWorkspace at(batch, q_tokens, k_tokens, num_heads,
+                        scratch_bytes(batch, q_tokens, max_len_q, max_len_k, num_heads, head_dim, dtype, path));
   if (workspace_bytes < at.bytes) return NTB200_WORKSPACE_TOO_SMALL;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return NTB200_MISALIGNED;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -827,9 +889,9 @@ int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_
                      batch, q_tokens, num_heads, head_dim, scaling};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case NTB200_F32: return launch_bwd<float>(a, k_tokens, ws, at, path, st);
-    case NTB200_F16: return launch_bwd<__half>(a, k_tokens, ws, at, path, st);
-    default: return launch_bwd<__nv_bfloat16>(a, k_tokens, ws, at, path, st);
+    case NTB200_F32: return launch_bwd<float>(a, k_tokens, max_len_q, max_len_k, ws, at, path, st);
+    case NTB200_F16: return launch_bwd<__half>(a, k_tokens, max_len_q, max_len_k, ws, at, path, st);
+    default: return launch_bwd<__nv_bfloat16>(a, k_tokens, max_len_q, max_len_k, ws, at, path, st);
   }
 }
 

@@ -85,5 +85,8 @@ __device__ __forceinline__ float grad_scale(const BwdArgs& a, const int* __restr
 bool attn_bwd_tcgen05_supported(const BwdArgs& a, int64_t k_tokens, int dtype);
 int attn_bwd_tcgen05_launch(const BwdArgs& a, int64_t k_tokens, int dtype, const ListOut& kv, const ListOut& qi, int64_t kv_capacity,
                             int64_t q_capacity, cudaStream_t st);
+// whole sequences as items, heads of 64: seqs lists (first key, keys, first query, queries) of every sequence with rows on either side;
+// scratch: H * 64 * q_tokens floats, 16-byte aligned (unused where no sequence has more than 128 keys)
+int attn_bwd_fused_launch(const BwdArgs& a, int64_t k_tokens, int dtype, const ListOut& seqs, float* scratch, cudaStream_t st);
 
 }  // namespace ntb200

@@ -50,7 +50,8 @@ struct Cfg {
   static constexpr int kStages = D == 64 ? 4 : 2; // other tile pairs
   static constexpr int kAcc1 = 256, kAcc2 = 256 + D;
   static constexpr int kStats = 2 * kTR * 4;      // -lse and -D of a stage
-  static constexpr int kSmem = 1024 + (kOwn + kStages) * 2 * kTile + kStages * kStats + 512;
+  static constexpr int kStaging = (kOwn + kStages) * 2 * kTile + kStages * kStats + 512;  // 2 KB a softmax warp for the outputs
+  static constexpr int kSmem = 1024 + kStaging + 8 * 2048;
   // tensor-memory columns of the packed P and dS of a chunk of 32 columns
   static __device__ __forceinline__ int p_col(int chunk) { return kSep ? 384 + 16 * chunk : 32 * chunk; }
   static __device__ __forceinline__ int ds_col(int chunk) { return kSep ? 448 + 16 * chunk : 128 + 32 * chunk; }
@@ -64,6 +65,50 @@ struct Ctrl {
   uint32_t tmem_base;
   volatile int abort;
 };
+
+// Columns past the end of the sequence have no probability, whatever was in their columns (in a loop of zero or one trips, so that
+// whole chunks do not pay for the selects).
+__device__ __forceinline__ void cut_columns(float (&x)[32], int c0, int nc) {
+#pragma unroll 1
+  for (int ragged = nc - c0 < 32 ? 1 : 0; ragged > 0; --ragged) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = c0 + i >= nc ? 0.0f : x[i];
+  }
+}
+
+// 32 columns of 32 rows (one row per lane, packed 16-bit, 64 bytes) to global memory through the warp's 2 KB of shared memory: stored
+// row by row from the lanes themselves, every 16-byte store would touch 32 lines.
+__device__ __forceinline__ void store_rows(uint32_t stage, const uint4 (&v)[4], uint8_t* out, int64_t row_bytes, int rows) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)), "r"(v[i].x), "r"(v[i].y),
+                 "r"(v[i].z), "r"(v[i].w)
+                 : "memory");
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + lane / 4, c = lane % 4;
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "r"(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4))
+                 : "memory");
+    if (r < rows) *reinterpret_cast<uint4*>(out + r * row_bytes + c * 16) = x;
+  }
+  __syncwarp();
+}
+
+template <int FMT>
+__device__ __forceinline__ void pack_row(const uint32_t (&r)[32], float f, uint4 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i].x = pack2<FMT>(__uint_as_float(r[8 * i]) * f, __uint_as_float(r[8 * i + 1]) * f);
+    v[i].y = pack2<FMT>(__uint_as_float(r[8 * i + 2]) * f, __uint_as_float(r[8 * i + 3]) * f);
+    v[i].z = pack2<FMT>(__uint_as_float(r[8 * i + 4]) * f, __uint_as_float(r[8 * i + 5]) * f);
+    v[i].w = pack2<FMT>(__uint_as_float(r[8 * i + 6]) * f, __uint_as_float(r[8 * i + 7]) * f);
+  }
+}
 
 struct TcArgs {
   BwdArgs a;
@@ -133,6 +178,8 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   auto head = [&](unsigned w) { return (int)((w < n_kv ? w : w - n_kv) % H); };
   auto tiles_of = [](const Item& it) { return (it.n_other + kTR - 1) / kTR; };
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_or_abort(ptx::smem_u32(bar), parity, &ctrl->abort); };
+  // for roles of whole warps: the lanes agree, so that none is left alone at a warp-wide instruction when a wait runs out
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_or_abort(ptx::smem_u32(bar), parity, &ctrl->abort)) != 0; };
 
   if (warp >= 8) {
     ptx::setmaxnreg_dec<kRegControl>();
@@ -353,7 +400,7 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           open();
         }
         if (w < n_all) load();
-        if (!wait(&ctrl->full[s], (g / C::kStages) & 1)) {
+        if (!wait_warp(&ctrl->full[s], (g / C::kStages) & 1)) {
           ok = false;
           break;
         }
@@ -397,13 +444,16 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     // The gradients of an item are written during the first tile of the next one (its last product retires meanwhile).
     struct Pending {
       bool any, live;
-      T* out;
+      T* out;             // of the warp's first row
+      int64_t row_bytes;
       int rows, cols, acc;
       float f;
-    } pend = {false, false, nullptr, 0, 0, 0, 0.0f};
-    auto write_out = [&](const Pending& o, bool zeros) {
+    } pend = {false, false, nullptr, 0, 0, 0, 0, 0.0f};
+    const uint32_t stage = ptx::smem_u32(smem) + (uint32_t)C::kStaging + (uint32_t)warp * 2048u;
+    auto write_out = [&](const Pending& o, bool zeros) {  // (whole warps: o.rows of this warp's 32 rows are valid)
       for (int c = 0; c < o.cols; c += 32) {
         uint32_t r[32];
+        uint4 v[4];
         if (!zeros) {
           ptx::tmem_ld_32x32b_x32(tl + o.acc + c, r);
           ptx::tmem_ld_wait();
@@ -411,23 +461,14 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 #pragma unroll
           for (int i = 0; i < 32; ++i) r[i] = 0u;
         }
-        if (row < o.rows) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint4 v;
-            v.x = pack2<FMT>(__uint_as_float(r[i]) * o.f, __uint_as_float(r[i + 1]) * o.f);
-            v.y = pack2<FMT>(__uint_as_float(r[i + 2]) * o.f, __uint_as_float(r[i + 3]) * o.f);
-            v.z = pack2<FMT>(__uint_as_float(r[i + 4]) * o.f, __uint_as_float(r[i + 5]) * o.f);
-            v.w = pack2<FMT>(__uint_as_float(r[i + 6]) * o.f, __uint_as_float(r[i + 7]) * o.f);
-            *reinterpret_cast<uint4*>(o.out + c + i) = v;
-          }
-        }
+        pack_row<FMT>(r, o.f, v);
+        store_rows(stage, v, reinterpret_cast<uint8_t*>(o.out + c), o.row_bytes, o.rows);
       }
     };
     uint32_t n = 0;  // items with tiles whose gradients have been written
     auto flush = [&]() {
       if (!pend.any) return;
-      if (ok && !wait(&ctrl->item_done, n & 1)) ok = false;
+      if (ok && !wait_warp(&ctrl->item_done, n & 1)) ok = false;
       ++n;
       if (ok && pend.live) {
         ptx::tc_fence_after_sync();
@@ -436,16 +477,7 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       arrive(&ctrl->acc_free);
       pend.any = false;
     };
-    // P of this thread's (up to) 64 columns, 2^(scale S - lse); lse per column (KV items, from shared memory) or per row.  Columns
-    // past the end of the sequence have no probability, whatever was in their columns (cut in a loop of zero or one trips, so
-    // that whole chunks do not pay for the selects).
-    auto cut = [&](float (&x)[32], int c0, int nc) {
-#pragma unroll 1
-      for (int ragged = nc - c0 < 32 ? 1 : 0; ragged > 0; --ragged) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = c0 + i >= nc ? 0.0f : x[i];
-      }
-    };
+    // P of this thread's (up to) 64 columns, 2^(scale S - lse); lse per column (KV items, from shared memory) or per row
     auto exponentials = [&](auto is_kv, const uint32_t (&sv)[2][32], float (&p)[2][32], const float* stats, uint64_t nl, int nc) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -465,7 +497,7 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             p[k][i + 2] = ptx::ex2_approx(e2);
             p[k][i + 3] = ptx::ex2_approx(e3);
           }
-          cut(p[k], c0, nc);
+          cut_columns(p[k], c0, nc);
         }
       }
     };
@@ -484,7 +516,7 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             ptx::f32x2_unpack(ptx::f32x2_mul(ptx::f32x2_pack(p[k][i], p[k][i + 1]), x0), p[k][i], p[k][i + 1]);
             ptx::f32x2_unpack(ptx::f32x2_mul(ptx::f32x2_pack(p[k][i + 2], p[k][i + 3]), x1), p[k][i + 2], p[k][i + 3]);
           }
-          cut(p[k], c0, nc);
+          cut_columns(p[k], c0, nc);
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) pk[i] = pack2<FMT>(p[k][2 * i], p[k][2 * i + 1]);
@@ -538,8 +570,8 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         uint32_t sv[2][32];
         float p[2][32];
         // ---- P
-        if (ok && !wait(&ctrl->s_ready, g & 1)) ok = false;
-        if (ok && kv && !wait(&ctrl->aux[s], (g / C::kStages) & 1)) ok = false;
+        if (ok && !wait_warp(&ctrl->s_ready, g & 1)) ok = false;
+        if (ok && kv && !wait_warp(&ctrl->aux[s], (g / C::kStages) & 1)) ok = false;
         if (ok && live) {
           ptx::tc_fence_after_sync();
 #pragma unroll
@@ -566,7 +598,7 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         arrive(&ctrl->p_ready);
         if (j == 0) flush();
         // ---- dS
-        if (ok && !wait(&ctrl->dp_ready, g & 1)) ok = false;
+        if (ok && !wait_warp(&ctrl->dp_ready, g & 1)) ok = false;
         if (ok && live) {
           ptx::tc_fence_after_sync();
 #pragma unroll
@@ -584,12 +616,13 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       Pending o;
       o.any = true;
       o.live = live;
-      o.rows = it.rows;
+      o.rows = it.rows - q * 32;
       o.cols = kv ? D : D / 2;
       o.acc = (kv && wg == 0 ? C::kAcc1 : C::kAcc2) + col0;
       o.f = kv && wg == 0 ? 1.0f : a.scaling / gs;
-      o.out = static_cast<T*>(kv ? (wg == 0 ? a.dv : a.dk) : a.dq) + (it.row0 + row) * (kv ? (wg == 0 ? a.lddv : a.lddk) : a.lddq) +
-              (int64_t)h * D + col0;
+      const int64_t ld = kv ? (wg == 0 ? a.lddv : a.lddk) : a.lddq;
+      o.row_bytes = ld * 2;
+      o.out = static_cast<T*>(kv ? (wg == 0 ? a.dv : a.dk) : a.dq) + (it.row0 + q * 32) * ld + (int64_t)h * D + col0;
       if (nt > 0) pend = o;
       else if (ok && live) write_out(o, true);  // nothing on the other side: zeros
     }
@@ -606,6 +639,628 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     ptx::tc_fence_after_sync();
     ptx::tmem_dealloc(tmem, 512);
   }
+}
+
+// ------------------------------------------------------------------ whole sequences: five products
+// The same roles for heads of 64, with an item per (sequence, head): all key tiles of the sequence in turn, each against all query
+// tiles.  S and dP are computed once for dV, dK and dQ: dS goes to shared memory as well-formed operand tiles (row = key, 64
+// queries a half), read K-major for dK += dS Q and MN-major for dQ = dS^T K.  Four more warps add the dQ tiles of successive key
+// tiles up in fp32 (scratch in global memory, one thread per row and always the same one: the order of the sum is fixed) and
+// write them out with the last key tile; a sequence of one key tile needs no scratch.
+// Half the exponentials and 5/7 of the products of the kernel above, but a sequence is one CTA's: for batches whose sequences are
+// short and many (attention_backward.cu chooses).
+constexpr int kFusedThreads = 512;
+constexpr int kFusedRegSoftmax = 168, kFusedRegAdd = 96, kFusedRegControl = 80, kFusedRegLaunch = 128;
+static_assert(2 * kFusedRegSoftmax + kFusedRegAdd + kFusedRegControl == 4 * kFusedRegLaunch && kFusedRegLaunch * kFusedThreads <= 65536,
+              "setmaxnreg exchange must balance");
+
+struct Fused {
+  static constexpr int D = 64, kTile = kHalf, kOwn = 2, kStages = 3;
+  static constexpr int kAccV = 256, kAccK = 320, kAccQ = 384, kP = 448;  // tensor-memory columns; S 0, dP 128
+  static constexpr int kStats = 2 * kTR * 4;
+  static constexpr int kDs = 2 * kHalf;  // dS: 128 keys x 128 queries
+  static constexpr int kStaging = (kOwn + kStages) * 2 * kTile + kDs + kStages * kStats + 512;  // 2 KB a warp for the outputs
+  static constexpr int kSmem = 1024 + kStaging + 12 * 2048;
+  static_assert(kSmem <= 227 * 1024, "more shared memory than a block has");
+};
+
+struct FusedCtrl {
+  uint64_t own_full[Fused::kOwn], own_empty[Fused::kOwn], own_aux[Fused::kOwn];
+  uint64_t full[Fused::kStages], empty[Fused::kStages], aux[Fused::kStages];
+  uint64_t s_ready, p_ready, dp_ready, ds_ready, dq_ready, dq_free, own_done, acc_free, done;
+  uint32_t tmem_base;
+  volatile int abort;
+};
+
+struct FusedArgs {
+  BwdArgs a;
+  ListOut seqs;     // an item per sequence: (first key, keys, first query, queries)
+  float4* scratch;  // [H][16][q_tokens]: dQ in fp32 while its key tiles are added up
+};
+
+template <int FMT>
+__global__ void __launch_bounds__(kFusedThreads, 1)
+attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g, const __grid_constant__ FusedArgs t) {
+  using C = Fused;
+  using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
+  static_assert(sizeof(FusedCtrl) <= 512, "control block exceeds its shared-memory slot");
+  const BwdArgs& a = t.a;
+  const unsigned H = (unsigned)a.H;
+  const unsigned n_all = (unsigned)*t.seqs.count * H;
+  if (blockIdx.x >= n_all) return;
+  extern __shared__ uint8_t bwd_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(bwd_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem_ds = smem + (C::kOwn + C::kStages) * 2 * C::kTile;
+  float* s_stats = reinterpret_cast<float*>(smem_ds + C::kDs);
+  FusedCtrl* ctrl = reinterpret_cast<FusedCtrl*>(reinterpret_cast<uint8_t*>(s_stats) + C::kStages * C::kStats);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kOwn; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&ctrl->own_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&ctrl->own_empty[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&ctrl->own_aux[s]), 1);
+    }
+    for (int s = 0; s < C::kStages; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&ctrl->full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&ctrl->empty[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&ctrl->aux[s]), 2);
+    }
+    ptx::mbar_init(ptx::smem_u32(&ctrl->s_ready), 1);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->p_ready), 8);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->dp_ready), 1);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->ds_ready), 8);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->dq_ready), 1);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->dq_free), 4);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->own_done), 1);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->acc_free), 8);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->done), 1);
+    ctrl->abort = 0;
+    ptx::fence_barrier_init();
+    ptx::prefetch_tensormap(&map_q);
+    ptx::prefetch_tensormap(&map_k);
+    ptx::prefetch_tensormap(&map_v);
+    ptx::prefetch_tensormap(&map_g);
+  }
+  if (warp == 13) {
+    ptx::tmem_alloc(ptx::smem_u32(&ctrl->tmem_base), 512);
+    ptx::tmem_relinquish();
+    ptx::tc_fence_before_sync();
+  }
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = ctrl->tmem_base;
+  const uint32_t s_own = ptx::smem_u32(smem);
+  const uint32_t s_oth = s_own + C::kOwn * 2 * C::kTile;
+  const uint32_t s_ds = ptx::smem_u32(smem_ds);
+
+  auto fetch = [&](unsigned w) { return w < n_all ? __ldg(t.seqs.items + w / H) : make_int4(0, 0, 0, 0); };
+  auto head = [&](unsigned w) { return (int)(w % H); };
+  auto tiles = [](int n) { return (n + kTR - 1) / kTR; };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_or_abort(ptx::smem_u32(bar), parity, &ctrl->abort); };
+  // for roles of whole warps: the lanes agree, so that none is left alone at a warp-wide instruction when a wait runs out
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_or_abort(ptx::smem_u32(bar), parity, &ctrl->abort)) != 0; };
+  // record: x first key, y keys, z first query, w queries.  Own tiles (keys) are counted by n, tiles (own x queries) by g.
+
+  if (warp >= 12) {
+    ptx::setmaxnreg_dec<kFusedRegControl>();
+    if (warp == 12 && ptx::elect_one()) {
+      // ------------------------------------------------------------ TMA producer
+      bool ok = true;
+      uint32_t g = 0, n = 0;
+      int4 rec = fetch(blockIdx.x);
+      for (unsigned w = blockIdx.x; w < n_all && ok; w += gridDim.x) {
+        const int4 it = rec;
+        rec = fetch(w + gridDim.x);
+        const int nk = tiles(it.y), nq = tiles(it.w), col = head(w) * C::D;
+        if (nq == 0) continue;
+        for (int kt = 0; kt < nk && ok; ++kt, ++n) {
+          const uint32_t o = n % C::kOwn;
+          if (!wait(&ctrl->own_empty[o], ((n / C::kOwn) & 1) ^ 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bo = ptx::smem_u32(&ctrl->own_full[o]);
+          ptx::mbar_arrive_expect_tx(bo, 2 * C::kTile);
+          ptx::tma_load_2d(s_own + o * 2 * C::kTile, &map_k, bo, col, it.x + kt * kTR);
+          ptx::tma_load_2d(s_own + o * 2 * C::kTile + C::kTile, &map_v, bo, col, it.x + kt * kTR);
+          for (int j = 0; j < nq; ++j, ++g) {
+            const uint32_t s = g % C::kStages;
+            if (!wait(&ctrl->empty[s], ((g / C::kStages) & 1) ^ 1)) {
+              ok = false;
+              ++n;  // this own pair was issued: part of the drain below
+              break;
+            }
+            const uint32_t b = ptx::smem_u32(&ctrl->full[s]);
+            ptx::mbar_arrive_expect_tx(b, 2 * C::kTile);
+            ptx::tma_load_2d(s_oth + s * 2 * C::kTile, &map_q, b, col, it.z + j * kTR);
+            ptx::tma_load_2d(s_oth + s * 2 * C::kTile + C::kTile, &map_g, b, col, it.z + j * kTR);
+          }
+          if (!ok) break;
+        }
+      }
+      if (!ok) {
+        ctrl->abort = 1;
+        atomicOr(&g_attn_bwd_error, 1);
+      }
+      for (uint32_t k = n > (uint32_t)C::kOwn ? n - C::kOwn : 0; k < n; ++k)
+        ptx::mbar_wait(ptx::smem_u32(&ctrl->own_full[k % C::kOwn]), (k / C::kOwn) & 1);
+      for (uint32_t k = g > (uint32_t)C::kStages ? g - C::kStages : 0; k < g; ++k)
+        ptx::mbar_wait(ptx::smem_u32(&ctrl->full[k % C::kStages]), (k / C::kStages) & 1);
+    } else if (warp == 13 && ptx::elect_one()) {
+      // ------------------------------------------------------------ MMA issuer
+      constexpr uint32_t idesc_acc = ptx::umma_idesc_f16(FMT, kTR, 64, 0, 1);  // A K-major (or tensor memory), B MN-major
+      constexpr uint32_t idesc_dq = ptx::umma_idesc_f16(FMT, kTR, 64, 1, 1);   // A MN-major: dS transposed
+      const uint64_t d_own = ptx::umma_desc_kmajor_sw128(s_own), d_oth = ptx::umma_desc_kmajor_sw128(s_oth);
+      const uint64_t d_own_mn = ptx::umma_desc_mnmajor_sw128(s_own), d_oth_mn = ptx::umma_desc_mnmajor_sw128(s_oth);
+      const uint64_t d_ds = ptx::umma_desc_kmajor_sw128(s_ds), d_ds_mn = ptx::umma_desc_mnmajor_sw128(s_ds, kHalf);
+      // cursor of the tile whose S and dP are issued next
+      unsigned wa = blockIdx.x;
+      uint32_t ga = 0, na = 0;
+      int ja = 0, ka = 0, nka = 0, nqa = 0, len_q = 0;
+      int4 rec_a = fetch(wa);
+      auto settle = [&]() {
+        while (wa < n_all) {
+          const int4 it = rec_a;
+          rec_a = fetch(wa + gridDim.x);
+          nka = tiles(it.y), nqa = tiles(it.w), len_q = it.w;
+          if (nka > 0 && nqa > 0) return;
+          wa += gridDim.x;
+        }
+      };
+      settle();
+      auto scores = [&](uint32_t tm, int which, uint64_t* ready) {
+        const uint32_t s = ga % C::kStages, o = na % C::kOwn;
+        int nc = len_q - ja * kTR;
+        nc = nc > kTR ? kTR : nc;
+        const uint32_t idesc = ptx::umma_idesc_f16(FMT, kTR, (nc + 15) & ~15);
+        const uint64_t da = d_own + (uint64_t)((o * 2 + which) * (C::kTile >> 4)), db = d_oth + (uint64_t)((s * 2 + which) * (C::kTile >> 4));
+#pragma unroll
+        for (int k = 0; k < C::D / 16; ++k) ptx::umma_f16(tm, da + 2 * k, db + 2 * k, idesc, k != 0 ? 1u : 0u);
+        ptx::umma_commit(ptx::smem_u32(ready));
+      };
+      auto issue_s = [&]() -> bool {
+        if (ja == 0 && !wait(&ctrl->own_full[na % C::kOwn], (na / C::kOwn) & 1)) return false;
+        if (!wait(&ctrl->full[ga % C::kStages], (ga / C::kStages) & 1)) return false;
+        ptx::tc_fence_after_sync();
+        scores(tmem, 0, &ctrl->s_ready);
+        return true;
+      };
+      auto issue_dp = [&]() {
+        scores(tmem + 128, 1, &ctrl->dp_ready);
+        ++ga;
+        if (++ja == nqa) {
+          ja = 0;
+          ++na;
+          if (++ka == nka) {
+            ka = 0;
+            wa += gridDim.x;
+            settle();
+          }
+        }
+      };
+      bool ok = true;
+      if (wa < n_all) {
+        ok = issue_s();
+        if (ok) issue_dp();
+      }
+      uint32_t g = 0, n = 0;
+      int4 rec = fetch(blockIdx.x);
+      for (unsigned w = blockIdx.x; w < n_all && ok; w += gridDim.x) {
+        const int4 it = rec;
+        rec = fetch(w + gridDim.x);
+        const int nk = tiles(it.y), nq = tiles(it.w);
+        if (nq == 0) continue;
+        for (int kt = 0; kt < nk && ok; ++kt, ++n) {
+          const uint32_t o = n % C::kOwn;
+          const int rows = it.y - kt * kTR < kTR ? it.y - kt * kTR : kTR;
+          for (int j = 0; j < nq && ok; ++j, ++g) {
+            const uint32_t s = g % C::kStages;
+            const bool more = wa < n_all;
+            int nc = it.w - j * kTR;
+            nc = nc > kTR ? kTR : nc;
+            const int ksteps = (nc + 15) >> 4;
+            if (!wait(&ctrl->aux[s], (g / C::kStages) & 1)) { ok = false; break; }
+            if (j == 0 && n > 0 && !wait(&ctrl->acc_free, (n - 1) & 1)) { ok = false; break; }
+            if (!wait(&ctrl->p_ready, g & 1)) { ok = false; break; }
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int ks = 0; ks < kTR / 16; ++ks)  // dV += P dO
+              if (ks < ksteps)
+                ptx::umma_f16_ts(tmem + C::kAccV, tmem + C::kP + 8 * ks, d_oth_mn + (uint64_t)((s * 2 + 1) * (C::kTile >> 4) + ks * (2048 >> 4)),
+                                 idesc_acc, (j | ks) != 0 ? 1u : 0u);
+            if (more && !issue_s()) { ok = false; break; }
+            if (!wait(&ctrl->ds_ready, g & 1)) { ok = false; break; }
+            if (j == 0 && !wait(&ctrl->own_aux[o], (n / C::kOwn) & 1)) { ok = false; break; }
+            if (g > 0 && !wait(&ctrl->dq_free, (g - 1) & 1)) { ok = false; break; }
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int ks = 0; ks < kTR / 16; ++ks)  // dQ = dS^T K, over the tile's keys
+              if (ks * 16 < rows)
+                ptx::umma_f16(tmem + C::kAccQ, d_ds_mn + (uint64_t)(ks * (2048 >> 4)), d_own_mn + (uint64_t)(o * 2 * (C::kTile >> 4) + ks * (2048 >> 4)),
+                              idesc_dq, ks != 0 ? 1u : 0u);
+            ptx::umma_commit(ptx::smem_u32(&ctrl->dq_ready));
+#pragma unroll
+            for (int ks = 0; ks < kTR / 16; ++ks)  // dK += dS Q
+              if (ks < ksteps)
+                ptx::umma_f16(tmem + C::kAccK, d_ds + (uint64_t)((ks / 4) * (kHalf >> 4) + 2 * (ks % 4)),
+                              d_oth_mn + (uint64_t)(s * 2 * (C::kTile >> 4) + ks * (2048 >> 4)), idesc_acc, (j | ks) != 0 ? 1u : 0u);
+            ptx::umma_commit(ptx::smem_u32(&ctrl->empty[s]));
+            if (j == nq - 1) {
+              ptx::umma_commit(ptx::smem_u32(&ctrl->own_done));
+              ptx::umma_commit(ptx::smem_u32(&ctrl->own_empty[o]));
+            }
+            if (more) issue_dp();
+          }
+        }
+      }
+      if (!ok) {
+        ctrl->abort = 1;
+        atomicOr(&g_attn_bwd_error, 2);
+      }
+      ptx::umma_commit(ptx::smem_u32(&ctrl->done));
+      ptx::mbar_wait(ptx::smem_u32(&ctrl->done), 0);
+    } else if (warp >= 14) {
+      // ------------------------------------------------------------ helpers: warp 14 lse, A tiles and own keys, warp 15 D and B tiles
+      const int me = warp - 14;
+      auto clear = [&](uint32_t tile, int from) {  // rows of a landed tile past the sequence's end, up to the next 16
+        const int to = (from + 15) & ~15;
+        for (int i = lane; i < (to - from) * 8; i += 32) {
+          const int r = from + i / 8;
+          const uint32_t addr = tile + (r >> 3) * 1024 + (r & 7) * 128 + (i % 8) * 16;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0u) : "memory");
+        }
+        ptx::fence_proxy_async();
+        __syncwarp();
+      };
+      bool ok = true;
+      uint32_t g = 0, n = 0;
+      auto fetch_seq = [&](unsigned w) { return me == 1 && a.top != nullptr && w < n_all ? __ldg(t.seqs.seq + w / H) : 0; };
+      unsigned w = blockIdx.x;
+      int4 rec = fetch(w), rec_next = fetch(w + gridDim.x);
+      int seq = fetch_seq(w), seq_next = fetch_seq(w + gridDim.x);
+      int j = 0, kt = 0, nk = 0, nq = 0;
+      unsigned top = 0;
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      auto step = [&]() {
+        w += gridDim.x;
+        rec = rec_next, seq = seq_next;
+        rec_next = fetch(w + gridDim.x), seq_next = fetch_seq(w + gridDim.x);
+      };
+      auto open = [&]() {
+        for (; w < n_all; step()) {
+          nk = tiles(rec.y), nq = tiles(rec.w);
+          if (nk > 0 && nq > 0) break;
+        }
+        if (me == 1 && a.top != nullptr && w < n_all) top = a.top[(int64_t)seq * H + head(w)];
+      };
+      auto load = [&]() {
+        const float* src = (me == 0 ? a.lse : a.delta) + (int64_t)head(w) * a.q_tokens + rec.z + j * kTR;
+        const int nc = rec.w - j * kTR;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = lane + 32 * k < nc ? src[lane + 32 * k] : 0.0f;
+      };
+      open();
+      if (w < n_all) load();
+      while (w < n_all) {
+        const uint32_t s = g % C::kStages, o = n % C::kOwn;
+        const unsigned top_c = top;
+        const float vc[4] = {v[0], v[1], v[2], v[3]};
+        const bool first = j == 0;
+        const uint32_t own_parity = (n / C::kOwn) & 1;
+        const int rows = rec.y - kt * kTR < kTR ? rec.y - kt * kTR : kTR;
+        int nc = rec.w - j * kTR;
+        nc = nc > kTR ? kTR : nc;
+        if (++j == nq) {  // on to the next tile, whose statistics are fetched before this one's are waited for
+          j = 0;
+          ++n;
+          if (++kt == nk) {
+            kt = 0;
+            step();
+            open();
+          }
+        }
+        if (w < n_all) load();
+        if (me == 0 && first) {
+          if (!wait_warp(&ctrl->own_full[o], own_parity)) {
+            ok = false;
+            break;
+          }
+          clear(s_own + o * 2 * C::kTile, rows);
+          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->own_aux[o]));
+        }
+        if (!wait_warp(&ctrl->full[s], (g / C::kStages) & 1)) {
+          ok = false;
+          break;
+        }
+        float* dst = s_stats + s * (C::kStats / 4) + me * kTR;
+        const float fc = me == 1 && a.top != nullptr ? -scale_of(top_c) : -1.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dst[lane + 32 * k] = vc[k] * fc;
+        clear(s_oth + (s * 2 + me) * C::kTile, nc);
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->aux[s]));
+        ++g;
+      }
+      if (!ok && lane == 0) {
+        ctrl->abort = 1;
+        atomicOr(&g_attn_bwd_error, 1);
+      }
+    }
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------ dQ: one thread per query row of the tile
+    ptx::setmaxnreg_dec<kFusedRegAdd>();
+    const int row = (warp - 8) * 32 + lane;
+    const uint32_t tl = tmem + ((uint32_t)((warp - 8) * 32) << 16) + C::kAccQ;
+    const uint32_t stage = ptx::smem_u32(smem) + (uint32_t)C::kStaging + (uint32_t)warp * 2048u;
+    bool ok = true;
+    uint32_t g = 0;
+    int4 rec = fetch(blockIdx.x);
+    for (unsigned w = blockIdx.x; w < n_all; w += gridDim.x) {
+      const int4 it = rec;
+      rec = fetch(w + gridDim.x);
+      const int nk = tiles(it.y), nq = tiles(it.w), h = head(w);
+      if (nk == 0) {  // queries without keys: zeros
+        for (int r = row; r < it.w; r += kTR) {
+          uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(a.dq) + ((int64_t)it.z + r) * a.lddq + (int64_t)h * C::D);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        continue;
+      }
+      const float f = a.scaling / grad_scale(a, t.seqs.seq, w / H, h);
+      for (int kt = 0; kt < nk; ++kt) {
+        for (int j = 0; j < nq; ++j, ++g) {
+          const bool live = j * kTR + row < it.w, first = kt == 0, last = kt == nk - 1;
+          const int64_t token = (int64_t)it.z + j * kTR + row;
+          float4* sc = t.scratch + (int64_t)h * 16 * a.q_tokens + token;
+          T* out = static_cast<T*>(a.dq) + (token - lane) * a.lddq + (int64_t)h * C::D;  // the warp's first row
+          float4 old[8];
+          if (!first && live) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) old[i] = sc[(int64_t)i * a.q_tokens];
+          }
+          if (ok && !wait_warp(&ctrl->dq_ready, g & 1)) ok = false;
+          if (ok) ptx::tc_fence_after_sync();
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t r[32];
+            if (ok) {
+              ptx::tmem_ld_32x32b_x32(tl + 32 * x, r);
+              ptx::tmem_ld_wait();
+            }
+            if (x == 1) {
+              ptx::tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->dq_free));
+            }
+            if (!ok) continue;
+            if (!first && live) {
+              if (x == 1) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) old[i] = sc[(int64_t)(8 + i) * a.q_tokens];
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                r[4 * i] = __float_as_uint(__uint_as_float(r[4 * i]) + old[i].x);
+                r[4 * i + 1] = __float_as_uint(__uint_as_float(r[4 * i + 1]) + old[i].y);
+                r[4 * i + 2] = __float_as_uint(__uint_as_float(r[4 * i + 2]) + old[i].z);
+                r[4 * i + 3] = __float_as_uint(__uint_as_float(r[4 * i + 3]) + old[i].w);
+              }
+            }
+            if (last) {
+              uint4 v[4];
+              pack_row<FMT>(r, f, v);
+              store_rows(stage, v, reinterpret_cast<uint8_t*>(out + 32 * x), a.lddq * 2, it.w - j * kTR - (warp - 8) * 32);
+            } else if (live) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                sc[(int64_t)(8 * x + i) * a.q_tokens] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
+                                                                    __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+            }
+          }
+        }
+      }
+    }
+    if (!ok && lane == 0) {
+      ctrl->abort = 1;
+      atomicOr(&g_attn_bwd_error, 4);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax, one thread per key row and half of the columns
+    ptx::setmaxnreg_inc<kFusedRegSoftmax>();
+    const int q = warp & 3, wg = warp >> 2;
+    const int row = q * 32 + lane;
+    const uint32_t tl = tmem + ((uint32_t)(q * 32) << 16);
+    const float scale = a.scaling * kLog2e;
+    const uint64_t sc2 = ptx::f32x2_pack(scale, scale);
+    bool ok = true;
+    uint32_t g = 0, n = 0;
+    auto arrive = [&](uint64_t* bar) {
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(bar));
+    };
+    struct Pending {
+      bool any, live;
+      T* out;  // of the warp's first row
+      int rows;
+      float f;
+    } pend = {false, false, nullptr, 0, 0.0f};
+    const uint32_t stage = ptx::smem_u32(smem) + (uint32_t)C::kStaging + (uint32_t)warp * 2048u;
+    const int64_t row_bytes = (wg == 0 ? a.lddv : a.lddk) * 2;
+    auto write_out = [&](const Pending& o, bool zeros) {  // warps 0-3: dV, warps 4-7: dK
+#pragma unroll
+      for (int c = 0; c < C::D; c += 32) {
+        uint32_t r[32];
+        uint4 v[4];
+        if (!zeros) {
+          ptx::tmem_ld_32x32b_x32(tl + (wg == 0 ? C::kAccV : C::kAccK) + c, r);
+          ptx::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0u;
+        }
+        pack_row<FMT>(r, o.f, v);
+        store_rows(stage, v, reinterpret_cast<uint8_t*>(o.out + c), row_bytes, o.rows);
+      }
+    };
+    auto flush = [&]() {
+      if (!pend.any) return;
+      if (ok && !wait_warp(&ctrl->own_done, n & 1)) ok = false;
+      ++n;
+      if (ok && pend.live) {
+        ptx::tc_fence_after_sync();
+        write_out(pend, false);
+      }
+      arrive(&ctrl->acc_free);
+      pend.any = false;
+    };
+    auto fetch_seq = [&](unsigned w) { return a.top != nullptr && w < n_all ? __ldg(t.seqs.seq + w / H) : 0; };
+    int4 rec = fetch(blockIdx.x), rec_next = fetch(blockIdx.x + gridDim.x);
+    int seq_next = fetch_seq(blockIdx.x + gridDim.x);
+    unsigned top = a.top != nullptr ? a.top[(int64_t)fetch_seq(blockIdx.x) * H + head(blockIdx.x)] : 0u;
+    for (unsigned w = blockIdx.x; w < n_all; w += gridDim.x) {
+      const int4 it = rec;
+      const float gs = a.top != nullptr ? scale_of(top) : 1.0f;
+      rec = rec_next;
+      if (a.top != nullptr && w + gridDim.x < n_all) top = a.top[(int64_t)seq_next * H + head(w + gridDim.x)];
+      rec_next = fetch(w + 2 * gridDim.x);
+      seq_next = fetch_seq(w + 2 * gridDim.x);
+      const int nk = tiles(it.y), nq = tiles(it.w), h = head(w);
+      const uint64_t gs2 = ptx::f32x2_pack(gs, gs);
+      for (int kt = 0; kt < nk; ++kt) {
+        const int rows = it.y - kt * kTR < kTR ? it.y - kt * kTR : kTR;
+        const bool live = q * 32 < rows, whole = q * 32 + 32 <= rows;  // warp-uniform
+        for (int j = 0; j < nq; ++j, ++g) {
+          const uint32_t s = g % C::kStages;
+          int nc = it.w - j * kTR;
+          nc = nc > kTR ? kTR : nc;
+          const float* stats = s_stats + s * (C::kStats / 4);
+          float p[2][32];
+          // ---- P
+          if (ok && !wait_warp(&ctrl->s_ready, g & 1)) ok = false;
+          if (ok && !wait_warp(&ctrl->aux[s], (g / C::kStages) & 1)) ok = false;
+          if (ok && live) {
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {  // (a chunk at a time: both with P do not fit the registers)
+              const int c0 = (wg + 2 * k) * 32;
+              if (c0 < nc) {
+                uint32_t sv[32], pk[16];
+                ptx::tmem_ld_32x32b_x32(tl + c0, sv);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                  const ulonglong2 nl = *reinterpret_cast<const ulonglong2*>(stats + c0 + i);
+                  const uint64_t x0 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), sc2, nl.x);
+                  const uint64_t x1 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), sc2, nl.y);
+                  float e0, e1, e2, e3;
+                  ptx::f32x2_unpack(x0, e0, e1);
+                  ptx::f32x2_unpack(x1, e2, e3);
+                  p[k][i] = ptx::ex2_approx(e0);
+                  p[k][i + 1] = ptx::ex2_approx(e1);
+                  p[k][i + 2] = ptx::ex2_approx(e2);
+                  p[k][i + 3] = ptx::ex2_approx(e3);
+                }
+                cut_columns(p[k], c0, nc);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) pk[i] = pack2<FMT>(p[k][2 * i], p[k][2 * i + 1]);
+                ptx::tmem_st_32x32b_x16(tl + C::kP + 16 * (wg + 2 * k), pk);
+              }
+            }
+            ptx::tmem_st_wait();
+          }
+          arrive(&ctrl->p_ready);
+          if (j == 0) flush();
+          // ---- dS
+          if (ok && !wait_warp(&ctrl->dp_ready, g & 1)) ok = false;
+          if (ok && live) {
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int chunk = wg + 2 * k, c0 = chunk * 32;
+              if (c0 < nc) {
+                uint32_t sv[32];
+                ptx::tmem_ld_32x32b_x32(tl + 128 + c0, sv);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                  const ulonglong2 nd = *reinterpret_cast<const ulonglong2*>(stats + kTR + c0 + i);
+                  const uint64_t x0 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), gs2, nd.x);
+                  const uint64_t x1 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), gs2, nd.y);
+                  ptx::f32x2_unpack(ptx::f32x2_mul(ptx::f32x2_pack(p[k][i], p[k][i + 1]), x0), p[k][i], p[k][i + 1]);
+                  ptx::f32x2_unpack(ptx::f32x2_mul(ptx::f32x2_pack(p[k][i + 2], p[k][i + 3]), x1), p[k][i + 2], p[k][i + 3]);
+                }
+                cut_columns(p[k], c0, nc);
+                uint32_t pk[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) pk[i] = pack2<FMT>(p[k][2 * i], p[k][2 * i + 1]);
+                // keys past the end are summed over by dQ: zeros (again in a loop of zero or one trips)
+#pragma unroll 1
+                for (int ragged = whole ? 0 : 1; ragged > 0; --ragged) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) pk[i] = row < rows ? pk[i] : 0u;
+                }
+                // row = key, 64 queries a half, 128-byte swizzle: eight rows' 16-byte pieces fall into different banks
+                const uint32_t base = s_ds + (chunk >> 1) * kHalf + (row >> 3) * 1024 + (row & 7) * 128;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t addr = base + ((((chunk & 1) * 4 + i) ^ (row & 7)) << 4);
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(pk[4 * i]), "r"(pk[4 * i + 1]), "r"(pk[4 * i + 2]),
+                               "r"(pk[4 * i + 3])
+                               : "memory");
+                }
+              }
+            }
+            ptx::fence_proxy_async();  // the tensor core reads dS
+          }
+          arrive(&ctrl->ds_ready);
+        }
+        Pending o;
+        o.any = true;
+        o.live = live;
+        o.rows = rows - q * 32;
+        o.f = wg == 0 ? 1.0f : a.scaling / gs;
+        o.out = static_cast<T*>(wg == 0 ? a.dv : a.dk) + ((int64_t)it.x + kt * kTR + q * 32) * (wg == 0 ? a.lddv : a.lddk) + (int64_t)h * C::D;
+        if (nq > 0) pend = o;
+        else if (ok && live) write_out(o, true);  // keys without queries: zeros
+      }
+    }
+    flush();
+    if (!ok && lane == 0) {
+      ctrl->abort = 1;
+      atomicOr(&g_attn_bwd_error, 4);
+    }
+  }
+
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 13) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int FMT>
+int launch_fused(const BwdArgs& a, int64_t k_tokens, int dtype, const ListOut& seqs, float* scratch, cudaStream_t st) {
+  using C = Fused;
+  const int64_t E = (int64_t)a.H * C::D;
+  CUtensorMap map_q, map_k, map_v, map_g;
+  if (!make_tile_map(&map_q, {a.q, a.q_tokens, E, a.ldq}, dtype) || !make_tile_map(&map_k, {a.k, k_tokens, E, a.ldk}, dtype) ||
+      !make_tile_map(&map_v, {a.v, k_tokens, E, a.ldv}, dtype) || !make_tile_map(&map_g, {a.grad, a.q_tokens, E, E}, dtype))
+    return NTB200_LAUNCH_FAILED;
+  static std::atomic<int> configured[kMaxDevices];
+  if (!once_per_device(configured, [] {
+        return cudaFuncSetAttribute(attn_bwd_fused_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) == cudaSuccess;
+      }))
+    return NTB200_LAUNCH_FAILED;
+  int dev = 0, sms = kNumSMs;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t grid = a.batch * a.H < sms ? a.batch * a.H : sms;
+  const FusedArgs t = {a, seqs, reinterpret_cast<float4*>(scratch)};
+  attn_bwd_fused_kernel<FMT><<<(unsigned)grid, kFusedThreads, C::kSmem, st>>>(map_q, map_k, map_v, map_g, t);
+  return status_from_cuda(cudaGetLastError());
 }
 
 template <int FMT, int D>
@@ -643,6 +1298,10 @@ int attn_bwd_tcgen05_launch(const BwdArgs& a, int64_t k_tokens, int dtype, const
   const int64_t items = (kv_capacity + q_capacity) * a.H;
   if (dtype == NTB200_F16) return a.d == 64 ? launch<0, 64>(a, k_tokens, dtype, kv, qi, items, st) : launch<0, 128>(a, k_tokens, dtype, kv, qi, items, st);
   return a.d == 64 ? launch<1, 64>(a, k_tokens, dtype, kv, qi, items, st) : launch<1, 128>(a, k_tokens, dtype, kv, qi, items, st);
+}
+
+int attn_bwd_fused_launch(const BwdArgs& a, int64_t k_tokens, int dtype, const ListOut& seqs, float* scratch, cudaStream_t st) {
+  return dtype == NTB200_F16 ? launch_fused<0>(a, k_tokens, dtype, seqs, scratch, st) : launch_fused<1>(a, k_tokens, dtype, seqs, scratch, st);
 }
 
 int attn_bwd_tcgen05_error_flags_read_and_clear() {

@@ -336,11 +336,11 @@ __device__ __forceinline__ uint64_t umma_desc_kmajor_sw128(uint32_t smem_addr) {
 
 // Descriptor for an MN-major operand tile written by TMA with 128-byte swizzle: each K index is one
 // 128-byte row of 64 two-byte elements along M/N, 8-row groups 1024 bytes apart (stride byte offset);
-// the leading byte offset would step to the next 64 elements along M/N and is unused for a 64-wide tile.
-__device__ __forceinline__ uint64_t umma_desc_mnmajor_sw128(uint32_t smem_addr) {
+// the leading byte offset steps to the next 64 elements along M/N (unused for a 64-wide tile).
+__device__ __forceinline__ uint64_t umma_desc_mnmajor_sw128(uint32_t smem_addr, uint32_t leading_bytes = 16) {
   uint64_t d = 0;
   d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(leading_bytes >> 4) << 16;
   d |= (uint64_t)(1024u >> 4) << 32;
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;

@@ -251,7 +251,7 @@ void attention_forward(const AttentionShape& s, const void* q, const void* k, co
 void attention_backward(const AttentionShape& s, const Tensor& grad, const void* q, const void* k, const void* v, int64_t ldq, int64_t ldkv,
                         const Tensor& out, const Tensor& lse, void* dq, void* dk, void* dv, const Tensor& meta_q, const Tensor& meta_k) {
   const int dt = dtype_code(out.scalar_type());
-  const size_t bytes = ntb200_varlen_attention_backward_workspace_bytes(s.B, s.Tq, s.Tk, (int)s.H, (int)s.d, dt);
+  const size_t bytes = ntb200_varlen_attention_backward_workspace_bytes(s.B, s.Tq, s.Tk, (int)s.H, (int)s.d, s.longest_q, s.longest_k, dt, 0);
   Tensor ws = byte_workspace(bytes, out);
   check_rc(ntb200_varlen_attention_backward(grad.data_ptr(), q, ldq, k, ldkv, v, ldkv, out.data_ptr(), lse.data_ptr<float>(), dq, ldq, dk, ldkv,
                                             dv, ldkv, meta_q.data_ptr<int64_t>(), s.row_q, meta_k.data_ptr<int64_t>(), s.row_k, s.B, s.Tq, s.Tk,

@@ -269,8 +269,8 @@ def _cabi_backward(q, k, v, g, lq, lk, heads, path, ld_extra=0):
     ws = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
     _cabi.check("train", lib.ntb200_varlen_attention_train(
         q.data_ptr(), E, k.data_ptr(), E, v.data_ptr(), E, out.data_ptr(), lse.data_ptr(), off[0].data_ptr(), 1, off[1].data_ptr(), 1, B, Tq, Tk,
-        heads, d, max(lq), scaling, code, path if path < 3 or d == 64 else 2, ws.data_ptr(), n, stream_ptr()))
-    n = lib.ntb200_varlen_attention_backward_workspace_bytes(B, Tq, Tk, heads, d, code)
+        heads, d, max(lq), scaling, code, min(path, 3) if path < 3 or d == 64 else 2, ws.data_ptr(), n, stream_ptr()))
+    n = lib.ntb200_varlen_attention_backward_workspace_bytes(B, Tq, Tk, heads, d, max(lq), max(lk), code, path)
     ws = torch.full((n + 64,), 0xAB, dtype=torch.uint8, device="cuda")
     wide = E + ld_extra
     grads = [torch.full((t.size(0) + 3, wide), 7.0, dtype=q.dtype, device="cuda") for t in (q, k, v)]
@@ -288,7 +288,8 @@ def _cabi_backward(q, k, v, g, lq, lk, heads, path, ld_extra=0):
 
 @pytest.mark.parametrize("path,dtype,d", [(1, torch.float32, 64), (1, torch.bfloat16, 64), (1, torch.float16, 72), (2, torch.float16, 32),
                                           (2, torch.bfloat16, 64), (2, torch.float16, 64), (2, torch.bfloat16, 128), (2, torch.float16, 128),
-                                          (3, torch.bfloat16, 64), (3, torch.float16, 64), (3, torch.bfloat16, 128), (3, torch.float16, 128)],
+                                          (3, torch.bfloat16, 64), (3, torch.float16, 64), (3, torch.bfloat16, 128), (3, torch.float16, 128), (4, torch.bfloat16, 64),
+                                          (4, torch.float16, 64)],
                          ids=str)
 def test_attention_backward_paths(cuda_device, path, dtype, d):
     nt.device_error_flags()

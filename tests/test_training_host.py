@@ -98,7 +98,7 @@ def test_cabi_rejects_bad_arguments_without_launching(native_libs):
         return lib.ntb200_varlen_attention_backward(g, 16, ld, 16, ld, 16, ld, 16, 16, dq, ld, 16, ld, 16, ld, offs, row, offs, row, batch, tq,
                                                     tk, heads, d, 4, 4, 0.125, dtype, path, ws, n, None)
 
-    need = lib.ntb200_varlen_attention_backward_workspace_bytes(1, 4, 4, 1, 64, 2)
+    need = lib.ntb200_varlen_attention_backward_workspace_bytes(1, 4, 4, 1, 64, 4, 4, 2, 0)
     assert need > 0
     assert backward(ld=63) == -1 and backward(g=None) == -1 and backward(dq=None) == -1 and backward(row=0) == -1 and backward(path=9) == -1
     assert backward(dtype=3) == -2 and backward(d=257, ld=300) == -7 and backward(ws=None) == -1 and backward(n=need - 1) == -6
