@@ -66,6 +66,27 @@ struct Ctrl {
   volatile int abort;
 };
 
+// Four exponentials 2^x.  bf16: two of every eight on the FMA pipe (a polynomial, relative error 1.9e-4 where rounding P to bf16
+// costs up to 3.9e-3): the 16 results per clock of the MUFU units are what the P phase waits for.  fp16 rounds to 4.9e-4, so there
+// all go through MUFU.
+template <int FMT, bool POLY>
+__device__ __forceinline__ void ex2_four(uint64_t x0, uint64_t x1, float* p) {
+  float e0, e1, e2, e3;
+  ptx::f32x2_unpack(x0, e0, e1);
+  p[0] = ptx::ex2_approx(e0);
+  p[1] = ptx::ex2_approx(e1);
+  ptx::f32x2_unpack(x1, e2, e3);
+  if (FMT == 1 && POLY) {
+    const uint64_t x = ptx::f32x2_pack(ptx::fmax_nan(e2, -126.0f), ptx::fmax_nan(e3, -126.0f));
+    ptx::ex2_poly_x2(x, p[2], p[3]);
+    // (the polynomial's exponent arithmetic loses a NaN: 0 x brings it back)
+    ptx::f32x2_unpack(ptx::f32x2_fma(x, ptx::f32x2_pack(0.0f, 0.0f), ptx::f32x2_pack(p[2], p[3])), p[2], p[3]);
+  } else {
+    p[2] = ptx::ex2_approx(e2);
+    p[3] = ptx::ex2_approx(e3);
+  }
+}
+
 // Columns past the end of the sequence have no probability, whatever was in their columns (in a loop of zero or one trips, so that
 // whole chunks do not pay for the selects).
 __device__ __forceinline__ void cut_columns(float (&x)[32], int c0, int nc) {
@@ -142,7 +163,7 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       ptx::mbar_init(ptx::smem_u32(&ctrl->empty[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&ctrl->aux[s]), 2);  // both helper warps
     }
-    ptx::mbar_init(ptx::smem_u32(&ctrl->s_ready), 1);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->s_ready), 3);  // the commit and both helper warps
     ptx::mbar_init(ptx::smem_u32(&ctrl->p_ready), 8);
     ptx::mbar_init(ptx::smem_u32(&ctrl->p_done), 1);
     ptx::mbar_init(ptx::smem_u32(&ctrl->dp_ready), 1);
@@ -419,6 +440,12 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         ptx::fence_proxy_async();  // the tensor core reads the cleared rows
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->aux[s]));
+        // the statistics count into s_ready of their tile, whose phase begins when the tile before it is ready
+        if (g > 0 && !wait_warp(&ctrl->s_ready, (g - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->s_ready));
         ++g;
       }
       if (!ok && lane == 0) {
@@ -489,13 +516,8 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             if constexpr (decltype(is_kv)::value) n = *reinterpret_cast<const ulonglong2*>(stats + c0 + i);
             const uint64_t x0 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[k][i]), __uint_as_float(sv[k][i + 1])), sc2, n.x);
             const uint64_t x1 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[k][i + 2]), __uint_as_float(sv[k][i + 3])), sc2, n.y);
-            float e0, e1, e2, e3;
-            ptx::f32x2_unpack(x0, e0, e1);
-            ptx::f32x2_unpack(x1, e2, e3);
-            p[k][i] = ptx::ex2_approx(e0);
-            p[k][i + 1] = ptx::ex2_approx(e1);
-            p[k][i + 2] = ptx::ex2_approx(e2);
-            p[k][i + 3] = ptx::ex2_approx(e3);
+            if (i & 4) ex2_four<FMT, true>(x0, x1, p[k] + i);
+            else ex2_four<FMT, false>(x0, x1, p[k] + i);
           }
           cut_columns(p[k], c0, nc);
         }
@@ -571,7 +593,6 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         float p[2][32];
         // ---- P
         if (ok && !wait_warp(&ctrl->s_ready, g & 1)) ok = false;
-        if (ok && kv && !wait_warp(&ctrl->aux[s], (g / C::kStages) & 1)) ok = false;
         if (ok && live) {
           ptx::tc_fence_after_sync();
 #pragma unroll
@@ -707,7 +728,7 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       ptx::mbar_init(ptx::smem_u32(&ctrl->empty[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&ctrl->aux[s]), 2);
     }
-    ptx::mbar_init(ptx::smem_u32(&ctrl->s_ready), 1);
+    ptx::mbar_init(ptx::smem_u32(&ctrl->s_ready), 3);  // the commit and both helper warps
     ptx::mbar_init(ptx::smem_u32(&ctrl->p_ready), 8);
     ptx::mbar_init(ptx::smem_u32(&ctrl->dp_ready), 1);
     ptx::mbar_init(ptx::smem_u32(&ctrl->ds_ready), 8);
@@ -980,6 +1001,12 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         for (int k = 0; k < 4; ++k) dst[lane + 32 * k] = vc[k] * fc;
         clear(s_oth + (s * 2 + me) * C::kTile, nc);
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->aux[s]));
+        // the statistics count into s_ready of their tile, whose phase begins when the tile before it is ready
+        if (g > 0 && !wait_warp(&ctrl->s_ready, (g - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->s_ready));
         ++g;
       }
       if (!ok && lane == 0) {
@@ -1140,7 +1167,6 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           float p[2][32];
           // ---- P
           if (ok && !wait_warp(&ctrl->s_ready, g & 1)) ok = false;
-          if (ok && !wait_warp(&ctrl->aux[s], (g / C::kStages) & 1)) ok = false;
           if (ok && live) {
             ptx::tc_fence_after_sync();
 #pragma unroll
@@ -1155,13 +1181,8 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                   const ulonglong2 nl = *reinterpret_cast<const ulonglong2*>(stats + c0 + i);
                   const uint64_t x0 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), sc2, nl.x);
                   const uint64_t x1 = ptx::f32x2_fma(ptx::f32x2_pack(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), sc2, nl.y);
-                  float e0, e1, e2, e3;
-                  ptx::f32x2_unpack(x0, e0, e1);
-                  ptx::f32x2_unpack(x1, e2, e3);
-                  p[k][i] = ptx::ex2_approx(e0);
-                  p[k][i + 1] = ptx::ex2_approx(e1);
-                  p[k][i + 2] = ptx::ex2_approx(e2);
-                  p[k][i + 3] = ptx::ex2_approx(e3);
+                  if (i & 4) ex2_four<FMT, true>(x0, x1, p[k] + i);
+                  else ex2_four<FMT, false>(x0, x1, p[k] + i);
                 }
                 cut_columns(p[k], c0, nc);
 #pragma unroll

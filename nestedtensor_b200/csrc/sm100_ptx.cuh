@@ -132,6 +132,12 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// maximum that is NaN when an operand is
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 // 2^x for a pair, same polynomial as ex2_poly; x must already be >= -126 (the caller clamps).
 __device__ __forceinline__ void ex2_poly_x2(uint64_t x, float& r0, float& r1) {
   const uint64_t magic = f32x2_pack(12582912.0f, 12582912.0f);

@@ -248,6 +248,23 @@ def test_attention_does_not_mix_sequences(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_attention_carries_nan(cuda_device, dtype):
+    """One NaN query reaches its own output row and dQ row and, through its probabilities, every dK and dV row of its sequence
+    and no other's, at every position in the kernels' tiles."""
+    lengths, H, d = [40, 150], 1, 64
+    q, k, v, g, qs, _ = _attend_inputs(lengths, lengths, H, d, dtype, 16)
+    for row in list(range(40, 56)) + [100, 167, 168, 189]:
+        q2 = q.clone()
+        q2[row] = float("nan")
+        got = _run_self(q2, k, v, g, qs, H)
+        for name in ("out", "dq"):
+            bad = torch.isnan(got[name]).all(1)
+            assert bool(bad[row]) and int(torch.isnan(got[name]).any(1).sum()) == 1, (name, row)
+        for name in ("dk", "dv"):
+            assert bool(torch.isnan(got[name][40:]).all()) and not bool(torch.isnan(got[name][:40]).any()), (name, row)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_attention_large_logits_and_gradients(cuda_device, dtype):
     """Probabilities that are one or nothing; gradients under and over the ordinary (fp16: a loss scale's)."""
     lengths = [64, 190]
