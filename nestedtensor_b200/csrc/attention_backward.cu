@@ -25,14 +25,26 @@ namespace ntb200 {
 namespace {
 
 // ------------------------------------------------------------------ work lists and D = rowsum(dO * O), one launch
-// An item for every `tile` rows of the own side (keys for dK / dV, queries for dQ), longest other side first.  A sequence whose other side is empty keeps its items: their gradients
-// are zeros, written by a block that walks no tile at all.  One block.
+// Which kernel takes a sequence depends on its own lengths only, so that a batch cut in parts gives the bits of the whole.  A class
+// of sequences: longest side in (over, to].
+struct Class {
+  int64_t over, to;
+  __host__ __device__ bool any() const { return to > over; }
+  __device__ __forceinline__ bool has(int64_t n, int64_t m) const {
+    const int64_t l = n > m ? n : m;
+    return l > over && l <= to;
+  }
+};
+
+// An item for every `tile` rows of the own side (keys for dK / dV, queries for dQ) of the class's sequences, longest other side first.
+// A sequence whose other side is empty keeps its items: their gradients are zeros, written by a block that walks no tile at
+// all.  One block.
 constexpr int kListBuckets = 32;
 constexpr int kPrepThreads = 256;
 
 __device__ __forceinline__ void build_backward_items(const int64_t* __restrict__ offsets_own, int64_t row_elems_own,
                                                      const int64_t* __restrict__ offsets_other, int64_t row_elems_other, int64_t batch,
-                                                     int tile, const ListOut& out) {
+                                                     int tile, const Class& cls, const ListOut& out) {
   __shared__ int s_cnt[kListBuckets], s_base[kListBuckets];
   if (threadIdx.x < kListBuckets) s_cnt[threadIdx.x] = 0;
   __syncthreads();
@@ -42,7 +54,7 @@ __device__ __forceinline__ void build_backward_items(const int64_t* __restrict__
   };
   for (int64_t b = threadIdx.x; b < batch; b += kPrepThreads) {
     const int64_t n = (offsets_own[b + 1] - offsets_own[b]) / row_elems_own, m = (offsets_other[b + 1] - offsets_other[b]) / row_elems_other;
-    if (n > 0) atomicAdd(&s_cnt[bucket(m)], (int)((n + tile - 1) / tile));
+    if (n > 0 && cls.has(n, m)) atomicAdd(&s_cnt[bucket(m)], (int)((n + tile - 1) / tile));
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -56,7 +68,7 @@ __device__ __forceinline__ void build_backward_items(const int64_t* __restrict__
   __syncthreads();
   for (int64_t b = threadIdx.x; b < batch; b += kPrepThreads) {
     const int64_t n = (offsets_own[b + 1] - offsets_own[b]) / row_elems_own, m = (offsets_other[b + 1] - offsets_other[b]) / row_elems_other;
-    if (n <= 0) continue;
+    if (n <= 0 || !cls.has(n, m)) continue;
     const int tiles = (int)((n + tile - 1) / tile);
     const int pos = atomicAdd(&s_base[bucket(m)], tiles);  // (the order inside a bucket decides nothing but the schedule)
     const int t0 = (int)(offsets_own[b] / row_elems_own), o0 = (int)(offsets_other[b] / row_elems_other);
@@ -69,11 +81,11 @@ __device__ __forceinline__ void build_backward_items(const int64_t* __restrict__
 }
 
 __global__ void __launch_bounds__(kPrepThreads) query_items_kernel(BwdArgs a, int tile, ListOut l) {
-  build_backward_items(a.offsets_q, a.row_elems_q, a.offsets_k, a.row_elems_k, a.batch, tile, l);
+  build_backward_items(a.offsets_q, a.row_elems_q, a.offsets_k, a.row_elems_k, a.batch, tile, Class{0, INT64_MAX}, l);
 }
 
-// An item for every sequence with rows on either side: (first key, keys, first query, queries), most tile pairs first.  One block.
-__device__ __forceinline__ void build_sequence_items(const BwdArgs& a, const ListOut& out) {
+// An item for every sequence of the class: (first key, keys, first query, queries), most tile pairs first.  One block.
+__device__ __forceinline__ void build_sequence_items(const BwdArgs& a, const Class& cls, const ListOut& out) {
   __shared__ int s_cnt[kListBuckets], s_base[kListBuckets];
   if (threadIdx.x < kListBuckets) s_cnt[threadIdx.x] = 0;
   __syncthreads();
@@ -88,7 +100,7 @@ __device__ __forceinline__ void build_sequence_items(const BwdArgs& a, const Lis
   };
   for (int64_t b = threadIdx.x; b < a.batch; b += kPrepThreads) {
     const int4 l = lengths(b);
-    if (l.y > 0 || l.w > 0) atomicAdd(&s_cnt[bucket(l)], 1);
+    if (cls.has(l.y, l.w)) atomicAdd(&s_cnt[bucket(l)], 1);
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -102,31 +114,37 @@ __device__ __forceinline__ void build_sequence_items(const BwdArgs& a, const Lis
   __syncthreads();
   for (int64_t b = threadIdx.x; b < a.batch; b += kPrepThreads) {
     const int4 l = lengths(b);
-    if (l.y <= 0 && l.w <= 0) continue;
+    if (!cls.has(l.y, l.w)) continue;
     const int pos = atomicAdd(&s_base[bucket(l)], 1);
     out.items[pos] = l;
     out.seq[pos] = (int)b;
   }
 }
 
-// Blocks 0 and 1 build the lists (tile 0: block 0 the list of sequences); every warp of the others takes one query token: D of all its heads, and (fp16) the largest
+// The lists of a backward pass: tiles of the short and the long class's sequences, the sequences of the middle class.
+struct Lists {
+  ListOut kv, qi, long_kv, long_qi, mid;
+};
+struct Plan {
+  Class short_, mid, long_;
+  int tile;  // rows of the short class's tiles; the long class's have 128
+};
+constexpr int kListBlocks = 5;
+
+// The first blocks build one list each; every warp of the others takes one query token: D of all its heads, and (fp16) the largest
 // |dO| of its sequence and head.  VEC: heads of 32, 64 or 128 elements on 16-byte boundaries: a head on d / 8 lanes.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kPrepThreads)
-backward_prepare_kernel(BwdArgs a, int tile, ListOut kv, ListOut qi, unsigned* __restrict__ top) {
-  if (tile == 0) {
-    if (blockIdx.x == 0) build_sequence_items(a, kv);
-    if (blockIdx.x <= 1) return;
+backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ top) {
+  switch (blockIdx.x) {  // (a class without sequences gives an empty list)
+    case 0: build_backward_items(a.offsets_k, a.row_elems_k, a.offsets_q, a.row_elems_q, a.batch, plan.tile, plan.short_, l.kv); return;
+    case 1: build_backward_items(a.offsets_q, a.row_elems_q, a.offsets_k, a.row_elems_k, a.batch, plan.tile, plan.short_, l.qi); return;
+    case 2: if (plan.long_.any()) build_backward_items(a.offsets_k, a.row_elems_k, a.offsets_q, a.row_elems_q, a.batch, 128, plan.long_, l.long_kv); return;
+    case 3: if (plan.long_.any()) build_backward_items(a.offsets_q, a.row_elems_q, a.offsets_k, a.row_elems_k, a.batch, 128, plan.long_, l.long_qi); return;
+    case 4: if (plan.mid.any()) build_sequence_items(a, plan.mid, l.mid); return;
+    default: break;
   }
-  if (blockIdx.x == 0) {
-    build_backward_items(a.offsets_k, a.row_elems_k, a.offsets_q, a.row_elems_q, a.batch, tile, kv);
-    return;
-  }
-  if (blockIdx.x == 1) {
-    build_backward_items(a.offsets_q, a.row_elems_q, a.offsets_k, a.row_elems_k, a.batch, tile, qi);
-    return;
-  }
-  const int64_t t = ((int64_t)blockIdx.x - 2) * (kPrepThreads / 32) + (threadIdx.x >> 5);
+  const int64_t t = ((int64_t)blockIdx.x - kListBlocks) * (kPrepThreads / 32) + (threadIdx.x >> 5);
   if (t >= a.q_tokens) return;
   const int lane = threadIdx.x & 31;
   const int64_t E = (int64_t)a.H * a.d;
@@ -136,27 +154,39 @@ backward_prepare_kernel(BwdArgs a, int tile, ListOut kv, ListOut qi, unsigned* _
   if (top != nullptr) b = find_entry_warp(a.offsets_q, 0, a.batch - 1, t * a.row_elems_q);
   if (VEC) {
     const int per = a.d / 8;  // lanes per head
-    for (int v0 = 0; v0 < E / 8; v0 += 32) {
-      const int v = v0 + lane;
-      float s = 0.0f, m = 0.0f;
-      if (v < E / 8) {
-        T x[8], y[8];
-        *reinterpret_cast<uint4*>(x) = reinterpret_cast<const uint4*>(g)[v];
-        *reinterpret_cast<uint4*>(y) = reinterpret_cast<const uint4*>(o)[v];
+    const int nv = (int)(E / 8);
+    constexpr int kAhead = 4;  // steps of 256 elements whose loads are in flight together
+    for (int v0 = lane; v0 < nv + lane; v0 += 32 * kAhead) {  // (the same trips for every lane: the sums are warp-wide)
+      uint4 x[kAhead], y[kAhead];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          s = fmaf(to_f32(x[k]), to_f32(y[k]), s);
-          m = fmaxf(m, fabsf(to_f32(x[k])));
+      for (int i = 0; i < kAhead; ++i) {
+        const int v = v0 + 32 * i;
+        x[i] = y[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (v < nv) {
+          x[i] = reinterpret_cast<const uint4*>(g)[v];
+          y[i] = reinterpret_cast<const uint4*>(o)[v];
         }
       }
-      for (int w = per / 2; w > 0; w >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, w);
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-      }
-      if (v < E / 8 && lane % per == 0) {
-        const int h = v / per;
-        a.delta[(int64_t)h * a.q_tokens + t] = s;
-        if (top != nullptr) atomicMax(top + b * a.H + h, __float_as_uint(m));
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (v0 - lane + 32 * i >= nv) break;
+        const T *xe = reinterpret_cast<const T*>(&x[i]), *ye = reinterpret_cast<const T*>(&y[i]);
+        float s = 0.0f, m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          s = fmaf(to_f32(xe[k]), to_f32(ye[k]), s);
+          m = fmaxf(m, fabsf(to_f32(xe[k])));
+        }
+        for (int w = per / 2; w > 0; w >>= 1) {
+          s += __shfl_xor_sync(0xffffffffu, s, w);
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+        }
+        const int v = v0 + 32 * i;
+        if (v < nv && lane % per == 0) {
+          const int h = v / per;
+          a.delta[(int64_t)h * a.q_tokens + t] = s;
+          if (top != nullptr) atomicMax(top + b * a.H + h, __float_as_uint(m));
+        }
       }
     }
   } else {
@@ -661,17 +691,18 @@ __device__ __forceinline__ void bwd_mma_tile(const BwdArgs& a, const Item& it, f
   }
 }
 
-// blocks [0, kv_blocks): dK and dV of a (key tile, head); the others dQ of a (query tile, head)
+// dK and dV of every (key tile, head), then dQ of every (query tile, head)
 template <typename T, int D>
-__global__ void __launch_bounds__(kMmaThreads) attn_bwd_mma_kernel(BwdArgs a, ListOut kv, ListOut qi, int64_t kv_blocks) {
+__global__ void __launch_bounds__(kMmaThreads) attn_bwd_mma_kernel(BwdArgs a, ListOut kv, ListOut qi) {
   extern __shared__ __align__(128) uint8_t mma_smem[];
-  const bool is_kv = (int64_t)blockIdx.x < kv_blocks;
-  const int64_t w = is_kv ? (int64_t)blockIdx.x : (int64_t)blockIdx.x - kv_blocks;
-  const int64_t i = w / a.H;
-  const int h = (int)(w - i * a.H);
-  if (i >= *(is_kv ? kv : qi).count) return;
-  if (is_kv) bwd_mma_tile<T, D, true>(a, decode(kv.items[i]), grad_scale(a, kv.seq, i, h), h, mma_smem);
-  else bwd_mma_tile<T, D, false>(a, decode(qi.items[i]), grad_scale(a, qi.seq, i, h), h, mma_smem);
+  const int64_t n_kv = (int64_t)*kv.count * a.H, n = n_kv + (int64_t)*qi.count * a.H;
+  for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
+    const bool is_kv = w < n_kv;
+    const int64_t i = (is_kv ? w : w - n_kv) / a.H;
+    const int h = (int)((is_kv ? w : w - n_kv) - i * a.H);
+    if (is_kv) bwd_mma_tile<T, D, true>(a, decode(kv.items[i]), grad_scale(a, kv.seq, i, h), h, mma_smem);
+    else bwd_mma_tile<T, D, false>(a, decode(qi.items[i]), grad_scale(a, qi.seq, i, h), h, mma_smem);
+  }
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -679,37 +710,39 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 int64_t item_capacity(int64_t batch, int64_t tokens, int tile) { return batch + tokens / tile + 1; }
 
-// delta | largest |dO| | count, KV items, their sequences | count, Q items, their sequences | dQ in fp32 (the tcgen05 kernel with
-// whole sequences as items); every part on a 16-byte boundary
+// delta | largest |dO| | five lists (count, items, their sequences) | dQ in fp32 (the kernel with whole sequences as items); every part
+// on a 16-byte boundary
 struct BwdWorkspace {
-  size_t delta, top, kv, kv_seq, q, q_seq, scratch, bytes;
+  size_t delta, top, lists[kListBlocks], seqs[kListBlocks], scratch, bytes;
   BwdWorkspace(int64_t batch, int64_t q_tokens, int64_t k_tokens, int H, size_t scratch_bytes) {
     auto up = [](size_t v) { return (v + 15) / 16 * 16; };
-    const size_t nk = (size_t)item_capacity(batch, k_tokens, 32), nq = (size_t)item_capacity(batch, q_tokens, 32);  // (tiles of 32 rows or more)
+    const int64_t n[kListBlocks] = {item_capacity(batch, k_tokens, 32), item_capacity(batch, q_tokens, 32), item_capacity(batch, k_tokens, 128),
+                                    item_capacity(batch, q_tokens, 128), batch};  // (tiles of 32 rows or more)
     delta = 0;
     top = up((size_t)q_tokens * H * 4);
-    kv = top + up((size_t)batch * H * 4);
-    kv_seq = kv + 16 + sizeof(int4) * nk;
-    q = kv_seq + up(4 * nk);
-    q_seq = q + 16 + sizeof(int4) * nq;
-    scratch = q_seq + up(4 * nq);
+    size_t at = top + up((size_t)batch * H * 4);
+    for (int i = 0; i < kListBlocks; ++i) {
+      lists[i] = at;
+      seqs[i] = at + 16 + sizeof(int4) * (size_t)n[i];
+      at = seqs[i] + up(4 * (size_t)n[i]);
+    }
+    scratch = at;
     bytes = scratch + up(scratch_bytes);
+  }
+  Lists make(uint8_t* ws) const {
+    auto list = [&](int i) {
+      return ListOut{reinterpret_cast<int4*>(ws + lists[i] + 16), reinterpret_cast<int*>(ws + seqs[i]), reinterpret_cast<int*>(ws + lists[i])};
+    };
+    return {list(0), list(1), list(2), list(3), list(4)};
   }
 };
 
-struct Lists {
-  ListOut kv, qi;
-  Lists(uint8_t* ws, const BwdWorkspace& at)
-      : kv{reinterpret_cast<int4*>(ws + at.kv + 16), reinterpret_cast<int*>(ws + at.kv_seq), reinterpret_cast<int*>(ws + at.kv)},
-        qi{reinterpret_cast<int4*>(ws + at.q + 16), reinterpret_cast<int*>(ws + at.q_seq), reinterpret_cast<int*>(ws + at.q)} {}
-};
-
 template <typename T, bool VEC>
-int launch_prepare(const BwdArgs& a, int tile, const Lists& l, unsigned* top, cudaStream_t st) {
-  const int64_t blocks = 2 + ceil_div(a.q_tokens, kPrepThreads / 32);
+int launch_prepare(const BwdArgs& a, const Plan& plan, const Lists& l, unsigned* top, cudaStream_t st) {
+  const int64_t blocks = kListBlocks + ceil_div(a.q_tokens, kPrepThreads / 32);
   if (blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
   if (top != nullptr && cudaMemsetAsync(top, 0, (size_t)a.batch * a.H * 4, st) != cudaSuccess) return NTB200_LAUNCH_FAILED;
-  backward_prepare_kernel<T, VEC><<<(unsigned)blocks, kPrepThreads, 0, st>>>(a, tile, l.kv, l.qi, top);
+  backward_prepare_kernel<T, VEC><<<(unsigned)blocks, kPrepThreads, 0, st>>>(a, plan, l, top);
   return status_from_cuda(cudaGetLastError());
 }
 
@@ -721,7 +754,7 @@ int launch_bwd_simt(const BwdArgs& a, int64_t k_tokens, const Lists& l, cudaStre
         return cudaFuncSetAttribute(attn_bwd_simt_kernel<T, BT, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess;
       }))
     return NTB200_LAUNCH_FAILED;
-  const int rc = launch_prepare<T, false>(a, BT, l, nullptr, st);
+  const int rc = launch_prepare<T, false>(a, Plan{{0, INT64_MAX}, {0, 0}, {0, 0}, BT}, l, nullptr, st);
   if (rc != NTB200_OK) return rc;
   const int per_sm = 227 * 1024 / (kSmem + 1024);
   const int64_t most = (item_capacity(a.batch, k_tokens, BT) + item_capacity(a.batch, a.q_tokens, BT)) * a.H;
@@ -754,67 +787,66 @@ int launch_fwd(const BwdArgs& a, void* out, float* lse, const ListOut& l, cudaSt
 }
 
 template <typename T, int D>
-int launch_bwd_mma(BwdArgs a, int64_t k_tokens, unsigned* top, const Lists& l, cudaStream_t st) {
+int launch_bwd_mma(const BwdArgs& a, int64_t k_tokens, const Lists& l, cudaStream_t st) {
   constexpr int kSmem = bwd_mma_smem<D>();
   static std::atomic<int> configured[kMaxDevices];
   if (!once_per_device(configured, [] {
         return cudaFuncSetAttribute(attn_bwd_mma_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess;
       }))
     return NTB200_LAUNCH_FAILED;
-  a.top = std::is_same<T, __half>::value ? top : nullptr;
-  const int rc = launch_prepare<T, true>(a, kMmaTile, l, const_cast<unsigned*>(a.top), st);
-  if (rc != NTB200_OK) return rc;
-  const int64_t kv_blocks = k_tokens > 0 ? item_capacity(a.batch, k_tokens, kMmaTile) * a.H : 0;
-  const int64_t q_blocks = a.q_tokens > 0 ? item_capacity(a.batch, a.q_tokens, kMmaTile) * a.H : 0;
-  if (kv_blocks + q_blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
-  attn_bwd_mma_kernel<T, D><<<(unsigned)(kv_blocks + q_blocks), kMmaThreads, kSmem, st>>>(a, l.kv, l.qi, kv_blocks);
+  const int64_t most = (item_capacity(a.batch, k_tokens, kMmaTile) + item_capacity(a.batch, a.q_tokens, kMmaTile)) * a.H;
+  const int64_t resident = (int64_t)kNumSMs * (D == 32 ? 8 : D == 64 ? 4 : 2);
+  attn_bwd_mma_kernel<T, D><<<(unsigned)(most < resident ? most : resident), kMmaThreads, kSmem, st>>>(a, l.kv, l.qi);
   return status_from_cuda(cudaGetLastError());
 }
 
+// Sequences of up to kShort tokens on both sides go to the mma.sync kernel, whose tiles have 64 rows: 21 000 tokens of lengths up to 64
+// take 272 us there and 413 on the tcgen05 kernels (16 heads of 64), 10 000 take 107 and 178 (8 heads of 128); of lengths up to
+// 128, 283 and 243, and 122 and 117.
+constexpr int64_t kShort = 64;
+// Heads of 64: sequences of up to kMid tokens as whole items (S and dP once for all three gradients): 128 sequences of 32 to 512 tokens, 12
+// heads: 417 us against 446 with an item per tile; beyond, a sequence would keep its one CTA busy for long (one of 1024, 16
+// heads: 207 us against 47).
+constexpr int64_t kMid = 512;
+
+Plan make_plan(int d, bool tc, int path) {
+  constexpr int64_t kAll = INT64_MAX;
+  if (!tc || path == 2) return {{0, kAll}, {0, 0}, {0, 0}, kMmaTile};
+  if (path == 3) return {{0, 0}, {0, 0}, {0, kAll}, kMmaTile};
+  if (path == 4) return {{0, 0}, {0, kAll}, {0, 0}, kMmaTile};
+  if (d == 64) return {{0, kShort}, {kShort, kMid}, {kMid, kAll}, kMmaTile};
+  return {{0, kShort}, {0, 0}, {kShort, kAll}, kMmaTile};
+}
+
+// fp32 sums of dQ over the key tiles of the middle class's sequences
+size_t scratch_bytes(int64_t q_tokens, int64_t max_len_k, int H, int d, int dtype, int path) {
+  return d == 64 && dtype != NTB200_F32 && (path == 0 || path == 4) && max_len_k > 128 ? (size_t)q_tokens * H * d * 4 : 0;
+}
+
 template <typename T>
-int launch_bwd_tcgen05(BwdArgs a, int64_t k_tokens, unsigned* top, int dtype, const Lists& l, cudaStream_t st) {
-  a.top = std::is_same<T, __half>::value ? top : nullptr;
-  const int rc = launch_prepare<T, true>(a, 128, l, const_cast<unsigned*>(a.top), st);
-  if (rc != NTB200_OK) return rc;
-  return attn_bwd_tcgen05_launch(a, k_tokens, dtype, l.kv, l.qi, item_capacity(a.batch, k_tokens, 128), item_capacity(a.batch, a.q_tokens, 128), st);
-}
-
-// Whether the tcgen05 kernel takes whole sequences as items (heads of 64).  It needs enough of them to fill the GPU, and none so
-// long that its CTA is still busy when the others are done.
-bool by_sequence(int64_t batch, int64_t max_len_q, int64_t max_len_k, int H, int d, int dtype, int path) {
-  if (d != 64 || dtype == NTB200_F32 || (path != 0 && path != 4)) return false;
-  return path == 4 || (batch * H >= 2 * kNumSMs && max_len_q <= 1024 && max_len_k <= 1024);
-}
-
-size_t scratch_bytes(int64_t batch, int64_t q_tokens, int64_t max_len_q, int64_t max_len_k, int H, int d, int dtype, int path) {
-  return by_sequence(batch, max_len_q, max_len_k, H, d, dtype, path) && max_len_k > 128 ? (size_t)q_tokens * H * d * 4 : 0;
-}
-
-template <typename T>
-int launch_bwd(const BwdArgs& a, int64_t k_tokens, int64_t max_len_q, int64_t max_len_k, uint8_t* ws, const BwdWorkspace& at, int path,
-               cudaStream_t st) {
-  const Lists l(ws, at);
+int launch_bwd(const BwdArgs& args, int64_t k_tokens, int64_t max_len, uint8_t* ws, const BwdWorkspace& at, int path, cudaStream_t st) {
+  const Lists l = at.make(ws);
+  BwdArgs a = args;
   if constexpr (!std::is_same<T, float>::value) {
+    constexpr int dtype = std::is_same<T, __half>::value ? NTB200_F16 : NTB200_BF16;
     const bool mma = (a.d == 32 || a.d == 64 || a.d == 128) && aligned16(a.grad) && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) &&
                      aligned16(a.out) && aligned16(a.dq) && aligned16(a.dk) && aligned16(a.dv) && a.ldq % 8 == 0 && a.ldk % 8 == 0 &&
                      a.ldv % 8 == 0 && a.lddq % 8 == 0 && a.lddk % 8 == 0 && a.lddv % 8 == 0;
-    if (path >= 2 && !mma) return NTB200_UNSUPPORTED_SHAPE;
-    constexpr int dtype = std::is_same<T, __half>::value ? NTB200_F16 : NTB200_BF16;
     const bool tc = mma && a.d >= 64 && attn_bwd_tcgen05_supported(a, k_tokens, dtype);
-    if ((path == 3 && !tc) || (path == 4 && (!tc || a.d != 64))) return NTB200_UNSUPPORTED_SHAPE;
-    if (tc && by_sequence(a.batch, max_len_q, max_len_k, a.H, a.d, dtype, path)) {
-      BwdArgs b = a;
-      b.top = std::is_same<T, __half>::value ? reinterpret_cast<unsigned*>(ws + at.top) : nullptr;
-      const int rc = launch_prepare<T, true>(b, 0, l, const_cast<unsigned*>(b.top), st);
-      if (rc != NTB200_OK) return rc;
-      return attn_bwd_fused_launch(b, k_tokens, dtype, l.kv, reinterpret_cast<float*>(ws + at.scratch), st);
-    }
-    if (tc && (path == 3 || path == 0)) return launch_bwd_tcgen05<T>(a, k_tokens, reinterpret_cast<unsigned*>(ws + at.top), dtype, l, st);
+    if ((path == 2 && !mma) || (path >= 3 && !tc) || (path == 4 && a.d != 64)) return NTB200_UNSUPPORTED_SHAPE;
     if (mma && path != 1) {
-      unsigned* top = reinterpret_cast<unsigned*>(ws + at.top);
-      if (a.d == 32) return launch_bwd_mma<T, 32>(a, k_tokens, top, l, st);
-      if (a.d == 64) return launch_bwd_mma<T, 64>(a, k_tokens, top, l, st);
-      return launch_bwd_mma<T, 128>(a, k_tokens, top, l, st);
+      const Plan plan = make_plan(a.d, tc, path);
+      a.top = dtype == NTB200_F16 ? reinterpret_cast<unsigned*>(ws + at.top) : nullptr;
+      int rc = launch_prepare<T, true>(a, plan, l, const_cast<unsigned*>(a.top), st);
+      if (rc == NTB200_OK && plan.long_.any() && max_len > plan.long_.over)
+        rc = attn_bwd_tcgen05_launch(a, k_tokens, dtype, l.long_kv, l.long_qi, item_capacity(a.batch, k_tokens, 128),
+                                     item_capacity(a.batch, a.q_tokens, 128), st);
+      if (rc == NTB200_OK && plan.mid.any() && max_len > plan.mid.over)
+        rc = attn_bwd_fused_launch(a, k_tokens, dtype, l.mid, reinterpret_cast<float*>(ws + at.scratch), st);
+      if (rc != NTB200_OK || !plan.short_.any()) return rc;
+      if (a.d == 32) return launch_bwd_mma<T, 32>(a, k_tokens, l, st);
+      if (a.d == 64) return launch_bwd_mma<T, 64>(a, k_tokens, l, st);
+      return launch_bwd_mma<T, 128>(a, k_tokens, l, st);
     }
   } else if (path > 1) {
     return NTB200_UNSUPPORTED_SHAPE;
@@ -857,8 +889,9 @@ extern "C" {
 
 size_t ntb200_varlen_attention_backward_workspace_bytes(int64_t batch, int64_t q_tokens, int64_t k_tokens, int num_heads, int head_dim,
                                                         int64_t max_len_q, int64_t max_len_k, int dtype, int path) {
+  (void)max_len_q;
   if (batch <= 0 || q_tokens < 0 || k_tokens < 0 || num_heads < 1 || head_dim < 1) return 0;
-  return BwdWorkspace(batch, q_tokens, k_tokens, num_heads, scratch_bytes(batch, q_tokens, max_len_q, max_len_k, num_heads, head_dim, dtype, path)).bytes;
+  return BwdWorkspace(batch, q_tokens, k_tokens, num_heads, scratch_bytes(q_tokens, max_len_k, num_heads, head_dim, dtype, path)).bytes;
 }
 
 int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
@@ -880,7 +913,7 @@ int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_
   if (q_tokens > 0 && (grad_out == nullptr || q == nullptr || out == nullptr || lse == nullptr || grad_q == nullptr)) return NTB200_INVALID_ARG;
   if (k_tokens > 0 && (k == nullptr || v == nullptr || grad_k == nullptr || grad_v == nullptr)) return NTB200_INVALID_ARG;
   const BwdWorkspace at(batch, q_tokens, k_tokens, num_heads,
-                        scratch_bytes(batch, q_tokens, max_len_q, max_len_k, num_heads, head_dim, dtype, path));
+                        scratch_bytes(q_tokens, max_len_k, num_heads, head_dim, dtype, path));
   if (workspace_bytes < at.bytes) return NTB200_WORKSPACE_TOO_SMALL;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return NTB200_MISALIGNED;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -888,10 +921,11 @@ int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_
                      ldq, ldk, ldv, ld_grad_q, ld_grad_k, ld_grad_v, offsets_q, offsets_k, row_elems_q, row_elems_k,
                      batch, q_tokens, num_heads, head_dim, scaling};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t max_len = max_len_q > max_len_k ? max_len_q : max_len_k;
   switch (dtype) {
-    case NTB200_F32: return launch_bwd<float>(a, k_tokens, max_len_q, max_len_k, ws, at, path, st);
-    case NTB200_F16: return launch_bwd<__half>(a, k_tokens, max_len_q, max_len_k, ws, at, path, st);
-    default: return launch_bwd<__nv_bfloat16>(a, k_tokens, max_len_q, max_len_k, ws, at, path, st);
+    case NTB200_F32: return launch_bwd<float>(a, k_tokens, max_len, ws, at, path, st);
+    case NTB200_F16: return launch_bwd<__half>(a, k_tokens, max_len, ws, at, path, st);
+    default: return launch_bwd<__nv_bfloat16>(a, k_tokens, max_len, ws, at, path, st);
   }
 }
 
