@@ -20,6 +20,7 @@
 #include "attention_internal.cuh"
 #include "attention_tiny.cuh"
 #include "common.cuh"
+#include "row_vec.cuh"
 
 namespace ntb200 {
 namespace {
@@ -152,7 +153,8 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
   const T* o = static_cast<const T*>(a.out) + t * E;
   int64_t b = 0;
   if (top != nullptr) b = find_entry_warp(a.offsets_q, 0, a.batch - 1, t * a.row_elems_q);
-  if (VEC) {
+  if constexpr (VEC) {
+    constexpr int kDtype = std::is_same<T, __half>::value ? NTB200_F16 : NTB200_BF16;  // (VEC: 16-bit types)
     const int per = a.d / 8;  // lanes per head
     const int nv = (int)(E / 8);
     constexpr int kAhead = 4;  // steps of 256 elements whose loads are in flight together
@@ -170,12 +172,13 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         if (v0 - lane + 32 * i >= nv) break;
-        const T *xe = reinterpret_cast<const T*>(&x[i]), *ye = reinterpret_cast<const T*>(&y[i]);
-        float s = 0.0f, m = 0.0f;
+        float s = 0.0f, m = 0.0f, xe[8], ye[8];
+        Vec16<kDtype>::unpack(x[i], xe);
+        Vec16<kDtype>::unpack(y[i], ye);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          s = fmaf(to_f32(xe[k]), to_f32(ye[k]), s);
-          m = fmaxf(m, fabsf(to_f32(xe[k])));
+          s = fmaf(xe[k], ye[k], s);
+          m = fmaxf(m, fabsf(xe[k]));
         }
         for (int w = per / 2; w > 0; w >>= 1) {
           s += __shfl_xor_sync(0xffffffffu, s, w);
@@ -706,8 +709,6 @@ __global__ void __launch_bounds__(kMmaThreads) attn_bwd_mma_kernel(BwdArgs a, Li
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 int64_t item_capacity(int64_t batch, int64_t tokens, int tile) { return batch + tokens / tile + 1; }
 
 // delta | largest |dO| | five lists (count, items, their sequences) | dQ in fp32 (the kernel with whole sequences as items); every part
