@@ -42,6 +42,26 @@ def build_meta(sizes: torch.Tensor, device) -> torch.Tensor:
     return host
 
 
+class _Ragged(object):
+    """What nested tensors over the same rows share: the sizes of the one they were made from (the first column holds the
+    lengths), its device offsets, and the elements per row in them.  Holds no values."""
+    __slots__ = ("sizes", "meta", "device", "row_elems")
+
+    def __init__(self, sizes, meta, device):
+        self.sizes, self.meta, self.device = sizes, meta, device
+        self.row_elems = 1
+        if sizes.size(0) > 0 and sizes.size(1) > 1:
+            self.row_elems = int(sizes[0, 1]) if sizes.size(1) == 2 else int(sizes[0, 1:].prod())
+
+    def on(self, device):
+        """The same structure with its offsets on `device`."""
+        if self.meta is None or self.meta.device != device:
+            if self.device != device:
+                return _Ragged(self.sizes, build_meta(self.sizes, device), device)
+            self.meta = build_meta(self.sizes, device)
+        return self
+
+
 class NestedTensor(object):
     def __init__(self, buffer: torch.Tensor, sizes: torch.Tensor, meta: Optional[torch.Tensor] = None,
                  channels_last: bool = False):
@@ -58,18 +78,18 @@ class NestedTensor(object):
         # the logical (C, H_i, W_i), every constituent is STORED as (H_i, W_i, C), i.e. with strides (1, W_i*C, C).
         self._channels_last = bool(channels_last)
         self._nchw = None  # cached contiguous copy of a channels_last tensor, made on first use by an operator
-        self._packed = None
-        self._root = None
+        self._packed = None  # set by _over()
+        self._ragged = None
 
     @classmethod
-    def _over(cls, packed, root):
+    def _over(cls, packed, ragged):
         """A nested tensor over the [rows, ...] matrix `packed` (contiguous; it carries the autograd graph) with the lengths of
-        `root`, whose offsets it shares; the flat buffer and the sizes are made when something asks for them."""
+        `ragged`; its flat buffer and its sizes are made when something asks for them."""
         out = cls.__new__(cls)
         out._flat = out._extents = out._meta = out._nchw = None
         out._channels_last = False
         out._packed = packed
-        out._root = root
+        out._ragged = ragged
         return out
 
     @property
@@ -81,7 +101,7 @@ class NestedTensor(object):
     @property
     def _sizes(self):
         if self._extents is None:
-            lengths, p = self._root._sizes, self._packed
+            lengths, p = self._ragged.sizes, self._packed
             sizes = torch.empty((lengths.size(0), p.dim()), dtype=torch.int64)
             if lengths.size(0) > 0:
                 sizes[:, 0] = lengths[:, 0]
@@ -138,24 +158,18 @@ class NestedTensor(object):
             raise RuntimeError("with_values(): values must be on the nested tensor's device")
         return self._with_rows(values.contiguous())
 
+    def _structure(self):
+        if self._ragged is None:
+            self._ragged = _Ragged(self._extents, self._meta, self.device)
+        return self._ragged
+
     def _with_rows(self, packed):
-        return NestedTensor._over(packed, self if self._root is None else self._root)
+        return NestedTensor._over(packed, self._structure())
 
     def _row_offsets(self):
         """(device offsets of the constituents, elements per row in them)."""
-        root = self if self._root is None else self._root
-        if root._meta is None or root._meta.device != self.device:
-            if root._buffer.device != self.device:  # moved away from the structure it was made from
-                self._meta = build_meta(self._sizes, self.device) if self._meta is None else self._meta
-                return self._meta, self._row_elems()
-            root._meta = build_meta(root._sizes, root._buffer.device)
-        return root._meta, root._row_elems()
-
-    def _row_elems(self):
-        sizes = self._sizes
-        if sizes.size(0) == 0 or sizes.size(1) == 1:
-            return 1
-        return int(sizes[0, 1]) if sizes.size(1) == 2 else int(sizes[0, 1:].prod())
+        r = self._ragged = self._structure().on(self.device)
+        return r.meta, r.row_elems
 
     def _tracked(self):
         """(rows, sizes, features) as an operator that tracks gradients takes them: the packed rows with their last extent and
@@ -163,7 +177,7 @@ class NestedTensor(object):
         if self._channels_last:
             raise RuntimeError("nestedtensor_b200: the training operators need contiguous constituents")
         if self._packed is not None:
-            return self._packed, self._root._sizes, self._packed.size(-1) if self._packed.dim() > 1 else 1
+            return self._packed, self._ragged.sizes, self._packed.size(-1) if self._packed.dim() > 1 else 1
         buf = self._flat
         base = buf._base
         if base is not None and base.requires_grad and base.numel() == buf.numel() and base.is_contiguous():
@@ -216,7 +230,7 @@ class NestedTensor(object):
         return 1 + self.tensor_dim()
 
     def __len__(self):
-        return int((self if self._root is None else self._root)._sizes.size(0))
+        return int((self._extents if self._ragged is None else self._ragged.sizes).size(0))
 
     def size(self, dim=None):
         """``None`` for ragged dimensions (nestedtensor/csrc/py_init.cpp:169-172)."""
@@ -309,7 +323,7 @@ class NestedTensor(object):
 
     def to(self, *args, **kwargs):
         if self._packed is not None:
-            return NestedTensor._over(self._packed.to(*args, **kwargs), self._root)
+            return NestedTensor._over(self._packed.to(*args, **kwargs), self._ragged)
         buf = self._buffer.to(*args, **kwargs)
         meta = self._meta if (self._meta is not None and self._meta.device == buf.device) else None
         return NestedTensor(buf, self._sizes, meta, channels_last=self._channels_last)

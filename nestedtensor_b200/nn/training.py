@@ -33,15 +33,15 @@ def _check(obj, name):
 
 def layer_norm(input: NestedTensor, normalized_shape, weight=None, bias=None, eps: float = 1e-5) -> NestedTensor:
     """``torch.nn.functional.layer_norm`` with gradients of the input, the weight and the bias.  As ``nn.layer_norm``, the last
-    dimension must be regular and equal ``normalized_shape``, a singleton, and weight and bias come together."""
+    dimension must be regular and equal ``normalized_shape``, a singleton, and weight and bias come together; the dimensions
+    between the first and the last must be regular here."""
     _check(input, "input")
     if isinstance(normalized_shape, int):
         normalized_shape = (normalized_shape,)
     x, sizes, features = input._tracked()
+    shape = None if input.tensor_dim() == 2 else input.values().shape  # (L_i, ..., E): the operator's rows are finer
     out = _ops.ops().layer_norm_train(x, sizes, features, normalized_shape, weight, bias, eps)
-    if input.tensor_dim() != 2:  # (L_i, ..., E): the rows of the operator are finer than the constituents'
-        out = out.view(input.values().shape)
-    return input._with_rows(out)
+    return input._with_rows(out if shape is None else out.view(shape))
 
 
 def embedding(input: NestedTensor, weight: torch.Tensor, padding_idx: Optional[int] = None, max_norm=None, norm_type=2.0,
@@ -81,7 +81,8 @@ def attention(query: NestedTensor, key: NestedTensor, value: NestedTensor, num_h
         _check(t, name)
         if t.dim() != 3 and len(t) > 0:
             raise RuntimeError(name + " needs to be 3 dim.")
-    if value is not key and not torch.equal(key._sizes, value._sizes):
+    if value is not key and not (key._packed is not None and value._packed is not None and key._ragged is value._ragged) \
+            and not torch.equal(key._sizes, value._sizes):
         raise RuntimeError("nestedtensor_b200: key and value must have the same nested size")
     q, q_sizes, features = query._tracked()
     k, k_sizes, k_features = key._tracked()
