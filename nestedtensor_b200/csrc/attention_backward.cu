@@ -8,12 +8,13 @@
 // P is computed again from the forward pass's row statistics, P_ij = 2^(a log2(e) q_i.k_j - lse_i) with lse_i the base-2
 // logarithm of the row's softmax denominator, so nothing of size L x L is ever stored.
 //
-// A sequence's gradients are sums over its own rows only, taken in a fixed order by one block: no atomics, the same bits on
-// every run and whatever the rest of the batch holds.
+// A sequence's gradients are sums over its own rows only, taken in a fixed order by one block, and its kernel is chosen by its own
+// lengths: no atomics, the same bits on every run and whatever the rest of the batch holds.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cstdint>
 #include <type_traits>
 
 #include "attention_backward.cuh"
@@ -132,10 +133,16 @@ struct Plan {
 };
 constexpr int kListBlocks = 5;
 
+// D from the rounded O is off by |dO| |O| times half a step of the 16-bit type, and that goes into every dS_ij = P_ij (dP_ij - D_i) of
+// the row alike.  Over many keys it is small next to dP; a sequence of one key has dS = 0, and all of its dQ and dK would be that
+// error.  So a row of up to kFewKeys keys sums D = sum_j P_ij dP_ij itself, in 32 bits.  (Relative error of bf16 dQ and dK, heads of
+// 64: 2 keys 0.0039 from O, 0.0024 from P; 4 keys 0.0029; 16 keys 0.0025; 64 keys 0.0024, the rounding of dS and of the result.)
+constexpr int kFewKeys = 16;
+
 // The first blocks build one list each; every warp of the others takes one query token: D of all its heads, and (fp16) the largest
 // |dO| of its sequence and head.  VEC: heads of 32, 64 or 128 elements on 16-byte boundaries: a head on d / 8 lanes.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kPrepThreads)
+__global__ void __launch_bounds__(kPrepThreads, 4)
 backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ top) {
   switch (blockIdx.x) {  // (a class without sequences gives an empty list)
     case 0: build_backward_items(a.offsets_k, a.row_elems_k, a.offsets_q, a.row_elems_q, a.batch, plan.tile, plan.short_, l.kv); return;
@@ -151,27 +158,87 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
   const int64_t E = (int64_t)a.H * a.d;
   const T* g = static_cast<const T*>(a.grad) + t * E;
   const T* o = static_cast<const T*>(a.out) + t * E;
-  int64_t b = 0;
-  if (top != nullptr) b = find_entry_warp(a.offsets_q, 0, a.batch - 1, t * a.row_elems_q);
+  constexpr bool kRounded = !std::is_same<T, float>::value;  // O has fewer bits than D
+  [[maybe_unused]] constexpr int kSteps = 4;                 // steps of 256 elements whose loads are in flight together
+  [[maybe_unused]] uint4 x[kSteps], y[kSteps];
+  [[maybe_unused]] const int nv = (int)(E / 8);
+  [[maybe_unused]] auto load = [&](int first) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int v = first + 32 * i;
+      x[i] = y[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (v < nv) {
+        x[i] = reinterpret_cast<const uint4*>(g)[v];
+        y[i] = reinterpret_cast<const uint4*>(o)[v];
+      }
+    }
+  };
+  if constexpr (VEC) load(lane);  // (in flight while the sequence is looked up)
+  int64_t b = 0, key0 = 0, keys = INT64_MAX;
+  if constexpr (kRounded) {
+    b = find_entry_warp(a.offsets_q, 0, a.batch - 1, t * a.row_elems_q);
+    if (t * a.row_elems_q >= a.offsets_q[b + 1]) return;  // behind the last sequence: nothing reads its D
+    key0 = a.offsets_k[b] / a.row_elems_k, keys = a.offsets_k[b + 1] / a.row_elems_k - key0;
+  }
+  const bool few = kRounded && keys <= kFewKeys;
+  const float scale = a.scaling * kLog2e;
+  const T* q = static_cast<const T*>(a.q) + t * a.ldq;
+  const T* k0 = static_cast<const T*>(a.k) + key0 * a.ldk;
+  const T* v0 = static_cast<const T*>(a.v) + key0 * a.ldv;
   if constexpr (VEC) {
     constexpr int kDtype = std::is_same<T, __half>::value ? NTB200_F16 : NTB200_BF16;  // (VEC: 16-bit types)
     const int per = a.d / 8;  // lanes per head
-    const int nv = (int)(E / 8);
-    constexpr int kAhead = 4;  // steps of 256 elements whose loads are in flight together
-    for (int v0 = lane; v0 < nv + lane; v0 += 32 * kAhead) {  // (the same trips for every lane: the sums are warp-wide)
-      uint4 x[kAhead], y[kAhead];
+    if (few) {
+      constexpr int kAhead = 4;  // keys whose rows are in flight together
+      for (int v = lane; v < nv + lane; v += 32) {  // (the same trips for every lane: the sums are warp-wide)
+        const bool live = v < nv;
+        const int h = live ? v / per : 0;
+        float xe[8], qe[8], s = 0.0f, m = 0.0f;
+        Vec16<kDtype>::unpack(live ? reinterpret_cast<const uint4*>(g)[v] : make_uint4(0u, 0u, 0u, 0u), xe);
+        Vec16<kDtype>::unpack(live ? reinterpret_cast<const uint4*>(q)[v] : make_uint4(0u, 0u, 0u, 0u), qe);
+        const float lse = live ? a.lse[(int64_t)h * a.q_tokens + t] : 0.0f;
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int v = v0 + 32 * i;
-        x[i] = y[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (v < nv) {
-          x[i] = reinterpret_cast<const uint4*>(g)[v];
-          y[i] = reinterpret_cast<const uint4*>(o)[v];
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(xe[e]));
+        for (int w = per / 2; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+        for (int j0 = 0; j0 < (int)keys; j0 += kAhead) {
+          uint4 kv[kAhead], vv[kAhead];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            kv[i] = vv[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (live && j0 + i < (int)keys) {
+              kv[i] = reinterpret_cast<const uint4*>(k0 + (j0 + i) * a.ldk)[v];
+              vv[i] = reinterpret_cast<const uint4*>(v0 + (j0 + i) * a.ldv)[v];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            float ke[8], ve[8], sij = 0.0f, dp = 0.0f;
+            Vec16<kDtype>::unpack(kv[i], ke);
+            Vec16<kDtype>::unpack(vv[i], ve);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              sij = fmaf(qe[e], ke[e], sij);
+              dp = fmaf(xe[e], ve[e], dp);
+            }
+            for (int w = per / 2; w > 0; w >>= 1) {
+              sij += __shfl_xor_sync(0xffffffffu, sij, w);
+              dp += __shfl_xor_sync(0xffffffffu, dp, w);
+            }
+            if (j0 + i < (int)keys) s = fmaf(exp2f(fmaf(sij, scale, -lse)), dp, s);
+          }
+        }
+        if (live && lane % per == 0) {
+          a.delta[(int64_t)h * a.q_tokens + t] = s;
+          if (top != nullptr) atomicMax(top + b * a.H + h, __float_as_uint(m));
         }
       }
+      return;
+    }
+    for (int first = lane; first < nv + lane; first += 32 * kSteps) {
+      if (first != lane) load(first);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (v0 - lane + 32 * i >= nv) break;
+      for (int i = 0; i < kSteps; ++i) {
+        if (first - lane + 32 * i >= nv) break;
         float s = 0.0f, m = 0.0f, xe[8], ye[8];
         Vec16<kDtype>::unpack(x[i], xe);
         Vec16<kDtype>::unpack(y[i], ye);
@@ -184,7 +251,7 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
           s += __shfl_xor_sync(0xffffffffu, s, w);
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
         }
-        const int v = v0 + 32 * i;
+        const int v = first + 32 * i;
         if (v < nv && lane % per == 0) {
           const int h = v / per;
           a.delta[(int64_t)h * a.q_tokens + t] = s;
@@ -195,9 +262,27 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
   } else {
     for (int h = 0; h < a.H; ++h) {
       float s = 0.0f;
-      for (int i = lane; i < a.d; i += 32) s = fmaf(to_f32(g[(int64_t)h * a.d + i]), to_f32(o[(int64_t)h * a.d + i]), s);
+      const int64_t col = (int64_t)h * a.d;
+      if (few) {
+        const float lse = a.lse[(int64_t)h * a.q_tokens + t];
+        for (int64_t j = 0; j < keys; ++j) {
+          float sij = 0.0f, dp = 0.0f;
+          for (int i = lane; i < a.d; i += 32) {
+            sij = fmaf(to_f32(q[col + i]), to_f32(k0[j * a.ldk + col + i]), sij);
+            dp = fmaf(to_f32(g[col + i]), to_f32(v0[j * a.ldv + col + i]), dp);
+          }
 #pragma unroll
-      for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+          for (int w = 16; w > 0; w >>= 1) {
+            sij += __shfl_xor_sync(0xffffffffu, sij, w);
+            dp += __shfl_xor_sync(0xffffffffu, dp, w);
+          }
+          s = fmaf(exp2f(fmaf(sij, scale, -lse)), dp, s);
+        }
+      } else {
+        for (int i = lane; i < a.d; i += 32) s = fmaf(to_f32(g[col + i]), to_f32(o[col + i]), s);
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+      }
       if (lane == 0) a.delta[(int64_t)h * a.q_tokens + t] = s;
     }
   }
@@ -843,7 +928,7 @@ int launch_bwd(const BwdArgs& args, int64_t k_tokens, int64_t max_len, uint8_t* 
         rc = attn_bwd_tcgen05_launch(a, k_tokens, dtype, l.long_kv, l.long_qi, item_capacity(a.batch, k_tokens, 128),
                                      item_capacity(a.batch, a.q_tokens, 128), st);
       if (rc == NTB200_OK && plan.mid.any() && max_len > plan.mid.over)
-        rc = attn_bwd_fused_launch(a, k_tokens, dtype, l.mid, reinterpret_cast<float*>(ws + at.scratch), st);
+        rc = attn_bwd_fused_launch(a, k_tokens, dtype, l.mid, at.bytes > at.scratch ? reinterpret_cast<float*>(ws + at.scratch) : nullptr, st);
       if (rc != NTB200_OK || !plan.short_.any()) return rc;
       if (a.d == 32) return launch_bwd_mma<T, 32>(a, k_tokens, l, st);
       if (a.d == 64) return launch_bwd_mma<T, 64>(a, k_tokens, l, st);

@@ -1038,7 +1038,8 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       const float f = a.scaling / grad_scale(a, t.seqs.seq, w / H, h);
       for (int kt = 0; kt < nk; ++kt) {
         for (int j = 0; j < nq; ++j, ++g) {
-          const bool live = j * kTR + row < it.w, first = kt == 0, last = kt == nk - 1;
+          // (no scratch was asked for where no sequence was to have more than one key tile: then none is touched)
+          const bool live = j * kTR + row < it.w && (nk == 1 || t.scratch != nullptr), first = kt == 0, last = kt == nk - 1;
           const int64_t token = (int64_t)it.z + j * kTR + row;
           float4* sc = t.scratch + (int64_t)h * 16 * a.q_tokens + token;
           T* out = static_cast<T*>(a.dq) + (token - lane) * a.lddq + (int64_t)h * C::D;  // the warp's first row

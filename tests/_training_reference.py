@@ -81,7 +81,8 @@ def attention(q, k, v, g, lq, lk, heads, scaling):
     dt = q.dtype
     d = q.size(1) // heads
     # 16-bit kernels round P and dS to the storage type before the products that use them (the forward pass P too) and D is
-    # taken from the rounded output; fp32 kernels round nothing.  The forward kernel for 16-bit types may take a quarter of its
+    # taken from the rounded output where a row has more than 16 keys, from the probabilities where it has fewer; fp32 kernels
+    # round nothing.  The forward kernel for 16-bit types may take a quarter of its
     # exponentials from a polynomial of relative error 1.9e-4, which also enters the row's denominator.
     half = dt != torch.float32
     u = rounding(dt)
@@ -110,6 +111,8 @@ def attention(q, k, v, g, lq, lk, heads, scaling):
         e_o = (e_p + up * P) @ V.abs() + (m + 4) * W * (P @ V.abs())
         e_d = (G.abs() * (e_o + (u if half else W) * (O.abs() + e_o))).sum(2, keepdim=True) + (d + 2) * W * (G * O).abs().sum(2, keepdim=True)
         e_dp = (d + 2) * W * (G.abs() @ V.abs().transpose(1, 2))
+        if half and m <= 16:  # D = sum_j P_ij dP_ij
+            e_d = (e_p * dP.abs() + P * e_dp).sum(2, keepdim=True) + (m + 4) * W * (P * dP).abs().sum(2, keepdim=True)
         e_ds = e_p * (dP - D).abs() + P * (e_dp + e_d + 2 * W * (dP.abs() + D.abs()))
         # rounded for the products; below the type's normal range by half its smallest step, where dS is held relative to the
         # power of two at or below the head's largest |dO| (at most that number times 2)

@@ -247,6 +247,18 @@ def test_attention_does_not_mix_sequences(cuda_device, dtype):
             assert torch.equal(part[name], clean[name][rows]), name
 
 
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_attention_over_one_key_has_no_score_gradient(cuda_device, dtype, d):
+    """The softmax of one score is 1 whatever the score is: dQ = dK = 0, up to what fp32 sums leave of dP - dP."""
+    heads, lq = 3, [1, 90, 1, 300]
+    q, k, v, g, qs, ks = _attend_inputs(lq, [1, 1, 1, 1], heads, d, dtype, 77)
+    got = _run_attend(q, k, v, g, qs, ks, heads)
+    want, bound = ref.attention(q, k, v, g, lq, [1, 1, 1, 1], heads, d ** -0.5)
+    assert float(want["dq"].abs().max()) < 1e-12 and float(want["dk"].abs().max()) < 1e-12
+    _check(got, want, bound, "one key")
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_attention_carries_nan(cuda_device, dtype):
     """One NaN query reaches its own output row and dQ row and, through its probabilities, every dK and dV row of its sequence
@@ -314,6 +326,24 @@ def test_attention_backward_paths(cuda_device, path, dtype, d):
     q, k, v, g, _, _ = _attend_inputs(lq, lk, 2, d, dtype, path + d)
     want, bound = ref.attention(q, k, v, g, lq, lk, 2, d ** -0.5)
     _check(_cabi_backward(q, k, v, g, lq, lk, 2, path, 24), want, bound, "path %d" % path)
+
+
+@pytest.mark.parametrize("path,dtype,d", [(0, torch.float32, 64), (0, torch.float16, 24), (0, torch.float16, 64), (0, torch.bfloat16, 128),
+                                          (2, torch.float16, 32), (3, torch.float16, 64), (4, torch.float16, 64), (4, torch.bfloat16, 64)], ids=str)
+def test_attention_rows_behind_the_last_sequence(cuda_device, path, dtype, d):
+    """Tokens that belong to no sequence hold anything: they are neither written nor do they reach a result (fp16: nor the power
+    of two that dO is brought to)."""
+    lq, lk = [70, 3, 200, 9], [65, 40, 140, 30]
+    q, k, v, g, _, _ = _attend_inputs(lq + [50], lk + [50], 2, d, dtype, 31)
+    for t in (q, k, v, g):
+        t[-50:-25] = float("nan")
+        t[-25:] = torch.finfo(dtype).max
+    nq, nk = sum(lq), sum(lk)
+    want, bound = ref.attention(q[:nq], k[:nk], v[:nk], g[:nq], lq, lk, 2, d ** -0.5)
+    got = _cabi_backward(q, k, v, g, lq, lk, 2, path)
+    for name, n in (("dq", nq), ("dk", nk), ("dv", nk)):
+        assert bool((got[name][n:] == 7.0).all())
+    _check({n: t[:nq if n in ("out", "dq") else nk] for n, t in got.items()}, want, bound, "path %d" % path)
 
 
 @pytest.mark.parametrize("op", ["norm", "attend"])
