@@ -494,6 +494,9 @@ int launch_attn_simt(const QkvSrc& s, void* out, int64_t batch, int64_t q_tokens
   return status_from_cuda(cudaGetLastError());
 }
 
+// the tcgen05 kernel stores its output 32 bytes at a time
+bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
+
 template <typename T, int D>
 int launch_attn_fa(const QkvSrc& s, void* out, int64_t batch, int H, int64_t max_len_q, float scale, cudaStream_t st) {
   constexpr int kSmem = 5 * kBKV * D * 2;  // 20 / 40 / 80 KB
@@ -568,7 +571,7 @@ extern "C" {
 
 size_t ntb200_varlen_attention_workspace_bytes(int64_t batch, int64_t total_tokens, int num_heads, int head_dim, int dtype) {
   if (batch <= 0 || total_tokens <= 0) return 0;
-  if (!attn_tcgen05_supported(batch, total_tokens, num_heads, head_dim, dtype)) return 0;
+  if (!attn_tcgen05_supported(batch, total_tokens, num_heads, head_dim, dtype, false)) return 0;
   return attn_tcgen05_workspace_bytes(batch, total_tokens);
 }
 
@@ -597,8 +600,8 @@ int ntb200_varlen_attention(const void* qkv, void* out, const int64_t* offsets, 
       return launch_attn_tiny<__nv_bfloat16>(src, out, batch, num_heads, head_dim, max_len, scaling, st);
     }
   }
-  const bool tc_ok = dtype != NTB200_F32 && (num_heads * (int64_t)head_dim) % 8 == 0 && aligned16(qkv) && aligned16(out) &&
-                     attn_tcgen05_supported(batch, total_tokens, num_heads, head_dim, dtype);
+  const bool tc_ok = dtype != NTB200_F32 && (num_heads * (int64_t)head_dim) % 8 == 0 && aligned16(qkv) && aligned32(out) &&
+                     attn_tcgen05_supported(batch, total_tokens, num_heads, head_dim, dtype, false);
   if (path == 3 || (path == 0 && tc_ok && workspace != nullptr)) {
     if (!tc_ok) return NTB200_UNSUPPORTED_SHAPE;
     const size_t need = attn_tcgen05_workspace_bytes(batch, total_tokens);
@@ -610,7 +613,7 @@ int ntb200_varlen_attention(const void* qkv, void* out, const int64_t* offsets, 
     // so a batch cut into shards or ranges reproduces the one-call result bit for bit.
     const int skip_short = path == 0 ? (int)kTinyMaxLen : 0;
     return attn_tcgen05_launch(qkv, out, AttnRows{offsets, offsets, (int64_t)num_heads * head_dim, (int64_t)num_heads * head_dim, nullptr},
-                               batch, total_tokens, num_heads, scaling, dtype, workspace, st, skip_short);
+                               batch, total_tokens, num_heads, head_dim, scaling, dtype, workspace, st, skip_short);
   }
   const int64_t E = (int64_t)num_heads * head_dim;
   const size_t es = dtype == NTB200_F32 ? 4 : 2;
@@ -638,7 +641,7 @@ int ntb200_varlen_cross_attention(const void* q, int64_t ldq, const void* k, int
 
 size_t ntb200_varlen_cross_attention_workspace_bytes(int64_t batch, int64_t q_tokens, int num_heads, int head_dim, int dtype) {
   if (batch <= 0 || q_tokens <= 0) return 0;
-  if (!attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype)) return 0;
+  if (!attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype, false)) return 0;
   return attn_tcgen05_workspace_bytes(batch, q_tokens);
 }
 
@@ -656,8 +659,8 @@ int ntb200_varlen_cross_attention_ws(const void* q, int64_t ldq, const void* k, 
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || offsets_q == nullptr || offsets_k == nullptr)
     return NTB200_INVALID_ARG;
   // path 0: tcgen05 when the shape allows it and a workspace is given, else the mma.sync kernel, else SIMT; 3: tcgen05 or error
-  const bool tc_ok = dtype != NTB200_F32 && attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype) && k_tokens > 0 &&
-                     k_tokens < (1ll << 31) - 128 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) &&
+  const bool tc_ok = dtype != NTB200_F32 && attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype, false) && k_tokens > 0 &&
+                     k_tokens < (1ll << 31) - 128 && aligned16(q) && aligned16(k) && aligned16(v) && aligned32(out) &&
                      ldq % 8 == 0 && ldk % 8 == 0 && ldv % 8 == 0;
   if (path == 3 || (path == 0 && tc_ok && workspace != nullptr)) {
     if (!tc_ok) return NTB200_UNSUPPORTED_SHAPE;
@@ -665,7 +668,7 @@ int ntb200_varlen_cross_attention_ws(const void* q, int64_t ldq, const void* k, 
     if (workspace == nullptr || workspace_bytes < need) return NTB200_WORKSPACE_TOO_SMALL;
     if (!aligned16(workspace)) return NTB200_MISALIGNED;
     return attn_tcgen05_cross_launch(q, ldq, k, ldk, v, ldv, out, AttnRows{offsets_q, offsets_k, E, E, nullptr}, batch, q_tokens, k_tokens,
-                                     num_heads, scaling, dtype, workspace, static_cast<cudaStream_t>(stream));
+                                     num_heads, head_dim, scaling, dtype, workspace, static_cast<cudaStream_t>(stream));
   }
   const QkvSrc src = {q, k, v, ldq, ldk, ldv, offsets_q, offsets_k, E, E};
   return launch_attn_generic(src, out, batch, q_tokens, num_heads, head_dim, max_len_q, scaling, dtype, path,
@@ -699,8 +702,8 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
     if (dtype == NTB200_F16) return launch_attn_tiny<__half>(src, out, batch, num_heads, head_dim, max_len_q, scaling, st);
     return launch_attn_tiny<__nv_bfloat16>(src, out, batch, num_heads, head_dim, max_len_q, scaling, st);
   }
-  const bool tc_ok = dtype != NTB200_F32 && attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype) && k_tokens > 0 &&
-                     k_tokens < (1ll << 31) - 128 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && ldq % 8 == 0 &&
+  const bool tc_ok = dtype != NTB200_F32 && attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype, true) && k_tokens > 0 &&
+                     k_tokens < (1ll << 31) - 128 && aligned16(q) && aligned16(k) && aligned16(v) && aligned32(out) && ldq % 8 == 0 &&
                      ldk % 8 == 0 && ldv % 8 == 0;
   if (path == 3 || (path == 0 && tc_ok && workspace != nullptr)) {
     if (!tc_ok) return NTB200_UNSUPPORTED_SHAPE;
@@ -708,8 +711,10 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
     if (!aligned16(workspace)) return NTB200_MISALIGNED;
     const AttnRows rows = {offsets_q, offsets_k, row_elems_q, row_elems_k, lse};
     if (packed)
-      return attn_tcgen05_launch(q, out, rows, batch, q_tokens, num_heads, scaling, dtype, workspace, st, path == 0 ? (int)kTinyMaxLen : 0);
-    return attn_tcgen05_cross_launch(q, ldq, k, ldk, v, ldv, out, rows, batch, q_tokens, k_tokens, num_heads, scaling, dtype, workspace, st);
+      return attn_tcgen05_launch(q, out, rows, batch, q_tokens, num_heads, head_dim, scaling, dtype, workspace, st,
+                                 path == 0 ? (int)kTinyMaxLen : 0);
+    return attn_tcgen05_cross_launch(q, ldq, k, ldk, v, ldv, out, rows, batch, q_tokens, k_tokens, num_heads, head_dim, scaling, dtype,
+                                     workspace, st);
   }
   if (path != 1 && dtype != NTB200_F32 && (head_dim == 32 || head_dim == 64 || head_dim == 128)) {
     const int rc = launch_attn_generic(src, out, batch, q_tokens, num_heads, head_dim, max_len_q, scaling, dtype, 2, st);
@@ -728,7 +733,7 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
 size_t ntb200_varlen_attention_train_workspace_bytes(int64_t batch, int64_t q_tokens, int num_heads, int head_dim, int dtype) {
   if (batch <= 0 || q_tokens <= 0) return 0;
   const size_t tiles = attn_fwd_tiles_workspace_bytes(batch, q_tokens);
-  const size_t tc = attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype) ? attn_tcgen05_workspace_bytes(batch, q_tokens) : 0;
+  const size_t tc = attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype, true) ? attn_tcgen05_workspace_bytes(batch, q_tokens) : 0;
   return tiles > tc ? tiles : tc;
 }
 

@@ -1,4 +1,5 @@
-// Variable-length self-attention on tcgen05 tensor cores, head_dim 64, fp16 / bf16.
+// Variable-length self-attention on tcgen05 tensor cores, fp16 / bf16, head_dim 64; with row statistics (the forward pass of
+// training) head_dim 128 too.  What follows describes 64; Cfg<128> says what differs.
 //
 // One CTA = one (sequence, head, 128-query tile).  For every block of 128 keys:
 //     S[128 x n]   = Q K^T          tcgen05.mma, both operands K-major in shared memory (TMA, 128-B swizzle)
@@ -34,9 +35,7 @@ __device__ int g_attn_error = 0;  // bit 0 producer, 1 MMA issuer, 2 softmax
 
 constexpr int kQT = 128;   // query rows per CTA (TMEM lanes)
 constexpr int kKV = 128;   // keys per block
-constexpr int kHD = 64;    // head dim
-constexpr int kTile = kQT * kHD * 2;  // 16 KB: one 128 x 64 two-byte tile
-constexpr int kStages = 2;
+constexpr int kHalf = kQT * 64 * 2;  // 16 KB: one 128 x 64 two-byte tile, as TMA writes it
 // Of the 16 key pairs of a 32-key chunk, pair 2k+1 is exponentiated by the polynomial when bit k is set
 // (0xff: half of all exponentials, 0xaa: a quarter, 0: none), the others on the MUFU unit.  A quarter measured
 // best on B200 at the BERT-large batch (none: +1 %, half: +6 %).
@@ -44,9 +43,7 @@ constexpr unsigned kPolyPairs = 0xaa;
 // A row's reference maximum is raised (and its running output rescaled) only when a block's maximum exceeds it
 // by more than this many powers of two.
 constexpr float kLazyRescale = 8.0f;
-constexpr int kTmemCols = 256;        // S: columns [0,128), P: [128,192), O: [192,256)
-constexpr int kPCol = 128;
-constexpr int kOCol = 192;
+constexpr int kTmemCols = 256;        // of each of the two CTAs of an SM
 constexpr int kAttnThreads = 256;     // warps 0-3 softmax, warp 4 TMA, warp 5 MMA, warps 6-7 idle
 // Register exchange of setmaxnreg.  A request for more registers than the other warps of the CTA give back blocks for
 // ever (it is not one of the bounded waits), so the two counts must add up to twice the count the kernel is launched
@@ -56,8 +53,23 @@ constexpr int kRegLaunch = 65536 / (2 * kAttnThreads);
 constexpr int kRegSoftmax = 208;
 constexpr int kRegControl = 48;
 static_assert(kRegSoftmax + kRegControl == 2 * kRegLaunch && kRegLaunch % 8 == 0, "setmaxnreg exchange must balance");
-constexpr int kAttnSmem = 1024 + kTile * (2 + 2 * kStages) + 256;  // 2 Q buffers + 2 stages of (K, V)
 
+// Head dim 64: S in tensor-memory columns [0,128), P [128,192), O [192,256); Q buffers and K, V stages of 16 KB, two of each.
+// Head dim 128: S [0,128) with P over its first half, O [128,256); one Q buffer and one stage of 32 KB, so that two CTAs still
+// share an SM: the next QK^T waits for this PV, and the other CTA's products run meanwhile.  Two sequences of about 4500
+// tokens, 8 heads, bf16: 197 us (0.83 PFLOP/s) against 564 on the mma.sync kernel; sequences of 1 to 512, 42 against 66; of
+// 1 to 128, 31 against 43.  Bound by the softmax warps' issue and latency, as at 64.
+template <int D>
+struct Cfg {
+  static constexpr bool kSepP = D == 64;  // P has columns of its own
+  static constexpr int kPCol = kSepP ? 128 : 0, kOCol = kSepP ? 192 : 128;
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTile = kHalves * kHalf;
+  static constexpr int kStages = D == 64 ? 2 : 1, kQBufs = kStages;
+  static constexpr int kSmem = 1024 + kTile * (kQBufs + 2 * kStages) + 256;
+};
+
+template <int kStages>
 struct Ctrl {
   uint64_t full_k[kStages];   // K tile (plus Q with the first block of an item) landed
   uint64_t empty_k[kStages];  // QK^T of that stage retired: K (and the Q buffer two items back) reusable
@@ -72,7 +84,7 @@ struct Ctrl {
   volatile int abort;
 };
 
-static_assert(sizeof(Ctrl) <= 256, "control block exceeds its shared-memory slot");
+static_assert(sizeof(Ctrl<2>) <= 256, "control block exceeds its shared-memory slot");
 
 // ------------------------------------------------------------------ work list
 // items[i] = (first query token of the tile, valid query rows in the tile, first key token of the sequence, number
@@ -161,9 +173,10 @@ __global__ void __launch_bounds__(kListThreads) build_items_kernel(const int64_t
 // of those sequences by itself (attn_tiny_warp; it returns at once for a longer sequence).  The short sequences thus
 // cost no launch of their own, and which kernel computes a sequence depends on its own length only.
 constexpr int kPrepWarps = 8;
-constexpr int kPrepSmem = kPrepWarps * 3 * (int)kTinyMaxLen * kHD * 2;  // 96 KB: Q, K, V tiles of 32 x 64 per warp
+template <int D>
+constexpr int kPrepSmem = kPrepWarps * 3 * (int)kTinyMaxLen * D * 2;  // 96 / 192 KB: Q, K, V tiles of 32 x D per warp
 
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(kPrepWarps * 32)
 prepare_self_attention_kernel(const int64_t* __restrict__ offsets, int64_t row_elems, int64_t batch, int64_t E,
                               int4* __restrict__ items, int* __restrict__ count, int64_t capacity, const T* __restrict__ qkv,
@@ -175,9 +188,9 @@ prepare_self_attention_kernel(const int64_t* __restrict__ offsets, int64_t row_e
     return;
   }
   const int warp = threadIdx.x >> 5;
-  attn_tiny_warp<T, kHD, (int)kTinyMaxLen>(qkv, 3 * E, qkv + E, 3 * E, qkv + 2 * E, 3 * E, out, offsets, offsets, row_elems, row_elems,
+  attn_tiny_warp<T, D, (int)kTinyMaxLen>(qkv, 3 * E, qkv + E, 3 * E, qkv + 2 * E, 3 * E, out, offsets, offsets, row_elems, row_elems,
                                            batch, H, scale_log2e, ((int64_t)blockIdx.x - 1) * kPrepWarps + warp,
-                                           (uint32_t)__cvta_generic_to_shared(prep_smem) + (uint32_t)warp * (uint32_t)(kPrepSmem / kPrepWarps),
+                                           (uint32_t)__cvta_generic_to_shared(prep_smem) + (uint32_t)warp * (uint32_t)(kPrepSmem<D> / kPrepWarps),
                                            lse);
 }
 
@@ -198,18 +211,20 @@ prepare_self_attention_kernel(const int64_t* __restrict__ offsets, int64_t row_e
 // because the write needs about 30 registers (it spilled, and lost 20 %, before the row sums were cut to two
 // packed accumulators).
 // STATS: the rows' softmax denominators are stored too (LseOut), for a backward pass.
-template <int FMT, bool STATS>
+template <int FMT, int D, bool STATS>
 __global__ void __launch_bounds__(kAttnThreads, 2)
 attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, int col_q, int col_k, int col_v, void* __restrict__ out,
                     const int4* __restrict__ items, const int* __restrict__ count, int H, float scale_log2e, LseOut lse) {
+  using C = Cfg<D>;
+  constexpr int kStages = C::kStages, kTile = C::kTile;
   const int n_items = *count;
   if ((int64_t)blockIdx.x >= (int64_t)n_items * H) return;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + kTile * (2 + 2 * kStages));
+  Ctrl<kStages>* ctrl = reinterpret_cast<Ctrl<kStages>*>(smem + kTile * (C::kQBufs + 2 * kStages));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t E = (int64_t)H * kHD;
+  const int64_t E = (int64_t)H * D;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -237,8 +252,8 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   __syncthreads();
   ptx::tc_fence_after_sync();
   const uint32_t tmem_base = ctrl->tmem_base;
-  const uint32_t s_q = ptx::smem_u32(smem);          // two Q buffers
-  const uint32_t s_k = s_q + 2 * kTile;              // K ring: stage s at s_k + s*kTile
+  const uint32_t s_q = ptx::smem_u32(smem);          // Q buffers
+  const uint32_t s_k = s_q + C::kQBufs * kTile;      // K ring: stage s at s_k + s*kTile
   const uint32_t s_v = s_k + kStages * kTile;        // V ring: stage s at s_v + s*kTile
 
   // One 16-byte record per work item; every role fetches the record of its NEXT item while it works on
@@ -293,9 +308,12 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           }
           const uint32_t fk = ptx::smem_u32(&ctrl->full_k[s]);
           ptx::mbar_arrive_expect_tx(fk, (j == 0 ? 2 : 1) * kTile);
-          // Q buffer n&1 was last read by item n-2, all of whose QK^T precede the release of this stage
-          if (j == 0) ptx::tma_load_2d(s_q + (n & 1) * kTile, &map_q, fk, col_q + it.h * kHD, it.tq);
-          ptx::tma_load_2d(s_k + s * kTile, &map_k, fk, col_k + it.h * kHD, it.tok0 + j * kKV);
+          // Q buffer n % kQBufs was last read by item n - kQBufs, all of whose QK^T precede the release of this stage
+#pragma unroll
+          for (int x = 0; x < C::kHalves; ++x) {
+            if (j == 0) ptx::tma_load_2d(s_q + (n % C::kQBufs) * kTile + x * kHalf, &map_q, fk, col_q + it.h * D + x * 64, it.tq);
+            ptx::tma_load_2d(s_k + s * kTile + x * kHalf, &map_k, fk, col_k + it.h * D + x * 64, it.tok0 + j * kKV);
+          }
           // ... V only once the PV that last read its stage has retired
           if (!wait_or_abort(ptx::smem_u32(&ctrl->empty_v[s]), ph ^ 1, &ctrl->abort)) {
             ok = false;
@@ -304,7 +322,9 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           }
           const uint32_t fv = ptx::smem_u32(&ctrl->full_v[s]);
           ptx::mbar_arrive_expect_tx(fv, kTile);
-          ptx::tma_load_2d(s_v + s * kTile, &map_v, fv, col_v + it.h * kHD, it.tok0 + j * kKV);
+#pragma unroll
+          for (int x = 0; x < C::kHalves; ++x)
+            ptx::tma_load_2d(s_v + s * kTile + x * kHalf, &map_v, fv, col_v + it.h * D + x * 64, it.tok0 + j * kKV);
         }
       }
       if (!ok) {
@@ -321,11 +341,11 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     } else if (warp == 5 && ptx::elect_one()) {
       // ------------------------------------------------------------ MMA issuer
       bool ok = true;
-      const uint32_t t_s = tmem_base, t_p = tmem_base + kPCol, t_o = tmem_base + kOCol;
-      constexpr uint32_t idesc_pv = ptx::umma_idesc_f16(FMT, kQT, kHD, 0, 1);  // B = V is MN-major
+      const uint32_t t_s = tmem_base, t_p = tmem_base + C::kPCol, t_o = tmem_base + C::kOCol;
+      constexpr uint32_t idesc_pv = ptx::umma_idesc_f16(FMT, kQT, D, 0, 1);  // B = V is MN-major
       const uint64_t desc_q0 = ptx::umma_desc_kmajor_sw128(s_q);
       const uint64_t desc_k0 = ptx::umma_desc_kmajor_sw128(s_k);
-      const uint64_t desc_v0 = ptx::umma_desc_mnmajor_sw128(s_v);
+      const uint64_t desc_v0 = ptx::umma_desc_mnmajor_sw128(s_v, C::kHalves > 1 ? kHalf : 16);
       // cursor A: the block whose QK^T is issued next (runs one block ahead of cursor B: PV)
       Pos ia = first;
       uint32_t ga = 0, na = 0;
@@ -339,10 +359,13 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         int nvalid = a.L - ja * kKV;
         nvalid = nvalid > kKV ? kKV : nvalid;
         const uint32_t idesc_qk = ptx::umma_idesc_f16(FMT, kQT, (nvalid + 15) & ~15);
-        const uint64_t dq = desc_q0 + (uint64_t)((na & 1) * (kTile >> 4));
+        const uint64_t dq = desc_q0 + (uint64_t)((na % C::kQBufs) * (kTile >> 4));
         const uint64_t dk = desc_k0 + (uint64_t)(s * (kTile >> 4));
 #pragma unroll
-        for (int k = 0; k < kHD / 16; ++k) ptx::umma_f16(t_s, dq + 2 * k, dk + 2 * k, idesc_qk, k != 0 ? 1u : 0u);
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t at = (uint64_t)((k / 4) * (kHalf >> 4) + 2 * (k % 4));
+          ptx::umma_f16(t_s, dq + at, dk + at, idesc_qk, k != 0 ? 1u : 0u);
+        }
         ptx::umma_commit(ptx::smem_u32(&ctrl->empty_k[s]));
         ptx::umma_commit(ptx::smem_u32(&ctrl->s_ready));
         ++ga;
@@ -363,7 +386,7 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         rec_b = fetch(next(ib));
         for (int jb = 0; jb < b.n_blk && ok; ++jb, ++gb) {
           // S of block gb is in the softmax warps' registers: the next QK^T may overwrite it
-          if (ia.item < n_items) {
+          if (C::kSepP && ia.item < n_items) {
             if (!wait_or_abort(ptx::smem_u32(&ctrl->s_free), gb & 1, &ctrl->abort)) { ok = false; break; }
             if (!issue_qk()) { ok = false; break; }
           }
@@ -380,8 +403,8 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             for (int r = nvalid; r < r_end; ++r) {
               const uint32_t addr = s_v + s * kTile + (uint32_t)((r >> 3) * 1024 + (r & 7) * 128);
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr + c * 16), "r"(0u) : "memory");
+              for (int c = 0; c < 8 * C::kHalves; ++c)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr + (c / 8) * kHalf + (c % 8) * 16), "r"(0u) : "memory");
             }
             ptx::fence_proxy_async();  // make the generic-proxy stores visible to the tensor core's reads
           }
@@ -397,6 +420,11 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           }
           ptx::umma_commit(ptx::smem_u32(&ctrl->empty_v[s]));
           ptx::umma_commit(ptx::smem_u32(&ctrl->o_ready));
+          if (!C::kSepP && ia.item < n_items) {
+            // P lies over S: the next QK^T waits for this PV (the SM's other CTA works meanwhile)
+            if (!wait_or_abort(ptx::smem_u32(&ctrl->o_ready), gb & 1, &ctrl->abort)) { ok = false; break; }
+            if (!issue_qk()) { ok = false; break; }
+          }
         }
       }
       if (!ok) {
@@ -413,7 +441,7 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const int q = warp;                              // TMEM lane quarter of this warp
     const int row = q * 32 + lane;                   // row inside the tile = TMEM lane
     const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
-    const uint32_t t_s = tmem_base + lane_addr, t_p = tmem_base + kPCol + lane_addr, t_o = tmem_base + kOCol + lane_addr;
+    const uint32_t t_s = tmem_base + lane_addr, t_p = tmem_base + C::kPCol + lane_addr, t_o = tmem_base + C::kOCol + lane_addr;
     bool ok = true;
     uint32_t g = 0;
 
@@ -433,7 +461,7 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const float inv = pend.inv;
         uint16_t* orow = reinterpret_cast<uint16_t*>(out) + pend.out_row0 + (int64_t)row * E;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < D / 16; ++c) {
           uint32_t r0[16];
           ptx::tmem_ld_32x32b_x16(t_o + c * 16, r0);
           ptx::tmem_ld_wait();
@@ -473,9 +501,11 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           ptx::tmem_ld_wait();
         }
         // S has been consumed: the MMA warp may issue the next block's QK^T
-        ptx::tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->s_free));
+        if (C::kSepP) {
+          ptx::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->s_free));
+        }
         float m_new = m, corr = 1.0f;
         bool any_up = false;
         if (ok && warp_active) {
@@ -537,7 +567,7 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           if (any_up) {
             // rescale the running output (only when some row of the warp raised its reference maximum)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {  // 16 columns at a time: the S row stays live in registers
+            for (int c = 0; c < D / 16; ++c) {  // 16 columns at a time: the S row stays live in registers
               uint32_t r0[16];
               ptx::tmem_ld_32x32b_x16(t_o + c * 16, r0);
               ptx::tmem_ld_wait();
@@ -567,7 +597,13 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const float p0 = ptx::ex2_approx(a0), p1 = ptx::ex2_approx(a1);
                 float p2, p3;
                 if ((kPolyPairs >> k) & 1) {
-                  ptx::ex2_poly_x2(ptx::f32x2_pack(fmaxf(b0, -126.0f), fmaxf(b1, -126.0f)), p2, p3);
+                  if (STATS) {  // (the polynomial's exponent arithmetic loses a NaN: 0 x brings it back)
+                    const uint64_t x = ptx::f32x2_pack(ptx::fmax_nan(b0, -126.0f), ptx::fmax_nan(b1, -126.0f));
+                    ptx::ex2_poly_x2(x, p2, p3);
+                    ptx::f32x2_unpack(ptx::f32x2_fma(x, ptx::f32x2_pack(0.0f, 0.0f), ptx::f32x2_pack(p2, p3)), p2, p3);
+                  } else {
+                    ptx::ex2_poly_x2(ptx::f32x2_pack(fmaxf(b0, -126.0f), fmaxf(b1, -126.0f)), p2, p3);
+                  }
                 } else {
                   p2 = ptx::ex2_approx(b0);
                   p3 = ptx::ex2_approx(b1);
@@ -599,7 +635,7 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       pend.warp_active = warp_active;
       pend.inv = 1.0f / l;
       pend.rows = it.rows;
-      pend.out_row0 = (int64_t)it.tq * E + (int64_t)it.h * kHD;
+      pend.out_row0 = (int64_t)it.tq * E + (int64_t)it.h * D;
       if (STATS && ok && row < it.rows) lse.ptr[(int64_t)it.h * lse.ld + it.tq + row] = m + log2f(l);
     }
     if (ok && pend.any) {  // the last item of this CTA
@@ -623,17 +659,17 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   }
 }
 
-template <int FMT, bool STATS>
+template <int FMT, int D, bool STATS>
 int launch(const TileSource& q, int col_q, const TileSource& k, int col_k, const TileSource& v, int col_v, void* out,
            const AttnRows& rows, int64_t batch, int64_t q_tokens, int H, float scaling, int dtype, void* workspace, cudaStream_t st,
            int skip_short) {  // skip_short > 0: self-attention only
-  const int64_t E = (int64_t)H * kHD;
+  const int64_t E = (int64_t)H * D;
   CUtensorMap map_q, map_k, map_v;
   if (!make_tile_map(&map_q, q, dtype) || !make_tile_map(&map_k, k, dtype) || !make_tile_map(&map_v, v, dtype))
     return NTB200_LAUNCH_FAILED;
   static std::atomic<int> attr_set[kMaxDevices];
   if (!once_per_device(attr_set, [] {
-        return cudaFuncSetAttribute(attn_tcgen05_kernel<FMT, STATS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnSmem) == cudaSuccess;
+        return cudaFuncSetAttribute(attn_tcgen05_kernel<FMT, D, STATS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem) == cudaSuccess;
       }))
     return NTB200_LAUNCH_FAILED;
   const int64_t capacity = attn_tcgen05_item_capacity(batch, q_tokens);
@@ -644,12 +680,13 @@ int launch(const TileSource& q, int col_q, const TileSource& k, int col_k, const
     using T16 = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
     static std::atomic<int> prep_set[kMaxDevices];
     if (!once_per_device(prep_set, [] {
-          return cudaFuncSetAttribute(prepare_self_attention_kernel<T16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrepSmem) == cudaSuccess;
+          return cudaFuncSetAttribute(prepare_self_attention_kernel<T16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrepSmem<D>) ==
+                 cudaSuccess;
         }))
       return NTB200_LAUNCH_FAILED;
     const int64_t blocks = 1 + (batch * H + kPrepWarps - 1) / kPrepWarps;
     if (blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
-    prepare_self_attention_kernel<T16><<<(unsigned)blocks, kPrepWarps * 32, kPrepSmem, st>>>(
+    prepare_self_attention_kernel<T16, D><<<(unsigned)blocks, kPrepWarps * 32, kPrepSmem<D>, st>>>(
         rows.offsets_q, rows.row_elems_q, batch, E, items, count, capacity, static_cast<const T16*>(q.base), static_cast<T16*>(out), H,
         scaling * 1.4426950408889634f, LseOut{rows.lse, q_tokens});
   } else {
@@ -660,8 +697,8 @@ int launch(const TileSource& q, int col_q, const TileSource& k, int col_k, const
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   int64_t grid = 2ll * sms;  // two resident CTAs per SM, each loops over its share of the items
   if (grid > capacity * H) grid = capacity * H;
-  attn_tcgen05_kernel<FMT, STATS><<<(unsigned)grid, kAttnThreads, kAttnSmem, st>>>(map_q, map_k, map_v, col_q, col_k, col_v, out, items, count, H,
-                                                                            scaling * 1.4426950408889634f, LseOut{rows.lse, q_tokens});
+  attn_tcgen05_kernel<FMT, D, STATS><<<(unsigned)grid, kAttnThreads, Cfg<D>::kSmem, st>>>(
+      map_q, map_k, map_v, col_q, col_k, col_v, out, items, count, H, scaling * 1.4426950408889634f, LseOut{rows.lse, q_tokens});
   return status_from_cuda(cudaGetLastError());
 }
 
@@ -673,29 +710,37 @@ size_t attn_tcgen05_workspace_bytes(int64_t batch, int64_t total_tokens) {
   return 16 + sizeof(int4) * (size_t)attn_tcgen05_item_capacity(batch, total_tokens);
 }
 
-bool attn_tcgen05_supported(int64_t batch, int64_t total_tokens, int num_heads, int head_dim, int dtype) {
-  return head_dim == kHD && (dtype == NTB200_F16 || dtype == NTB200_BF16) && num_heads <= 65535 &&
-         total_tokens < (1ll << 31) - kQT && 3ll * num_heads * kHD < (1ll << 31) &&
+bool attn_tcgen05_supported(int64_t batch, int64_t total_tokens, int num_heads, int head_dim, int dtype, bool stats) {
+  return (head_dim == 64 || (stats && head_dim == 128)) && (dtype == NTB200_F16 || dtype == NTB200_BF16) && num_heads <= 65535 &&
+         total_tokens < (1ll << 31) - kQT && 3ll * num_heads * head_dim < (1ll << 31) &&
          attn_tcgen05_item_capacity(batch, total_tokens) < (1ll << 31);
 }
 
-int attn_tcgen05_launch(const void* qkv, void* out, const AttnRows& rows, int64_t batch, int64_t total_tokens, int H, float scaling,
+namespace {
+
+using LaunchFn = decltype(&launch<0, 64, false>);
+
+LaunchFn pick(int dtype, int d, bool stats) {  // (head dim 128 comes with statistics only: attn_tcgen05_supported)
+  if (dtype == NTB200_F16) return d == 128 ? launch<0, 128, true> : stats ? launch<0, 64, true> : launch<0, 64, false>;
+  return d == 128 ? launch<1, 128, true> : stats ? launch<1, 64, true> : launch<1, 64, false>;
+}
+
+}  // namespace
+
+int attn_tcgen05_launch(const void* qkv, void* out, const AttnRows& rows, int64_t batch, int64_t total_tokens, int H, int d, float scaling,
                         int dtype, void* workspace, cudaStream_t st, int skip_short) {
-  const int64_t E = (int64_t)H * kHD;
+  const int64_t E = (int64_t)H * d;
   const TileSource src = {qkv, total_tokens, 3 * E, 3 * E};  // one map, three column offsets
-  const bool f16 = dtype == NTB200_F16, stats = rows.lse != nullptr;
-  auto fn = f16 ? (stats ? launch<0, true> : launch<0, false>) : (stats ? launch<1, true> : launch<1, false>);
-  return fn(src, 0, src, (int)E, src, (int)(2 * E), out, rows, batch, total_tokens, H, scaling, dtype, workspace, st, skip_short);
+  return pick(dtype, d, rows.lse != nullptr)(src, 0, src, (int)E, src, (int)(2 * E), out, rows, batch, total_tokens, H, scaling, dtype, workspace,
+                                             st, skip_short);
 }
 
 int attn_tcgen05_cross_launch(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* out,
-                              const AttnRows& rows, int64_t batch, int64_t q_tokens, int64_t k_tokens, int H, float scaling, int dtype,
+                              const AttnRows& rows, int64_t batch, int64_t q_tokens, int64_t k_tokens, int H, int d, float scaling, int dtype,
                               void* workspace, cudaStream_t st) {
-  const int64_t E = (int64_t)H * kHD;
+  const int64_t E = (int64_t)H * d;
   const TileSource sq = {q, q_tokens, E, ldq}, sk = {k, k_tokens, E, ldk}, sv = {v, k_tokens, E, ldv};
-  const bool f16 = dtype == NTB200_F16, stats = rows.lse != nullptr;
-  auto fn = f16 ? (stats ? launch<0, true> : launch<0, false>) : (stats ? launch<1, true> : launch<1, false>);
-  return fn(sq, 0, sk, 0, sv, 0, out, rows, batch, q_tokens, H, scaling, dtype, workspace, st, 0);
+  return pick(dtype, d, rows.lse != nullptr)(sq, 0, sk, 0, sv, 0, out, rows, batch, q_tokens, H, scaling, dtype, workspace, st, 0);
 }
 
 int attn_tcgen05_error_flags_read_and_clear() {

@@ -192,8 +192,8 @@ def test_attention_gradients_head_sizes(cuda_device, dtype, d):
 # tile borders of every kernel: 16, 32, 64, 128 rows and one more or less, lengths of zero and one, several tiles
 @pytest.mark.parametrize("lengths", [[1], [2, 15, 16, 17], [31, 32, 33, 0], [63, 64, 65], [127, 128, 129], [255, 256, 257], [640, 1], [0, 0, 3],
                                      [383, 511, 700]], ids=str)
-@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.float16, 64), (torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float16, 32)],
-                         ids=str)
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.float16, 64), (torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float16, 128),
+                                     (torch.float16, 32)], ids=str)
 def test_attention_gradients_lengths(cuda_device, dtype, d, lengths):
     q, k, v, g, qs, _ = _attend_inputs(lengths, lengths, 3, d, dtype, len(lengths))
     want, bound = ref.attention(q, k, v, g, lengths, lengths, 3, d ** -0.5)
@@ -259,11 +259,12 @@ def test_attention_over_one_key_has_no_score_gradient(cuda_device, dtype, d):
     _check(got, want, bound, "one key")
 
 
+@pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-def test_attention_carries_nan(cuda_device, dtype):
+def test_attention_carries_nan(cuda_device, dtype, d):
     """One NaN query reaches its own output row and dQ row and, through its probabilities, every dK and dV row of its sequence
     and no other's, at every position in the kernels' tiles."""
-    lengths, H, d = [40, 150], 1, 64
+    lengths, H = [40, 150], 1
     q, k, v, g, qs, _ = _attend_inputs(lengths, lengths, H, d, dtype, 16)
     for row in list(range(40, 56)) + [100, 167, 168, 189]:
         q2 = q.clone()
@@ -274,6 +275,21 @@ def test_attention_carries_nan(cuda_device, dtype):
             assert bool(bad[row]) and int(torch.isnan(got[name]).any(1).sum()) == 1, (name, row)
         for name in ("dk", "dv"):
             assert bool(torch.isnan(got[name][40:]).all()) and not bool(torch.isnan(got[name][:40]).any()), (name, row)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_attention_carries_nan_keys(cuda_device, dtype, d):
+    """One NaN key makes every probability of its sequence and head NaN, at every position in the kernels' tiles, and no other's."""
+    lengths = [40, 150]
+    q, k, v, g, qs, _ = _attend_inputs(lengths, lengths, 2, d, dtype, 17)
+    for row in list(range(40, 72)) + [100, 167, 168, 189]:
+        k2 = k.clone()
+        k2[row, :d] = float("nan")
+        got = _run_self(q, k2, v, g, qs, 2)
+        for name, t in got.items():
+            assert bool(torch.isnan(t[40:, :d]).all()), (name, row)
+            assert not bool(torch.isnan(t[:40]).any()) and not bool(torch.isnan(t[:, d:]).any()), (name, row)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
@@ -298,7 +314,7 @@ def _cabi_backward(q, k, v, g, lq, lk, heads, path, ld_extra=0):
     ws = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
     _cabi.check("train", lib.ntb200_varlen_attention_train(
         q.data_ptr(), E, k.data_ptr(), E, v.data_ptr(), E, out.data_ptr(), lse.data_ptr(), off[0].data_ptr(), 1, off[1].data_ptr(), 1, B, Tq, Tk,
-        heads, d, max(lq), scaling, code, min(path, 3) if path < 3 or d == 64 else 2, ws.data_ptr(), n, stream_ptr()))
+        heads, d, max(lq), scaling, code, min(path, 3), ws.data_ptr(), n, stream_ptr()))
     n = lib.ntb200_varlen_attention_backward_workspace_bytes(B, Tq, Tk, heads, d, max(lq), max(lk), code, path)
     ws = torch.full((n + 64,), 0xAB, dtype=torch.uint8, device="cuda")
     wide = E + ld_extra

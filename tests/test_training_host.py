@@ -86,13 +86,15 @@ def test_cabi_rejects_bad_arguments_without_launching(native_libs):
     assert lib.ntb200_embedding_backward(None, None, 8, None, 0, 0, 64, -1, 1.0, 0, None, 0, None) == 0
 
     # attention
-    def train(q=16, ld=64, k=16, out=16, lse=16, offs=16, row=64, batch=1, tq=4, tk=4, heads=1, d=64, dtype=2, path=0, ws=None, n=0):
+    def train(q=16, ld=64, k=16, out=32, lse=16, offs=16, row=64, batch=1, tq=4, tk=4, heads=1, d=64, dtype=2, path=0, ws=None, n=0):
         return lib.ntb200_varlen_attention_train(q, ld, k, ld, k, ld, out, lse, offs, row, offs, row, batch, tq, tk, heads, d, 4, 0.125, dtype,
                                                  path, ws, n, None)
 
     assert train(ld=63) == -1 and train(lse=None) == -1 and train(row=0) == -1 and train(path=4) == -1 and train(dtype=3) == -2
     assert train(d=257, ld=300) == -7 and train(batch=0) == 0 and train(tq=0) == 0 and train(k=None) == -1
     assert train(path=3, ws=16, n=3) == -6 and train(path=3, d=32) == -7
+    assert train(path=3, ws=16, n=1 << 20, out=16) == -7  # the tcgen05 kernel stores 32 bytes at a time
+    assert lib.ntb200_varlen_attention(16, 16, 16, 1, 4, 1, 64, 4, 0.125, 2, 3, 16, 1 << 20, None) == -7
 
     def backward(g=16, ld=64, offs=16, row=64, batch=1, tq=4, tk=4, heads=1, d=64, dtype=2, path=0, ws=16, n=1 << 20, dq=16):
         return lib.ntb200_varlen_attention_backward(g, 16, ld, 16, ld, 16, ld, 16, 16, dq, ld, 16, ld, 16, ld, offs, row, offs, row, batch, tq,
