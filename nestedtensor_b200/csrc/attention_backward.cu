@@ -296,9 +296,33 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
 // computes a (BT/16) x (BT/16) patch of S and dP and keeps BT/16 rows x DP/16 columns of each gradient in registers.
 template <typename T, int BT, int DP>
 __device__ __forceinline__ void load_rows(float* __restrict__ s, const T* __restrict__ g, int64_t ld, int rows, int d) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (d % 4 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0) {
+#pragma unroll
+      for (int i = threadIdx.x; i < BT * DP / 4; i += 256) {
+        const int r = i / (DP / 4), c = i % (DP / 4) * 4;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r < rows && c < d) v = *reinterpret_cast<const float4*>(g + (int64_t)r * ld + c);
+        *reinterpret_cast<float4*>(s + r * (DP + 4) + c) = v;
+      }
+      return;
+    }
+  }
   for (int i = threadIdx.x; i < BT * DP; i += 256) {
     const int r = i / DP, c = i % DP;
     s[r * (DP + 4) + c] = (r < rows && c < d) ? to_f32(g[(int64_t)r * ld + c]) : 0.0f;
+  }
+}
+
+// MI neighbouring values at a multiple of MI
+template <int MI>
+__device__ __forceinline__ void load_some(float (&v)[MI], const float* __restrict__ s) {
+  if constexpr (MI == 4) {
+    const float4 x = *reinterpret_cast<const float4*>(s);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) v[i] = s[i];
   }
 }
 
@@ -396,11 +420,8 @@ __device__ __forceinline__ void bwd_simt_item(const BwdArgs& a, const Item& it, 
     __syncthreads();
     for (int c = 0; c < nc; ++c) {
       float ds[MI], pv[MI];
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        ds[i] = s_ds[c * LS + ty * MI + i];
-        if (KV) pv[i] = s_p[c * LS + ty * MI + i];
-      }
+      load_some(ds, s_ds + c * LS + ty * MI);
+      if (KV) load_some(pv, s_p + c * LS + ty * MI);
 #pragma unroll
       for (int m = 0; m < NC / 4; ++m) {
         const float4 x = *reinterpret_cast<const float4*>(oth_a + c * LD + tx * 4 + 64 * m);
@@ -559,8 +580,7 @@ attn_fwd_simt_kernel(BwdArgs a, T* __restrict__ out, float* __restrict__ lse, co
       }
       for (int c = 0; c < nc; ++c) {
         float p[MI];
-#pragma unroll
-        for (int i = 0; i < MI; ++i) p[i] = s_p[c * LS + ty * MI + i];
+        load_some(p, s_p + c * LS + ty * MI);
 #pragma unroll
         for (int m = 0; m < NC / 4; ++m) {
           const float4 x = *reinterpret_cast<const float4*>(s_v + c * LD + tx * 4 + 64 * m);
