@@ -722,7 +722,7 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
   }
   if (path == 2) return NTB200_UNSUPPORTED_SHAPE;
   // what no tensor-core kernel takes: 32-bit tiles (the inference entry points' kernel, one warp per query and head, rereads its
-  // keys for every query: 242 us against 50 us for 16 sequences of up to 200 tokens, 4 heads of 64 in fp32)
+  // keys for every query: 242 us against 44 us for 16 sequences of up to 200 tokens, 4 heads of 64 in fp32)
   if (q_tokens >= (1ll << 31) - 256 || k_tokens >= (1ll << 31) - 256 || batch >= (1ll << 31) - 256) return NTB200_UNSUPPORTED_SHAPE;
   if (workspace == nullptr || workspace_bytes < attn_fwd_tiles_workspace_bytes(batch, q_tokens)) return NTB200_WORKSPACE_TOO_SMALL;
   if (!aligned16(workspace)) return NTB200_MISALIGNED;

@@ -293,7 +293,10 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
 //     KV:  r = keys,    A_own = K, B_own = V;   c = queries, A = Q, B = dO:   dV_r += P_cr dO_c,  dK_r += dS_cr Q_c
 //     !KV: r = queries, A_own = Q, B_own = dO;  c = keys,    A = K, B = V:    dQ_r += dS_cr K_c
 // with S_cr = A_own,r . A_c and dP_cr = B_own,r . B_c in both.  Everything is held in fp32 in shared memory, each thread
-// computes a (BT/16) x (BT/16) patch of S and dP and keeps BT/16 rows x DP/16 columns of each gradient in registers.
+// computes a (BT/16) x (BT/16) patch of S and dP and keeps BT/16 rows x DP/16 columns of each gradient in registers.  fp32 has no
+// tensor-core product of its precision, so this is bound by the FMA units and the shared-memory reads that feed them: 0.58
+// GFLOP in 16 sequences of up to 200 tokens (4 heads of 64) take 55 us, two waves of items of up to four tiles; 12 GFLOP in two
+// of up to 1400 (12 heads) 830 us, 15 TFLOP/s.
 template <typename T, int BT, int DP>
 __device__ __forceinline__ void load_rows(float* __restrict__ s, const T* __restrict__ g, int64_t ld, int rows, int d) {
   if constexpr (std::is_same<T, float>::value) {
@@ -618,7 +621,8 @@ attn_fwd_simt_kernel(BwdArgs a, T* __restrict__ out, float* __restrict__ lse, co
 //     S = A_own A_c^T,  dP = B_own B_c^T        (B operands: rows of the other side's tiles)
 //     acc1 += P B_c,    acc2 += dS A_c          (B operands: the same tiles, transposed by ldmatrix)
 // Other side's tiles of 64 rows come double-buffered through cp.async.  P and dS are rounded to the 16-bit type for the products
-// (as the forward pass rounds P); all sums are fp32.
+// (as the forward pass rounds P); all sums are fp32.  Bound by the ldmatrix and mma.sync issue of its 9 products, of which short
+// sequences leave part empty: 10 000 tokens of lengths up to 64, 8 heads of 128, 133 us with the lists and D.
 constexpr int kMmaThreads = 128, kMmaTile = 64;
 
 template <typename T, int D>
@@ -907,12 +911,12 @@ int launch_bwd_mma(const BwdArgs& a, int64_t k_tokens, const Lists& l, cudaStrea
 }
 
 // Sequences of up to kShort tokens on both sides go to the mma.sync kernel, whose tiles have 64 rows: 21 000 tokens of lengths up to 64
-// take 272 us there and 413 on the tcgen05 kernels (16 heads of 64), 10 000 take 107 and 178 (8 heads of 128); of lengths up to
-// 128, 283 and 243, and 122 and 117.
+// take 273 us there and 449 on the tcgen05 kernels (16 heads of 64), 10 000 take 133 and 204 (8 heads of 128); of lengths up to
+// 128, 291 and 265, and 148 and 141.
 constexpr int64_t kShort = 64;
 // Heads of 64: sequences of up to kMid tokens as whole items (S and dP once for all three gradients): 128 sequences of 32 to 512 tokens, 12
-// heads: 417 us against 446 with an item per tile; beyond, a sequence would keep its one CTA busy for long (one of 1024, 16
-// heads: 207 us against 47).
+// heads: 416 us against 445 with an item per tile; beyond, a sequence would keep its one CTA busy for long (one of 1024, 16
+// heads: 217 us against 47).
 constexpr int64_t kMid = 512;
 
 Plan make_plan(int d, bool tc, int path) {

