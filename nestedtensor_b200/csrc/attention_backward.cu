@@ -295,8 +295,8 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
 // with S_cr = A_own,r . A_c and dP_cr = B_own,r . B_c in both.  Everything is held in fp32 in shared memory, each thread
 // computes a (BT/16) x (BT/16) patch of S and dP and keeps BT/16 rows x DP/16 columns of each gradient in registers.  fp32 has no
 // tensor-core product of its precision, so this is bound by the FMA units and the shared-memory reads that feed them: 0.58
-// GFLOP in 16 sequences of up to 200 tokens (4 heads of 64) take 55 us, two waves of items of up to four tiles; 12 GFLOP in two
-// of up to 1400 (12 heads) 830 us, 15 TFLOP/s.
+// GFLOP in 16 sequences of up to 200 tokens (4 heads of 64) take 57 us, two waves of items of up to four tiles; two sequences
+// of up to 1400 (12 heads) 594 us, 22 TFLOP/s of its seven products (832 us before two blocks fitted an SM).
 template <typename T, int BT, int DP>
 __device__ __forceinline__ void load_rows(float* __restrict__ s, const T* __restrict__ g, int64_t ld, int rows, int d) {
   if constexpr (std::is_same<T, float>::value) {
@@ -467,7 +467,7 @@ __device__ __forceinline__ void bwd_simt_item(const BwdArgs& a, const Item& it, 
 
 // KV items, then Q items, in one launch: neither alone fills the GPU when the batch is small
 template <typename T, int BT, int DP>
-__global__ void __launch_bounds__(256) attn_bwd_simt_kernel(BwdArgs a, ListOut kv, ListOut qi) {
+__global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) attn_bwd_simt_kernel(BwdArgs a, ListOut kv, ListOut qi) {
   const int64_t n_kv = (int64_t)*kv.count * a.H, n = n_kv + (int64_t)*qi.count * a.H;
   for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
     if (w < n_kv) bwd_simt_item<T, BT, DP, true>(a, decode(kv.items[w / a.H]), (int)(w % a.H));
@@ -481,7 +481,7 @@ template <int BT, int DP>
 constexpr int fwd_simt_smem() { return (3 * BT * (DP + 4) + BT * (BT + 4) + 3 * BT) * 4; }
 
 template <typename T, int BT, int DP>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, DP == 64 ? 2 : 1)
 attn_fwd_simt_kernel(BwdArgs a, T* __restrict__ out, float* __restrict__ lse, const int4* __restrict__ items, const int* __restrict__ count) {
   constexpr int MI = BT / 16, LD = DP + 4, LS = BT + 4, NC = DP / 16;
   extern __shared__ __align__(16) float bwd_smem[];
