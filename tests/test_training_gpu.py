@@ -219,20 +219,22 @@ def test_attention_one_side_empty(cuda_device, dtype):
             assert torch.equal(t, torch.zeros_like(t)), name
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-def test_attention_does_not_mix_sequences(cuda_device, dtype):
+def test_attention_does_not_mix_sequences(cuda_device, dtype, d):
     """NaN and Inf in one sequence stay there, and the others' gradients have the bits they have alone."""
-    lengths, H, d = [20, 33, 130, 77], 2, 64
+    lengths, H = [20, 33, 130, 77, 530, 9], 2
     q, k, v, g, qs, _ = _attend_inputs(lengths, lengths, H, d, dtype, 6)
     clean = _run_self(q, k, v, g, qs, H)
-    for bad in (1, 2):
+    for bad in range(1, len(lengths)):
         a = sum(lengths[:bad])
         sl = slice(a, a + lengths[bad])
-        q2, v2, g2 = q.clone(), v.clone(), g.clone()
+        q2, k2, v2, g2 = q.clone(), k.clone(), v.clone(), g.clone()
         q2[sl] = float("nan")
+        k2[sl] = float("inf")
         v2[sl] = float("inf")
         g2[sl] = float("-inf")
-        got = _run_self(q2, k, v2, g2, qs, H)
+        got = _run_self(q2, k2, v2, g2, qs, H)
         for name in got:
             for other in range(len(lengths)):
                 o = sum(lengths[:other])
