@@ -2,7 +2,9 @@
 // C++ autograd function over the C ABI's forward pass (which keeps what the gradients need) and backward pass.  First
 // derivatives only: differentiating a gradient raises.  Host validation, allocation through torch's caching allocator and
 // launches on the current stream as in dispatch.cpp; nothing is kept between calls, so captured CUDA graphs share nothing.
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -27,9 +29,25 @@ struct FirstOrderOnly : public torch::autograd::Function<FirstOrderOnly> {
 
 c10::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
 
+// A leaf's gradient node belongs to the stream it was made on, and lives as long as any graph of that leaf.  In a capture, the engine
+// would make that stream wait for the captured one; the default stream must not, and the process does not survive it.
+void refuse_capture_into_default_stream() {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto& edge : node->next_edges()) {
+    if (!edge.is_valid()) continue;
+    const auto stream = edge.function->stream();
+    TORCH_CHECK(!stream || stream->device_type() != c10::DeviceType::CUDA || c10::cuda::CUDAStream(*stream).stream() != nullptr,
+                "nestedtensor_b200: a backward pass is being captured into a CUDA graph while an eager graph of the same leaves, made on the "
+                "default stream, is alive: drop it (its outputs, its loss) before the capture, or run it on another stream");
+  }
+}
+
 // Runs `compute` (the gradients) without recording it; with create_graph=True every result keeps its dependence on `deps`.
 template <typename F>
 variable_list first_order(const std::array<Tensor, 4>& deps, F&& compute) {
+  refuse_capture_into_default_stream();
   const bool create_graph = at::GradMode::is_enabled();
   variable_list grads;
   {

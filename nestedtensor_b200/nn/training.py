@@ -14,7 +14,8 @@ between them (projections, activations, residuals, losses) is plain torch on unp
 Gradients flow to the values of the inputs, to weights and biases; first derivatives only.  All tensors of a call have one
 device and one dtype (float32, float16 or bfloat16); statistics, sums and softmax denominators are fp32.  The gradients are
 sums in a fixed order: the same inputs give the same bits.  Work runs on the current stream, the gradients on the stream of
-their forward call; workspaces belong to the call.  The functions of ``nestedtensor_b200.nn`` itself are the inference forms:
+their forward call; workspaces belong to the call.  Forward and backward may be captured into a CUDA graph, unless an eager
+graph of the same leaves, made on the default stream, is still alive: that call raises.  The functions of ``nestedtensor_b200.nn`` itself are the inference forms:
 they do not track gradients, and refuse a NestedTensor that does."""
 from __future__ import annotations
 

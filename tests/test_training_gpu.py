@@ -504,6 +504,38 @@ def test_block_on_another_stream(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(one, want))
 
 
+def test_capture_beside_an_eager_graph_of_the_same_leaf(cuda_device):
+    """Refused with an error, and the process, the eager graph and a capture without it go on."""
+    sizes = torch.tensor([[3, 64], [5, 64]])
+    x = torch.randn(8, 64, device="cuda")
+    w, b = (torch.randn(64, device="cuda", requires_grad=True) for _ in range(2))
+    nested = nt.NestedTensor(x.view(-1), sizes)
+    g = torch.randn(8, 64, device="cuda")
+
+    def step():
+        y = training.layer_norm(nested, 64, w, b).values()
+        return torch.autograd.grad(y, [w, b], g)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = step()
+    torch.cuda.current_stream().wait_stream(side)
+    eager = training.layer_norm(nested, 64, w, b).values()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(eager, [w, b], g), want))
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
 def test_second_derivatives_are_refused(cuda_device):
     x = torch.randn(6, 32, device="cuda", requires_grad=True)
     sizes = torch.tensor([[2, 32], [4, 32]])
