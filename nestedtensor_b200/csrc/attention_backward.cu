@@ -174,25 +174,27 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
     }
   };
   if constexpr (VEC) load(lane);  // (in flight while the sequence is looked up)
-  int64_t b = 0, key0 = 0, keys = INT64_MAX;
+  int64_t b = 0, key0 = 0, keys = 0;
+  bool few = false;
   if constexpr (kRounded) {
     b = find_entry_warp(a.offsets_q, 0, a.batch - 1, t * a.row_elems_q);
     if (t * a.row_elems_q >= a.offsets_q[b + 1]) return;  // behind the last sequence: nothing reads its D
-    key0 = a.offsets_k[b] / a.row_elems_k, keys = a.offsets_k[b + 1] / a.row_elems_k - key0;
+    const int64_t k_first = a.offsets_k[b], k_elems = a.offsets_k[b + 1] - k_first;
+    few = k_elems <= kFewKeys * a.row_elems_k;
+    if (few) key0 = k_first / a.row_elems_k, keys = k_elems / a.row_elems_k;
   }
-  const bool few = kRounded && keys <= kFewKeys;
   const float scale = a.scaling * kLog2e;
   const T* q = static_cast<const T*>(a.q) + t * a.ldq;
   const T* k0 = static_cast<const T*>(a.k) + key0 * a.ldk;
   const T* v0 = static_cast<const T*>(a.v) + key0 * a.ldv;
   if constexpr (VEC) {
     constexpr int kDtype = std::is_same<T, __half>::value ? NTB200_F16 : NTB200_BF16;  // (VEC: 16-bit types)
-    const int per = a.d / 8;  // lanes per head
+    const int per = a.d / 8, log_per = 31 - __clz(per);  // lanes per head: 4, 8 or 16
     if (few) {
       constexpr int kAhead = 4;  // keys whose rows are in flight together
       for (int v = lane; v < nv + lane; v += 32) {  // (the same trips for every lane: the sums are warp-wide)
         const bool live = v < nv;
-        const int h = live ? v / per : 0;
+        const int h = live ? v >> log_per : 0;
         float xe[8], qe[8], s = 0.0f, m = 0.0f;
         Vec16<kDtype>::unpack(live ? reinterpret_cast<const uint4*>(g)[v] : make_uint4(0u, 0u, 0u, 0u), xe);
         Vec16<kDtype>::unpack(live ? reinterpret_cast<const uint4*>(q)[v] : make_uint4(0u, 0u, 0u, 0u), qe);
@@ -227,7 +229,7 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
             if (j0 + i < (int)keys) s = fmaf(exp2f(fmaf(sij, scale, -lse)), dp, s);
           }
         }
-        if (live && lane % per == 0) {
+        if (live && (lane & (per - 1)) == 0) {
           a.delta[(int64_t)h * a.q_tokens + t] = s;
           if (top != nullptr) atomicMax(top + b * a.H + h, __float_as_uint(m));
         }
@@ -252,8 +254,8 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
         }
         const int v = first + 32 * i;
-        if (v < nv && lane % per == 0) {
-          const int h = v / per;
+        if (v < nv && (lane & (per - 1)) == 0) {
+          const int h = v >> log_per;
           a.delta[(int64_t)h * a.q_tokens + t] = s;
           if (top != nullptr) atomicMax(top + b * a.H + h, __float_as_uint(m));
         }
