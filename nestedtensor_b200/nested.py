@@ -45,13 +45,20 @@ def build_meta(sizes: torch.Tensor, device) -> torch.Tensor:
 class _Ragged(object):
     """What nested tensors over the same rows share: the sizes of the one they were made from (the first column holds the
     lengths), its device offsets, and the elements per row in them.  Holds no values."""
-    __slots__ = ("sizes", "meta", "device", "row_elems")
+    __slots__ = ("sizes", "meta", "device", "_row_elems")
 
     def __init__(self, sizes, meta, device):
         self.sizes, self.meta, self.device = sizes, meta, device
-        self.row_elems = 1
-        if sizes.size(0) > 0 and sizes.size(1) > 1:
-            self.row_elems = int(sizes[0, 1]) if sizes.size(1) == 2 else int(sizes[0, 1:].prod())
+        self._row_elems = None
+
+    @property
+    def row_elems(self):
+        if self._row_elems is None:
+            n = 1
+            if self.sizes.size(0) > 0 and self.sizes.size(1) > 1:
+                n = int(self.sizes[0, 1]) if self.sizes.size(1) == 2 else int(self.sizes[0, 1:].prod())
+            self._row_elems = n
+        return self._row_elems
 
     def on(self, device):
         """The same structure with its offsets on `device`."""
