@@ -374,11 +374,13 @@ int ntb200_embedding_backward(const void* grad, const void* index, int index_byt
                               int64_t vocab, int64_t embed_dim, int64_t padding_idx, float scale, int dtype,
                               void* workspace, size_t workspace_bytes, void* stream);
 
-/* Attention: as ntb200_varlen_cross_attention_ws (self-attention: the same offsets twice; where q, k and v are the three
- * thirds of one [T, 3*H*d] matrix the kernels and results are those of ntb200_varlen_attention), and
+/* Attention: as ntb200_varlen_cross_attention_ws (self-attention: the same offsets twice, and in 16 bits with q, k and v the three
+ * thirds of one [T, 3*H*d] matrix as ntb200_varlen_attention; head_dim 128 and what no tensor-core kernel takes run on
+ * kernels of their own, off by roundings), and
  *   lse[h*q_tokens + t] = log2( sum_j exp2(scaling * log2(e) * q_t,h . k_j,h) )      (left unwritten for rows without keys)
  * offsets_q / offsets_k count elements of matrices with row_elems_q / row_elems_k elements per token (1: token offsets).
- *   path  0 = best available;  1 = 32-bit tiles;  2 = mma.sync kernel;  3 = tcgen05 kernel (1-3: for cross-checks)
+ *   path  0 = best available;  1 = 32-bit tiles;  2 = mma.sync kernel;  3 = tcgen05 kernel: head_dim 64 or 128, rows on
+ *         16-byte boundaries, out on a 32-byte one (1-3: for cross-checks)
  * workspace: 16-byte aligned.
  */
 size_t ntb200_varlen_attention_train_workspace_bytes(int64_t batch, int64_t q_tokens, int num_heads, int head_dim,

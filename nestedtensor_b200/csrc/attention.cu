@@ -696,7 +696,7 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
   const bool packed = offsets_q == offsets_k && row_elems_q == row_elems_k && q_tokens == k_tokens && ldq == 3 * E && ldk == 3 * E &&
                       ldv == 3 * E && static_cast<const char*>(k) == static_cast<const char*>(q) + E * es &&
                       static_cast<const char*>(v) == static_cast<const char*>(q) + 2 * E * es;
-  // the same choices as the inference entry points
+  // the same choices as the inference entry points, but for heads of 128, which the tcgen05 kernel takes with statistics
   if (path == 0 && packed && dtype != NTB200_F32 && (head_dim == 32 || head_dim == 64 || head_dim == 128) && E % 8 == 0 && aligned16(q) &&
       aligned16(out) && max_len_q >= 1 && max_len_q <= kTinyMaxLen) {
     if (dtype == NTB200_F16) return launch_attn_tiny<__half>(src, out, batch, num_heads, head_dim, max_len_q, scaling, st);
