@@ -44,29 +44,32 @@ def build_meta(sizes: torch.Tensor, device) -> torch.Tensor:
 
 class _Ragged(object):
     """What nested tensors over the same rows share: the sizes of the one they were made from (the first column holds the
-    lengths), its device offsets, and the elements per row in them.  Holds no values."""
-    __slots__ = ("sizes", "meta", "device", "_row_elems")
+    lengths) and its device offsets.  Holds no values."""
+    __slots__ = ("sizes", "meta", "device", "_rows")
 
     def __init__(self, sizes, meta, device):
         self.sizes, self.meta, self.device = sizes, meta, device
-        self._row_elems = None
-
-    @property
-    def row_elems(self):
-        if self._row_elems is None:
-            n = 1
-            if self.sizes.size(0) > 0 and self.sizes.size(1) > 1:
-                n = int(self.sizes[0, 1]) if self.sizes.size(1) == 2 else int(self.sizes[0, 1:].prod())
-            self._row_elems = n
-        return self._row_elems
+        self._rows = None
 
     def on(self, device):
-        """The same structure with its offsets on `device`."""
-        if self.meta is None or self.meta.device != device:
-            if self.device != device:
-                return _Ragged(self.sizes, build_meta(self.sizes, device), device)
-            self.meta = build_meta(self.sizes, device)
-        return self
+        """The same structure for tensors on `device`."""
+        return self if self.device == device else _Ragged(self.sizes, None, device)
+
+    def row_offsets(self):
+        """(device offsets of the constituents, what one row counts in them).  Element offsets where all rows have the same
+        number of elements, and at least one; otherwise only the lengths tell where a constituent begins, one a row."""
+        if self._rows is None:
+            width = 1
+            for j in range(1, self.sizes.size(1) if self.sizes.size(0) > 0 else 0):
+                extents = self.sizes[:, j]
+                width *= int(extents[0]) if bool((extents == extents[0]).all()) else 0
+            if width == 0:
+                self._rows = build_meta(self.sizes[:, :1].contiguous(), self.device), 1
+            else:
+                if self.meta is None or self.meta.device != self.device:
+                    self.meta = build_meta(self.sizes, self.device)
+                self._rows = self.meta, width
+        return self._rows
 
 
 class NestedTensor(object):
@@ -174,9 +177,9 @@ class NestedTensor(object):
         return NestedTensor._over(packed, self._structure())
 
     def _row_offsets(self):
-        """(device offsets of the constituents, elements per row in them)."""
-        r = self._ragged = self._structure().on(self.device)
-        return r.meta, r.row_elems
+        """(device offsets of the constituents, what one row counts in them)."""
+        self._ragged = self._structure().on(self.device)
+        return self._ragged.row_offsets()
 
     def _tracked(self):
         """(rows, sizes, features) as an operator that tracks gradients takes them: the packed rows with their last extent and
