@@ -42,6 +42,10 @@ def build_meta(sizes: torch.Tensor, device) -> torch.Tensor:
     return host
 
 
+def _capturing(device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class _Ragged(object):
     """What nested tensors over the same rows share: the sizes of the one they were made from (the first column holds the
     lengths) and its device offsets.  Holds no values."""
@@ -63,12 +67,17 @@ class _Ragged(object):
             for j in range(1, self.sizes.size(1) if self.sizes.size(0) > 0 else 0):
                 extents = self.sizes[:, j]
                 width *= int(extents[0]) if bool((extents == extents[0]).all()) else 0
-            if width == 0:
-                self._rows = build_meta(self.sizes[:, :1].contiguous(), self.device), 1
-            else:
-                if self.meta is None or self.meta.device != self.device:
-                    self.meta = build_meta(self.sizes, self.device)
+            if width > 0 and self.meta is not None and self.meta.device == self.device:
                 self._rows = self.meta, width
+                return self._rows
+            if _capturing(self.device):
+                raise RuntimeError("nestedtensor_b200: the offsets of this nested tensor are not on the device yet; make them before the "
+                                   "capture (by a pass over the same nested tensor, or one that shares its structure)")
+            if width > 0:
+                self.meta = build_meta(self.sizes, self.device)
+                self._rows = self.meta, width
+            else:
+                self._rows = build_meta(self.sizes[:, :1].contiguous(), self.device), 1
         return self._rows
 
 
@@ -83,7 +92,7 @@ class NestedTensor(object):
             raise RuntimeError("channels_last needs constituents of shape (C, H_i, W_i)")
         self._flat = buffer
         self._extents = sizes.contiguous()
-        self._meta = meta
+        self._offsets = meta
         # channels_last (nestedtensor/csrc/nested_tensor_impl.cpp:46, storage_is_contiguous_channels_last): the sizes are
         # the logical (C, H_i, W_i), every constituent is STORED as (H_i, W_i, C), i.e. with strides (1, W_i*C, C).
         self._channels_last = bool(channels_last)
@@ -96,7 +105,7 @@ class NestedTensor(object):
         """A nested tensor over the [rows, ...] matrix `packed` (contiguous; it carries the autograd graph) with the lengths of
         `ragged`; its flat buffer and its sizes are made when something asks for them."""
         out = cls.__new__(cls)
-        out._flat = out._extents = out._meta = out._nchw = None
+        out._flat = out._extents = out._offsets = out._nchw = None
         out._channels_last = False
         out._packed = packed
         out._ragged = ragged
@@ -120,6 +129,14 @@ class NestedTensor(object):
             self._extents = sizes
         return self._extents
 
+    @property
+    def _meta(self):
+        """The device offsets and sizes, or None as long as nothing has asked for them.  A tensor with the sizes that a structure was
+        made from shares them with it."""
+        if self._offsets is None and self._packed is None and self._ragged is not None:
+            self._offsets = self._ragged.meta
+        return self._offsets
+
     # ---- record access -------------------------------------------------------------------
     def _record(self):
         """(buffer, sizes, meta) in the contiguous layout every operator works on; a channels_last tensor is brought
@@ -131,9 +148,14 @@ class NestedTensor(object):
         if self._packed is not None and self._packed.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("nestedtensor_b200: this operator does not track gradients and would drop them; use "
                                "nestedtensor_b200.nn.training, torch.no_grad() or detach the values")
-        if self._meta is None or self._meta.device != self._buffer.device:
-            self._meta = build_meta(self._sizes, self._buffer.device)
-        return self._buffer, self._sizes, self._meta
+        meta = self._meta
+        if meta is None or meta.device != self._buffer.device:
+            meta = build_meta(self._sizes, self._buffer.device)
+            if not _capturing(meta.device):  # (made inside a capture, they belong to that graph and hold nothing before its replay)
+                self._offsets = meta
+                if self._packed is None and self._ragged is not None:
+                    self._ragged.meta = meta
+        return self._buffer, self._sizes, meta
 
     def _stored_sizes(self):
         """Constituent shapes as they lie in the buffer."""

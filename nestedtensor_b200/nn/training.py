@@ -14,9 +14,14 @@ between them (projections, activations, residuals, losses) is plain torch on unp
 Gradients flow to the values of the inputs, to weights and biases; first derivatives only.  All tensors of a call have one
 device and one dtype (float32, float16 or bfloat16); statistics, sums and softmax denominators are fp32.  The gradients are
 sums in a fixed order: the same inputs give the same bits.  Work runs on the current stream, the gradients on the stream of
-their forward call; workspaces belong to the call.  Forward and backward may be captured into a CUDA graph, unless an eager
-graph of the same leaves, made on the default stream, is still alive: that call raises.  The functions of ``nestedtensor_b200.nn`` itself are the inference forms:
-they do not track gradients, and refuse a NestedTensor that does."""
+their forward call; workspaces belong to the call.
+
+Forward and backward may be captured into a CUDA graph, with two exceptions, which raise: an eager graph of the same leaves,
+made on the default stream, is still alive; or attention needs the offsets of a nested tensor that are not on the device yet (a
+pass over it before the capture puts them there, and every nested tensor made from it shares them).
+
+The functions of ``nestedtensor_b200.nn`` itself are the inference forms: they do not track gradients, and refuse a NestedTensor
+that does."""
 from __future__ import annotations
 
 from typing import Optional

@@ -37,3 +37,48 @@ def test_attention_over_the_rows_of_irregular_constituents(cuda_device, dtype, h
         results.append((y, z, *torch.autograd.grad([y, z], [qkv, q, k, v], [g, g])))
     for x, want in zip(*results):
         assert torch.equal(x, want) and bool(torch.isfinite(x).all())
+
+
+def test_capture_needs_the_offsets_on_the_device(cuda_device):
+    """Made inside a capture, the offsets would be copied out of a host block that is no longer theirs at the replay: refused; and a
+    nested tensor whose offsets were made before is taken, by training and inference operators alike."""
+    sizes = torch.tensor([[3, 96], [50, 96]])
+    x = torch.randn(53, 96, device="cuda")
+    ready, late = nt.NestedTensor(x.view(-1), sizes), nt.NestedTensor(x.view(-1), sizes)
+    want = training.self_attention(ready, 2).values()
+    assert ready._meta is not None and late._meta is None
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            training.self_attention(late, 2)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            training.attention(ready, late, late, 2)
+    assert late._meta is None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = training.self_attention(ready, 2).values()
+    # eager passes over other lengths take whatever host and device memory is free
+    for n in range(1, 30):
+        other = nt.NestedTensor(x[:n + 20].reshape(-1), torch.tensor([[n, 96], [20, 96]]))
+        training.self_attention(other, 2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_offsets_made_inside_a_capture_are_not_kept(cuda_device):
+    """An inference operator makes the offsets in its graph, where they hold nothing before the replay: an eager call makes its own."""
+    sizes = torch.tensor([[3, 8], [50, 8]])
+    x = torch.randn(53, 8, device="cuda")
+    nested = nt.NestedTensor(x.view(-1), sizes)
+    want = nt.NestedTensor(x.view(-1), sizes).to_padded_tensor(0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = nested.to_padded_tensor(0)
+    assert nested._meta is None
+    assert torch.equal(nested.to_padded_tensor(0), want)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)

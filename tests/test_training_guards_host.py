@@ -26,3 +26,27 @@ def test_row_offsets_follow_the_lengths(shapes):
         assert (offsets % row == 0).all() and (offsets // row).tolist() == starts
         assert b.nested_size() == tuple(torch.Size([n, 6]) for n in lengths)
         assert b._record()[2][:len(lengths) + 1].tolist() == [6 * n for n in starts]
+
+
+def test_structure_and_record_share_their_offsets():
+    """One copy of the offsets, whichever operator asked first."""
+    for first in ("rows", "record"):
+        a = _nested([(3, 5), (4, 5)])
+        b = a.with_values(torch.zeros(7, 2))
+        assert a._meta is None
+        if first == "rows":
+            rows = a._row_offsets()[0]
+            assert a._meta is rows
+            meta = a._record()[2]
+        else:
+            meta = a._record()[2]
+            rows = a._row_offsets()[0]
+        assert rows is meta and b._row_offsets()[0] is meta and a._meta is meta
+        assert b._meta is None and b._record()[2].tolist() == [0, 6, 14, 3, 2, 4, 2]  # (its own sizes)
+    given = torch.tensor([0, 15, 35, 3, 5, 4, 5])
+    a = nt.NestedTensor(torch.zeros(35), torch.tensor([[3, 5], [4, 5]]), given)
+    assert a._meta is given and a._record()[2] is given and a._row_offsets() == (given, 5)
+    odd = _nested([(3, 5), (4, 7)])  # the record counts elements, the structure rows
+    assert odd._record()[2].tolist() == [0, 15, 43, 3, 5, 4, 7]
+    offsets, row = odd._row_offsets()
+    assert row == 1 and offsets[:3].tolist() == [0, 3, 7] and odd._record()[2].tolist() == [0, 15, 43, 3, 5, 4, 7]
