@@ -5,11 +5,14 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/library.h>
 
 #include <algorithm>
 #include <array>
 #include <cmath>
+#include <unordered_set>
+#include <vector>
 
 #include "dispatch_common.h"
 
@@ -30,17 +33,30 @@ struct FirstOrderOnly : public torch::autograd::Function<FirstOrderOnly> {
 c10::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
 
 // A leaf's gradient node belongs to the stream it was made on, and lives as long as any graph of that leaf.  In a capture, the engine
-// would make that stream wait for the captured one; the default stream must not, and the process does not survive it.
+// would make that stream wait for the captured one; the default stream must not, and the process does not survive it.  The leaf may
+// lie behind other nodes (views, projections): all that this pass will run from here on are looked at.
 void refuse_capture_into_default_stream() {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
-  for (const auto& edge : node->next_edges()) {
-    if (!edge.is_valid()) continue;
-    const auto stream = edge.function->stream();
-    TORCH_CHECK(!stream || stream->device_type() != c10::DeviceType::CUDA || c10::cuda::CUDAStream(*stream).stream() != nullptr,
-                "nestedtensor_b200: a backward pass is being captured into a CUDA graph while an eager graph of the same leaves, made on the "
-                "default stream, is alive: drop it (its outputs, its loss) before the capture, or run it on another stream");
+  const auto* wanted = torch::autograd::get_current_graph_task_exec_info();  // (empty: every node)
+  std::vector<torch::autograd::Node*> todo = {node.get()};
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!todo.empty()) {
+    const auto* at = todo.back();
+    todo.pop_back();
+    for (const auto& edge : at->next_edges()) {
+      if (!edge.is_valid() || !seen.insert(edge.function.get()).second) continue;
+      if (wanted != nullptr && !wanted->empty()) {
+        const auto it = wanted->find(edge.function.get());
+        if (it == wanted->end() || !it->second.should_execute()) continue;
+      }
+      const auto stream = edge.function->stream();
+      TORCH_CHECK(!stream || stream->device_type() != c10::DeviceType::CUDA || c10::cuda::CUDAStream(*stream).stream() != nullptr,
+                  "nestedtensor_b200: a backward pass is being captured into a CUDA graph while an eager graph of the same leaves, made on the "
+                  "default stream, is alive: drop it (its outputs, its loss) before the capture, or run it on another stream");
+      todo.push_back(edge.function.get());
+    }
   }
 }
 

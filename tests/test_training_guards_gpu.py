@@ -82,3 +82,48 @@ def test_offsets_made_inside_a_capture_are_not_kept(cuda_device):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def _in_a_capture(step):
+    """`step` run eagerly on a side stream (no graph of it stays alive), then captured: (eager result, result of one replay)."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    return want, got
+
+
+def test_capture_beside_an_eager_graph_of_a_leaf_behind_other_nodes(cuda_device):
+    """The leaf whose eager graph is alive need not be an input of the operator itself: a projection and a view lie between."""
+    sizes = torch.tensor([[3, 64], [5, 64]])
+    x, p = (torch.randn(s, device="cuda", requires_grad=True) for s in ((8, 32), (32, 64)))
+    w, b = (torch.randn(64, device="cuda", requires_grad=True) for _ in range(2))
+    g = torch.randn(8, 64, device="cuda")
+
+    def step(leaves=(x, p, w, b)):
+        rows = (x @ p).view(-1)
+        y = training.layer_norm(nt.NestedTensor(rows, sizes), 64, w, b).values()
+        return torch.autograd.grad(y, leaves, g)
+
+    want, got = _in_a_capture(step)  # no eager graph is alive (and cuBLAS is set up)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    for make in (lambda: x * 2, lambda: p.view(-1) * 3):
+        eager = make()
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                step()
+        want, got = _in_a_capture(lambda: step((w, b)))  # a pass that does not reach the leaf
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+        eager.sum().backward()
+        del eager
+        x.grad = p.grad = None
+    want, got = _in_a_capture(step)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
