@@ -210,11 +210,7 @@ class NestedTensor(object):
             raise RuntimeError("nestedtensor_b200: the training operators need contiguous constituents")
         if self._packed is not None:
             return self._packed, self._ragged.sizes, self._packed.size(-1) if self._packed.dim() > 1 else 1
-        buf = self._flat
-        base = buf._base
-        if base is not None and base.requires_grad and base.numel() == buf.numel() and base.is_contiguous():
-            buf = base  # a flat view of a whole tensor: the gradient goes to the tensor itself, without the view's own step
-        return buf, self._extents, -1
+        return self._flat, self._extents, -1
 
     # ---- attributes ----------------------------------------------------------------------
     @property

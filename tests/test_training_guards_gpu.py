@@ -127,3 +127,46 @@ def test_capture_beside_an_eager_graph_of_a_leaf_behind_other_nodes(cuda_device)
         x.grad = p.grad = None
     want, got = _in_a_capture(step)
     assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def _hooked(x, sizes):
+    """(leaf, the flat buffer made from it, a nested tensor over that buffer)"""
+    x = x.detach().requires_grad_()
+    buf = x.view(-1)
+    return x, buf, nt.NestedTensor(buf, sizes)
+
+
+def test_the_callers_buffer_is_in_the_graph(cuda_device):
+    """Hooks on the buffer that a nested tensor was made of see and change its gradient; it can keep it, and be differentiated."""
+    sizes = torch.tensor([[2, 96], [7, 96]])
+    data, g = torch.randn(9, 96, device="cuda"), torch.randn(9, 96, device="cuda")
+    ops = {"norm": lambda t: training.layer_norm(t, 96), "self": lambda t: training.self_attention(t, 2),
+           "query": lambda t: training.attention(t, t.with_values(data), t.with_values(data), 2)}
+    for name, op in ops.items():
+        x, buf, nested = _hooked(data, sizes)
+        y = op(nested).values()
+        go = g[:, :y.size(1)]
+        want, = torch.autograd.grad(y, x, go)
+        x, buf, nested = _hooked(data, sizes)
+        buf.register_hook(lambda t: t * 2)
+        y = op(nested).values()
+        y.backward(go)
+        assert torch.equal(x.grad, want * 2), name
+        x, buf, nested = _hooked(data, sizes)
+        got, = torch.autograd.grad(op(nested).values(), buf, go)
+        assert torch.equal(got, want.view(-1)), name
+        buf.retain_grad()
+        op(nested).values().backward(go)
+        assert torch.equal(buf.grad, want.view(-1)) and torch.equal(x.grad, want), name
+
+
+def test_a_buffer_cut_off_from_the_graph_stays_cut_off(cuda_device):
+    """No gradient flows through a view made under no_grad to its base."""
+    sizes = torch.tensor([[2, 64], [7, 64]])
+    x = torch.randn(9, 64, device="cuda", requires_grad=True)
+    w, b = (torch.randn(64, device="cuda", requires_grad=True) for _ in range(2))
+    with torch.no_grad():
+        buf = x.view(-1)
+    y = training.layer_norm(nt.NestedTensor(buf, sizes), 64, w, b).values()
+    y.sum().backward()
+    assert x.grad is None and w.grad is not None

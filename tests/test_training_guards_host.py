@@ -50,3 +50,14 @@ def test_structure_and_record_share_their_offsets():
     assert odd._record()[2].tolist() == [0, 15, 43, 3, 5, 4, 7]
     offsets, row = odd._row_offsets()
     assert row == 1 and offsets[:3].tolist() == [0, 3, 7] and odd._record()[2].tolist() == [0, 15, 43, 3, 5, 4, 7]
+
+
+def test_the_tracked_rows_are_the_callers_own_tensor():
+    """No base of a view in its place: that would pass by its hooks, and lead gradients around a no_grad block."""
+    x = torch.randn(7, 5, requires_grad=True)
+    sizes = torch.tensor([[3, 5], [4, 5]])
+    buf = x.view(-1)
+    assert nt.NestedTensor(buf, sizes)._tracked()[0] is buf
+    with torch.no_grad():
+        cut = x.view(-1)
+    assert nt.NestedTensor(cut, sizes)._tracked()[0] is cut
