@@ -125,6 +125,22 @@ Rows make_rows(const Tensor& t, const Tensor& sizes, int64_t features, const cha
   return r;
 }
 
+// Elements per row of constituents (L_i, ...), where all rows have the same number and at least one; 0 otherwise.
+int64_t row_elems(const Tensor& sizes) {
+  TORCH_CHECK(sizes.device().is_cpu() && sizes.scalar_type() == at::kLong && sizes.dim() == 2 && sizes.is_contiguous(),
+              "nestedtensor_b200: sizes must be a contiguous CPU int64 [B, tensor_dim] tensor");
+  const int64_t B = sizes.size(0), td = sizes.size(1);
+  const int64_t* p = sizes.data_ptr<int64_t>();
+  int64_t width = 1;
+  for (int64_t b = 0; b < B; ++b) {
+    int64_t n = 1;
+    for (int64_t j = 1; j < td; ++j) n *= p[b * td + j];
+    if (b == 0) width = n;
+    if (n != width || n < 1) return 0;
+  }
+  return width;
+}
+
 void check_meta(const Tensor& meta, int64_t row_elems, int64_t B, const Tensor& like) {
   TORCH_CHECK(meta.is_cuda() && meta.device() == like.device() && meta.scalar_type() == at::kLong && meta.is_contiguous() && meta.numel() >= B + 1,
               "nestedtensor_b200: meta must be a CUDA int64 tensor that begins with B+1 offsets, on the input's device");
@@ -410,6 +426,7 @@ TORCH_LIBRARY_FRAGMENT(nestedtensor, m) {
   m.def(
       "layer_norm_train(Tensor x, Tensor sizes, int features, int[] normalized_shape, Tensor? weight, Tensor? bias, float eps) -> Tensor",
       &layer_norm_train);
+  m.def("row_elems(Tensor sizes) -> int", &row_elems);
   m.def("embedding_train(Tensor weight, Tensor index, Tensor sizes, int? padding_idx, float scale) -> Tensor", &embedding_train);
   m.def(
       "self_attention_train(Tensor qkv, Tensor sizes, int features, Tensor meta, int row_elems, int num_heads, float? scaling) -> Tensor",

@@ -63,22 +63,21 @@ class _Ragged(object):
         """(device offsets of the constituents, what one row counts in them).  Element offsets where all rows have the same
         number of elements, and at least one; otherwise only the lengths tell where a constituent begins, one a row."""
         if self._rows is None:
-            width = 1
-            for j in range(1, self.sizes.size(1) if self.sizes.size(0) > 0 else 0):
-                extents = self.sizes[:, j]
-                width *= int(extents[0]) if bool((extents == extents[0]).all()) else 0
-            if width > 0 and self.meta is not None and self.meta.device == self.device:
-                self._rows = self.meta, width
-                return self._rows
-            if _capturing(self.device):
-                raise RuntimeError("nestedtensor_b200: the offsets of this nested tensor are not on the device yet; make them before the "
-                                   "capture (by a pass over the same nested tensor, or one that shares its structure)")
-            if width > 0:
-                self.meta = build_meta(self.sizes, self.device)
-                self._rows = self.meta, width
-            else:
+            width = _ops.ops().row_elems(self.sizes)
+            if width == 0:
+                self._refuse_capture()
                 self._rows = build_meta(self.sizes[:, :1].contiguous(), self.device), 1
+            else:
+                if self.meta is None or self.meta.device != self.device:
+                    self._refuse_capture()
+                    self.meta = build_meta(self.sizes, self.device)
+                self._rows = self.meta, width
         return self._rows
+
+    def _refuse_capture(self):
+        if _capturing(self.device):
+            raise RuntimeError("nestedtensor_b200: the offsets of this nested tensor are not on the device yet; make them before the "
+                               "capture (by a pass over the same nested tensor, or one that shares its structure)")
 
 
 class NestedTensor(object):

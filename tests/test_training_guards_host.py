@@ -14,7 +14,7 @@ def _nested(shapes, **kw):
 @pytest.mark.parametrize("shapes", [[(3, 5), (4, 5)], [(3, 5), (4, 7)], [(4, 7), (3, 5)], [(3, 0), (4, 7)], [(3, 5), (0, 0), (2, 5)],
                                     [(2, 0), (5, 0)], [(0, 4), (6, 9), (1, 1)], [(2, 3, 4), (5, 4, 3)], [(2, 3, 4), (5, 3, 4)],
                                     [(2, 3, 0), (5, 4, 0)], [(3,), (0,), (2,)]], ids=str)
-def test_row_offsets_follow_the_lengths(shapes):
+def test_row_offsets_follow_the_lengths(native_libs, shapes):
     """with_values() takes any constituents (L_i, ...): whatever their other dimensions, sequence i of the result begins at row
     L_0 + ... + L_(i-1)."""
     lengths = [s[0] for s in shapes]
@@ -28,7 +28,7 @@ def test_row_offsets_follow_the_lengths(shapes):
         assert b._record()[2][:len(lengths) + 1].tolist() == [6 * n for n in starts]
 
 
-def test_structure_and_record_share_their_offsets():
+def test_structure_and_record_share_their_offsets(native_libs):
     """One copy of the offsets, whichever operator asked first."""
     for first in ("rows", "record"):
         a = _nested([(3, 5), (4, 5)])
