@@ -140,13 +140,20 @@ class NestedTensor(object):
     def _record(self):
         """(buffer, sizes, meta) in the contiguous layout every operator works on; a channels_last tensor is brought
         there once (one transpose kernel) and the result is kept."""
+        self._refuse_tracked()
         if self._channels_last:
             if self._nchw is None:
                 self._nchw = self.contiguous()
             return self._nchw._record()
-        if self._packed is not None and self._packed.requires_grad and torch.is_grad_enabled():
+        return (self._buffer, *self._layout())
+
+    def _refuse_tracked(self):
+        if self.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("nestedtensor_b200: this operator does not track gradients and would drop them; use "
                                "nestedtensor_b200.nn.training, torch.no_grad() or detach the values")
+
+    def _layout(self):
+        """(sizes, meta) of the same record, for operators that read no values."""
         meta = self._meta
         if meta is None or meta.device != self._buffer.device:
             meta = build_meta(self._sizes, self._buffer.device)
@@ -154,7 +161,7 @@ class NestedTensor(object):
                 self._offsets = meta
                 if self._packed is None and self._ragged is not None:
                     self._ragged.meta = meta
-        return self._buffer, self._sizes, meta
+        return self._sizes, meta
 
     def _stored_sizes(self):
         """Constituent shapes as they lie in the buffer."""
@@ -226,7 +233,7 @@ class NestedTensor(object):
 
     @property
     def requires_grad(self):
-        return self._packed is not None and self._packed.requires_grad
+        return (self._flat if self._packed is None else self._packed).requires_grad
 
     @property
     def is_cuda(self):
@@ -319,6 +326,7 @@ class NestedTensor(object):
         if want_cl:
             buf, sizes, meta = self._record()
             return NestedTensor(ops.transpose_nchw_nhwc(buf, sizes, meta), sizes, meta, channels_last=True)
+        self._refuse_tracked()
         stored = self._stored_sizes()
         out = ops.transpose_nhwc_nchw(self._buffer, stored, build_meta(stored, self._buffer.device))
         return NestedTensor(out, self._sizes)
@@ -439,13 +447,13 @@ def _op_to_tensor_mask(nt, mask_dim=None):
 
 
 def _op_to_mask(nt, mask_dim=None):
-    _, sizes, meta = nt._record()
+    sizes, meta = nt._layout()
     return _ops.ops().to_mask(sizes, meta, mask_dim)
 
 
 def _op_from_padded_tensor(padded, target):
     """``from_padded_tensor(padded, sizes-of(target))`` (nestedtensor/csrc/masking.cpp:459-533)."""
-    _, sizes, meta = target._record()
+    sizes, meta = target._layout()
     if meta.device != padded.device:
         meta = build_meta(sizes, padded.device)
     return NestedTensor(_ops.ops().from_padded_tensor(padded, sizes, meta), sizes, meta)

@@ -56,6 +56,7 @@ def conv2d(input: NestedTensor, weight, bias=None, stride=1, padding=0, dilation
         # pointwise convolution: every pixel of every image is one row of a single packed GEMM.  A channels_last input is
         # stored pixel-major already and the result stays channels_last: no transpose on either side.
         cl = input._channels_last
+        input._refuse_tracked()
         pixels = input._buffer if cl else transpose_nchw_nhwc(input)._buffer
         cin = int(sizes[0, 0])
         y = ops.packed_linear(pixels.view(-1, cin), weight.reshape(cout, cin), None, 0, None)

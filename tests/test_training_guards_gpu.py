@@ -170,3 +170,42 @@ def test_a_buffer_cut_off_from_the_graph_stays_cut_off(cuda_device):
     y = training.layer_norm(nt.NestedTensor(buf, sizes), 64, w, b).values()
     y.sum().backward()
     assert x.grad is None and w.grad is not None
+
+
+def test_inference_functions_refuse_a_tracked_buffer(cuda_device):
+    """One answer for one object: what nn.training would track, the functions that track nothing refuse."""
+    x = torch.randn(6, 32, device="cuda", requires_grad=True)
+    nested = nt.NestedTensor(x.view(-1), torch.tensor([[2, 32], [4, 32]]))
+    assert nested.requires_grad and nested.values().requires_grad
+    for call in (lambda: nested.to_padded_tensor(0), lambda: nt.nn.layer_norm(nested, 32), lambda: nested.to_tensor_mask()):
+        with pytest.raises(RuntimeError, match="does not track gradients"):
+            call()
+    with torch.no_grad():
+        want = nt.nn.layer_norm(nested, 32)
+    assert torch.equal(training.layer_norm(nested, 32).values().view(-1), want._buffer)
+    assert torch.equal(nt.nn.layer_norm(nt.NestedTensor(x.detach().view(-1), nested._sizes), 32)._buffer, want._buffer)
+
+
+def test_operators_that_read_lengths_alone_take_tracked_tensors(cuda_device):
+    x = torch.randn(6, 32, device="cuda", requires_grad=True)
+    nested = nt.NestedTensor(x.view(-1), torch.tensor([[2, 32], [4, 32]]))
+    for t in (nested, nested.with_values(x * 1)):
+        mask = torch.ops.nestedtensor.to_mask(t, 2)
+        assert mask.tolist() == [[True, True, False, False], [True] * 4]
+        padded = torch.randn(2, 4, 32, device="cuda")
+        got = torch.ops.nestedtensor.from_padded_tensor(padded, t)
+        assert torch.equal(got._buffer.view(6, 32), torch.cat([padded[0, :2], padded[1]]))
+
+
+def test_channels_last_operators_refuse_a_tracked_buffer(cuda_device):
+    x = torch.randn(8 * 6, device="cuda", requires_grad=True)
+    images = nt.NestedTensor(x.view(-1), torch.tensor([[8, 2, 1], [8, 2, 2]]), channels_last=True)
+    weight = torch.randn(4, 8, 1, 1, device="cuda", requires_grad=True)
+    for call in (lambda: images.contiguous(), lambda: nt.nn.conv2d(images, weight), lambda: images.to_padded_tensor(0)):
+        with pytest.raises(RuntimeError, match="does not track gradients"):
+            call()
+    with torch.no_grad():
+        want = nt.nn.conv2d(images, weight)._buffer
+    got = nt.nn.conv2d(nt.NestedTensor(x.detach(), images._sizes, channels_last=True), weight)  # (the weight's gradient is not offered)
+    assert torch.equal(got._buffer, want) and not got.requires_grad
+    assert torch.ops.nestedtensor.to_mask(images, 2).shape[0] == 2

@@ -61,3 +61,16 @@ def test_the_tracked_rows_are_the_callers_own_tensor():
     with torch.no_grad():
         cut = x.view(-1)
     assert nt.NestedTensor(cut, sizes)._tracked()[0] is cut
+
+
+def test_a_tracked_buffer_is_known_as_one():
+    x = torch.randn(7, 5, requires_grad=True)
+    a = nt.NestedTensor(x.view(-1), torch.tensor([[3, 5], [4, 5]]))
+    assert a.requires_grad and a.values().requires_grad and a.with_values(x * 1).requires_grad
+    assert not a.with_values(x.detach()).requires_grad and not nt.NestedTensor(x.detach().view(-1), a._sizes).requires_grad
+    for t in (a, a.with_values(x * 1)):
+        with pytest.raises(RuntimeError, match="does not track gradients"):
+            t._record()
+        assert t._layout()[1].tolist() == [0, 15, 35, 3, 5, 4, 5]
+        with torch.no_grad():
+            assert t._record()[0].numel() == 35
