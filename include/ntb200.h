@@ -232,6 +232,8 @@ int ntb200_device_error_flags(void);
  *              1 = SIMT;  2 = mma.sync kernel;  3 = tcgen05 kernel for every sequence;
  *              4 = the warp-per-(sequence, head) kernel (1-4: for cross-checks, NTB200_UNSUPPORTED_SHAPE when
  *              the shape does not fit).  Sequences longer than max_len are not computed by paths 0, 2 and 4.
+ *              2-4 need scaling > 0, a normal number times log2(e); path 0 takes the SIMT kernel for any other (here
+ *              and for cross-attention)
  *   workspace  device scratch of ntb200_varlen_attention_workspace_bytes(...) bytes, 16-byte aligned
  *              (holds the device-built list of (sequence, query tile) work items); may be NULL
  * Replaces steps 2-8 of bt_min_mha (nestedtensor/csrc/cuda/mha.cpp:59-105) including
@@ -380,7 +382,8 @@ int ntb200_embedding_backward(const void* grad, const void* index, int index_byt
  *   lse[h*q_tokens + t] = log2( sum_j exp2(scaling * log2(e) * q_t,h . k_j,h) )      (left unwritten for rows without keys)
  * offsets_q / offsets_k count elements of matrices with row_elems_q / row_elems_k elements per token (1: token offsets).
  *   path  0 = best available;  1 = 32-bit tiles;  2 = mma.sync kernel;  3 = tcgen05 kernel: head_dim 64 or 128, rows on
- *         16-byte boundaries, out on a 32-byte one (1-3: for cross-checks)
+ *         16-byte boundaries, out on a 32-byte one (1-3: for cross-checks).  2 and 3 need scaling > 0, a normal number times
+ *         log2(e); path 0 takes the 32-bit tiles for any other finite scaling
  * workspace: 16-byte aligned.
  */
 size_t ntb200_varlen_attention_train_workspace_bytes(int64_t batch, int64_t q_tokens, int num_heads, int head_dim,

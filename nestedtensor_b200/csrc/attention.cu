@@ -16,6 +16,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cfloat>
+#include <cmath>
+
 #include "attention_internal.cuh"
 #include "attention_tiny.cuh"
 #include "common.cuh"
@@ -494,6 +497,14 @@ int launch_attn_simt(const QkvSrc& s, void* out, int64_t batch, int64_t q_tokens
   return status_from_cuda(cudaGetLastError());
 }
 
+// The tensor-core kernels mark what lies past a sequence's keys with -inf, and take a row's maximum, before they multiply by the
+// factor: right for positive factors that fp32 holds as normal numbers (their packed products flush others to zero, and
+// -inf * 0 is NaN).  The kernels on fp32 values multiply first and take any.
+bool keeps_order(float scaling) {
+  const float f = scaling * 1.4426950408889634f;
+  return f >= FLT_MIN && f <= FLT_MAX;
+}
+
 // the tcgen05 kernel stores its output 32 bytes at a time
 bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 
@@ -578,12 +589,15 @@ size_t ntb200_varlen_attention_workspace_bytes(int64_t batch, int64_t total_toke
 int ntb200_varlen_attention(const void* qkv, void* out, const int64_t* offsets, int64_t batch, int64_t total_tokens,
                             int num_heads, int head_dim, int64_t max_len, float scaling, int dtype, int path,
                             void* workspace, size_t workspace_bytes, void* stream) {
-  const int force_simt = path == 1;
   if (batch < 0 || total_tokens < 0 || num_heads < 1 || head_dim < 1 || max_len < 0) return NTB200_INVALID_ARG;
   if (dtype != NTB200_F32 && dtype != NTB200_F16 && dtype != NTB200_BF16) return NTB200_UNSUPPORTED_DTYPE;
   if (head_dim > kMaxHeadDim) return NTB200_UNSUPPORTED_SHAPE;
   if (batch == 0 || total_tokens == 0) return NTB200_OK;
   if (qkv == nullptr || out == nullptr || offsets == nullptr) return NTB200_INVALID_ARG;
+  if (path != 1 && !keeps_order(scaling)) {
+    if (path != 0) return NTB200_UNSUPPORTED_SHAPE;
+    path = 1;
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // path 0: best available (the warp-per-(sequence, head) kernel when no sequence is longer than 32 tokens, else tcgen05
   // when a workspace is given and the shape is supported, else mma.sync, else SIMT); 1: SIMT; 2: mma.sync flash kernel;
@@ -619,7 +633,7 @@ int ntb200_varlen_attention(const void* qkv, void* out, const int64_t* offsets, 
   const size_t es = dtype == NTB200_F32 ? 4 : 2;
   const char* base = static_cast<const char*>(qkv);
   const QkvSrc src = {base, base + E * es, base + 2 * E * es, 3 * E, 3 * E, 3 * E, offsets, offsets, E, E};
-  return launch_attn_generic(src, out, batch, total_tokens, num_heads, head_dim, max_len, scaling, dtype, force_simt ? 1 : path, st);
+  return launch_attn_generic(src, out, batch, total_tokens, num_heads, head_dim, max_len, scaling, dtype, path, st);
 }
 
 int ntb200_varlen_cross_attention(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* out,
@@ -634,6 +648,10 @@ int ntb200_varlen_cross_attention(const void* q, int64_t ldq, const void* k, int
   if (batch == 0 || q_tokens == 0) return NTB200_OK;
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || offsets_q == nullptr || offsets_k == nullptr)
     return NTB200_INVALID_ARG;
+  if (path != 1 && !keeps_order(scaling)) {
+    if (path == 2) return NTB200_UNSUPPORTED_SHAPE;
+    path = 1;
+  }
   const QkvSrc src = {q, k, v, ldq, ldk, ldv, offsets_q, offsets_k, E, E};
   return launch_attn_generic(src, out, batch, q_tokens, num_heads, head_dim, max_len_q, scaling, dtype, path,
                              static_cast<cudaStream_t>(stream));
@@ -658,6 +676,10 @@ int ntb200_varlen_cross_attention_ws(const void* q, int64_t ldq, const void* k, 
   if (batch == 0 || q_tokens == 0) return NTB200_OK;
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || offsets_q == nullptr || offsets_k == nullptr)
     return NTB200_INVALID_ARG;
+  if (path != 1 && !keeps_order(scaling)) {
+    if (path != 0) return NTB200_UNSUPPORTED_SHAPE;
+    path = 1;
+  }
   // path 0: tcgen05 when the shape allows it and a workspace is given, else the mma.sync kernel, else SIMT; 3: tcgen05 or error
   const bool tc_ok = dtype != NTB200_F32 && attn_tcgen05_supported(batch, q_tokens, num_heads, head_dim, dtype, false) && k_tokens > 0 &&
                      k_tokens < (1ll << 31) - 128 && aligned16(q) && aligned16(k) && aligned16(v) && aligned32(out) &&
@@ -680,7 +702,7 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
                                   int64_t batch, int64_t q_tokens, int64_t k_tokens, int num_heads, int head_dim, int64_t max_len_q,
                                   float scaling, int dtype, int path, void* workspace, size_t workspace_bytes, void* stream) {
   if (batch < 0 || q_tokens < 0 || k_tokens < 0 || num_heads < 1 || head_dim < 1 || max_len_q < 0 || row_elems_q < 1 || row_elems_k < 1 ||
-      path < 0 || path > 3)
+      path < 0 || path > 3 || !std::isfinite(scaling * 1.4426950408889634f))
     return NTB200_INVALID_ARG;
   if (dtype != NTB200_F32 && dtype != NTB200_F16 && dtype != NTB200_BF16) return NTB200_UNSUPPORTED_DTYPE;
   if (head_dim > kMaxHeadDim) return NTB200_UNSUPPORTED_SHAPE;
@@ -689,6 +711,10 @@ int ntb200_varlen_attention_train(const void* q, int64_t ldq, const void* k, int
   if (batch == 0 || q_tokens == 0) return NTB200_OK;
   if (q == nullptr || out == nullptr || lse == nullptr || offsets_q == nullptr || offsets_k == nullptr) return NTB200_INVALID_ARG;
   if (k_tokens > 0 && (k == nullptr || v == nullptr)) return NTB200_INVALID_ARG;
+  if (path != 1 && !keeps_order(scaling)) {
+    if (path != 0) return NTB200_UNSUPPORTED_SHAPE;
+    path = 1;
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const QkvSrc src = {q, k, v, ldq, ldk, ldv, offsets_q, offsets_k, row_elems_q, row_elems_k, {lse, q_tokens}};
   // one packed [T, 3E] matrix of a self-attention: q, k and v are its three column blocks over the same sequences

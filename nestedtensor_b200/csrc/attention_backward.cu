@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -1013,7 +1014,7 @@ int ntb200_varlen_attention_backward(const void* grad_out, const void* q, int64_
                                      int num_heads, int head_dim, int64_t max_len_q, int64_t max_len_k, float scaling, int dtype, int path,
                                      void* workspace, size_t workspace_bytes, void* stream) {
   if (batch < 0 || q_tokens < 0 || k_tokens < 0 || num_heads < 1 || head_dim < 1 || row_elems_q < 1 || row_elems_k < 1 || max_len_q < 0 ||
-      max_len_k < 0 || path < 0 || path > 4)
+      max_len_k < 0 || path < 0 || path > 4 || !std::isfinite(scaling * kLog2e))
     return NTB200_INVALID_ARG;
   if (dtype != NTB200_F32 && dtype != NTB200_F16 && dtype != NTB200_BF16) return NTB200_UNSUPPORTED_DTYPE;
   if (head_dim > kMaxHeadDim) return NTB200_UNSUPPORTED_SHAPE;

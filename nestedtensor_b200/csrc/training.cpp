@@ -384,7 +384,11 @@ int64_t check_heads(int64_t num_heads, int64_t E) {
   return E / num_heads;
 }
 
-double scaling_or_default(c10::optional<double> scaling, int64_t d) { return scaling ? *scaling : 1.0 / std::sqrt((double)d); }
+double scaling_or_default(c10::optional<double> scaling, int64_t d) {
+  if (!scaling) return 1.0 / std::sqrt((double)d);
+  TORCH_CHECK(std::isfinite((float)*scaling * 1.4426950408889634f), "nestedtensor_b200: scaling must be finite in 32 bits, got ", *scaling);
+  return *scaling;
+}
 
 // Self-attention of packed q|k|v rows: qkv is the buffer of (L_i, 3E) constituents in any contiguous shape; [T, E].
 Tensor self_attention_train(const Tensor& qkv, const Tensor& sizes, int64_t features, const Tensor& meta, int64_t row_elems, int64_t num_heads,

@@ -67,8 +67,8 @@ def embedding(input: NestedTensor, weight: torch.Tensor, padding_idx: Optional[i
 
 def self_attention(qkv: NestedTensor, num_heads: int, scaling: Optional[float] = None) -> NestedTensor:
     """softmax(scaling q k^T) v within every sequence, per head, for a NestedTensor of ``(L_i, 3 * E)`` rows q | k | v (the packed
-    projection of ``torch.nn.MultiheadAttention``); ``(L_i, E)``.  ``scaling`` defaults to ``head_dim ** -0.5``.  The gradient
-    of ``qkv`` has the same packed form."""
+    projection of ``torch.nn.MultiheadAttention``); ``(L_i, E)``.  ``scaling``, any finite number (the tensor-core kernels take
+    positive ones), defaults to ``head_dim ** -0.5``.  The gradient of ``qkv`` has the same packed form."""
     _check(qkv, "qkv")
     if qkv.dim() != 3 and len(qkv) > 0:
         raise RuntimeError("query needs to be 3 dim.")
@@ -82,7 +82,7 @@ def attention(query: NestedTensor, key: NestedTensor, value: NestedTensor, num_h
               scaling: Optional[float] = None) -> NestedTensor:
     """softmax(scaling q k^T) v of the queries of sequence b over the keys and values of sequence b, per head, for already projected
     NestedTensors ``(Lq_i, E)``, ``(Lk_i, E)``, ``(Lk_i, E)``; ``(Lq_i, E)``.  A sequence without keys gives zeros and passes no
-    gradient.  ``scaling`` defaults to ``head_dim ** -0.5``."""
+    gradient.  ``scaling`` as in ``self_attention``."""
     for t, name in ((query, "query"), (key, "key"), (value, "value")):
         _check(t, name)
         if t.dim() != 3 and len(t) > 0:

@@ -3,6 +3,8 @@ import pytest
 import torch
 
 import nestedtensor_b200 as nt
+from nestedtensor_b200 import _cabi
+from nestedtensor_b200.nn import training
 
 
 def _nested(shapes, **kw):
@@ -74,3 +76,27 @@ def test_a_tracked_buffer_is_known_as_one():
         assert t._layout()[1].tolist() == [0, 15, 35, 3, 5, 4, 5]
         with torch.no_grad():
             assert t._record()[0].numel() == 35
+
+
+@pytest.mark.parametrize("scaling", [float("nan"), float("inf"), -float("inf"), 1e39, 3e38])
+def test_attention_refuses_scalings_that_are_not_finite(native_libs, scaling):
+    """Times log2(e), as the kernels hold it in 32 bits."""
+    lib = _cabi.load()
+    for path in (0, 1, 2, 3):
+        assert lib.ntb200_varlen_attention_train(16, 64, 16, 64, 16, 64, 32, 16, 16, 64, 16, 64, 1, 4, 4, 1, 64, 4, scaling, 2, path, 16, 1 << 20,
+                                                 None) == -1
+        assert lib.ntb200_varlen_attention_backward(16, 16, 64, 16, 64, 16, 64, 16, 16, 16, 64, 16, 64, 16, 64, 16, 64, 16, 64, 1, 4, 4, 1, 64, 4, 4,
+                                                    scaling, 2, path, 16, 1 << 20, None) == -1
+
+
+def test_tensor_core_kernels_refuse_scalings_that_are_not_positive(native_libs):
+    lib = _cabi.load()
+    for scaling in (0.0, -0.125, 2.0 ** -130):
+        for path in (2, 3):
+            assert lib.ntb200_varlen_attention_train(16, 64, 16, 64, 16, 64, 32, 16, 16, 64, 16, 64, 1, 4, 4, 1, 64, 4, scaling, 2, path, 16, 1 << 20,
+                                                     None) == -7
+            assert lib.ntb200_varlen_cross_attention_ws(16, 64, 16, 64, 16, 64, 32, 16, 16, 1, 4, 4, 1, 64, 4, scaling, 2, path, 16, 1 << 20,
+                                                        None) == -7
+        for path in (2, 3, 4):
+            assert lib.ntb200_varlen_attention(16, 32, 16, 1, 4, 1, 64, 4, scaling, 2, path, 16, 1 << 20, None) == -7
+        assert lib.ntb200_varlen_cross_attention(16, 64, 16, 64, 16, 64, 32, 16, 16, 1, 4, 1, 64, 4, scaling, 2, 2, None) == -7
