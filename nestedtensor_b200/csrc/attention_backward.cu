@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -140,11 +141,61 @@ constexpr int kListBlocks = 5;
 // 64: 2 keys 0.0039 from O, 0.0024 from P; 4 keys 0.0029; 16 keys 0.0025; 64 keys 0.0024, the rounding of dS and of the result.)
 constexpr int kFewKeys = 16;
 
-// The first blocks build one list each; every warp of the others takes one query token: D of all its heads, and (fp16) the largest
-// |dO| of its sequence and head.  VEC: heads of 32, 64 or 128 elements on 16-byte boundaries: a head on d / 8 lanes.
+// Raises the largest squared 2-norm of a sequence and head.  A row that holds Inf or NaN does not count: no factor mends it, and the
+// others' gradients are held as if it were not there.
+__device__ __forceinline__ void raise_norm(unsigned* at, float m) {
+  if (m <= FLT_MAX) atomicMax(at, __float_as_uint(m));
+}
+
+// Rows of V a warp takes.  One pass over V, 13 us of the launch's 46 for 34 000 tokens of 12 heads; one row a warp, each with a search
+// of its own, takes 24.
+constexpr int kValueRows = 8;
+__host__ __device__ __forceinline__ int64_t prepare_blocks(int64_t tokens, int rows) {
+  return (tokens + rows * (kPrepThreads / 32) - 1) / (rows * (kPrepThreads / 32));
+}
+
+// |V_j|^2 of the rows from t0 on, one warp, into the largest of their sequence and head
+__device__ __forceinline__ void value_norms(const BwdArgs& a, uint2* __restrict__ top, int64_t k_tokens, int64_t t0) {
+  if (t0 >= k_tokens) return;
+  const int lane = threadIdx.x & 31, n = (int)(k_tokens - t0 < kValueRows ? k_tokens - t0 : kValueRows);
+  const int nv = a.H * a.d / 8, per = a.d / 8, log_per = 31 - __clz(per);
+  // lane i: the sequence of row i (-1: behind the last one)
+  const int64_t e = (t0 + lane % kValueRows) * a.row_elems_k;
+  const int64_t b = find_entry(a.offsets_k, 0, a.batch - 1, e);
+  const int seq = e < a.offsets_k[b + 1] ? (int)b : -1;
+  for (int v = lane; v < nv + lane; v += 32) {  // (the same trips for every lane: the sums are warp-wide)
+    uint4 x[kValueRows];
+#pragma unroll
+    for (int i = 0; i < kValueRows; ++i)
+      x[i] = i < n && v < nv ? reinterpret_cast<const uint4*>(static_cast<const __half*>(a.v) + (t0 + i) * a.ldv)[v] : make_uint4(0u, 0u, 0u, 0u);
+    const bool writes = v < nv && (lane & (per - 1)) == 0;
+    float most = 0.0f;
+    int of = __shfl_sync(0xffffffffu, seq, 0);
+#pragma unroll
+    for (int i = 0; i < kValueRows; ++i) {
+      float f[8], m = 0.0f;
+      Vec16<NTB200_F16>::unpack(x[i], f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = fmaf(f[k], f[k], m);
+      for (int w = per / 2; w > 0; w >>= 1) m += __shfl_xor_sync(0xffffffffu, m, w);
+      const int s = __shfl_sync(0xffffffffu, seq, i);
+      if (i < n && s != of) {
+        if (writes && of >= 0) raise_norm(&top[(int64_t)of * a.H + (v >> log_per)].y, most);
+        most = 0.0f;
+        of = s;
+      }
+      if (i < n && m <= FLT_MAX) most = fmaxf(most, m);
+    }
+    if (writes && of >= 0) raise_norm(&top[(int64_t)of * a.H + (v >> log_per)].y, most);
+  }
+}
+
+// The first blocks build one list each; every warp of the others takes one query token: D of all its heads, and (fp16) |dO|^2 for the
+// largest of its sequence and head; behind them (fp16) the rows of V likewise.  VEC: heads of 32, 64 or 128 elements on
+// 16-byte boundaries: a head on d / 8 lanes.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kPrepThreads, 4)
-backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ top) {
+backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, uint2* top, int64_t k_tokens) {
   switch (blockIdx.x) {  // (a class without sequences gives an empty list)
     case 0: build_backward_items(a.offsets_k, a.row_elems_k, a.offsets_q, a.row_elems_q, a.batch, plan.tile, plan.short_, l.kv); return;
     case 1: build_backward_items(a.offsets_q, a.row_elems_q, a.offsets_k, a.row_elems_k, a.batch, plan.tile, plan.short_, l.qi); return;
@@ -153,10 +204,17 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
     case 4: if (plan.mid.any()) build_sequence_items(a, plan.mid, l.mid); return;
     default: break;
   }
-  const int64_t t = ((int64_t)blockIdx.x - kListBlocks) * (kPrepThreads / 32) + (threadIdx.x >> 5);
-  if (t >= a.q_tokens) return;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t block = (int64_t)blockIdx.x - kListBlocks, q_blocks = prepare_blocks(a.q_tokens, 1);
   const int64_t E = (int64_t)a.H * a.d;
+  if constexpr (VEC && std::is_same<T, __half>::value) {
+    if (block >= q_blocks) {
+      value_norms(a, top, k_tokens, ((block - q_blocks) * (kPrepThreads / 32) + warp) * kValueRows);
+      return;
+    }
+  }
+  const int64_t t = block * (kPrepThreads / 32) + warp;
+  if (t >= a.q_tokens) return;
   const T* g = static_cast<const T*>(a.grad) + t * E;
   const T* o = static_cast<const T*>(a.out) + t * E;
   constexpr bool kRounded = !std::is_same<T, float>::value;  // O has fewer bits than D
@@ -201,8 +259,8 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
         Vec16<kDtype>::unpack(live ? reinterpret_cast<const uint4*>(q)[v] : make_uint4(0u, 0u, 0u, 0u), qe);
         const float lse = live ? a.lse[(int64_t)h * a.q_tokens + t] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(xe[e]));
-        for (int w = per / 2; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+        for (int e = 0; e < 8; ++e) m = fmaf(xe[e], xe[e], m);
+        for (int w = per / 2; w > 0; w >>= 1) m += __shfl_xor_sync(0xffffffffu, m, w);
         for (int j0 = 0; j0 < (int)keys; j0 += kAhead) {
           uint4 kv[kAhead], vv[kAhead];
 #pragma unroll
@@ -232,7 +290,7 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
         }
         if (live && (lane & (per - 1)) == 0) {
           a.delta[(int64_t)h * a.q_tokens + t] = s;
-          if (top != nullptr) atomicMax(top + b * a.H + h, __float_as_uint(m));
+          if (top != nullptr) raise_norm(&top[b * a.H + h].x, m);
         }
       }
       return;
@@ -248,17 +306,17 @@ backward_prepare_kernel(BwdArgs a, Plan plan, Lists l, unsigned* __restrict__ to
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           s = fmaf(xe[k], ye[k], s);
-          m = fmaxf(m, fabsf(xe[k]));
+          m = fmaf(xe[k], xe[k], m);
         }
         for (int w = per / 2; w > 0; w >>= 1) {
           s += __shfl_xor_sync(0xffffffffu, s, w);
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+          m += __shfl_xor_sync(0xffffffffu, m, w);
         }
         const int v = first + 32 * i;
         if (v < nv && (lane & (per - 1)) == 0) {
           const int h = v >> log_per;
           a.delta[(int64_t)h * a.q_tokens + t] = s;
-          if (top != nullptr) atomicMax(top + b * a.H + h, __float_as_uint(m));
+          if (top != nullptr) raise_norm(&top[b * a.H + h].x, m);
         }
       }
     }
@@ -823,7 +881,7 @@ __global__ void __launch_bounds__(kMmaThreads) attn_bwd_mma_kernel(BwdArgs a, Li
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t item_capacity(int64_t batch, int64_t tokens, int tile) { return batch + tokens / tile + 1; }
 
-// delta | largest |dO| | five lists (count, items, their sequences) | dQ in fp32 (the kernel with whole sequences as items); every part
+// delta | largest |dO|^2 and |V|^2 | five lists (count, items, their sequences) | dQ in fp32 (the kernel with whole sequences as items); every part
 // on a 16-byte boundary
 struct BwdWorkspace {
   size_t delta, top, lists[kListBlocks], seqs[kListBlocks], scratch, bytes;
@@ -833,7 +891,7 @@ struct BwdWorkspace {
                                     item_capacity(batch, q_tokens, 128), batch};  // (tiles of 32 rows or more)
     delta = 0;
     top = up((size_t)q_tokens * H * 4);
-    size_t at = top + up((size_t)batch * H * 4);
+    size_t at = top + up((size_t)batch * H * sizeof(uint2));
     for (int i = 0; i < kListBlocks; ++i) {
       lists[i] = at;
       seqs[i] = at + 16 + sizeof(int4) * (size_t)n[i];
@@ -851,11 +909,11 @@ struct BwdWorkspace {
 };
 
 template <typename T, bool VEC>
-int launch_prepare(const BwdArgs& a, const Plan& plan, const Lists& l, unsigned* top, cudaStream_t st) {
-  const int64_t blocks = kListBlocks + ceil_div(a.q_tokens, kPrepThreads / 32);
+int launch_prepare(const BwdArgs& a, const Plan& plan, const Lists& l, uint2* top, int64_t k_tokens, cudaStream_t st) {
+  const int64_t blocks = kListBlocks + prepare_blocks(a.q_tokens, 1) + (top != nullptr ? prepare_blocks(k_tokens, kValueRows) : 0);
   if (blocks > 0x7fffffffll) return NTB200_UNSUPPORTED_SHAPE;
-  if (top != nullptr && cudaMemsetAsync(top, 0, (size_t)a.batch * a.H * 4, st) != cudaSuccess) return NTB200_LAUNCH_FAILED;
-  backward_prepare_kernel<T, VEC><<<(unsigned)blocks, kPrepThreads, 0, st>>>(a, plan, l, top);
+  if (top != nullptr && cudaMemsetAsync(top, 0, (size_t)a.batch * a.H * sizeof(uint2), st) != cudaSuccess) return NTB200_LAUNCH_FAILED;
+  backward_prepare_kernel<T, VEC><<<(unsigned)blocks, kPrepThreads, 0, st>>>(a, plan, l, top, k_tokens);
   return status_from_cuda(cudaGetLastError());
 }
 
@@ -867,7 +925,7 @@ int launch_bwd_simt(const BwdArgs& a, int64_t k_tokens, const Lists& l, cudaStre
         return cudaFuncSetAttribute(attn_bwd_simt_kernel<T, BT, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) == cudaSuccess;
       }))
     return NTB200_LAUNCH_FAILED;
-  const int rc = launch_prepare<T, false>(a, Plan{{0, INT64_MAX}, {0, 0}, {0, 0}, BT}, l, nullptr, st);
+  const int rc = launch_prepare<T, false>(a, Plan{{0, INT64_MAX}, {0, 0}, {0, 0}, BT}, l, nullptr, k_tokens, st);
   if (rc != NTB200_OK) return rc;
   const int per_sm = 227 * 1024 / (kSmem + 1024);
   const int64_t most = (item_capacity(a.batch, k_tokens, BT) + item_capacity(a.batch, a.q_tokens, BT)) * a.H;
@@ -949,8 +1007,8 @@ int launch_bwd(const BwdArgs& args, int64_t k_tokens, int64_t max_len, uint8_t* 
     if ((path == 2 && !mma) || (path >= 3 && !tc) || (path == 4 && a.d != 64)) return NTB200_UNSUPPORTED_SHAPE;
     if (mma && path != 1) {
       const Plan plan = make_plan(a.d, tc, path);
-      a.top = dtype == NTB200_F16 ? reinterpret_cast<unsigned*>(ws + at.top) : nullptr;
-      int rc = launch_prepare<T, true>(a, plan, l, const_cast<unsigned*>(a.top), st);
+      a.top = dtype == NTB200_F16 ? reinterpret_cast<uint2*>(ws + at.top) : nullptr;
+      int rc = launch_prepare<T, true>(a, plan, l, const_cast<uint2*>(a.top), k_tokens, st);
       if (rc == NTB200_OK && plan.long_.any() && max_len > plan.long_.over)
         rc = attn_bwd_tcgen05_launch(a, k_tokens, dtype, l.long_kv, l.long_qi, item_capacity(a.batch, k_tokens, 128),
                                      item_capacity(a.batch, a.q_tokens, 128), st);

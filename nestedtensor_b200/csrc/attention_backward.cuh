@@ -37,7 +37,7 @@ struct BwdArgs {
   const void *grad, *q, *k, *v, *out;
   const float* lse;  // [H, q_tokens]
   float* delta;      // [H, q_tokens]: D
-  const unsigned* top;  // [batch, H]: bits of the largest |dO| of the sequence and head (fp16 kernels only, else NULL)
+  const uint2* top;  // [batch, H]: bits of the largest |dO_i|^2 and |V_j|^2 of the sequence and head (fp16 kernels only, else NULL)
   void *dq, *dk, *dv;
   int64_t ldq, ldk, ldv, lddq, lddk, lddv;  // grad and out are contiguous: their stride is H * d
   const int64_t *offsets_q, *offsets_k;
@@ -67,13 +67,14 @@ namespace {
 
 __device__ __forceinline__ Item decode(const int4& w) { return {w.x, w.y, w.z, w.w}; }
 
-// fp16 holds dS only between 2^-24 and 65504, while gradients come at any scale: dS is computed from dO times a power of two
-// that brings the largest |dO| of the sequence and head to [1, 2), and the product's sum is divided by it again (both exact).
-__device__ __forceinline__ float scale_of(unsigned top) {
-  const int e = (int)(top >> 23);       // biased exponent of a non-negative number
-  if (e == 0 || e == 255) return 1.0f;  // zeros; Inf or NaN, which no factor mends
-  const int f = 254 - e;                // 2^(127 - e)
-  return __uint_as_float((unsigned)(f < 27 ? 27 : (f > 227 ? 227 : f)) << 23);
+// fp16 holds dS only between 2^-24 and 65504, while gradients and values come at any scale: dS is computed from dO times a power of
+// two, and the product's sum is divided by it again (both exact).  With R = max |dO_i| max |V_j| over the sequence and head (2-norms),
+// |dS_ij| = P_ij (1 - P_ij) |dP_ij - (mean of the other dP, weighted by P)| <= 1/4 2R.  So the factor brings R to (2^15, 2^16]: dS
+// stays under 2^15, and as little as possible of it falls under fp16's normal numbers.
+__device__ __forceinline__ float scale_of(const uint2& top) {
+  const int e = (int)(__float_as_uint(__uint_as_float(top.x) * __uint_as_float(top.y)) >> 23);  // R^2 in [2^(e - 127), 2^(e - 126))
+  if (e == 0) return 1.0f;                                                                      // nothing but zeros (or Inf and NaN)
+  return __uint_as_float((unsigned)(127 + 16 - ((e - 126 + 1) >> 1)) << 23);                    // (e in 31 .. 207)
 }
 __device__ __forceinline__ float grad_scale(const BwdArgs& a, const int* __restrict__ seq, int64_t i, int h) {
   return a.top == nullptr ? 1.0f : scale_of(a.top[(int64_t)seq[i] * a.H + h]);

@@ -51,7 +51,7 @@ struct Cfg {
   static constexpr int kOwn = D == 64 ? 2 : 1;    // own tile pairs in shared memory
   static constexpr int kStages = D == 64 ? 4 : 2; // other tile pairs
   static constexpr int kAcc1 = 256, kAcc2 = 256 + D;
-  static constexpr int kStats = 2 * kTR * 4;      // -lse and -D of a stage
+  static constexpr int kStats = 2 * kTR * 4 + 16; // -lse and -D of a stage; (fp16) dO's factor
   static constexpr int kStaging = (kOwn + kStages) * 2 * kTile + kStages * kStats + 512;  // 2 KB a softmax warp for the outputs
   static constexpr int kSmem = 1024 + kStaging + 8 * 2048;
   // tensor-memory columns of the packed P and dS of a chunk of 32 columns
@@ -381,11 +381,14 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       uint32_t g = 0;
       // cursor over the tiles, one ahead: its statistics are on the way while the current tile is waited for
       unsigned w = blockIdx.x;
-      auto fetch_seq = [&](unsigned w) { return me == 1 && a.top != nullptr && w < n_kv ? __ldg(t.kv.seq + w / H) : 0; };
+      auto fetch_seq = [&](unsigned w) {
+        if (FMT != 0 || me != 1 || w >= n_all) return 0;
+        return __ldg(w < n_kv ? t.kv.seq + w / H : t.qi.seq + (w - n_kv) / H);
+      };
       int4 rec = fetch(w), rec_next = fetch(w + gridDim.x);
       int seq = fetch_seq(w), seq_next = fetch_seq(w + gridDim.x);
       int j = 0, nt = 0;
-      unsigned top = 0;
+      uint2 top = make_uint2(0u, 0u);
       float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       Item it = decode(rec);
       auto step = [&]() {
@@ -400,7 +403,7 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           if (nt > 0) break;
         }
         j = 0;
-        if (me == 1 && a.top != nullptr && w < n_kv) top = a.top[(int64_t)seq * H + head(w)];
+        if (FMT == 0 && me == 1 && w < n_all) top = a.top[(int64_t)seq * H + head(w)];
       };
       auto load = [&]() {
         if (w >= n_kv) return;
@@ -414,7 +417,7 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       while (w < n_all) {
         const uint32_t s = g % C::kStages;
         const bool kv = w < n_kv;
-        const unsigned top_c = top;
+        const uint2 top_c = top;
         const float vc[4] = {v[0], v[1], v[2], v[3]};
         int nc = it.n_other - j * kTR;
         nc = nc > kTR ? kTR : nc;
@@ -427,11 +430,12 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           ok = false;
           break;
         }
+        float* dst = s_stats + s * (C::kStats / 4);
+        const float gs = FMT == 0 && me == 1 ? scale_of(top_c) : 1.0f;
+        if (FMT == 0 && me == 1 && lane == 0) dst[2 * kTR] = gs;
         if (kv) {
-          float* dst = s_stats + s * (C::kStats / 4) + me * kTR;
-          const float fc = me == 1 && a.top != nullptr ? -scale_of(top_c) : -1.0f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) dst[lane + 32 * k] = vc[k] * fc;
+          for (int k = 0; k < 4; ++k) dst[me * kTR + lane + 32 * k] = vc[k] * -gs;
         }
         const int r_end = (nc + 15) & ~15;
         for (int i = lane; i < (r_end - nc) * 8 * C::kHalves; i += 32) {
@@ -551,41 +555,30 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     // what an item needs from memory is fetched one item ahead (its record two)
     struct Ahead {
       int4 rec;
-      unsigned top;    // bits of the largest |dO| (fp16)
       float lse, delta;  // of this row (Q items)
     };
-    auto fetch_seq = [&](unsigned w) {
-      if (a.top == nullptr || w >= n_all) return 0;
-      return __ldg(w < n_kv ? t.kv.seq + w / H : t.qi.seq + (w - n_kv) / H);
-    };
-    auto look = [&](unsigned w, const int4& r, int seq) {
-      Ahead x = {r, 0u, 0.0f, 0.0f};
-      if (w >= n_all) return x;
-      if (a.top != nullptr) x.top = a.top[(int64_t)seq * H + head(w)];
-      if (w >= n_kv && row < r.y && r.w > 0) {
+    auto look = [&](unsigned w, const int4& r) {
+      Ahead x = {r, 0.0f, 0.0f};
+      if (w >= n_kv && w < n_all && row < r.y && r.w > 0) {
         const int64_t i = (int64_t)head(w) * a.q_tokens + r.x + row;
         x.lse = a.lse[i];
         x.delta = a.delta[i];
       }
       return x;
     };
-    int4 rec = fetch(blockIdx.x), rec2 = fetch(blockIdx.x + gridDim.x);
-    int seq2 = fetch_seq(blockIdx.x + gridDim.x);
-    Ahead next = look(blockIdx.x, rec, fetch_seq(blockIdx.x));
+    int4 rec2 = fetch(blockIdx.x + gridDim.x);
+    Ahead next = look(blockIdx.x, fetch(blockIdx.x));
     for (unsigned w = blockIdx.x; w < n_all; w += gridDim.x) {
       const Ahead cur = next;
-      next = look(w + gridDim.x, rec2, seq2);
+      next = look(w + gridDim.x, rec2);
       rec2 = fetch(w + 2 * gridDim.x);
-      seq2 = fetch_seq(w + 2 * gridDim.x);
       const Item it = decode(cur.rec);
       const bool kv = w < n_kv;
       const int h = head(w);
       const int nt = tiles_of(it);
       const bool live = q * 32 < it.rows;  // warp-uniform: this warp owns valid rows
-      const float gs = a.top != nullptr ? scale_of(cur.top) : 1.0f;
-      const uint64_t gs2 = ptx::f32x2_pack(gs, gs);
+      float gs = 1.0f;                     // (fp16) dO's factor, beside the statistics of every tile
       const uint64_t nl2 = ptx::f32x2_pack(-cur.lse, -cur.lse);  // (Q items)
-      const uint64_t nd2 = ptx::f32x2_pack(-cur.delta * gs, -cur.delta * gs);
       for (int j = 0; j < nt; ++j, ++g) {
         const uint32_t s = g % C::kStages;
         int nc = it.n_other - j * kTR;
@@ -628,8 +621,10 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
           for (int k = 0; k < 2; ++k)
             if ((wg + 2 * k) * 32 < nc) ptx::tmem_ld_32x32b_x32(tl + 128 + (wg + 2 * k) * 32, sv[k]);
           ptx::tmem_ld_wait();
+          if (FMT == 0) gs = stats[2 * kTR];
+          const uint64_t gs2 = ptx::f32x2_pack(gs, gs);
           if (kv) products(std::true_type{}, sv, p, stats + kTR, 0, gs2, nc);
-          else products(std::false_type{}, sv, p, nullptr, nd2, gs2, nc);
+          else products(std::false_type{}, sv, p, nullptr, ptx::f32x2_pack(-cur.delta * gs, -cur.delta * gs), gs2, nc);
           ptx::tmem_st_wait();
         }
         arrive(&ctrl->ds_ready);
@@ -681,7 +676,7 @@ static_assert(2 * kFusedRegSoftmax + kFusedRegAdd + kFusedRegControl == 4 * kFus
 struct Fused {
   static constexpr int D = 64, kTile = kHalf, kOwn = 2, kStages = 3;
   static constexpr int kAccV = 256, kAccK = 320, kAccQ = 384, kP = 448;  // tensor-memory columns; S 0, dP 128
-  static constexpr int kStats = 2 * kTR * 4;
+  static constexpr int kStats = 2 * kTR * 4 + 16;
   static constexpr int kDs = 2 * kHalf;  // dS: 128 keys x 128 queries
   static constexpr int kStaging = (kOwn + kStages) * 2 * kTile + kDs + kStages * kStats + 512;  // 2 KB a warp for the outputs
   static constexpr int kSmem = 1024 + kStaging + 12 * 2048;
@@ -940,12 +935,12 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       };
       bool ok = true;
       uint32_t g = 0, n = 0;
-      auto fetch_seq = [&](unsigned w) { return me == 1 && a.top != nullptr && w < n_all ? __ldg(t.seqs.seq + w / H) : 0; };
+      auto fetch_seq = [&](unsigned w) { return FMT == 0 && me == 1 && w < n_all ? __ldg(t.seqs.seq + w / H) : 0; };
       unsigned w = blockIdx.x;
       int4 rec = fetch(w), rec_next = fetch(w + gridDim.x);
       int seq = fetch_seq(w), seq_next = fetch_seq(w + gridDim.x);
       int j = 0, kt = 0, nk = 0, nq = 0;
-      unsigned top = 0;
+      uint2 top = make_uint2(0u, 0u);
       float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       auto step = [&]() {
         w += gridDim.x;
@@ -957,7 +952,7 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           nk = tiles(rec.y), nq = tiles(rec.w);
           if (nk > 0 && nq > 0) break;
         }
-        if (me == 1 && a.top != nullptr && w < n_all) top = a.top[(int64_t)seq * H + head(w)];
+        if (FMT == 0 && me == 1 && w < n_all) top = a.top[(int64_t)seq * H + head(w)];
       };
       auto load = [&]() {
         const float* src = (me == 0 ? a.lse : a.delta) + (int64_t)head(w) * a.q_tokens + rec.z + j * kTR;
@@ -969,7 +964,7 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (w < n_all) load();
       while (w < n_all) {
         const uint32_t s = g % C::kStages, o = n % C::kOwn;
-        const unsigned top_c = top;
+        const uint2 top_c = top;
         const float vc[4] = {v[0], v[1], v[2], v[3]};
         const bool first = j == 0;
         const uint32_t own_parity = (n / C::kOwn) & 1;
@@ -998,10 +993,11 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           ok = false;
           break;
         }
-        float* dst = s_stats + s * (C::kStats / 4) + me * kTR;
-        const float fc = me == 1 && a.top != nullptr ? -scale_of(top_c) : -1.0f;
+        float* dst = s_stats + s * (C::kStats / 4);
+        const float gs = FMT == 0 && me == 1 ? scale_of(top_c) : 1.0f;
+        if (FMT == 0 && me == 1 && lane == 0) dst[2 * kTR] = gs;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) dst[lane + 32 * k] = vc[k] * fc;
+        for (int k = 0; k < 4; ++k) dst[me * kTR + lane + 32 * k] = vc[k] * -gs;
         clear(s_oth + (s * 2 + me) * C::kTile, nc);
         if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&ctrl->aux[s]));
         // the statistics count into s_ready of their tile, whose phase begins when the tile before it is ready
@@ -1147,19 +1143,12 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       arrive(&ctrl->acc_free);
       pend.any = false;
     };
-    auto fetch_seq = [&](unsigned w) { return a.top != nullptr && w < n_all ? __ldg(t.seqs.seq + w / H) : 0; };
-    int4 rec = fetch(blockIdx.x), rec_next = fetch(blockIdx.x + gridDim.x);
-    int seq_next = fetch_seq(blockIdx.x + gridDim.x);
-    unsigned top = a.top != nullptr ? a.top[(int64_t)fetch_seq(blockIdx.x) * H + head(blockIdx.x)] : 0u;
+    int4 rec = fetch(blockIdx.x);
     for (unsigned w = blockIdx.x; w < n_all; w += gridDim.x) {
       const int4 it = rec;
-      const float gs = a.top != nullptr ? scale_of(top) : 1.0f;
-      rec = rec_next;
-      if (a.top != nullptr && w + gridDim.x < n_all) top = a.top[(int64_t)seq_next * H + head(w + gridDim.x)];
-      rec_next = fetch(w + 2 * gridDim.x);
-      seq_next = fetch_seq(w + 2 * gridDim.x);
+      float gs = 1.0f;  // (fp16) dO's factor, beside the statistics of every tile
+      rec = fetch(w + gridDim.x);
       const int nk = tiles(it.y), nq = tiles(it.w), h = head(w);
-      const uint64_t gs2 = ptx::f32x2_pack(gs, gs);
       for (int kt = 0; kt < nk; ++kt) {
         const int rows = it.y - kt * kTR < kTR ? it.y - kt * kTR : kTR;
         const bool live = q * 32 < rows, whole = q * 32 + 32 <= rows;  // warp-uniform
@@ -1202,6 +1191,8 @@ attn_bwd_fused_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           if (ok && !wait_warp(&ctrl->dp_ready, g & 1)) ok = false;
           if (ok && live) {
             ptx::tc_fence_after_sync();
+            if (FMT == 0) gs = stats[2 * kTR];
+            const uint64_t gs2 = ptx::f32x2_pack(gs, gs);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const int chunk = wg + 2 * k, c0 = chunk * 32;

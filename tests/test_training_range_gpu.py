@@ -84,3 +84,82 @@ def test_inference_attention_scaling_of_any_sign(cuda_device, dtype, d, scaling)
         want, bound = ref.attention(q, k, v, g, lengths, lengths, heads, scaling)
         for name, got in (("self", out), ("cross", crossed)):
             ref.assert_within(got, want["out"], bound["out"], name)
+
+
+def _half_steps(q, k, v, g, lq, lk, heads, scaling):
+    """What the last place of a subnormal fp16 dS may add to dQ and dK: dS is held relative to a power of two that brings R = max|dO_i|
+    max|V_j| (2-norms, of the sequence and head) to (2^15, 2^16], so half a step of 2^-24 is at most R 2^-40."""
+    d = q.size(1) // heads
+    extra = {"dq": torch.zeros(q.shape, dtype=torch.float64, device=q.device), "dk": torch.zeros(k.shape, dtype=torch.float64, device=q.device)}
+    a = c = 0
+    for n, m in zip(lq, lk):
+        rows, cols = slice(a, a + n), slice(c, c + m)
+        a, c = a + n, c + m
+        if n == 0 or m == 0:
+            continue
+        Q, G = (t[rows].double().view(n, heads, d) for t in (q, g))
+        K, V = (t[cols].double().view(m, heads, d) for t in (k, v))
+        R = G.norm(dim=2).amax(0) * V.norm(dim=2).amax(0)
+        e = (abs(scaling) * R * 2.0 ** -40)[None, :, None]
+        extra["dq"][rows] = (e * K.abs().sum(0)).expand(n, heads, d).reshape(n, -1)
+        extra["dk"][cols] = (e * Q.abs().sum(0)).expand(m, heads, d).reshape(m, -1)
+    return extra
+
+
+# each kernel's range of lengths: mma.sync, whole sequences, tiles
+@pytest.mark.parametrize("lengths", [[40, 3, 64], [130, 20, 500], [700, 33]], ids=str)
+@pytest.mark.parametrize("d", [32, 64, 72, 128])
+def test_attention_fp16_large_values(cuda_device, d, lengths):
+    """|V| near fp16's largest against small dO that lie along single rows of it: dO . V is in the millions relative to the largest
+    |dO|, dQ and dK are ordinary."""
+    H, gen = 2, torch.Generator().manual_seed(d)
+    q, k, v, g = _inputs(lengths, lengths, H, d, torch.float16, d)
+    v = (torch.sign(v.float()) * 30000).half()
+    pick = torch.cat([torch.randint(0, n, (n,), generator=gen) + sum(lengths[:i]) for i, n in enumerate(lengths)]).cuda()
+    g = (torch.sign(v[pick].float()) * 1e-3).half()
+    scaling = d ** -0.5
+    want, bound = ref.attention(q, k, v, g, lengths, lengths, H, scaling)
+    for name, e in _half_steps(q, k, v, g, lengths, lengths, H, scaling).items():
+        bound[name] = bound[name] + e
+        assert float(want[name].abs().max()) < 30000
+    _check(_self(q, k, v, g, lengths, H), want, bound, "large values")
+
+
+@pytest.mark.parametrize("lengths", [[40, 3, 64], [130, 20, 500], [700, 33]], ids=str)
+@pytest.mark.parametrize("d", [32, 64, 72, 128])
+def test_attention_fp16_rows_of_different_magnitude(cuda_device, d, lengths):
+    """Rows of dO from 2^8 down to 2^-8 of the ordinary in one sequence: dQ of a row is linear in the row's dO, and is held as well as
+    that of a row among its like."""
+    H = 2
+    q, k, v, g = _inputs(lengths, lengths, H, d, torch.float16, d + 7)
+    g = torch.where(g < 0, g - 1, g + 1)  # (at least 1: the powers of two below stay exact)
+    scaling = d ** -0.5
+    want, bound = ref.attention(q, k, v, g, lengths, lengths, H, scaling)
+    s = torch.pow(2.0, torch.arange(g.size(0), device="cuda") * 5 % 17 - 8).double()[:, None]
+    scaled = (g.double() * s).half()
+    assert torch.equal(scaled.double(), g.double() * s)
+    got = _self(q, k, v, scaled, lengths, H)
+    extra = _half_steps(q, k, v, scaled, lengths, lengths, H, scaling)["dq"]
+    ref.assert_within(got["dq"], want["dq"] * s, bound["dq"] * s + extra + ref.tiny(torch.float16), "dq")
+    want, bound = ref.attention(q, k, v, scaled, lengths, lengths, H, scaling)
+    _check({n: got[n] for n in ("dk", "dv")}, {n: want[n] for n in ("dk", "dv")}, bound, "all rows")
+
+
+@pytest.mark.parametrize("lengths", [[40, 3, 64], [130, 20, 500], [700, 33]], ids=str)
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_attention_fp16_one_row_of_no_number(cuda_device, d, lengths):
+    """A row of dO that holds Inf or NaN is lost, and with it its sequence's dK and dV; the small gradients of the other rows are not."""
+    H = 2
+    q, k, v, g = _inputs(lengths, lengths, H, d, torch.float16, d + 9)
+    g = torch.where(g < 0, g - 1, g + 1) * 2.0 ** -12
+    scaling = d ** -0.5
+    want, bound = ref.attention(q, k, v, g * 2.0 ** 12, lengths, lengths, H, scaling)
+    for bad in (float("inf"), float("nan")):
+        g2 = g.clone()
+        g2[::37] = bad
+        rows = torch.ones(g.size(0), dtype=torch.bool, device="cuda")
+        rows[::37] = False
+        got = _self(q, k, v, g2, lengths, H)
+        extra = _half_steps(q, k, v, g, lengths, lengths, H, scaling)["dq"]
+        s = 2.0 ** -12
+        ref.assert_within(got["dq"][rows], (want["dq"] * s)[rows], (bound["dq"] * s + extra + ref.tiny(torch.float16))[rows], "dq")
