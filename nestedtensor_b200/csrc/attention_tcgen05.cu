@@ -38,8 +38,11 @@ constexpr int kKV = 128;   // keys per block
 constexpr int kHalf = kQT * 64 * 2;  // 16 KB: one 128 x 64 two-byte tile, as TMA writes it
 // Of the 16 key pairs of a 32-key chunk, pair 2k+1 is exponentiated by the polynomial when bit k is set
 // (0xff: half of all exponentials, 0xaa: a quarter, 0: none), the others on the MUFU unit.  A quarter measured
-// best on B200 at the BERT-large batch (none: +1 %, half: +6 %).
-constexpr unsigned kPolyPairs = 0xaa;
+// best on B200 at the BERT-large batch (none: +1 %, half: +6 %).  The polynomial is off by up to 1.9e-4, where rounding P costs
+// 3.9e-3 in bf16 and 4.9e-4 in fp16; a training pass in fp16 does without it: the gradients compute P again from the row's
+// denominator with exponentials that are right to 2^-22, and the two should agree.
+template <int FMT, bool STATS>
+constexpr unsigned kPolyPairs = STATS && FMT == 0 ? 0u : 0xaau;
 // A row's reference maximum is raised (and its running output rescaled) only when a block's maximum exceeds it
 // by more than this many powers of two.
 constexpr float kLazyRescale = 8.0f;
@@ -596,7 +599,7 @@ attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 ptx::f32x2_unpack(xb, b0, b1);
                 const float p0 = ptx::ex2_approx(a0), p1 = ptx::ex2_approx(a1);
                 float p2, p3;
-                if ((kPolyPairs >> k) & 1) {
+                if ((kPolyPairs<FMT, STATS> >> k) & 1) {
                   if (STATS) {  // (the polynomial's exponent arithmetic loses a NaN: 0 x brings it back)
                     const uint64_t x = ptx::f32x2_pack(ptx::fmax_nan(b0, -126.0f), ptx::fmax_nan(b1, -126.0f));
                     ptx::ex2_poly_x2(x, p2, p3);

@@ -163,3 +163,35 @@ def test_attention_fp16_one_row_of_no_number(cuda_device, d, lengths):
         extra = _half_steps(q, k, v, g, lengths, lengths, H, scaling)["dq"]
         s = 2.0 ** -12
         ref.assert_within(got["dq"][rows], (want["dq"] * s)[rows], (bound["dq"] * s + extra + ref.tiny(torch.float16))[rows], "dq")
+
+
+@pytest.mark.parametrize("d", [32, 64, 80, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=str)
+def test_attention_row_statistics_hold_32_bits(cuda_device, dtype, d):
+    """The base-2 logarithm of a row's softmax denominator where the scores are exact: one key at 0, the others all at -c / 128, for
+    every c up to d.  Exponentials are off by 2^-22, their sum by 2^-24 a term."""
+    lib, code = _cabi.load(), {torch.float32: 0, torch.float16: 1}[dtype]
+    lengths = [33, 100, 130]
+    T, B = sum(lengths), len(lengths)
+    q = torch.eye(d, dtype=dtype, device="cuda")[torch.arange(T, device="cuda") % d].contiguous()
+    k = (torch.arange(d, device="cuda") / -128).to(dtype).expand(T, d).contiguous()
+    for i in range(B):
+        k[sum(lengths[:i])] = 0
+    v = torch.ones(T, d, dtype=dtype, device="cuda")
+    out, lse = torch.empty_like(q), torch.empty(1, T, device="cuda")
+    off = torch.tensor([0] + lengths).cumsum(0).cuda()
+    n = lib.ntb200_varlen_attention_train_workspace_bytes(B, T, 1, d, code)
+    ws = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
+    _cabi.check("train", lib.ntb200_varlen_attention_train(
+        q.data_ptr(), d, k.data_ptr(), d, v.data_ptr(), d, out.data_ptr(), lse.data_ptr(), off.data_ptr(), 1, off.data_ptr(), 1, B, T, T, 1, d,
+        max(lengths), 1.0, code, 0, ws.data_ptr(), n, stream_ptr()))
+    a = 0
+    for m in lengths:
+        S = q[a:a + m].double() @ k[a:a + m].double().t()
+        want = torch.logsumexp(S, 1) / 0.6931471805599453
+        # exponents of at most 1.45 after two roundings, exponentials, m additions: as parts of the denominator, times log2(e); the
+        # logarithm and the sum with the row's maximum
+        bound = (3 * 1.45 + 4 + m) * ref.W * 1.45 + 4 * ref.W * want.abs()
+        off_by = (lse[0, a:a + m].double() - want).abs()
+        assert bool((off_by <= bound).all()), (m, float((off_by / bound).max()), int((off_by / bound).argmax()))
+        a += m
