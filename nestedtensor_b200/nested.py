@@ -102,7 +102,7 @@ class NestedTensor(object):
     @classmethod
     def _over(cls, packed, ragged):
         """A nested tensor over the [rows, ...] matrix `packed` (contiguous; it carries the autograd graph) with the lengths of
-        `ragged`; its flat buffer and its sizes are made when something asks for them."""
+        `ragged`; its sizes are made when something asks for them, its flat buffer (a view) every time."""
         out = cls.__new__(cls)
         out._flat = out._extents = out._offsets = out._nchw = None
         out._channels_last = False
@@ -112,9 +112,8 @@ class NestedTensor(object):
 
     @property
     def _buffer(self):
-        if self._flat is None:
-            self._flat = self._packed.view(-1)
-        return self._flat
+        # (not kept: a view made under no_grad would stay without the matrix's graph)
+        return self._packed.view(-1) if self._flat is None else self._flat
 
     @property
     def _sizes(self):

@@ -100,3 +100,23 @@ def test_tensor_core_kernels_refuse_scalings_that_are_not_positive(native_libs):
         for path in (2, 3, 4):
             assert lib.ntb200_varlen_attention(16, 32, 16, 1, 4, 1, 64, 4, scaling, 2, path, 16, 1 << 20, None) == -7
         assert lib.ntb200_varlen_cross_attention(16, 64, 16, 64, 16, 64, 32, 16, 16, 1, 4, 1, 64, 4, scaling, 2, 2, None) == -7
+
+
+def test_a_pass_without_gradients_leaves_the_graph_alone():
+    """What an operator under no_grad looked at is not kept: gradients flow through the constituents afterwards."""
+    x = torch.randn(7, 5, requires_grad=True)
+    a = _nested([(3, 5), (4, 5)])
+    for rows in (x, x * 1):
+        b = a.with_values(rows)
+        with torch.no_grad():
+            b._record()
+            assert b.numel() == 35
+        x.grad = None
+        b.unbind()[1].sum().backward()
+        assert torch.equal(x.grad, torch.cat([torch.zeros(3, 5), torch.ones(4, 5)]))
+    later = torch.randn(7, 5)
+    b = a.with_values(later)
+    b._record()
+    later.requires_grad_()
+    b.unbind()[0].sum().backward()
+    assert torch.equal(later.grad, torch.cat([torch.ones(3, 5), torch.zeros(4, 5)]))
