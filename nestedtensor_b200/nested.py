@@ -46,38 +46,60 @@ def _capturing(device) -> bool:
     return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
 
 
+class _Offsets(object):
+    """The device offsets and sizes of one set of sizes, made when something first asks for them and kept."""
+    __slots__ = ("tensor", "_copied")
+
+    def __init__(self, tensor=None):
+        self.tensor = tensor
+        self._copied = None  # an event behind their copy, until it has been seen to be through
+
+    def on(self, sizes, device):
+        """The offsets on `device`, or None where they would have to be made inside a graph capture: there they would belong to the
+        graph, and hold nothing before its replay."""
+        if self.tensor is None or self.tensor.device != device:
+            if _capturing(device):
+                return None
+            self.tensor = build_meta(sizes, device)
+            if device.type == "cuda":
+                self._copied = torch.cuda.current_stream(device).record_event()
+        elif self._copied is not None and not _capturing(device):
+            # the copy runs on the stream that first asked; another one waits for it
+            if self._copied.query():
+                self._copied = None
+            else:
+                torch.cuda.current_stream(device).wait_event(self._copied)
+        return self.tensor
+
+
 class _Ragged(object):
     """What nested tensors over the same rows share: the sizes of the one they were made from (the first column holds the
     lengths) and its device offsets.  Holds no values."""
-    __slots__ = ("sizes", "meta", "device", "_rows")
+    __slots__ = ("sizes", "offsets", "device", "_width", "_lengths")
 
-    def __init__(self, sizes, meta, device):
-        self.sizes, self.meta, self.device = sizes, meta, device
-        self._rows = None
+    def __init__(self, sizes, offsets, device):
+        self.sizes, self.offsets, self.device = sizes, offsets, device
+        self._width = self._lengths = None
 
     def on(self, device):
         """The same structure for tensors on `device`."""
-        return self if self.device == device else _Ragged(self.sizes, None, device)
+        return self if self.device == device else _Ragged(self.sizes, _Offsets(), device)
 
     def row_offsets(self):
         """(device offsets of the constituents, what one row counts in them).  Element offsets where all rows have the same
         number of elements, and at least one; otherwise only the lengths tell where a constituent begins, one a row."""
-        if self._rows is None:
-            width = _ops.ops().row_elems(self.sizes)
-            if width == 0:
-                self._refuse_capture()
-                self._rows = build_meta(self.sizes[:, :1].contiguous(), self.device), 1
-            else:
-                if self.meta is None or self.meta.device != self.device:
-                    self._refuse_capture()
-                    self.meta = build_meta(self.sizes, self.device)
-                self._rows = self.meta, width
-        return self._rows
-
-    def _refuse_capture(self):
-        if _capturing(self.device):
+        if self._width is None:
+            self._width = _ops.ops().row_elems(self.sizes)
+            if self._width == 0:
+                self._lengths = _Offsets()
+        if self._width > 0:
+            tensor = self.offsets.on(self.sizes, self.device)
+        else:
+            tensor = self._lengths.on(self.sizes[:, :1].contiguous(), self.device)
+        if tensor is None:
             raise RuntimeError("nestedtensor_b200: the offsets of this nested tensor are not on the device yet; make them before the "
                                "capture (by a pass over the same nested tensor, or one that shares its structure)")
+        return tensor, self._width or 1
 
 
 class NestedTensor(object):
@@ -91,7 +113,7 @@ class NestedTensor(object):
             raise RuntimeError("channels_last needs constituents of shape (C, H_i, W_i)")
         self._flat = buffer
         self._extents = sizes.contiguous()
-        self._offsets = meta
+        self._offsets = _Offsets(meta)
         # channels_last (nestedtensor/csrc/nested_tensor_impl.cpp:46, storage_is_contiguous_channels_last): the sizes are
         # the logical (C, H_i, W_i), every constituent is STORED as (H_i, W_i, C), i.e. with strides (1, W_i*C, C).
         self._channels_last = bool(channels_last)
@@ -104,7 +126,8 @@ class NestedTensor(object):
         """A nested tensor over the [rows, ...] matrix `packed` (contiguous; it carries the autograd graph) with the lengths of
         `ragged`; its sizes are made when something asks for them, its flat buffer (a view) every time."""
         out = cls.__new__(cls)
-        out._flat = out._extents = out._offsets = out._nchw = None
+        out._flat = out._extents = out._nchw = None
+        out._offsets = _Offsets()
         out._channels_last = False
         out._packed = packed
         out._ragged = ragged
@@ -129,11 +152,8 @@ class NestedTensor(object):
 
     @property
     def _meta(self):
-        """The device offsets and sizes, or None as long as nothing has asked for them.  A tensor with the sizes that a structure was
-        made from shares them with it."""
-        if self._offsets is None and self._packed is None and self._ragged is not None:
-            self._offsets = self._ragged.meta
-        return self._offsets
+        """The device offsets and sizes, or None as long as nothing has asked for them."""
+        return self._offsets.tensor
 
     # ---- record access -------------------------------------------------------------------
     def _record(self):
@@ -153,14 +173,8 @@ class NestedTensor(object):
 
     def _layout(self):
         """(sizes, meta) of the same record, for operators that read no values."""
-        meta = self._meta
-        if meta is None or meta.device != self._buffer.device:
-            meta = build_meta(self._sizes, self._buffer.device)
-            if not _capturing(meta.device):  # (made inside a capture, they belong to that graph and hold nothing before its replay)
-                self._offsets = meta
-                if self._packed is None and self._ragged is not None:
-                    self._ragged.meta = meta
-        return self._sizes, meta
+        meta = self._offsets.on(self._sizes, self.device)
+        return self._sizes, build_meta(self._sizes, self.device) if meta is None else meta
 
     def _stored_sizes(self):
         """Constituent shapes as they lie in the buffer."""
@@ -197,7 +211,7 @@ class NestedTensor(object):
 
     def _structure(self):
         if self._ragged is None:
-            self._ragged = _Ragged(self._extents, self._meta, self.device)
+            self._ragged = _Ragged(self._extents, self._offsets, self.device)
         return self._ragged
 
     def _with_rows(self, packed):

@@ -209,3 +209,28 @@ def test_channels_last_operators_refuse_a_tracked_buffer(cuda_device):
     got = nt.nn.conv2d(nt.NestedTensor(x.detach(), images._sizes, channels_last=True), weight)  # (the weight's gradient is not offered)
     assert torch.equal(got._buffer, want) and not got.requires_grad
     assert torch.ops.nestedtensor.to_mask(images, 2).shape[0] == 2
+
+
+def test_offsets_made_on_a_busy_stream_are_waited_for(cuda_device):
+    """The first call puts the offsets' copy on its stream, behind what is queued there; a call on another stream, over values that are
+    ready, does not run ahead of it."""
+    sizes = torch.tensor([[30, 192], [7, 192], [200, 192]])
+    x = torch.randn(237, 192, device="cuda")
+    want = training.self_attention(nt.NestedTensor(x.view(-1), sizes), 1).values()
+    padded = nt.NestedTensor(x.view(-1), sizes).to_padded_tensor(0)
+    torch.cuda.synchronize()
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    for irregular in (False, True):
+        nested = nt.NestedTensor(x.view(-1), sizes)
+        if irregular:
+            nested = nt.NestedTensor(torch.zeros(37 * 3 + 200, device="cuda"), torch.tensor([[30, 3], [7, 3], [200, 1]])).with_values(x)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(busy):
+            torch.cuda._sleep(200_000_000)  # about a tenth of a second
+            first = training.self_attention(nested, 1).values()
+        with torch.cuda.stream(other):
+            second = training.self_attention(nested, 1).values()
+            third = nested.to_padded_tensor(0)
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(second, want) and torch.equal(third, padded)
+        assert nested._row_offsets()[0].device == x.device and torch.equal(training.self_attention(nested, 1).values(), want)
