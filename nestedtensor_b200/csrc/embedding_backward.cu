@@ -477,9 +477,11 @@ int sums(const SumArgs& a, cudaStream_t st) {
     if (nv <= 96) return launch_sums<DT, EPV, 3>(a, st);
     return launch_sums<DT, EPV, 4>(a, st);
   }
+  // Single elements, several slabs of columns for wide rows.  Twelve a lane: four rows of them are in flight beside the sums, and 16
+  // spill (394 bytes stored; 12: 128).  15 000 tokens, fp32, 16 and 12 a lane: 131 columns 32 and 16 us, 333 41 and 19, 513 42 and 20,
+  // 1001 50 and 30, 2055 75 and 65; bf16: 29 and 23, 32 and 25, 33 and 26, 36 and 30, 56 and 56.
   if (a.cols <= 128) return launch_sums<DT, 1, 4>(a, st);
-  if (a.cols <= 384) return launch_sums<DT, 1, 12>(a, st);
-  return launch_sums<DT, 1, 16>(a, st);
+  return launch_sums<DT, 1, 12>(a, st);
 }
 
 }  // namespace
