@@ -18,8 +18,9 @@
 // they come from (a thread overwrites only what it has read itself), and the next S waits for this P's product.
 // Every step between the roles costs a warp some 150-200 cycles whether it waits or not, and eight warps hide little of that, so
 // a tile takes a softmax warp only two waits (S, dP) and two arrivals (P, dS): each commit also covers the product before it.
-// Measured: two sequences of about 4500 tokens, 8 heads of 128, bf16: 655 us, 0.63 PFLOP/s of the five products.  Tensor pipe 17 to
-// 26 %, exponentials 14 %, issue slots 32 %: nothing is full; what a tile waits for is the latency of the chain S, P, dP, dS.
+// Measured: two sequences of about 4500 tokens, 8 heads of 128, bf16: 619 us, 0.67 PFLOP/s of the five products.  Tensor pipe 46 %,
+// exponentials 20 %, issue slots 35 %: nothing is full; what a tile waits for is the latency of the chain S, P, dP, dS.  The compiler
+// works within the 168 registers of the launch: heads of 128 spill 80 bytes a thread (stores; 156 loads), heads of 64 24 (52).
 // All barriers count tiles g of the CTA over its items.  Every wait is bounded: a wait that runs out sets an error flag, the
 // roles fall through and the CTA frees its tensor memory.
 
@@ -666,8 +667,10 @@ attn_bwd_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 // tiles up in fp32 (scratch in global memory, one thread per row and always the same one: the order of the sum is fixed) and
 // write them out with the last key tile; a sequence of one key tile needs no scratch.
 // Half the exponentials and 5/7 of the products of the kernel above, but a sequence is one CTA's: for batches whose sequences are
-// short and many (attention_backward.cu chooses).  34 000 tokens in 128 sequences of 32 to 512, 12 heads, fp16: 372 us, 0.24
-// PFLOP/s of the five products; bound, like the kernel above, by the chain S, P, dP, dS, product through each softmax warp.
+// short and many (attention_backward.cu chooses).  34 000 tokens in 128 sequences of 32 to 512, 12 heads, fp16: 356 us, 0.25
+// PFLOP/s of the five products; bound, like the kernel above, by the chain S, P, dP, dS, product through each softmax warp (tensor
+// pipe 16 %, exponentials 12 %, issue slots 25 %, and 15 % of the time some SMs have no sequence left).  The 128 registers of the launch
+// spill 226 bytes a thread in fp16 (stores; 278 loads) and 196 (248) in bf16.
 constexpr int kFusedThreads = 512;
 constexpr int kFusedRegSoftmax = 168, kFusedRegAdd = 96, kFusedRegControl = 80, kFusedRegLaunch = 128;
 static_assert(2 * kFusedRegSoftmax + kFusedRegAdd + kFusedRegControl == 4 * kFusedRegLaunch && kFusedRegLaunch * kFusedThreads <= 65536,

@@ -12,7 +12,8 @@
 //
 // Measured at 150 000 tokens of a table of 50 000 x 1024 bf16, frequencies falling as 1 / rank: sort 34 us (two passes of 8 bits, each
 // a count and a scatter that wait on one another, far from any rate), sums 74 us (0.41 GB: 5.5 TB/s), runs over several
-// warps 24 us (most tokens belong to a few hundred indices, whose partial rows are read again).
+// warps 24 us (most tokens belong to a few hundred indices, whose partial rows are read again).  Up to a few thousand tokens the
+// launches one after another are the time: 310 tokens of 256 fp32 columns take 24 us in three kernels.
 
 #include "row_vec.cuh"
 
@@ -470,6 +471,7 @@ int launch_sums(const SumArgs& a, cudaStream_t st) {
 template <int DT>
 int sums(const SumArgs& a, cudaStream_t st) {
   constexpr int EPV = Vec16<DT>::kElems;
+  // (four 16-byte vectors a lane, over 96 of them a row, spill 36 bytes beside the four rows in flight)
   if (a.cols % EPV == 0 && aligned16(a.grad) && aligned16(a.dw)) {
     const int64_t nv = a.cols / EPV;
     if (nv <= 32) return launch_sums<DT, EPV, 1>(a, st);

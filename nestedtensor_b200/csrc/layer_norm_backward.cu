@@ -9,9 +9,12 @@
 // column sums stay in their registers (fp32) over all rows of a persistent block; every block leaves one [2, E] partial, and a
 // second, small kernel adds the partials in block order.  No atomics: the same bits on every run.
 //
-// Measured: 976 000 rows of 1024 bf16 in 942 us (6.4 TB/s, 0.97 of a copy); 37 000 of 768 fp16 in 43 us (4.0 TB/s: one to two waves
-// of rows a block, whose first loads and column sums do not overlap); 24 000 of 771 bf16, element by element, in 56 us (2.0
-// TB/s, bound by instruction issue).
+// Measured: 976 000 rows of 1024 bf16 in 942 us alone (6.4 TB/s, 0.97 of a copy), 1040 back to back with the forward pass; 37 000 of
+// 768 fp16 in 43 us (4.0 TB/s): 18 us of that do not depend on the rows (4 700 take 19, 75 000 70, 303 000 224; the rest goes at
+// 6.8 TB/s), and most of those are the column sums at the end, eight turns of a block with a barrier after each (30 % of the warps' time
+// is spent at barriers, of which the rows have none); 24 000 of 771 bf16, element by element, in 56 us (2.0 TB/s, bound by
+// instruction issue).  Rows that neither form holds in registers are read again: 20 000 of 8200 bf16 take 900 us (1.1 TB/s) and of
+// 4100 462, where 8192 take 212.
 
 #include "row_vec.cuh"
 
@@ -399,6 +402,8 @@ int launch_backward(const BwdCall& c, int* blocks, cudaStream_t st) {
     if (nv <= 768) return launch_rows<DT, EPV, 3, 256, AFFINE>(c, blocks, st);
     if (nv <= 1024) return launch_rows<DT, EPV, 4, 256, AFFINE>(c, blocks, st);
   } else {
+    // (13 elements a thread beside 16: the two sums of each are registers too.  24 000 rows of 515 bf16 take 47 us with 13 and 56 with
+    // 16, of 705 55 and 66, of 831 58 and 72; in fp32 the two are within 1.5 us)
     if (c.cols <= 128) return launch_rows<DT, 1, 4, 32, AFFINE>(c, blocks, st);
     if (c.cols <= 256) return launch_rows<DT, 1, 8, 32, AFFINE>(c, blocks, st);
     if (c.cols <= 512) return launch_rows<DT, 1, 8, 64, AFFINE>(c, blocks, st);

@@ -337,6 +337,7 @@ int launch_layer_norm(const void* x, const void* residual, const void* bias, con
     layer_norm_elements_kernel<DT, VPL, GROUP><<<(unsigned)(need < 148 * 32 ? need : 148 * 32), kLnThreads, 0, st>>>(      \
         x, gamma, beta, eps, out, rows, (int)cols, stats);                                                                 \
   } while (0)
+    // (13 elements a thread beside 16: 24 000 rows of 515 bf16 take 33 us with 13 and 35 with 16, of 705 36 and 39, of 831 37 and 43)
     if (cols <= 128) NTB200_LN_ELEMENTS(4, 32);
     else if (cols <= 512) NTB200_LN_ELEMENTS(16, 32);
     else if (cols <= 832) NTB200_LN_ELEMENTS(13, 64);
