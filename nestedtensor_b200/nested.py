@@ -54,6 +54,11 @@ class _Offsets(object):
         self.tensor = tensor
         self._copied = None  # an event behind their copy, until it has been seen to be through
 
+    def __reduce__(self):  # (copies and pickles of a nested tensor: events are none of theirs)
+        if self._copied is not None:
+            self._copied.synchronize()
+        return _Offsets, (self.tensor,)
+
     def on(self, sizes, device):
         """The offsets on `device`, or None where they would have to be made inside a graph capture: there they would belong to the
         graph, and hold nothing before its replay."""

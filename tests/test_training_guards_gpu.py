@@ -1,5 +1,8 @@
 """The training operators where a call could go wrong unseen: structures of any trailing sizes, what autograd sees of the caller's
 tensors, captured graphs."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -234,3 +237,16 @@ def test_offsets_made_on_a_busy_stream_are_waited_for(cuda_device):
         torch.cuda.synchronize()
         assert torch.equal(first, want) and torch.equal(second, want) and torch.equal(third, padded)
         assert nested._row_offsets()[0].device == x.device and torch.equal(training.self_attention(nested, 1).values(), want)
+
+
+def test_copies_and_pickles(cuda_device):
+    """Of a nested tensor whose offsets have just been made, and of one made from it."""
+    sizes = torch.tensor([[3, 96], [50, 96]])
+    x = torch.randn(53, 96, device="cuda")
+    a = nt.NestedTensor(x.view(-1), sizes)
+    b = a.with_values(x * 2)
+    want = [training.self_attention(t, 2).values() for t in (a, b)]
+    padded = [t.to_padded_tensor(0) for t in (a, b)]
+    for again in (copy.deepcopy((a, b)), pickle.loads(pickle.dumps((a, b)))):
+        for t, w, p in zip(again, want, padded):
+            assert torch.equal(training.self_attention(t, 2).values(), w) and torch.equal(t.to_padded_tensor(0), p)
